@@ -393,6 +393,84 @@ int okc_tp_oproj_allreduce_residual(const void* x, int ldx, const void* w, int l
                                     void* workspace, okc_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
+ * The 8-bit projection path and ragged batches.  No reference counterpart: the reference
+ * projects in bf16, rotates with one axis and masks causally (or in a window) only.
+ *
+ * These entry points keep no state in their workspace: it needs no initialisation, and calls
+ * that may overlap (on two streams, or two captured graphs replayed side by side) are given
+ * different ones.  `error` is a 32-bit device word, zeroed once by the caller, into which
+ * OKC_DEVERR_* bits are OR'd (okc_read_device_error reads and clears it); overlapping calls may
+ * share it.  T (M) = 0 is a call that does nothing.
+ *
+ * Ragged batches: cu_q int32 [B + 1] ascending from 0; request b owns the rows cu_q[b] ..
+ * cu_q[b+1]-1, and row t sits at the cache position seq_lens[b] - (cu_q[b+1] - t): seq_lens int32 [B]
+ * counts the cached positions with the new ones.  Rows from cu_q[B] to T-1 (a padded batch) are
+ * neither read nor written.
+ * ---------------------------------------------------------------------------------- */
+
+/* Residual add + RMSNorm to e4m3: s = x + residual rounded to the residual's type and stored in
+ * residual_out (which may be residual); y = s * rsqrt(mean(s^2) + eps) * g, g = w or 1 + w
+ * (unit_offset); scale[t] = max|y[t]| / 448, 1 for a row of zeros; q = e4m3(y / scale), RNE.  Without
+ * residual (NULL, residual_out NULL) s = x.  x bf16 [T][ldx], residual bf16 or fp32
+ * (residual_fp32) [T][ldr], residual_out [T][ldo] of the same type, w bf16 [H], q e4m3 [T][ldq],
+ * scale fp32 [T].  H a multiple of 16, <= 16384; rows 16-byte aligned.  A row that holds an
+ * infinity or a NaN gets an infinite or NaN scale.  Beside okc_rmsnorm_bf16. */
+int okc_add_rmsnorm_fp8(const void* x, int64_t ldx, const void* residual, int64_t ldr, int residual_fp32,
+                        const void* w, void* residual_out, int64_t ldo, void* q, int64_t ldq, float* scale,
+                        int T, int H, float eps, int unit_offset, okc_stream_t stream);
+
+/* Projection with an epilogue: y = act(x w^T * x_scale[m] * w_scale[n] + bias[n]) + residual.  x [M][ldx] and
+ * w [N][ldw] both bf16 (e4m3 = 0) or both e4m3 (e4m3 = 1); x_scale fp32 [M], w_scale fp32 [N] or, with
+ * w_scale_one, [1]; bias bf16 [N]; residual bf16 or fp32 (residual_fp32) [M][ldr]; each of the four may be
+ * NULL.  y bf16 or fp32 (out_fp32) [M][ldy].  act: 0 none, 1 relu, 2 silu, 3 gelu (erf), 4 gelu
+ * (tanh form).  fp32 accumulation and epilogue, one rounding.  x and w rows are 16-byte aligned
+ * (base, and ld x element size a multiple of 16 bytes); K itself is a multiple of 16 (e4m3) or 8 (bf16).
+ * y may be residual.  Beside okc_gemm_bf16. */
+size_t okc_linear_workspace_bytes(int M, int N, int K, int e4m3);
+int okc_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int e4m3, const float* x_scale,
+               const float* w_scale, int w_scale_one, const void* bias, int act, const void* residual,
+               int64_t ldr, int residual_fp32, void* y, int64_t ldy, int out_fp32, int M, int N, int K,
+               void* workspace, size_t workspace_bytes, int32_t* error, okc_stream_t stream);
+
+/* Rotary positions with several axes and the FP8 KV-append of a ragged batch.  qkv bf16 [T][ldqkv] =
+ * q (Hq*D) | k (Hkv*D) | v (Hkv*D); positions int64 [axes][ld_pos], axes 1..4; pair i < pairs of every q
+ * and k head turns by positions[axis_of_pair[i]][t] * inv_freq[i], formed in 64 bits; axis_of_pair is
+ * a HOST array of `pairs` bytes.  A pair is (2i, 2i+1), or (i, i + pairs) with half_split; elements
+ * from 2*pairs on pass.  q goes to bf16 q_out [T][ldq], k / k_scale[h] and v / v_scale[h] to the e4m3
+ * caches [num_pages, P, Hkv, D] (RNE, overflow -> NaN) at page_table[b][pos / P] * P + pos % P, pos the
+ * row's cache position above, which its rotary positions need not equal.  A position outside the
+ * table or the pool is skipped (OKC_DEVERR_PAGE; its q row is still written).  D a multiple of 8,
+ * <= 256, pairs a multiple of 8, 2*pairs <= D, rows 16-byte aligned.  Beside okc_rope_kv_append. */
+int okc_rope_axes_kv_append(const void* qkv, int64_t ldqkv, const int64_t* positions, int64_t ld_pos, int axes,
+                            const uint8_t* axis_of_pair, const float* inv_freq, int pairs, int half_split,
+                            const int32_t* cu_q, const int32_t* seq_lens, int B, const int32_t* page_table,
+                            int64_t table_ld, int max_pages, const float* k_scale, const float* v_scale,
+                            void* q_out, int64_t ldq, void* k_cache, void* v_cache, int T, int Hq, int Hkv,
+                            int D, int page_size, int64_t num_pages, int32_t* error, okc_stream_t stream);
+
+/* Attention of ragged chunks of new tokens (their keys appended) over the paged e4m3 cache.  The
+ * row of a token at position p sees the positions [lo, hi):
+ *   lo = max(0, doc_start[t], p + 1 - window),  hi = min(seq_len, max(p + 1, prefix_lens[b])),
+ * doc_start int32 [T] (packed documents), prefix_lens int32 [B] (a prefix that every token sees),
+ * window 0 = none; NULL leaves either out.  Scores: s_j = q.k_j * sm_scale, with softcap > 0
+ * softcap * tanh(s_j / softcap), then minus slopes[h] * |p - j| (fp32 [Hq] or NULL).  out = softmax(s) v,
+ * zero for a row that sees nothing; a position that a row does not see does not reach it whatever
+ * the cache holds there.  q bf16 [T][ldq], out bf16 [T][ldo] (Hq heads of D), caches e4m3
+ * [num_pages, P, Hkv, D] with scales fp32 [Hkv], page_table int32 [B][table_ld] (max_pages columns).  A
+ * position on a page outside the pool reads zeros, one past the table does not exist (both
+ * OKC_DEVERR_PAGE).  max_q: the longest chunk (0 = unknown); it only chooses kernels.  D 64 or
+ * 128, B <= 2048, Hq / Hkv whole, 16-byte aligned rows.  Beside okc_attn_decode_fp8 and
+ * okc_attn_prefill_fp8. */
+size_t okc_attn_chunk_workspace_bytes(int T, int B, int Hq, int Hkv, int D);
+int okc_attn_chunk_fp8(const void* q, int64_t ldq, const void* k_cache, const void* v_cache,
+                       const int32_t* page_table, int64_t table_ld, int max_pages, const int32_t* cu_q,
+                       const int32_t* seq_lens, const float* k_scale, const float* v_scale,
+                       const float* slopes, const int32_t* prefix_lens, const int32_t* doc_start, void* out,
+                       int64_t ldo, int T, int B, int Hq, int Hkv, int D, int page_size, int64_t num_pages,
+                       float sm_scale, float softcap, int window, int max_q, void* workspace,
+                       size_t workspace_bytes, int32_t* error, okc_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
  * The short names of the decode-path contract (the C-ABI list the drop-in boundary
  * names), as thin forms of the entry points above:
  *   okc_gemv_bf16       = okc_gemm_bf16 with contiguous x [M,K], W [N,K], y [M,N] (bf16,

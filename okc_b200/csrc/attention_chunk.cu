@@ -1,0 +1,657 @@
+// Attention of ragged chunks of new tokens over the paged e4m3 cache, for chunks of few rows
+// (decode tokens, verify blocks): split over the keys, joined by a log-sum-exp merge.
+//
+// Query row (token t, head h) of request b, at position p, sees the positions [lo, hi) with
+//   lo = max(0, doc_start[t], p + 1 - window),   hi = min(seq_len, max(p + 1, prefix_len)),
+// so every mask here (causal, sliding window, packed documents, a prefix that all tokens see) is one
+// interval per row.  Its scores are
+//   s_j = cap * tanh(q.k_j * sm_scale / cap) - slope[h] * |p - j|,   o = sum_j softmax(s)_j v_j,
+// and a row that sees nothing is zero.
+//
+// Bound by the cache read (2 D bytes a key and KV head).  The rows of one KV head's query group
+// (token-major, G heads a token) fill the 16 rows of mma.sync tiles; e4m3 keys and values are exact in
+// f16, the query too once its row is scaled by a power of two, and P is rounded to f16 (2^-11).
+//  * units of 32 keys x (8 / nh) subgroups of a (request, row tile, nh heads) are numbered in order
+//    and split evenly over a persistent grid (ragged contexts stay balanced); the nh heads of a
+//    key lie side by side in the cache, so the block's warps read whole token rows together;
+//  * a warp owns a ring of key blocks in shared memory that it fills with cp.async and reads as MMA
+//    fragments: no block barrier in the loop.  Page ids are fetched a block ahead.  Positions outside the
+//    tile's interval, or on a page outside the pool, are zero-filled, never read;
+//  * a K fragment's k slots and a V fragment's columns are permuted so that each lane's share is
+//    whole 16-byte chunks (a sum over k does not depend on its order).
+// Partial sums go to the workspace as fp32 with their running maximum and sum; segments are joined
+// in block order, so results repeat bit for bit.
+#include "chunk_common.cuh"
+
+namespace okc {
+
+namespace {
+
+constexpr int kStep = 32;      // keys per warp step
+constexpr int kWarps = 8;
+constexpr int kRows = 16;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// tanh(x) from exp(2x) given x * 2 log2(e): 1 - 2 / (1 + e^2x); off by a few 2^-24 absolute, which a cap of
+// 50 turns into 10^-5 of a score.
+__device__ __forceinline__ float tanh_from_2l2e(float x) { return 1.f - __fdividef(2.f, 1.f + ex2(x)); }
+
+__device__ __forceinline__ uint32_t e4m3x2_h2(uint32_t two) {
+  uint32_t h;
+  asm("{\n .reg .b16 t;\n cvt.u16.u32 t, %1;\n cvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(h) : "r"(two));
+  return h;
+}
+
+__device__ __forceinline__ uint32_t h2(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
+template <int D>
+struct ChunkCfg {
+  static constexpr int STAGE = 2 * kStep * D;  // K and V of a step
+  static constexpr int STAGES = 3;
+  static constexpr int RING = STAGE * STAGES;
+  static constexpr int SMEM = RING * kWarps;
+};
+
+struct SplitPlan {
+  int nh, nsub, hg;   // heads side by side in a block, key subgroups, head groups
+  int step_keys;      // keys of a unit
+  int ctas;
+  int* pre_u;         // [B + 1] units before a request
+  int* pre_t;         // [B + 1] row tiles (times head groups) before a request
+  float* ml;          // [slot][nh][16][2]
+  float* acc;         // [slot][nh][16][D]
+  int most_rows;      // requests of more rows are served by the other kernel
+};
+
+struct Req {
+  int n, len, lo, hi, prefix;  // new tokens, cached tokens, union of the rows' key intervals
+};
+
+__device__ __forceinline__ Req request(const ChunkArgs& a, int b) {
+  Req r;
+  r.n = max(0, a.cu_q[b + 1] - a.cu_q[b]);
+  r.len = max(0, a.seq_lens[b]);
+  r.prefix = a.prefix_lens ? a.prefix_lens[b] : 0;
+  r.lo = a.window > 0 ? max(0, r.len - r.n + 1 - a.window) : 0;
+  r.hi = min(r.len, a.max_keys);  // positions past the table's columns do not exist
+  return r;
+}
+
+__device__ __forceinline__ void unit_split(int U, int C, int c, int& u0, int& u1) {
+  const int q = U / C, r = U % C;
+  u0 = c * q + min(c, r);
+  u1 = u0 + q + (c < r ? 1 : 0);
+}
+__device__ __forceinline__ int unit_owner(int U, int C, int u) {
+  const int q = U / C, r = U % C, big = r * (q + 1);
+  return u < big ? u / (q + 1) : r + (u - big) / q;
+}
+
+// Units and row tiles before each request, by one warp.
+__device__ __forceinline__ void split_prefix(const ChunkArgs& a, const SplitPlan& pl, int* pre_u, int* pre_t) {
+  const int lane = threadIdx.x & 31;
+  int cu = 0, ct = 0;
+  for (int base = 0; base < a.B; base += 32) {
+    const int b = base + lane;
+    int u = 0, t = 0;
+    if (b < a.B) {
+      const Req r = request(a, b);
+      const int rows = r.n * a.G;
+      if (r.len > a.max_keys && blockIdx.x == 0) atomicOr(a.err, OKC_DEVERR_PAGE);
+      if (rows <= pl.most_rows) {
+        t = (rows + kRows - 1) / kRows * pl.hg;
+        u = t * ((max(0, r.hi - r.lo) + pl.step_keys - 1) / pl.step_keys);
+      }
+    }
+    int su = u, st = t;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, su, o), y = __shfl_up_sync(0xffffffffu, st, o);
+      if (lane >= o) {
+        su += x;
+        st += y;
+      }
+    }
+    if (b < a.B) {
+      pre_u[b] = cu + su - u;
+      pre_t[b] = ct + st - t;
+    }
+    cu += __shfl_sync(0xffffffffu, su, 31);
+    ct += __shfl_sync(0xffffffffu, st, 31);
+  }
+  if (lane == 0) {
+    pre_u[a.B] = cu;
+    pre_t[a.B] = ct;
+  }
+}
+
+template <int D, bool CAP>
+__global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs a, SplitPlan pl) {
+  using C = ChunkCfg<D>;
+  constexpr int KS = D / 16;   // k16 steps of QK
+  constexpr int ND = D / 8;    // n8 blocks of PV
+  constexpr int NCH = D / 16;  // 16-byte chunks of a key
+  extern __shared__ __align__(128) uint8_t smem[];
+  int* pre_u = reinterpret_cast<int*>(smem + C::SMEM);
+  int* pre_t = pre_u + a.B + 1;
+
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  if (warp == 0) split_prefix(a, pl, pre_u, pre_t);
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i <= a.B; i += blockDim.x) {
+      pl.pre_u[i] = pre_u[i];
+      pl.pre_t[i] = pre_t[i];
+    }
+  int u0, u1;
+  unit_split(pre_u[a.B], gridDim.x, blockIdx.x, u0, u1);
+  const int hw = warp % pl.nh, sub = warp / pl.nh;
+  uint8_t* ring = smem + warp * C::RING;
+  const uint32_t ring_s = smem_u32(ring);
+
+  while (u0 < u1) {
+    int b, hi_b = a.B - 1;
+    for (b = 0; b < hi_b;) {  // largest b with pre_u[b] <= u0 (requests without units share a prefix)
+      const int mid = (b + hi_b + 1) >> 1;
+      if (pre_u[mid] <= u0) b = mid; else hi_b = mid - 1;
+    }
+    const Req rq = request(a, b);
+    const int nc = (max(0, rq.hi - rq.lo) + pl.step_keys - 1) / pl.step_keys;
+    const int in_b = u0 - pre_u[b], tile = in_b / nc, c0 = in_b - tile * nc;
+    const int c1 = min(nc, c0 + (u1 - u0));
+    const int rt = tile / pl.hg, head = (tile - rt * pl.hg) * pl.nh + hw;
+    const int slot = blockIdx.x + pre_t[b] + tile;
+    u0 += c1 - c0;
+
+    // ---- the lane's two rows ----
+    const int rows = rq.n * a.G, r0 = rt * kRows;
+    const int row0 = a.cu_q[b], p_base = rq.len - rq.n;
+    int lo[2], hi[2], pos[2];
+    bool live[2];
+    float slope[2], fac[2];
+    uint32_t qf[KS][4];
+    const bool two = rows - r0 > 8;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = r0 + g + 8 * e;
+      live[e] = r < rows;
+      const int i = live[e] ? r / a.G : 0, hq = head * a.G + (live[e] ? r - i * a.G : 0);
+      pos[e] = p_base + i;
+      lo[e] = hi[e] = 0;
+      slope[e] = 0.f;
+      uint2 qv[KS];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) qv[k] = make_uint2(0u, 0u);
+      if (live[e]) {
+        hi[e] = min(rq.hi, max(pos[e] + 1, rq.prefix));
+        if (a.window > 0) lo[e] = max(0, pos[e] + 1 - a.window);
+        if (a.doc_start) lo[e] = max(lo[e], a.doc_start[row0 + i]);
+        if (a.slopes) slope[e] = a.slopes[hq] * 1.4426950408889634f;
+        const __nv_bfloat16* qp = a.q + (size_t)(row0 + i) * a.ldq + (size_t)hq * D;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)  // the four elements of step k's slots
+          qv[k] = *reinterpret_cast<const uint2*>(qp + 64 * (k >> 2) + 16 * c + 4 * (k & 3));
+      }
+      // scale the row by 2^-s so that its largest magnitude lies in [2^13, 2^14): exact in f16 down to 2^-27 of it
+      uint32_t top = 0;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        top = max(max(top, max(qv[k].x & 0x7fffu, (qv[k].x >> 16) & 0x7fffu)),
+                  max(qv[k].y & 0x7fffu, (qv[k].y >> 16) & 0x7fffu));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int sh = max(-100, (int)(top >> 7) - 127 - 13);
+      const float down = __uint_as_float((uint32_t)(127 - sh) << 23);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        qf[k][e] = h2(bf16_lo(qv[k].x) * down, bf16_hi(qv[k].x) * down);
+        qf[k][2 + e] = h2(bf16_lo(qv[k].y) * down, bf16_hi(qv[k].y) * down);
+      }
+      // without a cap: log2 units; with one: the argument of tanh times 2 log2(e)
+      fac[e] = a.k_scale[head] * a.sm_scale * (CAP ? 2.f / a.softcap : 1.f) * 1.4426950408889634f *
+               __uint_as_float((uint32_t)(127 + sh) << 23);
+    }
+    const float cap2 = CAP ? a.softcap * 1.4426950408889634f : 0.f;
+    // keys that every live row sees need no mask; keys outside [t_lo, t_hi) are not read
+    int full_lo = max(live[0] ? lo[0] : 0, live[1] ? lo[1] : 0);
+    int full_hi = min(live[0] ? hi[0] : 0x7fffffff, live[1] ? hi[1] : 0x7fffffff);
+    int t_lo = min(live[0] ? lo[0] : 0x7fffffff, live[1] ? lo[1] : 0x7fffffff);
+    int t_hi = max(live[0] ? hi[0] : 0, live[1] ? hi[1] : 0);
+    full_lo = __reduce_max_sync(0xffffffffu, full_lo);
+    full_hi = __reduce_min_sync(0xffffffffu, full_hi);
+    t_lo = __reduce_min_sync(0xffffffffu, t_lo);
+    t_hi = __reduce_max_sync(0xffffffffu, t_hi);
+
+    // ---- the warp's steps: keys [k0 + s * step_keys, + 32), those that meet [t_lo, t_hi) ----
+    const int k0 = rq.lo + c0 * pl.step_keys + sub * kStep;
+    int s_lo = 0, s_hi = c1 - c0;
+    if (t_lo > k0 + kStep - 1) s_lo = (t_lo - (k0 + kStep - 1) + pl.step_keys - 1) / pl.step_keys;
+    if (t_hi < k0 + (s_hi - 1) * pl.step_keys + 1) s_hi = t_hi <= k0 ? 0 : (t_hi - k0 + pl.step_keys - 1) / pl.step_keys;
+    const int32_t* trow = a.page_table + (size_t)b * a.table_ld;
+    const size_t hoff = (size_t)head * D;
+    auto fetch_page = [&](int s) -> int {  // this lane's key of step s; -1: not read
+      const int key = k0 + s * pl.step_keys + lane;
+      if (s >= s_hi || key < t_lo || key >= t_hi) return -1;
+      const int page = trow[key / a.P];
+      if (page < 0 || page >= a.num_pages) {
+        atomicOr(a.err, OKC_DEVERR_PAGE);
+        return -1;
+      }
+      return page;
+    };
+    auto issue = [&](int s, int page) {
+      if (s < s_hi) {
+        const int key = k0 + s * pl.step_keys + lane;
+        const long long off = page < 0 ? -1 : ((long long)page * a.P + key % a.P) * a.Hkv * D + (long long)hoff;
+        const uint32_t st = ring_s + (uint32_t)((s - s_lo) % C::STAGES) * C::STAGE;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          const int k = i * (32 / NCH) + lane / NCH, ch = lane % NCH;
+          const long long o = __shfl_sync(0xffffffffu, off, k);
+          const bool on = o >= 0;
+          const size_t src = on ? (size_t)o + ch * 16 : 0;
+          int kc = ch, vc = ch;
+          if (D == 128) {
+            kc ^= 4 * (k & 1);
+            vc ^= 2 * ((k >> 2) & 3);
+          }
+          cp16(st + k * D + kc * 16, a.k_cache + src, on);
+          cp16(st + kStep * D + k * D + vc * 16, a.v_cache + src, on);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    float o_acc[ND][4];
+#pragma unroll
+    for (int n = 0; n < ND; ++n) o_acc[n][0] = o_acc[n][1] = o_acc[n][2] = o_acc[n][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    int page = fetch_page(s_lo);
+#pragma unroll
+    for (int i = 0; i < C::STAGES - 1; ++i) {
+      const int next = fetch_page(s_lo + i + 1);
+      issue(s_lo + i, page);
+      page = next;
+    }
+
+    for (int s = s_lo; s < s_hi; ++s) {
+      const int next = fetch_page(s + C::STAGES);
+      __syncwarp();  // every lane has read the stage that is filled now
+      issue(s + C::STAGES - 1, page);
+      page = next;
+      asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 1) : "memory");
+      __syncwarp();
+      const uint8_t* ks = ring + ((s - s_lo) % C::STAGES) * C::STAGE;
+      const uint8_t* vs = ks + kStep * D;
+      const int kb0 = k0 + s * pl.step_keys;
+
+      // S: block 2 kb + h, column n <-> key 16 kb + 4 (n / 2) + n % 2 + 2 h
+      float sc[4][4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+        const int k = 16 * (n >> 1) + 4 * (g >> 1) + (g & 1) + 2 * (n & 1);
+#pragma unroll
+        for (int v = 0; v < D / 64; ++v) {
+          int ch = c + 4 * v;
+          if (D == 128) ch ^= 4 * (k & 1);
+          const uint4 kv = *reinterpret_cast<const uint4*>(ks + k * D + ch * 16);
+          const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            mma_f16_16816(sc[n], qf[4 * v + i][0], qf[4 * v + i][1], qf[4 * v + i][2], qf[4 * v + i][3],
+                          e4m3x2_h2(w[i] & 0xffffu), e4m3x2_h2(w[i] >> 16));
+        }
+      }
+      // scores, running maximum, P
+      const bool edge = kb0 < full_lo || kb0 + kStep > full_hi;
+      uint32_t pf[2][4];
+      float corr[2] = {1.f, 1.f};
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (e == 1 && !two) {
+          pf[0][1] = pf[0][3] = pf[1][1] = pf[1][3] = 0u;
+          break;
+        }
+        float x[8];  // block n, column 2 c + i: key 16 (n / 2) + 4 c + i + 2 (n % 2)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float v = sc[n][2 * e + i] * fac[e];
+            if (CAP) v = cap2 * tanh_from_2l2e(v);
+            x[2 * n + i] = v;
+          }
+        if (a.slopes) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int key = kb0 + 16 * (n >> 1) + 4 * c + i + 2 * (n & 1);
+              x[2 * n + i] -= slope[e] * (float)abs(pos[e] - key);
+            }
+        }
+        if (edge) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int key = kb0 + 16 * (n >> 1) + 4 * c + i + 2 * (n & 1);
+              if (key < lo[e] || key >= hi[e]) x[2 * n + i] = -INFINITY;
+            }
+        }
+        float top = x[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float nm = fmaxf(m[e], top);
+        const float org = nm == -INFINITY ? 0.f : nm;  // nothing seen yet: any finite origin
+        corr[e] = ex2(m[e] - org);
+        m[e] = nm;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = ex2(x[i] - org);
+          sum += x[i];
+        }
+        l[e] = l[e] * corr[e] + sum;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          pf[kb][e] = h2(x[4 * kb], x[4 * kb + 1]);
+          pf[kb][2 + e] = h2(x[4 * kb + 2], x[4 * kb + 3]);
+        }
+      }
+      if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+          o_acc[n][0] *= corr[0];
+          o_acc[n][1] *= corr[0];
+          o_acc[n][2] *= corr[1];
+          o_acc[n][3] *= corr[1];
+        }
+      }
+      // O += P V: column n of block nb <-> d = (D / 8) n + nb
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        constexpr int W = D / 32;  // words of a lane's share of a key
+        uint32_t vw[4][W];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = 16 * kb + 4 * c + i;
+          if (D == 128) {
+            const uint4 t4 = *reinterpret_cast<const uint4*>(vs + k * D + (g ^ (2 * ((k >> 2) & 3))) * 16);
+            vw[i][0] = t4.x;
+            vw[i][1] = t4.y;
+            vw[i][W - 2] = t4.z;
+            vw[i][W - 1] = t4.w;
+          } else {
+            const uint2 t2 = *reinterpret_cast<const uint2*>(vs + k * D + g * 8);
+            vw[i][0] = t2.x;
+            vw[i][1] = t2.y;
+          }
+        }
+        // A NaN value in a position that a row does not see must not reach it through 0 * NaN: on a step
+        // with such positions NaN values are taken out of the product and put into the rows that see them.
+        if (edge) {
+          uint32_t bad = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+              const uint32_t nan = ((vw[i][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+              bad |= nan;
+              vw[i][w] &= ~((nan >> 7) * 0xffu);
+            }
+          if (__any_sync(0xffffffffu, bad != 0)) {
+            for (int k = 0; k < 16; ++k)
+#pragma unroll
+              for (int n = 0; n < ND; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const int kk = 16 * kb + k, d = (D / 8) * (2 * c + i) + n, key = kb0 + kk;
+                  int ch = d / 16;
+                  if (D == 128) ch ^= 2 * ((kk >> 2) & 3);
+                  if ((vs[kk * D + ch * 16 + d % 16] & 0x7f) == 0x7f) {
+                    if (key >= lo[0] && key < hi[0]) o_acc[n][i] = __uint_as_float(0x7fffffffu);
+                    if (key >= lo[1] && key < hi[1]) o_acc[n][2 + i] = __uint_as_float(0x7fffffffu);
+                  }
+                }
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const uint32_t a01 = prmt(vw[0][w], vw[1][w], 0x5140), b01 = prmt(vw[0][w], vw[1][w], 0x7362);
+          const uint32_t a23 = prmt(vw[2][w], vw[3][w], 0x5140), b23 = prmt(vw[2][w], vw[3][w], 0x7362);
+          mma_f16_16816(o_acc[4 * w + 0], pf[kb][0], pf[kb][1], pf[kb][2], pf[kb][3], e4m3x2_h2(a01 & 0xffffu),
+                        e4m3x2_h2(a23 & 0xffffu));
+          mma_f16_16816(o_acc[4 * w + 1], pf[kb][0], pf[kb][1], pf[kb][2], pf[kb][3], e4m3x2_h2(a01 >> 16),
+                        e4m3x2_h2(a23 >> 16));
+          mma_f16_16816(o_acc[4 * w + 2], pf[kb][0], pf[kb][1], pf[kb][2], pf[kb][3], e4m3x2_h2(b01 & 0xffffu),
+                        e4m3x2_h2(b23 & 0xffffu));
+          mma_f16_16816(o_acc[4 * w + 3], pf[kb][0], pf[kb][1], pf[kb][2], pf[kb][3], e4m3x2_h2(b01 >> 16),
+                        e4m3x2_h2(b23 >> 16));
+        }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+    }
+
+    // ---- join the key subgroups of a head in shared memory, in order ----
+    if (pl.nsub > 1) {
+      float* mine = reinterpret_cast<float*>(ring);  // [16][D] and [16][2]
+      __syncwarp();
+      if (sub > 0) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float* dst = mine + (g + 8 * e) * D + (D / 4) * c;
+#pragma unroll
+          for (int n = 0; n < ND; ++n) {
+            dst[n] = o_acc[n][2 * e];
+            dst[D / 8 + n] = o_acc[n][2 * e + 1];
+          }
+          if (c == 0) {
+            mine[kRows * D + 2 * (g + 8 * e)] = m[e];
+            mine[kRows * D + 2 * (g + 8 * e) + 1] = l[e];
+          }
+        }
+      }
+      __syncthreads();
+      if (sub == 0) {
+        for (int s2 = 1; s2 < pl.nsub; ++s2) {
+          const float* from = reinterpret_cast<const float*>(smem + (warp + s2 * pl.nh) * C::RING);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float om = from[kRows * D + 2 * (g + 8 * e)], ol = from[kRows * D + 2 * (g + 8 * e) + 1];
+            const float nm = fmaxf(m[e], om), org = nm == -INFINITY ? 0.f : nm;
+            const float fa = ex2(m[e] - org), fb = ex2(om - org);
+            m[e] = nm;
+            l[e] = l[e] * fa + ol * fb;
+            const float* src = from + (g + 8 * e) * D + (D / 4) * c;
+#pragma unroll
+            for (int n = 0; n < ND; ++n) {
+              o_acc[n][2 * e] = o_acc[n][2 * e] * fa + src[n] * fb;
+              o_acc[n][2 * e + 1] = o_acc[n][2 * e + 1] * fa + src[D / 8 + n] * fb;
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (sub == 0) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (!live[e]) continue;
+        const size_t r = ((size_t)slot * pl.nh + hw) * kRows + g + 8 * e;
+        float4* dst = reinterpret_cast<float4*>(pl.acc + r * D + (D / 4) * c);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int n = 0; n < ND; n += 4)
+            dst[(i * ND + n) / 4] = make_float4(o_acc[n][2 * e + i], o_acc[n + 1][2 * e + i], o_acc[n + 2][2 * e + i],
+                                                o_acc[n + 3][2 * e + i]);
+        if (c == 0) *reinterpret_cast<float2*>(pl.ml + r * 2) = make_float2(m[e], l[e]);
+      }
+    }
+    __syncwarp();  // the ring is refilled
+  }
+}
+
+// Joins the segments of one output row (token, query head): warps w, w + WPR, .. of the row take
+// its segments, then warp 0 the warps' sums.  o = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s.
+template <int D, int WPR>
+__global__ void __launch_bounds__(256) attn_chunk_merge_kernel(ChunkArgs a, SplitPlan pl) {
+  constexpr int E = D / 32;  // elements a lane
+  __shared__ float part[8][D + 2];
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long item = (long long)blockIdx.x * (8 / WPR) + warp / WPR;
+  const int sub = warp % WPR;
+  const int t = (int)(item / a.Hq), hq = (int)(item - (long long)t * a.Hq);
+  int b = -1;
+  if (t < a.T) b = find_request(a.cu_q, a.B, t);
+  bool mine = false;
+  float M = -INFINITY, L = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  if (b >= 0) {
+    const Req rq = request(a, b);
+    mine = rq.n * a.G <= pl.most_rows;
+    const int nc = (max(0, rq.hi - rq.lo) + pl.step_keys - 1) / pl.step_keys;
+    if (mine && nc > 0) {
+      const int h = hq / a.G, r = (t - a.cu_q[b]) * a.G + hq - h * a.G;
+      const int in_t = (r / kRows) * pl.hg + h / pl.nh, tile = pl.pre_t[b] + in_t;
+      const int U = pl.pre_u[a.B], first = pl.pre_u[b] + in_t * nc;
+      const int s0 = unit_owner(U, pl.ctas, first), s1 = unit_owner(U, pl.ctas, first + nc - 1) + 1;
+      const size_t in_slot = (size_t)(h % pl.nh) * kRows + r % kRows, per = (size_t)pl.nh * kRows;
+      for (int base = s0 + sub * 32; base < s1; base += 32 * WPR) {
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (base + lane < s1) ml = *reinterpret_cast<const float2*>(pl.ml + ((size_t)(base + lane + tile) * per + in_slot) * 2);
+        const float nm = fmaxf(M, warp_max(ml.x)), org = nm == -INFINITY ? 0.f : nm;
+        const float old = ex2(M - org), w = ex2(ml.x - org);
+        M = nm;
+        L = L * old + warp_sum(w * ml.y);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] *= old;
+        const int cnt = min(32, s1 - base);
+#pragma unroll 4
+        for (int i = 0; i < cnt; ++i) {
+          const float wi = __shfl_sync(0xffffffffu, w, i);
+          const float* src = pl.acc + ((size_t)(base + i + tile) * per + in_slot) * D + lane * E;
+          if (E == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(src);
+            o[0] += wi * v.x;
+            o[1] += wi * v.y;
+            o[E - 2] += wi * v.z;
+            o[E - 1] += wi * v.w;
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(src);
+            o[0] += wi * v.x;
+            o[1] += wi * v.y;
+          }
+        }
+      }
+    }
+  }
+  if (WPR > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) part[warp][lane * E + e] = o[e];
+    if (lane == 0) {
+      part[warp][D] = M;
+      part[warp][D + 1] = L;
+    }
+    __syncthreads();
+    if (sub != 0) return;
+    for (int w = 1; w < WPR; ++w) {
+      const float om = part[warp + w][D], ol = part[warp + w][D + 1];
+      const float nm = fmaxf(M, om), org = nm == -INFINITY ? 0.f : nm;
+      const float fa = ex2(M - org), fb = ex2(om - org);
+      M = nm;
+      L = L * fa + ol * fb;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = o[e] * fa + part[warp + w][lane * E + e] * fb;
+    }
+  }
+  if (!mine) return;
+  const float inv = L == 0.f ? 0.f : __fdividef(a.v_scale[hq / a.G], L);
+  __nv_bfloat16* dst = a.out + (size_t)t * a.ldo + (size_t)hq * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; e += 2)
+    *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(o[e] * inv, o[e + 1] * inv);
+}
+
+int heads_a_block(int Hkv) { return Hkv % 8 == 0 ? 8 : Hkv % 4 == 0 ? 4 : Hkv % 2 == 0 ? 2 : 1; }
+
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+
+size_t split_slots(int T, int B, int Hq, int Hkv) {
+  const size_t hg = Hkv / heads_a_block(Hkv);
+  return okc_host::num_sms() + (((size_t)T * (Hq / Hkv) + kRows - 1) / kRows + B) * hg;
+}
+
+template <int D, bool CAP>
+int launch_split(const ChunkArgs& a, SplitPlan& pl, cudaStream_t stream) {
+  using C = ChunkCfg<D>;
+  const int smem = C::SMEM + 2 * (a.B + 1) * 4;
+  static okc_host::PerDevice configured;
+  if (int st = configured.smem(attn_chunk_split_kernel<D, CAP>, C::SMEM + 2 * (kMaxChunkRequests + 1) * 4)) return st;
+  if (int st = okc_host::launch_k(attn_chunk_split_kernel<D, CAP>, dim3(pl.ctas), dim3(32 * kWarps), smem, stream,
+                                  dim3(1), a, pl))
+    return st;
+  const long long items = (long long)a.T * a.Hq;
+  // few rows: eight warps share a row's segments
+  if (items <= 1024)
+    return okc_host::launch_k(attn_chunk_merge_kernel<D, 8>, dim3((unsigned)items), dim3(256), 0, stream, dim3(1), a, pl);
+  return okc_host::launch_k(attn_chunk_merge_kernel<D, 1>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, stream,
+                            dim3(1), a, pl);
+}
+
+}  // namespace
+
+size_t attn_chunk_ws_bytes(int T, int B, int Hq, int Hkv, int D) {
+  const size_t rows = split_slots(T, B, Hq, Hkv) * heads_a_block(Hkv) * kRows;
+  return 2 * up((size_t)(B + 1) * 4) + up(rows * 8) + up(rows * D * 4);
+}
+
+int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
+  SplitPlan pl;
+  pl.nh = heads_a_block(a.Hkv);
+  pl.nsub = kWarps / pl.nh;
+  pl.hg = a.Hkv / pl.nh;
+  pl.step_keys = kStep * pl.nsub;
+  pl.ctas = okc_host::num_sms();
+  pl.most_rows = 0x7fffffff;
+  const size_t rows = split_slots(a.T, a.B, a.Hq, a.Hkv) * pl.nh * kRows;
+  uint8_t* p = reinterpret_cast<uint8_t*>(a.ws);
+  pl.pre_u = reinterpret_cast<int*>(p);
+  p += up((size_t)(a.B + 1) * 4);
+  pl.pre_t = reinterpret_cast<int*>(p);
+  p += up((size_t)(a.B + 1) * 4);
+  pl.ml = reinterpret_cast<float*>(p);
+  p += up(rows * 8);
+  pl.acc = reinterpret_cast<float*>(p);
+  if (a.D == 64) return a.softcap > 0.f ? launch_split<64, true>(a, pl, stream) : launch_split<64, false>(a, pl, stream);
+  return a.softcap > 0.f ? launch_split<128, true>(a, pl, stream) : launch_split<128, false>(a, pl, stream);
+}
+
+}  // namespace okc

@@ -214,6 +214,24 @@ inline int launch_status() {
 
 int num_sms();  // cached per device (defined in capi.cu)
 
+// Raises a kernel's dynamic shared-memory limit once per device (the attribute belongs to the
+// device that is current at the call).
+struct PerDevice {
+  bool done[64] = {};
+  template <typename K>
+  int smem(K kernel, int bytes) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return OKC_ERR_DEVICE;
+    if (done[dev]) return OKC_OK;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+      cudaGetLastError();
+      return OKC_ERR_LAUNCH;
+    }
+    done[dev] = true;
+    return OKC_OK;
+  }
+};
+
 // PDL on by default; OKC_PDL=0 launches every kernel with plain stream order.
 inline bool pdl_enabled() {
   static int v = -1;

@@ -84,6 +84,82 @@ int launch_rope_append(const void* qkv, int ldqkv, const int64_t* positions,
                        void* v_cache, int64_t* slots_out, int B, int Hq, int Hkv, int D, int P,
                        long long num_pages, float q_scale, int qk_norm, float norm_eps, int* err,
                        cudaStream_t stream);
+// Residual add + RMSNorm to e4m3 rows with scales (norm_fp8.cu).
+int launch_add_rmsnorm_fp8(const void* x, long long ldx, const void* res, long long ldr, int res_fp32, const void* w,
+                           void* res_out, long long ldo, void* q, long long ldq, float* scale, int T, int H, float eps,
+                           int unit_offset, cudaStream_t stream);
+// Multi-axis RoPE + FP8 KV-append of a ragged batch (rope_axes.cu).
+struct RopeAxesArgs {
+  const __nv_bfloat16* qkv;
+  long long ldqkv;
+  const int64_t* positions;  // [axes][ld_pos]
+  long long ld_pos;
+  unsigned long long axis_bits[4];  // two bits a pair: the axis that turns it
+  const float* inv_freq;     // [R]
+  int R, half;
+  const int32_t* cu_q;
+  const int32_t* seq_lens;
+  const int32_t* page_table;
+  long long table_ld;
+  int max_pages;
+  const float* k_scale;
+  const float* v_scale;
+  __nv_bfloat16* q_out;
+  long long ldq;
+  uint8_t* k_cache;
+  uint8_t* v_cache;
+  int T, B, Hq, Hkv, D, P;
+  long long num_pages;
+  int* err;
+};
+int launch_rope_axes_append(const RopeAxesArgs& a, cudaStream_t stream);
+// Ragged chunk attention over the paged cache (attention_chunk.cu).
+struct ChunkArgs {
+  const __nv_bfloat16* q;  // [T][ldq]
+  long long ldq;
+  const uint8_t* k_cache;
+  const uint8_t* v_cache;
+  const int32_t* page_table;
+  long long table_ld;
+  int max_keys;  // positions that a table row covers
+  const int32_t* cu_q;
+  const int32_t* seq_lens;
+  const float* k_scale;
+  const float* v_scale;
+  const float* slopes;         // [Hq] or null
+  const int32_t* prefix_lens;  // [B] or null
+  const int32_t* doc_start;    // [T] or null
+  __nv_bfloat16* out;          // [T][ldo]
+  long long ldo;
+  int T, B, Hq, Hkv, G, D, P, window;
+  long long num_pages;
+  float sm_scale, softcap;
+  int max_q;
+  void* ws;
+  int* err;
+};
+size_t attn_chunk_ws_bytes(int T, int B, int Hq, int Hkv, int D);
+int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream);
+// Projection with an epilogue (linear.cu, linear_split.cu).
+struct LinearArgs {
+  const void* x;   // [M][ldx] bf16 or e4m3
+  const void* w;   // [N][ldw]
+  long long ldx, ldw;
+  void* y;         // [M][ldy] bf16 or fp32
+  long long ldy;
+  const float* x_scale;  // [M] or null
+  const float* w_scale;  // [N], [1] or null
+  int w_scale_one;
+  const __nv_bfloat16* bias;  // [N] or null
+  const void* res;            // [M][ldr] or null
+  long long ldr;
+  int res_fp32, out_fp32, act;
+  int M, N, K;
+  int e4m3;
+  int* err;
+};
+int launch_linear(const LinearArgs& a, cudaStream_t stream);
+int launch_linear_split(const LinearArgs& a, cudaStream_t stream);
 int launch_moe_route(const void* x, const void* wr, int32_t* ids, float* wts, float* logits, int T,
                      int H, int E, int topk, int renormalize, cudaStream_t stream);
 int launch_moe_permute(const int32_t* ids, int n, int expert_lo, int E, int bm, int32_t* counts,

@@ -1,0 +1,96 @@
+// What the projection kernels with an epilogue share (linear.cu: tall token blocks, linear_split.cu:
+// few tokens): tensor maps over 8- and 16-bit rows, the instruction descriptors and the epilogue's
+// arithmetic.  A K step is 128 bytes of a row for either type (128 e4m3 or 64 bf16 values: one
+// swizzle atom), an MMA 32 bytes of it, so the kernels differ only in kind and descriptor.
+#pragma once
+
+#include "kernels.cuh"
+#include "tcgen05.cuh"
+
+namespace okc {
+
+constexpr int LIN_KB = 128;  // bytes of a row per K block
+
+// D fp32, both operands K-major, M x N; e4m3 (kind::f8f6f4, type code 0) or bf16 (kind::f16, type code 1).
+__host__ __device__ constexpr uint32_t lin_idesc(bool e4m3, int m, int n) {
+  return (1u << 4) | (e4m3 ? 0u : ((1u << 7) | (1u << 10))) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+template <bool E4M3>
+__device__ __forceinline__ void lin_mma(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if constexpr (E4M3)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+  else
+    umma_bf16(tmem_d, a, b, idesc, acc);
+}
+
+enum { LIN_ACT_NONE = 0, LIN_ACT_RELU = 1, LIN_ACT_SILU = 2, LIN_ACT_GELU = 3, LIN_ACT_GELU_TANH = 4 };
+
+// Activations in fp32.  tanh and the logistic function go through one exponential:
+// 0.5 (1 + tanh(u)) = 1 / (1 + exp(-2u)).  A NaN stays a NaN (relu included: fmaxf would drop it).
+__device__ __forceinline__ float lin_act(float v, int act) {
+  switch (act) {
+    case LIN_ACT_RELU: return v < 0.f ? 0.f : v;
+    case LIN_ACT_SILU: return __fdividef(v, 1.f + __expf(-v));
+    case LIN_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.7071067811865476f));
+    case LIN_ACT_GELU_TANH:
+      return __fdividef(v, 1.f + __expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
+    default: return v;
+  }
+}
+
+// One output: the fp32 sum times its row and channel scales, plus the bias, through the activation,
+// plus the residual; rounded once if the output is bf16.
+__device__ __forceinline__ void lin_store(const LinearArgs& a, int m, int n, float v, float sx, float sw, float bias) {
+  v = lin_act(fmaf(v * sx, sw, bias), a.act);
+  if (a.res) {
+    const size_t i = (size_t)m * a.ldr + n;
+    v += a.res_fp32 ? reinterpret_cast<const float*>(a.res)[i]
+                    : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.res)[i]);
+  }
+  const size_t o = (size_t)m * a.ldy + n;
+  if (a.out_fp32)
+    reinterpret_cast<float*>(a.y)[o] = v;
+  else
+    reinterpret_cast<__nv_bfloat16*>(a.y)[o] = __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ float lin_row_scale(const LinearArgs& a, int m) { return a.x_scale ? a.x_scale[m] : 1.f; }
+__device__ __forceinline__ float lin_col_scale(const LinearArgs& a, int n) {
+  return a.w_scale ? a.w_scale[a.w_scale_one ? 0 : n] : 1.f;
+}
+
+// 32 consecutive TMEM columns of this warp's 32 lanes.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Host: a 2-D map over [rows][inner] of 8- or 16-bit elements, boxes of LIN_KB bytes x box_rows rows.
+inline bool lin_make_map(CUtensorMap* m, const void* base, int inner, int rows, long long ld, int box_rows, bool e4m3) {
+  auto fn = tensor_map_encoder();
+  if (!fn) return false;
+  const int es = e4m3 ? 1 : 2;
+  cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * es};
+  cuuint32_t box[2] = {(cuuint32_t)(LIN_KB / es), (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(m, e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base),
+            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace okc

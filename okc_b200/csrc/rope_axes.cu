@@ -1,0 +1,140 @@
+// Rotary positions with several axes (time, height, width) and the FP8 KV-append of a ragged
+// batch.  Token t of request b (cu_q[b] <= t < cu_q[b+1]) sits at the cache position
+// seq_lens[b] - (cu_q[b+1] - t), which its rotary positions need not equal; pair i turns by
+//   angle = positions[axis(i)][t] * inv_freq[i],   i < R,
+// with pair i = (2i, 2i+1), or (i, i + R) in the half-split form; elements from 2R on pass through.
+//
+// The angle is a product and a reduction to [-pi, pi] in 64 bits: in 32 bits the product alone is
+// off by half a unit of its last place, 0.03 rad at position 10^6.  One angle serves every head of
+// the token, so this costs R 64-bit reductions a token against (Hq + Hkv) D / 2 rotations.
+// Rotations are fp32; q is rounded once to bf16 and k, v once to e4m3 (RNE, overflow -> NaN).
+//
+// HBM-bound: 2 (Hq + 2 Hkv) D bytes in, 2 Hq D + 2 Hkv D bytes out per token.  A block takes one token;
+// each thread moves 16-byte vectors.
+#include "chunk_common.cuh"
+
+namespace okc {
+
+namespace {
+
+constexpr int kRopeThreads = 256;
+constexpr int kMaxPairs = 128;
+
+__device__ __forceinline__ uint32_t e4m3x4_nosat(float a, float b, float c, float d) {
+  return (uint32_t)f_to_e4m3_nosat(a) | ((uint32_t)f_to_e4m3_nosat(b) << 8) | ((uint32_t)f_to_e4m3_nosat(c) << 16) |
+         ((uint32_t)f_to_e4m3_nosat(d) << 24);
+}
+
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    f[2 * k] = bf16_lo(w[k]);
+    f[2 * k + 1] = bf16_hi(w[k]);
+  }
+}
+
+__device__ __forceinline__ void store8_bf16(__nv_bfloat16* p, const float (&f)[8]) {
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+}
+
+__device__ __forceinline__ void store8_e4m3(uint8_t* p, const float (&f)[8], float scale) {
+  float e[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) e[k] = __fdiv_rn(f[k], scale);
+  *reinterpret_cast<uint2*>(p) = make_uint2(e4m3x4_nosat(e[0], e[1], e[2], e[3]), e4m3x4_nosat(e[4], e[5], e[6], e[7]));
+}
+
+__global__ void __launch_bounds__(kRopeThreads) rope_axes_append_kernel(RopeAxesArgs a) {
+  __shared__ float cs[kMaxPairs], sn[kMaxPairs];
+  __shared__ int req;
+  pdl_trigger();
+  pdl_wait();
+  const int t = blockIdx.x;
+  if (threadIdx.x < 32) {
+    const int b = find_request(a.cu_q, a.B, t);
+    if (threadIdx.x == 0) req = b;
+  }
+  for (int i = threadIdx.x; i < a.R; i += kRopeThreads) {
+    const int axis = (int)((a.axis_bits[i >> 5] >> (2 * (i & 31))) & 3u);
+    const double ang = (double)a.positions[(size_t)axis * a.ld_pos + t] * (double)a.inv_freq[i];
+    const double turns = rint(ang * 0.15915494309189535);                 // 1 / (2 pi)
+    const float r = (float)fma(turns, -6.283185307179586, ang);           // 2 pi; in [-pi, pi]
+    sincosf(r, &sn[i], &cs[i]);
+  }
+  __syncthreads();
+  const int b = req;
+  if (b < 0) return;  // a row behind the last request
+  const long long pos = (long long)a.seq_lens[b] - a.cu_q[b + 1] + t;
+  long long slot = -1;
+  if (pos >= 0 && pos / a.P < a.max_pages) {
+    const int page = a.page_table[(size_t)b * a.table_ld + pos / a.P];
+    if (page >= 0 && page < a.num_pages) slot = (long long)page * a.P + pos % a.P;
+  }
+  if (slot < 0 && threadIdx.x == 0) atomicOr(a.err, OKC_DEVERR_PAGE);
+
+  const __nv_bfloat16* row = a.qkv + (size_t)t * a.ldqkv;
+  __nv_bfloat16* qo = a.q_out + (size_t)t * a.ldq;
+  const size_t kv_row = slot < 0 ? 0 : (size_t)slot * a.Hkv * a.D;
+  const int D = a.D, R = a.R;
+  // items: 8 pairs of a q or k head, then 8 passed elements of a q or k head, then 8 of a v head
+  const int rp = R / 8, pp = (D - 2 * R) / 8, vp = D / 8, hqk = a.Hq + a.Hkv;
+  const int n_rot = hqk * rp, n_pass = hqk * pp, n_all = n_rot + n_pass + a.Hkv * vp;
+  for (int it = threadIdx.x; it < n_all; it += kRopeThreads) {
+    if (it < n_rot) {
+      const int head = it / rp, i0 = (it - head * rp) * 8;
+      const int u0 = a.half ? i0 : 2 * i0, u1 = a.half ? i0 + R : 2 * i0 + 8;
+      float x[8], y[8], p[8], q[8];
+      unpack8(*reinterpret_cast<const uint4*>(row + (size_t)head * D + u0), x);
+      unpack8(*reinterpret_cast<const uint4*>(row + (size_t)head * D + u1), y);
+      if (a.half) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float c = cs[i0 + k], s = sn[i0 + k];
+          p[k] = x[k] * c - y[k] * s;
+          q[k] = x[k] * s + y[k] * c;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float c0 = cs[i0 + k], s0 = sn[i0 + k], c1 = cs[i0 + 4 + k], s1 = sn[i0 + 4 + k];
+          p[2 * k] = x[2 * k] * c0 - x[2 * k + 1] * s0;
+          p[2 * k + 1] = x[2 * k] * s0 + x[2 * k + 1] * c0;
+          q[2 * k] = y[2 * k] * c1 - y[2 * k + 1] * s1;
+          q[2 * k + 1] = y[2 * k] * s1 + y[2 * k + 1] * c1;
+        }
+      }
+      if (head < a.Hq) {
+        store8_bf16(qo + (size_t)head * D + u0, p);
+        store8_bf16(qo + (size_t)head * D + u1, q);
+      } else if (slot >= 0) {
+        uint8_t* dst = a.k_cache + kv_row + (size_t)(head - a.Hq) * D;
+        store8_e4m3(dst + u0, p, a.k_scale[head - a.Hq]);
+        store8_e4m3(dst + u1, q, a.k_scale[head - a.Hq]);
+      }
+    } else {
+      const int j = it - n_rot;
+      const bool is_v = j >= n_pass;
+      const int per = is_v ? vp : pp, k = is_v ? j - n_pass : j;
+      const int h = k / per, d = (k - h * per) * 8 + (is_v ? 0 : 2 * R);
+      const int head = is_v ? hqk + h : h;
+      float x[8];
+      unpack8(*reinterpret_cast<const uint4*>(row + (size_t)head * D + d), x);
+      if (head < a.Hq) {
+        store8_bf16(qo + (size_t)head * D + d, x);
+      } else if (slot >= 0) {
+        const int kh = is_v ? h : h - a.Hq;
+        store8_e4m3((is_v ? a.v_cache : a.k_cache) + kv_row + (size_t)kh * D + d, x, is_v ? a.v_scale[kh] : a.k_scale[kh]);
+      }
+    }
+  }
+}
+
+}  // namespace
+
+int launch_rope_axes_append(const RopeAxesArgs& a, cudaStream_t stream) {
+  return okc_host::launch_k(rope_axes_append_kernel, dim3(a.T), dim3(kRopeThreads), 0, stream, dim3(1), a);
+}
+
+}  // namespace okc

@@ -367,6 +367,252 @@ def attn_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     return out
 
 
+# --------------------------------------------------- 8-bit projections, ragged batches
+# These operators keep nothing between calls: outputs and scratch come from torch's caching
+# allocator (ordered with the stream; a captured call's belong to its graph), so calls on two
+# streams and graphs replayed side by side do not meet.  Only the word that device errors are OR'd into
+# is kept per device (read_device_error(tag, device)).
+def _error_word(dev: int, tag: str) -> int:
+    buf = _WS.get((dev, tag))
+    if buf is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise _lib.OkcError(f"{tag}: the first call on a device allocates its error word; make it before a capture")
+        buf = workspace(dev, tag, 256)
+        torch.cuda.current_stream(dev).synchronize()  # zeroed before a call on any stream
+    return buf.data_ptr()
+
+
+def _call(dev: int, name: str, *args) -> None:
+    """Calls the C entry point on the current stream of `dev`, with `dev` current."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == dev:
+        st = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, _stream(dev))
+    if st != _lib.OKC_OK:
+        check(st, name)
+
+
+def _tensor(t: torch.Tensor, name: str, dtype, shape: tuple, dev: int, rows: bool = False) -> None:
+    """Checks dtype, device, shape (None = any) and strides: contiguous, or with `rows` only inside
+    each row (the first dimension's stride is free)."""
+    if t.dtype != dtype and not (isinstance(dtype, tuple) and t.dtype in dtype):
+        raise _lib.OkcError(f"{name}: expected {dtype}, got {t.dtype}")
+    if not t.is_cuda or t.device.index != dev:
+        raise _lib.OkcError(f"{name}: expected a tensor on cuda:{dev}, got {t.device}")
+    ts = t.shape
+    if len(ts) != len(shape):
+        raise _lib.OkcError(f"{name}: expected shape {shape}, got {tuple(ts)}")
+    for have, want in zip(ts, shape):
+        if want is not None and have != want:
+            raise _lib.OkcError(f"{name}: expected shape {shape}, got {tuple(ts)}")
+    if t.is_contiguous():
+        return
+    if rows:
+        want = 1
+        for d in range(len(ts) - 1, 0, -1):
+            if ts[d] != 1 and t.stride(d) != want:
+                break
+            want *= ts[d]
+        else:
+            if ts[0] <= 1 or t.stride(0) >= want:
+                return
+    raise _lib.OkcError(f"{name}: unsupported strides {t.stride()} for shape {tuple(ts)}")
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row stride in elements; a single row has the length of one."""
+    return t.stride(0) if t.shape[0] > 1 else math.prod(t.shape[1:])
+
+
+_E4M3 = torch.float8_e4m3fn
+_STREAM_TYPES = (torch.bfloat16, torch.float32)
+
+
+def add_rmsnorm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float, residual: torch.Tensor | None = None,
+                    unit_offset: bool = False, residual_out: torch.Tensor | None = None):
+    """Residual add + RMSNorm with an e4m3 output (okc_add_rmsnorm_fp8): s = x + residual rounded to
+    the residual's type, y = s * rsqrt(mean(s^2) + eps) * (w or 1 + w), scale = max|y| / 448 per row
+    (1 for a row of zeros), q = e4m3(y / scale).  x bf16 [T, H] and w bf16 [H]; residual bf16 or
+    fp32 [T, H]; H a multiple of 16 up to 16384.  Returns (q e4m3 [T, H], scale fp32 [T], s or
+    None); s goes to `residual_out`, which may be `residual`."""
+    dev = _dev_index(x)
+    if x.dim() != 2:
+        raise _lib.OkcError(f"x: expected [T, H], got {tuple(x.shape)}")
+    T, H = x.shape
+    _tensor(x, "x", torch.bfloat16, (T, H), dev, rows=True)
+    _tensor(w, "w", torch.bfloat16, (H,), dev)
+    q = torch.empty((T, H), dtype=_E4M3, device=x.device)
+    scale = torch.empty(T, dtype=torch.float32, device=x.device)
+    rp, rld, op, old, r32 = None, 0, None, 0, 0
+    if residual is not None:
+        _tensor(residual, "residual", _STREAM_TYPES, (T, H), dev, rows=True)
+        if residual_out is None:
+            residual_out = torch.empty((T, H), dtype=residual.dtype, device=x.device)
+        else:
+            _tensor(residual_out, "residual_out", residual.dtype, (T, H), dev, rows=True)
+        rp, rld, op, old = residual.data_ptr(), _ld(residual), residual_out.data_ptr(), _ld(residual_out)
+        r32 = int(residual.dtype == torch.float32)
+    elif residual_out is not None:
+        raise _lib.OkcError("residual_out without residual")
+    if T:
+        _call(dev, "okc_add_rmsnorm_fp8", x.data_ptr(), _ld(x), rp, rld, r32, w.data_ptr(), op, old, q.data_ptr(), H,
+              scale.data_ptr(), T, H, float(eps), int(unit_offset))
+    return q, scale, residual_out
+
+
+LINEAR_ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor | None = None, w_scale: torch.Tensor | None = None,
+           bias: torch.Tensor | None = None, act: str | None = None, residual: torch.Tensor | None = None,
+           out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """y = act(x w^T * x_scale[:, None] * w_scale + bias) + residual (okc_linear), fp32 accumulation and
+    epilogue, one rounding.  x [M, K] and w [N, K] both e4m3 or both bf16; x_scale fp32 [M]; w_scale fp32
+    [N] or [1]; bias bf16 [N]; act None, "relu", "silu", "gelu" or "gelu_tanh"; residual bf16 or
+    fp32 [M, N]; y bf16 or fp32 [M, N] (`out`, which may be `residual`, or a new tensor of `out_dtype`).
+    K is a multiple of 16 (e4m3) or 8 (bf16), x and w rows 16-byte aligned."""
+    dev = _dev_index(x)
+    if x.dim() != 2 or w.dim() != 2:
+        raise _lib.OkcError(f"x and w: expected [M, K] and [N, K], got {tuple(x.shape)} and {tuple(w.shape)}")
+    if act not in LINEAR_ACTS:
+        raise _lib.OkcError(f"act: expected one of {sorted(k for k in LINEAR_ACTS if k)}, got {act!r}")
+    (M, K), N = x.shape, w.shape[0]
+    _tensor(x, "x", (_E4M3, torch.bfloat16), (M, K), dev, rows=True)
+    _tensor(w, "w", x.dtype, (N, K), dev, rows=True)
+    if out is None:
+        if out_dtype not in _STREAM_TYPES:
+            raise _lib.OkcError(f"out_dtype: expected bfloat16 or float32, got {out_dtype}")
+        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    else:
+        _tensor(out, "out", _STREAM_TYPES, (M, N), dev, rows=True)
+    sx = sw = bp = rp = None
+    one = rld = r32 = 0
+    if x_scale is not None:
+        _tensor(x_scale, "x_scale", torch.float32, (M,), dev)
+        sx = x_scale.data_ptr()
+    if w_scale is not None:
+        one = int(w_scale.numel() == 1)
+        _tensor(w_scale, "w_scale", torch.float32, (1,) if one else (N,), dev)
+        sw = w_scale.data_ptr()
+    if bias is not None:
+        _tensor(bias, "bias", torch.bfloat16, (N,), dev)
+        bp = bias.data_ptr()
+    if residual is not None:
+        _tensor(residual, "residual", _STREAM_TYPES, (M, N), dev, rows=True)
+        rp, rld, r32 = residual.data_ptr(), _ld(residual), int(residual.dtype == torch.float32)
+    if not M:
+        return out
+    e4m3 = int(x.dtype == _E4M3)
+    _call(dev, "okc_linear", x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), e4m3, sx, sw, one, bp, LINEAR_ACTS[act], rp,
+          rld, r32, out.data_ptr(), _ld(out), int(out.dtype == torch.float32), M, N, K, None, 0,
+          _error_word(dev, "linear"))
+    return out
+
+
+def rope_sections(sizes) -> tuple[int, ...]:
+    """The axis of each pair when the pairs are dealt in sections: sizes[0] pairs to axis 0, and so on."""
+    return tuple(a for a, n in enumerate(sizes) for _ in range(n))
+
+
+def _ragged(cu_q, seq_lens, page_table, dev: int) -> int:
+    B = seq_lens.shape[0]
+    _tensor(seq_lens, "seq_lens", torch.int32, (B,), dev)
+    _tensor(cu_q, "cu_q", torch.int32, (B + 1,), dev)
+    _tensor(page_table, "page_table", torch.int32, (B, None), dev, rows=True)
+    return B
+
+
+def _caches(k_cache, v_cache, k_scale, v_scale, Hkv, D: int, dev: int):
+    _tensor(k_cache, "k_cache", _E4M3, (None, None, Hkv, D), dev)
+    pages, P, Hkv, _ = k_cache.shape
+    _tensor(v_cache, "v_cache", _E4M3, (pages, P, Hkv, D), dev)
+    _tensor(k_scale, "k_scale", torch.float32, (Hkv,), dev)
+    _tensor(v_scale, "v_scale", torch.float32, (Hkv,), dev)
+    return pages, P, Hkv
+
+
+def rope_axes_kv_append(qkv: torch.Tensor, positions: torch.Tensor, axes, inv_freq: torch.Tensor,
+                        cu_q: torch.Tensor, seq_lens: torch.Tensor, page_table: torch.Tensor, k_cache: torch.Tensor,
+                        v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, Hq: int, Hkv: int,
+                        D: int, half: bool = False, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions with several axes (time, height, width) and the e4m3 KV-append of a ragged
+    batch (okc_rope_axes_kv_append).  qkv bf16 [T, (Hq + 2 Hkv) * D]; request b owns the rows cu_q[b] ..
+    cu_q[b + 1] - 1 (int32 [B + 1]) and ends, with them, at seq_lens[b] cached positions (int32 [B]).
+    positions int64 [A, T] holds each row's position on A <= 4 axes; `axes` the axis that turns each
+    pair (see rope_sections; its length, a multiple of 8, is the number of pairs), inv_freq fp32 [len(axes)].
+    A pair is (2i, 2i + 1), or with `half` (i, i + len(axes)); the head's other elements pass.  Returns
+    q bf16 [T, Hq, D]; rows behind cu_q[B] are left as they are."""
+    dev = _dev_index(qkv)
+    if qkv.dim() != 2 or positions.dim() != 2:
+        raise _lib.OkcError(f"qkv and positions: expected [T, C] and [A, T], got {tuple(qkv.shape)}, {tuple(positions.shape)}")
+    T = qkv.shape[0]
+    _tensor(qkv, "qkv", torch.bfloat16, (T, (Hq + 2 * Hkv) * D), dev, rows=True)
+    _tensor(positions, "positions", torch.int64, (None, T), dev, rows=True)
+    axes = bytes(axes)
+    _tensor(inv_freq, "inv_freq", torch.float32, (len(axes),), dev)
+    B = _ragged(cu_q, seq_lens, page_table, dev)
+    pages, P, _ = _caches(k_cache, v_cache, k_scale, v_scale, Hkv, D, dev)
+    if q_out is None:
+        q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=qkv.device)
+    else:
+        _tensor(q_out, "q_out", torch.bfloat16, (T, Hq, D), dev, rows=True)
+    if T:
+        _call(dev, "okc_rope_axes_kv_append", qkv.data_ptr(), _ld(qkv), positions.data_ptr(), _ld(positions),
+              positions.shape[0], axes, inv_freq.data_ptr(), len(axes), int(half), cu_q.data_ptr(),
+              seq_lens.data_ptr(), B, page_table.data_ptr(), _ld(page_table), page_table.shape[1],
+              k_scale.data_ptr(), v_scale.data_ptr(), q_out.data_ptr(), _ld(q_out), k_cache.data_ptr(),
+              v_cache.data_ptr(), T, Hq, Hkv, D, P, pages, _error_word(dev, "rope_axes"))
+    return q_out
+
+
+def attn_chunk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+               cu_q: torch.Tensor, seq_lens: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+               sm_scale: float, softcap: float = 0.0, slopes: torch.Tensor | None = None, window: int = 0,
+               prefix_lens: torch.Tensor | None = None, doc_start: torch.Tensor | None = None,
+               max_q: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of ragged chunks of new tokens (their keys appended) over the paged e4m3 cache
+    (okc_attn_chunk_fp8).  q bf16 [T, Hq, D]; the ragged batch as in rope_axes_kv_append.  A token at
+    position p sees the positions [max(0, doc_start, p + 1 - window), max(p + 1, prefix_len)) of its
+    request: doc_start int32 [T] the first position of its packed document, prefix_lens int32 [B] a prefix
+    that every token sees, window 0 = none.  Scores are capped as softcap * tanh(s / softcap)
+    (0 = uncapped), then lowered by slopes[h] * |p - j| (fp32 [Hq]).  max_q, the longest chunk if the
+    caller knows it, only chooses kernels.  Returns bf16 [T, Hq, D]: zero for a row that sees nothing, rows
+    behind cu_q[B] as they were."""
+    dev = _dev_index(q)
+    if q.dim() != 3:
+        raise _lib.OkcError(f"q: expected [T, Hq, D], got {tuple(q.shape)}")
+    T, Hq, D = q.shape
+    _tensor(q, "q", torch.bfloat16, (T, Hq, D), dev, rows=True)
+    B = _ragged(cu_q, seq_lens, page_table, dev)
+    pages, P, Hkv = _caches(k_cache, v_cache, k_scale, v_scale, None, D, dev)
+    sp = pp = dp = None
+    if slopes is not None:
+        _tensor(slopes, "slopes", torch.float32, (Hq,), dev)
+        sp = slopes.data_ptr()
+    if prefix_lens is not None:
+        _tensor(prefix_lens, "prefix_lens", torch.int32, (B,), dev)
+        pp = prefix_lens.data_ptr()
+    if doc_start is not None:
+        _tensor(doc_start, "doc_start", torch.int32, (T,), dev)
+        dp = doc_start.data_ptr()
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=q.device)
+    else:
+        _tensor(out, "out", torch.bfloat16, (T, Hq, D), dev, rows=True)
+    if not T:
+        return out
+    error = _error_word(dev, "attn_chunk")
+    nbytes = _lib.load().okc_attn_chunk_workspace_bytes(T, B, Hq, Hkv, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _call(dev, "okc_attn_chunk_fp8", q.data_ptr(), _ld(q), k_cache.data_ptr(), v_cache.data_ptr(),
+          page_table.data_ptr(), _ld(page_table), page_table.shape[1], cu_q.data_ptr(), seq_lens.data_ptr(),
+          k_scale.data_ptr(), v_scale.data_ptr(), sp, pp, dp, out.data_ptr(), _ld(out), T, B, Hq, Hkv, D, P, pages,
+          float(sm_scale), float(softcap), int(window), int(max_q or 0), ws.data_ptr(), nbytes, error)
+    return out
+
+
 def attn_workspace_bytes(B: int, Hq: int, Hkv: int, D: int, num_ctas: int = 0) -> int:
     return int(_lib.load().okc_attn_decode_workspace_bytes(B, Hq, Hkv, D, num_ctas))
 
