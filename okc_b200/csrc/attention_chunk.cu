@@ -31,27 +31,6 @@ constexpr int kStep = 32;      // keys per warp step
 constexpr int kWarps = 8;
 constexpr int kRows = 16;
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// tanh(x) from exp(2x) given x * 2 log2(e): 1 - 2 / (1 + e^2x); off by a few 2^-24 absolute, which a cap of
-// 50 turns into 10^-5 of a score.
-__device__ __forceinline__ float tanh_from_2l2e(float x) { return 1.f - __fdividef(2.f, 1.f + ex2(x)); }
-
-__device__ __forceinline__ uint32_t e4m3x2_h2(uint32_t two) {
-  uint32_t h;
-  asm("{\n .reg .b16 t;\n cvt.u16.u32 t, %1;\n cvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(h) : "r"(two));
-  return h;
-}
-
-__device__ __forceinline__ uint32_t h2(float x, float y) {
-  const __half2 h = __floats2half2_rn(x, y);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
@@ -72,22 +51,9 @@ struct SplitPlan {
   int* pre_t;         // [B + 1] row tiles (times head groups) before a request
   float* ml;          // [slot][nh][16][2]
   float* acc;         // [slot][nh][16][D]
-  int most_rows;      // requests of more rows are served by the other kernel
+  int most_rows;      // requests of more rows are served by the tensor-memory kernel
+  int merge_tokens;   // > 0: requests have at most this many tokens here; 0: rows are looked up
 };
-
-struct Req {
-  int n, len, lo, hi, prefix;  // new tokens, cached tokens, union of the rows' key intervals
-};
-
-__device__ __forceinline__ Req request(const ChunkArgs& a, int b) {
-  Req r;
-  r.n = max(0, a.cu_q[b + 1] - a.cu_q[b]);
-  r.len = max(0, a.seq_lens[b]);
-  r.prefix = a.prefix_lens ? a.prefix_lens[b] : 0;
-  r.lo = a.window > 0 ? max(0, r.len - r.n + 1 - a.window) : 0;
-  r.hi = min(r.len, a.max_keys);  // positions past the table's columns do not exist
-  return r;
-}
 
 __device__ __forceinline__ void unit_split(int U, int C, int c, int& u0, int& u1) {
   const int q = U / C, r = U % C;
@@ -180,7 +146,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
 
     // ---- the lane's two rows ----
     const int rows = rq.n * a.G, r0 = rt * kRows;
-    const int row0 = a.cu_q[b], p_base = rq.len - rq.n;
+    const int row0 = a.cu_q[b];
     int lo[2], hi[2], pos[2];
     bool live[2];
     float slope[2], fac[2];
@@ -191,23 +157,23 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
       const int r = r0 + g + 8 * e;
       live[e] = r < rows;
       const int i = live[e] ? r / a.G : 0, hq = head * a.G + (live[e] ? r - i * a.G : 0);
-      pos[e] = p_base + i;
+      pos[e] = 0;
       lo[e] = hi[e] = 0;
       slope[e] = 0.f;
       uint2 qv[KS];
 #pragma unroll
       for (int k = 0; k < KS; ++k) qv[k] = make_uint2(0u, 0u);
       if (live[e]) {
-        hi[e] = min(rq.hi, max(pos[e] + 1, rq.prefix));
-        if (a.window > 0) lo[e] = max(0, pos[e] + 1 - a.window);
-        if (a.doc_start) lo[e] = max(lo[e], a.doc_start[row0 + i]);
+        const RowSpan sp = row_span(a, rq, row0, i);
+        pos[e] = sp.pos;
+        lo[e] = sp.lo;
+        hi[e] = sp.hi;
         if (a.slopes) slope[e] = a.slopes[hq] * 1.4426950408889634f;
         const __nv_bfloat16* qp = a.q + (size_t)(row0 + i) * a.ldq + (size_t)hq * D;
 #pragma unroll
         for (int k = 0; k < KS; ++k)  // the four elements of step k's slots
           qv[k] = *reinterpret_cast<const uint2*>(qp + 64 * (k >> 2) + 16 * c + 4 * (k & 3));
       }
-      // scale the row by 2^-s so that its largest magnitude lies in [2^13, 2^14): exact in f16 down to 2^-27 of it
       uint32_t top = 0;
 #pragma unroll
       for (int k = 0; k < KS; ++k)
@@ -215,8 +181,8 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
                   max(qv[k].y & 0x7fffu, (qv[k].y >> 16) & 0x7fffu));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int sh = max(-100, (int)(top >> 7) - 127 - 13);
-      const float down = __uint_as_float((uint32_t)(127 - sh) << 23);
+      const int sh = f16_shift(top);
+      const float down = pow2(-sh);
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         qf[k][e] = h2(bf16_lo(qv[k].x) * down, bf16_hi(qv[k].x) * down);
@@ -224,7 +190,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
       }
       // without a cap: log2 units; with one: the argument of tanh times 2 log2(e)
       fac[e] = a.k_scale[head] * a.sm_scale * (CAP ? 2.f / a.softcap : 1.f) * 1.4426950408889634f *
-               __uint_as_float((uint32_t)(127 + sh) << 23);
+               pow2(sh);
     }
     const float cap2 = CAP ? a.softcap * 1.4426950408889634f : 0.f;
     // keys that every live row sees need no mask; keys outside [t_lo, t_hi) are not read
@@ -333,8 +299,9 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
         for (int n = 0; n < 4; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float v = sc[n][2 * e + i] * fac[e];
-            if (CAP) v = cap2 * tanh_from_2l2e(v);
+            // rounded here: fused into the subtraction below, a large score could exceed the maximum
+            float v = __fmul_rn(sc[n][2 * e + i], fac[e]);
+            if (CAP) v = __fmul_rn(cap2, tanh_from_2l2e(v));
             x[2 * n + i] = v;
           }
         if (a.slopes) {
@@ -527,9 +494,16 @@ __global__ void __launch_bounds__(256) attn_chunk_merge_kernel(ChunkArgs a, Spli
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long item = (long long)blockIdx.x * (8 / WPR) + warp / WPR;
   const int sub = warp % WPR;
-  const int t = (int)(item / a.Hq), hq = (int)(item - (long long)t * a.Hq);
-  int b = -1;
-  if (t < a.T) b = find_request(a.cu_q, a.B, t);
+  int t = (int)(item / a.Hq), b = -1;
+  const int hq = (int)(item - (long long)t * a.Hq);
+  if (pl.merge_tokens > 0) {  // the first merge_tokens tokens of every request
+    b = t / pl.merge_tokens;
+    const int i = t - b * pl.merge_tokens;
+    if (b >= a.B || i >= a.cu_q[b + 1] - a.cu_q[b]) b = -1;
+    else t = a.cu_q[b] + i;
+  } else if (t < a.T) {
+    b = find_request(a.cu_q, a.B, t);
+  }
   bool mine = false;
   float M = -INFINITY, L = 0.f, o[E];
 #pragma unroll
@@ -618,7 +592,7 @@ int launch_split(const ChunkArgs& a, SplitPlan& pl, cudaStream_t stream) {
   if (int st = okc_host::launch_k(attn_chunk_split_kernel<D, CAP>, dim3(pl.ctas), dim3(32 * kWarps), smem, stream,
                                   dim3(1), a, pl))
     return st;
-  const long long items = (long long)a.T * a.Hq;
+  const long long items = (long long)(pl.merge_tokens > 0 ? (long long)a.B * pl.merge_tokens : a.T) * a.Hq;
   // few rows: eight warps share a row's segments
   if (items <= 1024)
     return okc_host::launch_k(attn_chunk_merge_kernel<D, 8>, dim3((unsigned)items), dim3(256), 0, stream, dim3(1), a, pl);
@@ -630,7 +604,7 @@ int launch_split(const ChunkArgs& a, SplitPlan& pl, cudaStream_t stream) {
 
 size_t attn_chunk_ws_bytes(int T, int B, int Hq, int Hkv, int D) {
   const size_t rows = split_slots(T, B, Hq, Hkv) * heads_a_block(Hkv) * kRows;
-  return 2 * up((size_t)(B + 1) * 4) + up(rows * 8) + up(rows * D * 4);
+  return 2 * up((size_t)(B + 1) * 4) + up(rows * 8) + up(rows * D * 4) + attn_chunk_tc_ws_bytes(T, B, Hq, Hkv, D);
 }
 
 int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
@@ -640,7 +614,10 @@ int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
   pl.hg = a.Hkv / pl.nh;
   pl.step_keys = kStep * pl.nsub;
   pl.ctas = okc_host::num_sms();
-  pl.most_rows = 0x7fffffff;
+  // every request short: this kernel alone; else each kernel serves its requests
+  const bool split_only = a.max_q > 0 ? (long long)a.max_q * a.G <= kSplitRows : (long long)a.T * a.G <= kSplitRows;
+  pl.most_rows = split_only ? 0x7fffffff : kSplitRows;
+  pl.merge_tokens = split_only ? 0 : kSplitRows / a.G;
   const size_t rows = split_slots(a.T, a.B, a.Hq, a.Hkv) * pl.nh * kRows;
   uint8_t* p = reinterpret_cast<uint8_t*>(a.ws);
   pl.pre_u = reinterpret_cast<int*>(p);
@@ -650,6 +627,11 @@ int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
   pl.ml = reinterpret_cast<float*>(p);
   p += up(rows * 8);
   pl.acc = reinterpret_cast<float*>(p);
+  p += up(rows * a.D * 4);
+  if (!split_only) {
+    if (int st = launch_attn_chunk_tc(a, p, stream)) return st;
+    if (pl.merge_tokens == 0) return OKC_OK;  // no request is short enough
+  }
   if (a.D == 64) return a.softcap > 0.f ? launch_split<64, true>(a, pl, stream) : launch_split<64, false>(a, pl, stream);
   return a.softcap > 0.f ? launch_split<128, true>(a, pl, stream) : launch_split<128, false>(a, pl, stream);
 }

@@ -1,0 +1,675 @@
+// Attention of ragged chunks over the paged e4m3 cache for chunks of many rows: both products on the
+// tensor cores with scores, probabilities and outputs in tensor memory.  The masks and the scores
+// are those of attention_chunk.cu, which serves the short chunks.
+//
+// Compute-bound: 4 D operations per (row, visible key) against 2 D cache bytes per key and 256 rows.
+// A block takes 256 rows (token-major, the G query heads of one KV head side by side) as two tiles
+// of 128 and streams the keys that any of them sees in blocks of 128:
+//  * two softmax warpgroups, one thread a row: S is read from tensor memory twice (the maximum, then the
+//    exponentials), P goes back over S as f16 and is the next product's A operand there.  A row's sums
+//    never leave its thread;
+//  * four warps fetch key and value rows by page, turn e4m3 into f16 (exact) and store both as the
+//    swizzled rows that the MMAs read (keys K-major, values MN-major: no transpose);
+//  * one thread issues the MMAs: while one tile's softmax runs, the other tile's products do;
+//  * O is rescaled only when a row's maximum has grown by more than 2^8 since the last time, so P
+//    stays below 2^8 and a rescale is rare after the first blocks.
+// Blocks of a request are taken from its last rows on: the longest causal spans start first.  With few
+// blocks the keys are split over several, which leave fp32 partial sums for a merge.
+#include "chunk_common.cuh"
+#include "tcgen05.cuh"
+
+namespace okc {
+
+namespace {
+
+constexpr int kTile = 128;                 // rows of a tile, keys of a block
+constexpr int kPair = 2 * kTile;           // rows of a CTA
+constexpr int kSoftmaxThreads = 256;
+constexpr int kLoadThreads = 128;
+constexpr int kTcThreads = kSoftmaxThreads + kLoadThreads + 32;
+constexpr float kSlack = 8.f;              // log2 growth of the maximum that O tolerates
+
+template <int D>
+struct TcCfgA {
+  static constexpr int SUB = kTile * 128;              // 128 rows x 64 f16, one swizzled panel
+  static constexpr int PANELS = D / 64;
+  static constexpr int TILE_B = SUB * PANELS;          // a 128 x D f16 tile
+  static constexpr int Q0 = 0;
+  static constexpr int K0 = 2 * TILE_B;                // two K blocks
+  static constexpr int V0 = K0 + 2 * TILE_B;           // two V blocks
+  static constexpr int OFF0 = V0 + 2 * TILE_B;         // [2][128] row offsets of the keys
+  static constexpr int BAR0 = OFF0 + 2 * kTile * 8;
+  static constexpr int SMEM = 1024 + BAR0 + 512;
+};
+
+struct TcPlanA {
+  int splits;
+  float* acc;  // [splits][T * Hq][D]
+  float* ml;   // [splits][T * Hq][2]
+};
+
+__device__ __forceinline__ uint32_t umma_idesc_f16(int n, bool b_mn_major) {
+  return (1u << 4) | (b_mn_major ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+
+// A from shared memory, K-major.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// A from tensor memory: lane = row, column = two consecutive k.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// MN-major SWIZZLE_128B: 64-element panels `panel` bytes apart (LBO), 8-row groups 1024 B apart (SBO).
+__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t saddr, uint32_t panel) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ void tm_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Barriers and words shared by the roles.
+struct TcShared {
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drain;
+  uint32_t tmem;
+  int abort;
+  int b, tile;             // the block's request (-1: none) and row tile pair
+  int lo, hi;              // union of its rows' intervals
+  int full_lo, full_hi;    // intersection: keys in it need no mask
+  uint32_t nan[2][4];      // per V block: its keys that hold a NaN that was taken out
+};
+
+template <int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs a, TcPlanA pl) {
+  using C = TcCfgA<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  TcShared& sh = *reinterpret_cast<TcShared*>(smem + C::BAR0);
+  long long* offs = reinterpret_cast<long long*>(smem + C::OFF0);
+  static_assert(sizeof(TcShared) <= 512, "barrier area");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    mbar_init(&sh.q_full, kSoftmaxThreads / 32);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.k_full[i], kLoadThreads / 32);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_full[i], kLoadThreads / 32);
+      mbar_init(&sh.v_empty[i], 1);
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.o_full[i], 1);
+      for (int w = 0; w < 4; ++w) sh.nan[i][w] = 0;
+    }
+    mbar_init(&sh.drain, 1);
+    sh.abort = 0;
+    sh.lo = 0x7fffffff;
+    sh.hi = 0;
+    sh.full_lo = 0;
+    sh.full_hi = 0x7fffffff;
+    fence_mbar_init();
+  }
+  if (warp == kTcThreads / 32 - 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pdl_wait();
+  const int head = blockIdx.x % a.Hkv, split = blockIdx.x / a.Hkv;
+  if (warp == 0) {  // the blockIdx.y-th tile pair of the requests above kSplitRows
+    int before = 0, found = -1, tile = 0;
+    for (int base = 0; base < a.B && found < 0; base += 32) {
+      const int b = base + lane;
+      int n = 0;
+      if (b < a.B) {
+        const Req r = request(a, b);
+        const int rows = r.n * a.G;
+        if (rows > kSplitRows) n = (rows + kPair - 1) / kPair;
+        if (r.len > a.max_keys && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(a.err, OKC_DEVERR_PAGE);
+      }
+      int sum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+      }
+      const bool here = before + sum > (int)blockIdx.y;
+      const uint32_t who = __ballot_sync(0xffffffffu, here);
+      if (who) {
+        const int l = __ffs(who) - 1;
+        found = base + l;
+        // from the request's last tile pair on
+        tile = __shfl_sync(0xffffffffu, before + sum, l) - 1 - (int)blockIdx.y;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) {
+      sh.b = found;
+      sh.tile = tile;
+    }
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = sh.tmem;
+  const int b = sh.b;
+  Req rq = {};
+  int rows = 0, row0 = 0, r0 = 0;
+  if (b >= 0) {
+    rq = request(a, b);
+    rows = rq.n * a.G;
+    row0 = a.cu_q[b];
+    r0 = sh.tile * kPair;
+  }
+  // a softmax thread's row
+  RowSpan me = {0, 0, 0};
+  const int r = r0 + threadIdx.x;
+  const bool live = threadIdx.x < kSoftmaxThreads && r < rows;
+  const int tok = live ? row0 + r / a.G : 0, hq = live ? head * a.G + r % a.G : 0;
+  if (live) me = row_span(a, rq, row0, r / a.G);
+  if (threadIdx.x < kSoftmaxThreads) {
+    const int lo = __reduce_min_sync(0xffffffffu, live && me.lo < me.hi ? me.lo : 0x7fffffff);
+    const int hi = __reduce_max_sync(0xffffffffu, live && me.lo < me.hi ? me.hi : 0);
+    const int flo = __reduce_max_sync(0xffffffffu, live ? me.lo : 0);
+    const int fhi = __reduce_min_sync(0xffffffffu, live ? me.hi : 0x7fffffff);
+    if (lane == 0) {
+      atomicMin(&sh.lo, lo);
+      atomicMax(&sh.hi, hi);
+      atomicMax(&sh.full_lo, flo);
+      atomicMin(&sh.full_hi, fhi);
+    }
+  }
+  __syncthreads();
+  // this split's key blocks
+  const int k_lo = sh.lo, k_hi = sh.hi;
+  int nb = k_hi > k_lo ? (k_hi - k_lo + kTile - 1) / kTile : 0, first = 0;
+  if (pl.splits > 1) {
+    const int per = (nb + pl.splits - 1) / pl.splits;
+    first = min(nb, split * per);
+    nb = min(nb, first + per) - first;
+  }
+  const int key0 = k_lo + first * kTile;
+  const bool two = rows - r0 > kTile;
+  volatile int* abort_flag = &sh.abort;
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------ softmax
+    const int w = warp >> 2;  // tile
+    const bool on = w == 0 || two;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + w * kTile, to = tmem + lanes + 2 * kTile + w * D;
+    float fac = 0.f, slope = 0.f, m_ref = -INFINITY, l = 0.f;
+    uint32_t nan_d[D / 32];  // output columns that a visible NaN value reaches
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) nan_d[i] = 0;
+    const float cap2 = CAP ? a.softcap * 1.4426950408889634f : 0.f;
+    if (nb > 0 && on) {
+      // the row in f16, scaled by a power of two, into the swizzled panels
+      uint4 qv[D / 8];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        qv[i] = live ? *reinterpret_cast<const uint4*>(a.q + (size_t)tok * a.ldq + (size_t)hq * D + 8 * i)
+                     : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t u[4] = {qv[i].x, qv[i].y, qv[i].z, qv[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
+      }
+      const int shf = f16_shift(top);
+      fac = a.k_scale[head] * a.sm_scale * (CAP ? 2.f / a.softcap : 1.f) * 1.4426950408889634f * pow2(shf);
+      // a negative factor goes into the query, so that the largest score is the largest sum
+      const float down = fac < 0.f ? -pow2(-shf) : pow2(-shf);
+      fac = fabsf(fac);
+      if (BIAS && live) slope = a.slopes[hq] * 1.4426950408889634f;
+      uint8_t* qs = smem + C::Q0 + w * C::TILE_B;
+      const int lr = threadIdx.x & (kTile - 1);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t u[4] = {qv[i].x, qv[i].y, qv[i].z, qv[i].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = h2(bf16_lo(u[k]) * down, bf16_hi(u[k]) * down);
+        *reinterpret_cast<uint4*>(qs + (i / 8) * C::SUB + lr * 128 + (((i % 8) ^ (lr & 7)) * 16)) =
+            make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.q_full);
+
+    bool ok = true;
+    for (int j = 0; j < nb && on; ++j) {
+      const int kb = key0 + j * kTile;
+      ok = mbar_wait(&sh.s_full[w], (uint32_t)j & 1u, a.err, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) {
+        *abort_flag = 1;
+        break;
+      }
+      tc_after();
+      const bool edge = !__all_sync(0xffffffffu, !live || (me.lo <= kb && me.hi >= kb + kTile));
+      // the log2 score of raw sum v at key kb + c is u * f, or with a distance bias u * f - slope * distance
+      const float f = CAP ? cap2 : fac;
+      auto unit = [&](float v) -> float { return CAP ? tanh_from_2l2e(v * fac) : v; };
+      auto biased = [&](float v, int c) -> float {
+        return fmaf(unit(v), f, -__fmul_rn(slope, (float)abs(me.pos - (kb + c))));
+      };
+      const int vis_lo = live ? me.lo - kb : 0, vis_n = live ? me.hi - me.lo : 0;  // visible columns [vis_lo, vis_lo + vis_n)
+      // ---- the row's maximum over the block ----
+      float mx = -INFINITY;
+#pragma unroll 1
+      for (int c0 = 0; c0 < kTile; c0 += 32) {
+        uint32_t v[32];
+        tm_ld32(ts + c0, v);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          float x = __uint_as_float(v[c]);
+          if (BIAS) x = biased(x, c0 + c);
+          if (edge && !((unsigned)(c0 + c - vis_lo) < (unsigned)max(0, vis_n))) x = -INFINITY;
+          mx = fmaxf(mx, x);
+        }
+      }
+      // without a bias the score grows with the raw sum; rounded up, so that no fused u * f - org is positive
+      if (!BIAS && mx != -INFINITY) mx = __fmul_ru(unit(mx), f);
+      if (m_ref == -INFINITY) {
+        m_ref = mx;  // nothing before it: O and l are zero
+      }
+      const bool grow = mx > m_ref + kSlack;
+      if (__any_sync(0xffffffffu, grow)) {
+        // the block before is complete: its product was issued before this block's scores
+        const float down = grow ? ex2(m_ref - mx) : 1.f;
+        if (grow) m_ref = mx;
+        l *= down;
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t v[32];
+          tm_ld32(to + c0, v);
+          uint32_t o[16];
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(v[16 * hh + c]) * down);
+            tm_st16(to + c0 + 16 * hh, o);
+          }
+        }
+      }
+      const float org = m_ref == -INFINITY ? 0.f : m_ref;
+      // ---- P = 2^(score - org), as f16 over the scores ----
+#pragma unroll 1
+      for (int c0 = 0; c0 < kTile; c0 += 32) {
+        uint32_t v[32], o[16];
+        tm_ld32(ts + c0, v);
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          float p[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float raw = __uint_as_float(v[c + i]);
+            p[i] = ex2(BIAS ? biased(raw, c0 + c + i) - org : fmaf(unit(raw), f, -org));
+            if (edge && !((unsigned)(c0 + c + i - vis_lo) < (unsigned)max(0, vis_n))) p[i] = 0.f;
+          }
+          sum += p[0] + p[1];
+          o[c / 2] = h2(p[0], p[1]);
+        }
+        l += sum;
+        tm_st16(ts + c0 / 2, o);
+      }
+      tm_wait_st();
+      if (kb < sh.full_lo || kb + kTile > sh.full_hi) {  // as the loading warps decide it
+        // NaN values of keys that some rows do not see were taken out of V: put them into the rows that do
+        if (!mbar_wait(&sh.v_full[j & 1], (uint32_t)(j >> 1) & 1u, a.err, abort_flag)) *abort_flag = 1;
+        for (int q = 0; q < 4; ++q) {
+          for (uint32_t bits = *reinterpret_cast<volatile uint32_t*>(&sh.nan[j & 1][q]); bits; bits &= bits - 1) {
+            const int key = kb + 32 * q + __ffs(bits) - 1;
+            if (!live || key < me.lo || key >= me.hi) continue;
+            const int page = a.page_table[(size_t)b * a.table_ld + key / a.P];
+            const uint8_t* vr = a.v_cache + (((size_t)page * a.P + key % a.P) * a.Hkv + head) * D;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+              for (int c = 0; c < 32; ++c) nan_d[i] |= (uint32_t)((vr[32 * i + c] & 0x7f) == 0x7f) << c;
+          }
+        }
+      }
+      tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full[w]);
+    }
+    // ---- output ----
+    if (nb > 0 && on && ok) ok = mbar_wait(&sh.o_full[w], 0, a.err, abort_flag);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_after();
+    const bool have = nb > 0 && on && ok;
+    const size_t orow = (size_t)tok * a.Hq + hq;
+    const float vs = a.v_scale[head];
+    const float inv = l == 0.f ? 0.f : __fdividef(vs, l);
+    if (pl.splits > 1 && live) {
+      const size_t at = (size_t)split * a.T * a.Hq + orow;
+      *reinterpret_cast<float2*>(pl.ml + at * 2) = make_float2(m_ref, l);
+    }
+#pragma unroll 1
+    for (int c0 = 0; c0 < D; c0 += 32) {
+      uint32_t v[32];
+      if (have) {
+        tm_ld32(to + c0, v);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = 0u;
+      }
+      uint32_t nan = 0;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) nan = 32 * i == c0 ? nan_d[i] : nan;
+      if (nan) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+          if ((nan >> c) & 1u) v[c] = 0x7fffffffu;
+      }
+      if (!live) continue;
+      if (pl.splits > 1) {
+        float4* dst = reinterpret_cast<float4*>(pl.acc + ((size_t)split * a.T * a.Hq + orow) * D + c0);
+#pragma unroll
+        for (int c = 0; c < 32; c += 4)
+          dst[c / 4] = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]),
+                                   __uint_as_float(v[c + 3]));
+      } else {
+        uint4* dst = reinterpret_cast<uint4*>(a.out + (size_t)tok * a.ldo + (size_t)hq * D + c0);
+#pragma unroll
+        for (int c = 0; c < 32; c += 8) {
+          uint32_t o[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            o[k] = pack_bf16x2(__uint_as_float(v[c + 2 * k]) * inv, __uint_as_float(v[c + 2 * k + 1]) * inv);
+          dst[c / 8] = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+    }
+  } else if (warp < (kSoftmaxThreads + kLoadThreads) / 32) {
+    // ------------------------------------------------------------------ keys and values
+    const int lt = threadIdx.x - kSoftmaxThreads;  // 0 .. 127
+    const int f_lo = sh.full_lo, f_hi = sh.full_hi;
+    auto offset = [&](int j) {  // where key j * 128 + lt lies; -1: reads zeros
+      const int key = key0 + j * kTile + lt;
+      long long off = -1;
+      if (j < nb && key < k_hi) {
+        const int page = a.page_table[(size_t)b * a.table_ld + key / a.P];
+        if (page >= 0 && page < a.num_pages)
+          off = (((long long)page * a.P + key % a.P) * a.Hkv + head) * D;
+        else
+          atomicOr(a.err, OKC_DEVERR_PAGE);
+      }
+      offs[(j & 1) * kTile + lt] = off;
+    };
+    // the loading warps' barrier: whether any of them gave up (they leave together)
+    auto sync_any = [&](bool bad) {
+      uint32_t any;
+      asm volatile(
+          "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n"
+          " selp.b32 %0, 1, 0, q;\n}\n"
+          : "=r"(any)
+          : "r"((uint32_t)bad)
+          : "memory");
+      return any != 0;
+    };
+    // a thread's 16-byte chunks: eight lanes take four chunks of two neighbouring keys, which the
+    // swizzle puts into different banks
+    constexpr int NCH = D / 16, PER = kTile * NCH / kLoadThreads;
+    auto place = [&](int i, int& key, int& ch) {
+      const int u = i * kLoadThreads + lt;  // (key pair, chunk group of four, key of the pair, chunk)
+      ch = (u & 3) + 4 * ((u >> 3) % (NCH / 4));
+      key = 2 * (u / (2 * NCH)) + ((u >> 2) & 1);
+    };
+    auto store = [&](uint8_t* base, int key, int ch, const uint4& raw) {
+      const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
+      uint32_t o[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        o[2 * k] = e4m3x2_h2(x[k] & 0xffffu);
+        o[2 * k + 1] = e4m3x2_h2(x[k] >> 16);
+      }
+      uint8_t* row = base + (ch / 4) * C::SUB + key * 128;
+      const int c8 = 2 * (ch % 4);
+      *reinterpret_cast<uint4*>(row + ((c8 ^ (key & 7)) * 16)) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4*>(row + (((c8 + 1) ^ (key & 7)) * 16)) = make_uint4(o[4], o[5], o[6], o[7]);
+    };
+    offset(0);
+    sync_any(false);
+    for (int j = 0; j < nb; ++j) {
+      uint4 kr[PER], vr[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        int key, ch;
+        place(i, key, ch);
+        const long long off = offs[(j & 1) * kTile + key];
+        kr[i] = vr[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (off >= 0) {
+          kr[i] = *reinterpret_cast<const uint4*>(a.k_cache + off + ch * 16);
+          vr[i] = *reinterpret_cast<const uint4*>(a.v_cache + off + ch * 16);
+        }
+      }
+      offset(j + 1);
+      const int st = j & 1;
+      const uint32_t ph = ((uint32_t)(j >> 1) & 1u) ^ 1u;
+      bool ok = mbar_wait(&sh.k_empty[st], ph, a.err, abort_flag);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        int key, ch;
+        place(i, key, ch);
+        store(smem + C::K0 + st * C::TILE_B, key, ch, kr[i]);
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.k_full[st]);
+      ok &= mbar_wait(&sh.v_empty[st], ph, a.err, abort_flag);
+      const int kb = key0 + j * kTile;
+      const bool edge = kb < f_lo || kb + kTile > f_hi;
+      if (edge) {
+        if (lt < 4) sh.nan[st][lt] = 0;
+        sync_any(false);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          int key, ch;
+          place(i, key, ch);
+          uint32_t x[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w}, bad = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t nan = ((x[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            bad |= nan;
+            x[k] &= ~((nan >> 7) * 0xffu);
+          }
+          if (bad) atomicOr(&sh.nan[st][key >> 5], 1u << (key & 31));
+          vr[i] = make_uint4(x[0], x[1], x[2], x[3]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        int key, ch;
+        place(i, key, ch);
+        store(smem + C::V0 + st * C::TILE_B, key, ch, vr[i]);
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.v_full[st]);
+      // the offsets of block j + 1 are there, those of block j read
+      if (sync_any(!ok)) {
+        *abort_flag = 1;
+        break;
+      }
+    }
+  } else if (lane == 0) {
+    // ------------------------------------------------------------------ MMA issue
+    const uint32_t id_s = umma_idesc_f16(kTile, false), id_o = umma_idesc_f16(D, true);
+    auto scores = [&](int w, int st) {
+      const uint64_t qa = umma_desc_sw128(smem_u32(smem + C::Q0 + w * C::TILE_B));
+      const uint64_t ka = umma_desc_sw128(smem_u32(smem + C::K0 + st * C::TILE_B));
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t at = ((k / 4) * C::SUB + (k % 4) * 32) >> 4;
+        umma_ss(tmem + w * kTile, qa + at, ka + at, id_s, k != 0);
+      }
+      umma_commit(&sh.s_full[w]);
+    };
+    auto output = [&](int w, int st, bool acc) {
+      const uint64_t va = umma_desc_mn(smem_u32(smem + C::V0 + st * C::TILE_B), C::SUB);
+#pragma unroll
+      for (int k = 0; k < kTile / 16; ++k)
+        umma_ts(tmem + 2 * kTile + w * D, tmem + w * kTile + 8 * k, va + k * (2048 >> 4), id_o, acc || k != 0);
+    };
+    bool ok = nb == 0 || mbar_wait(&sh.q_full, 0, a.err, abort_flag);
+    if (ok && nb > 0) {
+      ok = mbar_wait(&sh.k_full[0], 0, a.err, abort_flag);
+      if (ok) {
+        tc_after();
+        scores(0, 0);
+        if (two) scores(1, 0);
+        umma_commit(&sh.k_empty[0]);
+      }
+    }
+    for (int j = 0; ok && j < nb; ++j) {
+      const int st = j & 1, nx = st ^ 1;
+      ok = mbar_wait(&sh.v_full[st], (uint32_t)(j >> 1) & 1u, a.err, abort_flag);
+      if (ok && j + 1 < nb) ok = mbar_wait(&sh.k_full[nx], (uint32_t)((j + 1) >> 1) & 1u, a.err, abort_flag);
+      for (int w = 0; ok && w < (two ? 2 : 1); ++w) {
+        ok = mbar_wait(&sh.p_full[w], (uint32_t)j & 1u, a.err, abort_flag);
+        if (!ok) break;
+        tc_after();
+        output(w, st, j > 0);
+        if (j + 1 < nb)
+          scores(w, nx);  // over P, which the product above has read by then
+        else
+          umma_commit(&sh.o_full[w]);
+      }
+      if (!ok) break;
+      umma_commit(&sh.v_empty[st]);
+      if (j + 1 < nb) umma_commit(&sh.k_empty[nx]);
+    }
+    if (!ok) *abort_flag = 1;
+    umma_commit(&sh.drain);  // no MMA may be in flight when the tensor memory is released
+    mbar_wait(&sh.drain, 0, a.err);
+  }
+
+  tc_before();
+  __syncthreads();
+  if (warp == kTcThreads / 32 - 1) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// Joins the key splits of a row (token, query head), one warp a row.
+template <int D>
+__global__ void __launch_bounds__(256) attn_chunk_tc_merge_kernel(ChunkArgs a, TcPlanA pl) {
+  constexpr int E = D / 32;
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), all = (long long)a.T * a.Hq;
+  if (item >= all) return;
+  const int t = (int)(item / a.Hq), hq = (int)(item - (long long)t * a.Hq);
+  const int b = find_request(a.cu_q, a.B, t);
+  if (b < 0 || (a.cu_q[b + 1] - a.cu_q[b]) * a.G <= kSplitRows) return;
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < pl.splits) ml = *reinterpret_cast<const float2*>(pl.ml + ((size_t)lane * all + item) * 2);
+  const float M = warp_max(ml.x), org = M == -INFINITY ? 0.f : M;
+  const float w = ex2(ml.x - org), L = warp_sum(w * ml.y);
+  float o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int s = 0; s < pl.splits; ++s) {
+    const float ws = __shfl_sync(0xffffffffu, w, s);
+    const float* src = pl.acc + ((size_t)s * all + item) * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(src + e);
+      o[e] += ws * v.x;
+      o[e + 1] += ws * v.y;
+    }
+  }
+  const float inv = L == 0.f ? 0.f : __fdividef(a.v_scale[hq / a.G], L);
+  __nv_bfloat16* dst = a.out + (size_t)t * a.ldo + (size_t)hq * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(o[e] * inv, o[e + 1] * inv);
+}
+
+// Tile pairs of the requests above kSplitRows, at most.
+long long tc_tiles(int T, int B, int G) {
+  const long long rows = (long long)T * G, big = rows / (kSplitRows + 1);
+  return rows / kPair + (big < B ? big : B);
+}
+
+int tc_splits(int T, int B, int Hq, int Hkv, long long max_keys) {
+  const long long ctas = tc_tiles(T, B, Hq / Hkv) * Hkv;
+  if (ctas <= 0) return 1;
+  long long s = okc_host::num_sms() / ctas;
+  const long long most = max_keys / 512;  // at least four key blocks a split
+  if (s > most) s = most;
+  return s < 1 ? 1 : s > 32 ? 32 : (int)s;
+}
+
+template <int D, bool CAP, bool BIAS>
+int launch_tc(const ChunkArgs& a, const TcPlanA& pl, cudaStream_t stream) {
+  using C = TcCfgA<D>;
+  static okc_host::PerDevice configured;
+  if (int st = configured.smem(attn_chunk_tc_kernel<D, CAP, BIAS>, C::SMEM)) return st;
+  const long long tiles = tc_tiles(a.T, a.B, a.G);
+  if (tiles > 65535) return OKC_ERR_TOO_LARGE;
+  if (int st = okc_host::launch_k(attn_chunk_tc_kernel<D, CAP, BIAS>, dim3(a.Hkv * pl.splits, (unsigned)tiles),
+                                  dim3(kTcThreads), C::SMEM, stream, dim3(1), a, pl))
+    return st;
+  if (pl.splits == 1) return OKC_OK;
+  return okc_host::launch_k(attn_chunk_tc_merge_kernel<D>, dim3((unsigned)(((long long)a.T * a.Hq + 7) / 8)), dim3(256),
+                            0, stream, dim3(1), a, pl);
+}
+
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+size_t attn_chunk_tc_ws_bytes(int T, int B, int Hq, int Hkv, int D) {
+  const int s = tc_splits(T, B, Hq, Hkv, 1ll << 31);
+  if (s == 1) return 0;
+  const size_t rows = (size_t)s * T * Hq;
+  return up(rows * D * 4) + up(rows * 8);
+}
+
+int launch_attn_chunk_tc(const ChunkArgs& a, void* ws, cudaStream_t stream) {
+  TcPlanA pl;
+  pl.splits = tc_splits(a.T, a.B, a.Hq, a.Hkv, a.max_keys);
+  pl.acc = reinterpret_cast<float*>(ws);
+  pl.ml = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + up((size_t)pl.splits * a.T * a.Hq * a.D * 4));
+  const bool cap = a.softcap > 0.f, bias = a.slopes != nullptr;
+  if (a.D == 64) {
+    if (cap) return bias ? launch_tc<64, true, true>(a, pl, stream) : launch_tc<64, true, false>(a, pl, stream);
+    return bias ? launch_tc<64, false, true>(a, pl, stream) : launch_tc<64, false, false>(a, pl, stream);
+  }
+  if (cap) return bias ? launch_tc<128, true, true>(a, pl, stream) : launch_tc<128, true, false>(a, pl, stream);
+  return bias ? launch_tc<128, false, true>(a, pl, stream) : launch_tc<128, false, false>(a, pl, stream);
+}
+
+}  // namespace okc

@@ -25,4 +25,67 @@ __device__ __forceinline__ int find_request(const int32_t* cu_q, int B, int t) {
   return lo < B ? lo : -1;
 }
 
+// 2^x; ex2(-inf) = 0.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// tanh(x) from exp(2x) given x * 2 log2(e): 1 - 2 / (1 + e^2x); off by a few 2^-24 absolute, which a cap of
+// 50 turns into 10^-5 of a score.
+__device__ __forceinline__ float tanh_from_2l2e(float x) { return 1.f - __fdividef(2.f, 1.f + ex2(x)); }
+
+__device__ __forceinline__ uint32_t e4m3x2_h2(uint32_t two) {
+  uint32_t h;
+  asm("{\n .reg .b16 t;\n cvt.u16.u32 t, %1;\n cvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(h) : "r"(two));
+  return h;
+}
+
+__device__ __forceinline__ uint32_t h2(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A request: its rows' key intervals all lie in [lo, hi).
+struct Req {
+  int n, len, lo, hi, prefix;  // new tokens, cached tokens, union of the rows' key intervals
+};
+
+__device__ __forceinline__ Req request(const ChunkArgs& a, int b) {
+  Req r;
+  r.n = max(0, a.cu_q[b + 1] - a.cu_q[b]);
+  r.len = max(0, a.seq_lens[b]);
+  r.prefix = a.prefix_lens ? a.prefix_lens[b] : 0;
+  r.lo = a.window > 0 ? max(0, r.len - r.n + 1 - a.window) : 0;
+  r.hi = min(r.len, a.max_keys);  // positions past the table's columns do not exist
+  return r;
+}
+
+// One query row: its position and the interval [lo, hi) that it sees (hi <= lo: nothing).
+struct RowSpan {
+  int pos, lo, hi;
+};
+__device__ __forceinline__ RowSpan row_span(const ChunkArgs& a, const Req& rq, int row0, int i) {
+  RowSpan r;
+  r.pos = rq.len - rq.n + i;
+  r.lo = a.window > 0 ? max(0, r.pos + 1 - a.window) : 0;
+  if (a.doc_start) r.lo = max(r.lo, a.doc_start[row0 + i]);
+  r.hi = min(rq.hi, max(r.pos + 1, rq.prefix));
+  return r;
+}
+
+// The power of two that brings a bf16 row whose largest magnitude has the bits `top` into
+// [2^13, 2^14): the row is then exact in f16 down to 2^-27 of that magnitude.
+__device__ __forceinline__ int f16_shift(uint32_t top) { return max(-100, (int)(top >> 7) - 127 - 13); }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// A kernel of this file family serves the requests of at most / more than this many rows a KV
+// head (new tokens x query heads of one KV head).
+constexpr int kSplitRows = 64;
+
+// The tensor-memory kernel (attention_chunk_tc.cu) for the requests above kSplitRows.
+size_t attn_chunk_tc_ws_bytes(int T, int B, int Hq, int Hkv, int D);
+int launch_attn_chunk_tc(const ChunkArgs& a, void* ws, cudaStream_t stream);
+
 }  // namespace okc
