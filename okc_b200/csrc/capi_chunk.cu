@@ -68,6 +68,8 @@ int okc_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int e4m3,
   a.N = N;
   a.K = K;
   a.e4m3 = e4m3;
+  a.pairs = ldy % 2 == 0 && aligned_to(y, out_fp32 ? 8 : 4) &&
+            (!residual || (ldr % 2 == 0 && aligned_to(residual, residual_fp32 ? 8 : 4)));
   a.err = error;
   (void)workspace;
   if (workspace_bytes < okc_linear_workspace_bytes(M, N, K, e4m3)) return OKC_ERR_WORKSPACE;

@@ -156,6 +156,7 @@ struct LinearArgs {
   int res_fp32, out_fp32, act;
   int M, N, K;
   int e4m3;
+  int pairs;  // y's and the residual's rows take aligned accesses of two columns
   int* err;
 };
 int launch_linear(const LinearArgs& a, cudaStream_t stream);

@@ -2,10 +2,19 @@
 // e4m3 or bf16 operands, fp32 accumulation in tensor memory.
 //
 // Compute-bound from a few hundred tokens on (2MNK operations against (M + N) K bytes in).
-//  * a CTA owns a 128-token x BN-channel tile; persistent grid, one CTA per SM; tiles are taken
-//    in groups of 16 token tiles per channel column so that the CTAs in flight share operands in L2;
-//  * warp 0 streams K blocks of 128 bytes a row of both operands with TMA into a ring, warp 1 issues
-//    the MMAs into one of two TMEM accumulators, warps 2-5 drain the other one;
+//  * a CTA pair owns a tile of 256 tokens x bn channels (tcgen05 cta_group::2): each CTA loads its 128
+//    token rows and half of the channel rows, 32 KB a K block for 256 x 256 x 128 bytes of products,
+//    so shared-memory traffic stays below what the 8-bit MMA rate takes (a single CTA's 128 x 256 tile
+//    needs 48 KB for half the products);
+//  * persistent grid of pairs; tiles are taken in groups of 8 token tiles per channel column, so that the
+//    pairs in flight share operands in L2; bn (a multiple of 32) is chosen so that the last
+//    wave is full;
+//  * warp 0 streams K blocks of 256 bytes a row with TMA into a ring, warp 1 of the leading CTA issues
+//    the MMAs, warps 2-9 of both CTAs drain the accumulators;
+//  * the MMA truncates as it accumulates (3e-6 relative over K = 4104 in bf16).  A bf16 output does
+//    not see that; for an fp32 output an accumulator takes kSegment K blocks only, and the draining warps
+//    add the segments in fp32 registers (which bounds bn by 128) while the next one runs in the
+//    other accumulator: 3e-7;
 //  * the epilogue turns each 32 x 32 block through shared memory, so that a warp reads the residual
 //    and writes y a row at a time whatever their strides and alignment.
 #include "linear.cuh"
@@ -14,193 +23,411 @@ namespace okc {
 
 namespace {
 
-template <int BN, int STAGES>
-struct LinCfg {
-  static constexpr int A_BYTES = 128 * LIN_KB;
-  static constexpr int B_BYTES = BN * LIN_KB;
-  static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int TURN = 4 * 32 * 33 * 4;  // a 32 x 32 fp32 block per epilogue warp
-  static constexpr int BODY = STAGE * STAGES + TURN;
-  static constexpr int SMEM = 1024 + BODY + 256;
-  static constexpr int TMEM_COLS = 2 * BN;
+constexpr int kStages = 3;
+constexpr int kPanels = 2;       // 128-byte K panels of a stage: one barrier and one commit for eight MMAs
+constexpr int kSegment = 4;      // stages an accumulator takes, for an fp32 output
+constexpr int kDrainWarps = 8;   // a CTA's
+constexpr int kTallThreads = 64 + 32 * kDrainWarps;
+constexpr int kGroup = 8;        // token tiles of a group
+
+template <bool OUT32>
+struct TallSmem {
+  static constexpr int BN = OUT32 ? 128 : 256;       // channels of a tile, at most
+  static constexpr int A_PANEL = 128 * LIN_KB;       // this CTA's 128 token rows
+  static constexpr int B_PANEL = BN / 2 * LIN_KB;    // its channel rows
+  static constexpr int STAGE = kPanels * (A_PANEL + B_PANEL);
+  static constexpr int BLOCK = 32 * 32;              // a 32 x 32 fp32 block
+  static constexpr int BLOCKS = OUT32 ? 2 : 1;       // per draining warp
+  static constexpr int TURN = kDrainWarps * BLOCKS * BLOCK * 4;
+  static constexpr int BAR0 = STAGE * kStages + TURN;
+  static constexpr int TOTAL = 1024 + BAR0 + 256;
 };
 
-// Tile order: groups of 16 token tiles, channel tiles outer within a group.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The shared-memory address of `bar` in the pair's leading CTA.
+__device__ __forceinline__ uint32_t in_leader(uint64_t* bar) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
+  return r;
+}
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+template <bool E4M3>
+__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if constexpr (E4M3)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// Arrives on `bar` of both CTAs when every MMA issued so far is done.
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+// Tile order: groups of kGroup token tiles, channel tiles outer within a group.
 __device__ __forceinline__ void lin_tile(int u, int mt, int nt, int& tm, int& tn) {
-  constexpr int GM = 16;
-  const int per = GM * nt, g = u / per, first = g * GM, rows = min(GM, mt - first);
+  const int per = kGroup * nt, g = u / per, first = g * kGroup, rows = min(kGroup, mt - first);
   const int r = u - g * per;
   tn = r / rows;
   tm = first + r - tn * rows;
 }
 
-template <bool E4M3, int BN, int STAGES>
-__global__ void __launch_bounds__(192) linear_tall_kernel(const __grid_constant__ CUtensorMap map_x,
-                                                          const __grid_constant__ CUtensorMap map_w, LinearArgs a) {
-  using C = LinCfg<BN, STAGES>;
+// A lane's row into a 32 x 32 block, two columns at a time; the pairs of a row are permuted by it, so
+// that rows are written and read without bank conflicts.
+__device__ __forceinline__ void block_put(float* block, int row, int pair, float x, float y) {
+  reinterpret_cast<float2*>(block)[row * 16 + (pair ^ (row & 15))] = make_float2(x, y);
+}
+
+// Writes a 32 x 32 block of y (`rows` x `cols` of it exist): a lane has two neighbouring columns of
+// every second row.  Residual rows are fetched eight at a time ahead of the stores, which may
+// overwrite them.  Whole blocks whose rows take aligned accesses of two columns use them.
+template <bool OUT32>
+__device__ __forceinline__ void tall_block(const float* block, int rows, int cols, float my_sx, const LinearArgs& a,
+                                           int m0, int n0) {
+  constexpr int B = 4;  // a lane's rows in flight
+  const int lane = threadIdx.x & 31, odd = lane >> 4, pair = lane & 15;
+  const int oe = OUT32 ? 4 : 2, re = a.res_fp32 ? 4 : 2;
+  const int have = min(2, max(0, cols - 2 * pair));  // columns this lane has
+  float sw[2], bias[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int n = n0 + 2 * pair + i;
+    sw[i] = i < have ? lin_col_scale(a, n) : 0.f;
+    bias[i] = i < have && a.bias ? __bfloat162float(a.bias[n]) : 0.f;
+  }
+  uint8_t* y = reinterpret_cast<uint8_t*>(a.y) + ((size_t)(m0 + odd) * a.ldy + n0 + 2 * pair) * oe;
+  const uint8_t* res = reinterpret_cast<const uint8_t*>(a.res) + ((size_t)(m0 + odd) * a.ldr + n0 + 2 * pair) * re;
+  const long long y_step = 2 * a.ldy * oe, r_step = 2 * a.ldr * re;
+  const bool whole = a.pairs && rows == 32 && cols >= 32;
+#pragma unroll 1
+  for (int i0 = 0; i0 < 16; i0 += B) {
+    float2 r[B], v[B];
+    if (a.res) {
+      if (whole) {
+        if (a.res_fp32) {
+#pragma unroll
+          for (int i = 0; i < B; ++i) r[i] = *reinterpret_cast<const float2*>(res + i * r_step);
+        } else {
+#pragma unroll
+          for (int i = 0; i < B; ++i) {
+            const uint32_t b = *reinterpret_cast<const uint32_t*>(res + i * r_step);
+            r[i] = make_float2(bf16_lo(b), bf16_hi(b));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+          const int h = 2 * (i0 + i) + odd < rows ? have : 0;
+          r[i].x = h > 0 ? lin_get(res + i * r_step, a.res_fp32) : 0.f;
+          r[i].y = h > 1 ? lin_get(res + i * r_step + re, a.res_fp32) : 0.f;
+        }
+      }
+      res += B * r_step;
+    } else {
+#pragma unroll
+      for (int i = 0; i < B; ++i) r[i] = make_float2(0.f, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const int row = 2 * (i0 + i) + odd;
+      v[i] = reinterpret_cast<const float2*>(block)[row * 16 + (pair ^ (row & 15))];
+      const float sx = __shfl_sync(0xffffffffu, my_sx, row);
+      v[i].x = fmaf(v[i].x * sx, sw[0], bias[0]);
+      v[i].y = fmaf(v[i].y * sx, sw[1], bias[1]);
+    }
+    lin_act_switch(a.act, [&](auto act) {
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        v[i].x = lin_act<decltype(act)::value>(v[i].x);
+        v[i].y = lin_act<decltype(act)::value>(v[i].y);
+      }
+    });
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      v[i].x += r[i].x;
+      v[i].y += r[i].y;
+    }
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        if (OUT32)
+          *reinterpret_cast<float2*>(y + i * y_step) = v[i];
+        else
+          *reinterpret_cast<uint32_t*>(y + i * y_step) = pack_bf16x2(v[i].x, v[i].y);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        const int h = 2 * (i0 + i) + odd < rows ? have : 0;
+        if (h > 0) lin_put<OUT32>(y + i * y_step, v[i].x);
+        if (h > 1) lin_put<OUT32>(y + i * y_step + oe, v[i].y);
+      }
+    }
+    y += B * y_step;
+  }
+}
+
+template <bool E4M3, bool OUT32>
+__global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __grid_constant__ CUtensorMap map_x,
+                                                                      const __grid_constant__ CUtensorMap map_w,
+                                                                      const __grid_constant__ LinearArgs a, int bn) {
+  using C = TallSmem<OUT32>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* turn = reinterpret_cast<float*>(smem + C::STAGE * STAGES);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BODY);
-  uint64_t* empty = full + STAGES;
-  uint64_t* accf = empty + STAGES;
-  uint64_t* acce = accf + 2;
+  float* turn = reinterpret_cast<float*>(smem + C::STAGE * kStages);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR0);  // the leader's count both CTAs' bytes
+  uint64_t* empty = full + kStages;
+  uint64_t* accf = empty + kStages;
+  uint64_t* acce = accf + 2;  // the leader's count both CTAs' draining warps
   uint64_t* drain = acce + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int KE = E4M3 ? LIN_KB : LIN_KB / 2;  // K elements per block
-  const int nkb = (a.K + KE - 1) / KE;
-  const int mt = (a.M + 127) / 128, nt = (a.N + BN - 1) / BN, tiles = mt * nt;
+  const uint32_t rank = cluster_rank();
+  constexpr int KE = E4M3 ? LIN_KB : LIN_KB / 2;  // K elements of a panel
+  const int nkb = (a.K + KE * kPanels - 1) / (KE * kPanels);
+  const int mt = (a.M + 255) / 256, nt = (a.N + bn - 1) / bn, tiles = mt * nt;
+  const int u_first = blockIdx.x >> 1, u_step = gridDim.x >> 1;
 
   pdl_trigger();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&accf[i], 1);
-      mbar_init(&acce[i], 4);
+      mbar_init(&acce[i], 2 * kDrainWarps);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(C::TMEM_COLS));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  cluster_sync();  // both CTAs' barriers and tensor memory are there
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
 
   if (warp == 0) {
     if (lane == 0) {
+      const int half = bn / 2;
+      const uint32_t bytes = 2 * kPanels * (C::A_PANEL + half * LIN_KB);
       int it = 0;
       bool ok = true;
-      for (int u = blockIdx.x; u < tiles && ok; u += gridDim.x) {
+      for (int u = u_first; u < tiles && ok; u += u_step) {
         int tm, tn;
         lin_tile(u, mt, nt, tm, tn);
         for (int kb = 0; kb < nkb; ++kb, ++it) {
-          const int s = it % STAGES;
-          if (!mbar_wait(&empty[s], ((uint32_t)(it / STAGES) & 1u) ^ 1u, a.err, abort_flag)) {
+          const int s = it % kStages;
+          if (!mbar_wait(&empty[s], ((uint32_t)(it / kStages) & 1u) ^ 1u, a.err, abort_flag)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&full[s], C::STAGE);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
           uint8_t* sa = smem + s * C::STAGE;
-          tma_load_2d(sa, &map_x, kb * KE, tm * 128, &full[s]);
-          tma_load_2d(sa + C::A_BYTES, &map_w, kb * KE, tn * BN, &full[s]);
+          const uint32_t bar = in_leader(&full[s]);
+#pragma unroll
+          for (int p = 0; p < kPanels; ++p) {
+            const int k = (kb * kPanels + p) * KE;
+            tma_load_pair(sa + p * C::A_PANEL, &map_x, k, tm * 256 + (int)rank * 128, bar);
+            tma_load_pair(sa + kPanels * C::A_PANEL + p * C::B_PANEL, &map_w, k, tn * bn + (int)rank * half, bar);
+          }
         }
       }
       if (!ok) *abort_flag = 1;
-      // no copy may be in flight when the block ends
-      for (int i = max(0, it - STAGES); i < it; ++i)
-        if (!mbar_wait(&full[i % STAGES], (uint32_t)(i / STAGES) & 1u, a.err)) break;
+      // a stage is left once its MMAs are done, so no copy is in flight after these waits (where a
+      // role gave up, it waited for longer than any copy takes)
+      for (int i = max(0, it - kStages); i < it; ++i)
+        if (!mbar_wait(&empty[i % kStages], (uint32_t)(i / kStages) & 1u, a.err, abort_flag)) break;
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = lin_idesc(E4M3, 128, BN);
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = lin_idesc(E4M3, 256, bn);
       int it = 0, seg = 0;
       bool ok = true;
-      for (int u = blockIdx.x; u < tiles && ok; u += gridDim.x, ++seg) {
-        const int buf = seg & 1;
-        if (!mbar_wait(&acce[buf], ((uint32_t)(seg >> 1) & 1u) ^ 1u, a.err, abort_flag)) {
-          ok = false;
-          break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      for (int u = u_first; u < tiles && ok; u += u_step) {
         for (int kb = 0; kb < nkb; ++kb, ++it) {
-          const int s = it % STAGES;
-          if (!mbar_wait(&full[s], (uint32_t)(it / STAGES) & 1u, a.err, abort_flag)) {
-            ok = false;
-            break;
+          const int buf = seg & 1;
+          const bool begin = OUT32 ? kb % kSegment == 0 : kb == 0;
+          if (begin) {
+            ok = mbar_wait(&acce[buf], ((uint32_t)(seg >> 1) & 1u) ^ 1u, a.err, abort_flag);
+            if (!ok) break;
           }
+          const int s = it % kStages;
+          ok = mbar_wait(&full[s], (uint32_t)(it / kStages) & 1u, a.err, abort_flag);
+          if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t sa = smem_u32(smem + s * C::STAGE);
-          const uint64_t da = umma_desc_sw128(sa), db = umma_desc_sw128(sa + C::A_BYTES);
+          const uint64_t da = umma_desc_sw128(sa), db = umma_desc_sw128(sa + kPanels * C::A_PANEL);
 #pragma unroll
-          for (int j = 0; j < LIN_KB / 32; ++j)
-            lin_mma<E4M3>(tmem + buf * BN, da + 2 * j, db + 2 * j, idesc, (kb | j) != 0);
-          umma_commit(&empty[s]);
+          for (int p = 0; p < kPanels; ++p)
+#pragma unroll
+            for (int j = 0; j < LIN_KB / 32; ++j)
+              pair_mma<E4M3>(tmem + buf * 256, da + ((p * C::A_PANEL + 32 * j) >> 4),
+                             db + ((p * C::B_PANEL + 32 * j) >> 4), idesc, !(begin && p == 0 && j == 0));
+          pair_commit(&empty[s]);
+          if (kb == nkb - 1 || (OUT32 && kb % kSegment == kSegment - 1)) {
+            pair_commit(&accf[buf]);
+            ++seg;
+          }
         }
-        if (ok) umma_commit(&accf[buf]);
       }
       if (!ok) *abort_flag = 1;
-      umma_commit(drain);  // no MMA may be in flight when the tensor memory is released
+      pair_commit(drain);  // no MMA may be in flight when the tensor memory is released
       mbar_wait(drain, 0, a.err);
     }
   } else {
-    const int q4 = warp & 3;
-    float* st = turn + q4 * 32 * 33;
+    const int q4 = warp & 3, half = (warp - 2) >> 2;
+    const int chunks = bn / 32, c_first = half * ((chunks + 1) / 2), c_n = half ? chunks / 2 : (chunks + 1) / 2;
+    const int nseg = OUT32 ? (nkb + kSegment - 1) / kSegment : 1;
+    const uint32_t lanes = tmem + ((uint32_t)(q4 * 32) << 16) + c_first * 32;
+    float* st = turn + (warp - 2) * C::BLOCKS * C::BLOCK;
     int seg = 0;
-    for (int u = blockIdx.x; u < tiles; u += gridDim.x, ++seg) {
-      int tm, tn;
-      lin_tile(u, mt, nt, tm, tn);
-      const int buf = seg & 1;
-      const bool ok = mbar_wait(&accf[buf], (uint32_t)(seg >> 1) & 1u, a.err, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) break;
+    bool ok = true;
+    auto wait_acc = [&](int buf) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&accf[buf], (uint32_t)(seg >> 1) & 1u, a.err, abort_flag));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int m0 = tm * 128 + q4 * 32;
-      const float my_sx = m0 + lane < a.M ? lin_row_scale(a, m0 + lane) : 0.f;
-      const int rows = min(32, a.M - m0);
-#pragma unroll 1
-      for (int c0 = 0; c0 < BN; c0 += 32) {
-        const int n = tn * BN + c0 + lane;
-        if (tn * BN + c0 >= a.N || rows <= 0) break;
-        float v[32];
-        tmem_ld32(tmem + ((uint32_t)(q4 * 32) << 16) + buf * BN + c0, v);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) st[lane * 33 + j] = v[j];
-        __syncwarp();
-        const bool on = n < a.N;
-        const float sw = on ? lin_col_scale(a, n) : 0.f;
-        const float bias = on && a.bias ? __bfloat162float(a.bias[n]) : 0.f;
-#pragma unroll 8
-        for (int i = 0; i < rows; ++i) {
-          const float sx = __shfl_sync(0xffffffffu, my_sx, i);
-          if (on) lin_store(a, m0 + i, n, st[i * 33 + lane], sx, sw, bias);
-        }
-        __syncwarp();
-      }
+      return ok;
+    };
+    auto free_acc = [&](int buf) {
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acce[buf]);
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(&acce[buf])) : "memory");
+    };
+    for (int u = u_first; u < tiles; u += u_step) {
+      int tm, tn;
+      lin_tile(u, mt, nt, tm, tn);
+      const int m0 = tm * 256 + (int)rank * 128 + q4 * 32, rows = min(32, a.M - m0);
+      const float my_sx = lane < rows ? lin_row_scale(a, m0 + lane) : 0.f;
+      auto emit = [&](int c, const float* block) {
+        const int n0 = tn * bn + (c_first + c) * 32;
+        __syncwarp();
+        tall_block<OUT32>(block, rows, a.N - n0, my_sx, a, m0, n0);
+        __syncwarp();
+      };
+      const int c_live = rows > 0 ? min(c_n, (a.N - tn * bn + 31) / 32 - c_first) : 0;
+      if constexpr (OUT32) {
+        float acc[2][32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[c][j] = 0.f;
+        for (int i = 0; i < nseg; ++i, ++seg) {
+          if (!wait_acc(seg & 1)) break;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if (c >= c_n) break;
+#pragma unroll
+            for (int h = 0; h < 32; h += 16) {
+              float v[16];
+              tmem_ld16(lanes + (seg & 1) * 256 + c * 32 + h, v);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) acc[c][h + j] += v[j];
+            }
+          }
+          free_acc(seg & 1);
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) block_put(st + c * C::BLOCK, lane, j, acc[c][2 * j], acc[c][2 * j + 1]);
+#pragma unroll 1
+        for (int c = 0; c < c_live; ++c) emit(c, st + c * C::BLOCK);
+      } else {
+        if (!wait_acc(seg & 1)) break;
+#pragma unroll 1
+        for (int c = 0; c < c_live; ++c) {
+          float v[32];
+          tmem_ld32(lanes + (seg & 1) * 256 + c * 32, v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) block_put(st, lane, j, v[2 * j], v[2 * j + 1]);
+          if (c == c_live - 1) free_acc(seg & 1);
+          emit(c, st);
+        }
+        if (c_live <= 0) free_acc(seg & 1);
+        ++seg;
+      }
     }
+    if (!ok) *abort_flag = 1;
   }
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other may signal it or use its shared memory
   if (warp == 0) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS));
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
 }
 
-template <bool E4M3, int BN, int STAGES>
+// Channels a tile: the multiple of 32 from 64 to `most` whose waves cost least (a tile's time goes with its
+// width, plus a constant of 16 channels' worth for its ends).
+int tall_bn(int M, int N, int pairs, int most) {
+  int best = most;
+  long long cost = -1;
+  for (int bn = most; bn >= 64; bn -= 32) {
+    const long long tiles = (long long)((M + 255) / 256) * ((N + bn - 1) / bn);
+    const long long c = (tiles + pairs - 1) / pairs * (bn + 16);
+    if (cost < 0 || c < cost) {
+      cost = c;
+      best = bn;
+    }
+  }
+  return best;
+}
+
+template <bool E4M3, bool OUT32>
 int launch_tall(const LinearArgs& a, cudaStream_t stream) {
-  using C = LinCfg<BN, STAGES>;
+  const int pairs = okc_host::num_sms() / 2;
+  const int bn = tall_bn(a.M, a.N, pairs, OUT32 ? 128 : 256);
   CUtensorMap mx, mw;
-  if (!lin_make_map(&mx, a.x, a.K, a.M, a.ldx, 128, E4M3) || !lin_make_map(&mw, a.w, a.K, a.N, a.ldw, BN, E4M3))
+  if (!lin_make_map(&mx, a.x, a.K, a.M, a.ldx, 128, E4M3) || !lin_make_map(&mw, a.w, a.K, a.N, a.ldw, bn / 2, E4M3))
     return OKC_ERR_INVALID;
   static okc_host::PerDevice configured;
-  if (int st = configured.smem(linear_tall_kernel<E4M3, BN, STAGES>, C::SMEM)) return st;
-  const long long tiles = (long long)((a.M + 127) / 128) * ((a.N + BN - 1) / BN);
+  if (int st = configured.smem(linear_tall_kernel<E4M3, OUT32>, TallSmem<OUT32>::TOTAL)) return st;
+  const long long tiles = (long long)((a.M + 255) / 256) * ((a.N + bn - 1) / bn);
   if (tiles > 0x7fffffff) return OKC_ERR_TOO_LARGE;
-  const int grid = (int)(tiles < okc_host::num_sms() ? tiles : okc_host::num_sms());
-  return okc_host::launch_k(linear_tall_kernel<E4M3, BN, STAGES>, dim3(grid), dim3(192), C::SMEM, stream, dim3(1), mx,
-                            mw, a);
+  const int grid = 2 * (int)(tiles < pairs ? tiles : pairs);
+  return okc_host::launch_k(linear_tall_kernel<E4M3, OUT32>, dim3(grid), dim3(kTallThreads), TallSmem<OUT32>::TOTAL, stream, dim3(2),
+                            mx, mw, a, bn);
 }
 
 }  // namespace
 
 int launch_linear(const LinearArgs& a, cudaStream_t stream) {
-  return a.e4m3 ? launch_tall<true, 256, 4>(a, stream) : launch_tall<false, 256, 4>(a, stream);
+  if (a.out_fp32) return a.e4m3 ? launch_tall<true, true>(a, stream) : launch_tall<false, true>(a, stream);
+  return a.e4m3 ? launch_tall<true, false>(a, stream) : launch_tall<false, false>(a, stream);
 }
 
 }  // namespace okc

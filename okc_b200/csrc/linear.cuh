@@ -4,6 +4,8 @@
 // swizzle atom), an MMA 32 bytes of it, so the kernels differ only in kind and descriptor.
 #pragma once
 
+#include <type_traits>
+
 #include "kernels.cuh"
 #include "tcgen05.cuh"
 
@@ -31,31 +33,37 @@ enum { LIN_ACT_NONE = 0, LIN_ACT_RELU = 1, LIN_ACT_SILU = 2, LIN_ACT_GELU = 3, L
 
 // Activations in fp32.  tanh and the logistic function go through one exponential:
 // 0.5 (1 + tanh(u)) = 1 / (1 + exp(-2u)).  A NaN stays a NaN (relu included: fmaxf would drop it).
-__device__ __forceinline__ float lin_act(float v, int act) {
+template <int ACT>
+__device__ __forceinline__ float lin_act(float v) {
+  if constexpr (ACT == LIN_ACT_RELU) return v < 0.f ? 0.f : v;
+  if constexpr (ACT == LIN_ACT_SILU) return __fdividef(v, 1.f + __expf(-v));
+  if constexpr (ACT == LIN_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.7071067811865476f));
+  if constexpr (ACT == LIN_ACT_GELU_TANH)
+    return __fdividef(v, 1.f + __expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
+  return v;
+}
+
+// Calls f(integral_constant<ACT>) for the run-time activation.
+template <typename F>
+__device__ __forceinline__ void lin_act_switch(int act, F&& f) {
   switch (act) {
-    case LIN_ACT_RELU: return v < 0.f ? 0.f : v;
-    case LIN_ACT_SILU: return __fdividef(v, 1.f + __expf(-v));
-    case LIN_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.7071067811865476f));
-    case LIN_ACT_GELU_TANH:
-      return __fdividef(v, 1.f + __expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
-    default: return v;
+    case LIN_ACT_RELU: f(std::integral_constant<int, LIN_ACT_RELU>()); break;
+    case LIN_ACT_SILU: f(std::integral_constant<int, LIN_ACT_SILU>()); break;
+    case LIN_ACT_GELU: f(std::integral_constant<int, LIN_ACT_GELU>()); break;
+    case LIN_ACT_GELU_TANH: f(std::integral_constant<int, LIN_ACT_GELU_TANH>()); break;
+    default: f(std::integral_constant<int, LIN_ACT_NONE>()); break;
   }
 }
 
-// One output: the fp32 sum times its row and channel scales, plus the bias, through the activation,
-// plus the residual; rounded once if the output is bf16.
-__device__ __forceinline__ void lin_store(const LinearArgs& a, int m, int n, float v, float sx, float sw, float bias) {
-  v = lin_act(fmaf(v * sx, sw, bias), a.act);
-  if (a.res) {
-    const size_t i = (size_t)m * a.ldr + n;
-    v += a.res_fp32 ? reinterpret_cast<const float*>(a.res)[i]
-                    : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.res)[i]);
-  }
-  const size_t o = (size_t)m * a.ldy + n;
-  if (a.out_fp32)
-    reinterpret_cast<float*>(a.y)[o] = v;
+__device__ __forceinline__ float lin_get(const uint8_t* p, bool fp32) {
+  return fp32 ? *reinterpret_cast<const float*>(p) : __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p));
+}
+template <bool OUT32>
+__device__ __forceinline__ void lin_put(uint8_t* p, float v) {
+  if constexpr (OUT32)
+    *reinterpret_cast<float*>(p) = v;
   else
-    reinterpret_cast<__nv_bfloat16*>(a.y)[o] = __float2bfloat16_rn(v);
+    *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v);
 }
 
 __device__ __forceinline__ float lin_row_scale(const LinearArgs& a, int m) { return a.x_scale ? a.x_scale[m] : 1.f; }
