@@ -426,6 +426,7 @@ int launch_tall(const LinearArgs& a, cudaStream_t stream) {
 }  // namespace
 
 int launch_linear(const LinearArgs& a, cudaStream_t stream) {
+  if (a.M <= kSplitTokens) return launch_linear_split(a, stream);
   if (a.out_fp32) return a.e4m3 ? launch_tall<true, true>(a, stream) : launch_tall<false, true>(a, stream);
   return a.e4m3 ? launch_tall<true, false>(a, stream) : launch_tall<false, false>(a, stream);
 }

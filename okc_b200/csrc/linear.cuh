@@ -13,6 +13,9 @@ namespace okc {
 
 constexpr int LIN_KB = 128;  // bytes of a row per K block
 
+// Up to this many tokens the K-split kernel (linear_split.cu), the CTA-pair kernel (linear.cu) beyond.
+constexpr int kSplitTokens = 128;
+
 // D fp32, both operands K-major, M x N; e4m3 (kind::f8f6f4, type code 0) or bf16 (kind::f16, type code 1).
 __host__ __device__ constexpr uint32_t lin_idesc(bool e4m3, int m, int n) {
   return (1u << 4) | (e4m3 ? 0u : ((1u << 7) | (1u << 10))) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);

@@ -1,0 +1,271 @@
+// Projection with an epilogue, few tokens: the weight is the MMA's 128-row operand and the tokens its N
+// side, so one CTA tile covers 128 channels x up to BN tokens and the weight is read once.
+//
+// HBM-bound on the weight stream (N K bytes in e4m3).
+//  * K is split over the S CTAs of a cluster, S the largest of 1, 2, 4, 8 whose CTAs are all resident
+//    at once (every CTA then streams at the same rate whatever N is), so that the whole card reads;
+//  * warp 0 streams K blocks of 256 bytes a weight row with TMA into a ring, warp 1 issues the
+//    MMAs, warps 2-9 drain the accumulator; for an fp32 output every kSplitSegment stages, summed in
+//    registers, because the MMA truncates as it accumulates;
+//  * each CTA leaves its fp32 sums in its shared memory; the cluster's CTAs take the tokens in turn, add
+//    the S sums in rank order over distributed shared memory (the result repeats bit for bit), apply
+//    the epilogue and write y 128 channels a row: no workspace, no second launch.
+#include "linear.cuh"
+
+namespace okc {
+
+namespace {
+
+constexpr int kSplitPanels = 2;
+constexpr int kSplitSegment = 4;
+constexpr int kSplitDrain = 8;
+constexpr int kSplitThreads = 64 + 32 * kSplitDrain;
+
+template <int BN>
+struct SplitCfg {
+  static constexpr int A_PANEL = 128 * LIN_KB;
+  static constexpr int B_PANEL = BN * LIN_KB;
+  static constexpr int STAGE = kSplitPanels * (A_PANEL + B_PANEL);
+  static constexpr int STAGES = 3;
+  static constexpr int BODY = STAGE * STAGES;
+  static constexpr int SMEM = 1024 + BODY + 256;
+  static constexpr int ACC = BN < 32 ? 32 : BN;  // TMEM columns of an accumulator
+  static_assert(BODY >= BN * 128 * 4, "the sums reuse the ring");
+};
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t local, uint32_t rank) {
+  uint32_t addr;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(local), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <bool E4M3, bool OUT32, int BN>
+__global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __grid_constant__ CUtensorMap map_x,
+                                                                     const __grid_constant__ CUtensorMap map_w,
+                                                                     const __grid_constant__ LinearArgs a) {
+  using C = SplitCfg<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BODY);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* accf = empty + C::STAGES;
+  uint64_t* acce = accf + 2;
+  uint64_t* drain = acce + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int KE = E4M3 ? LIN_KB : LIN_KB / 2;
+  const int S = gridDim.x, rank = blockIdx.x;
+  const int nkb = (a.K + KE * kSplitPanels - 1) / (KE * kSplitPanels);
+  const int per = nkb / S, rest = nkb % S;  // this CTA's stages [k_first, k_first + k_n)
+  const int k_first = rank * per + min(rank, rest), k_n = per + (rank < rest ? 1 : 0);
+  const int n0 = blockIdx.y * 128, m0 = blockIdx.z * BN;
+
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&accf[i], 1);
+      mbar_init(&acce[i], kSplitDrain);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(2 * C::ACC));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  constexpr int COLS = BN >= 64 ? BN / 2 : BN < 32 ? 16 : 32;  // a draining warp's tokens
+  const int q4 = warp & 3, half = (warp - 2) >> 2;
+  const bool drains = warp >= 2 && half * COLS < BN;
+  float acc[COLS];
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      for (; it < k_n; ++it) {
+        const int s = it % C::STAGES;
+        if (!mbar_wait(&empty[s], ((uint32_t)(it / C::STAGES) & 1u) ^ 1u, a.err, abort_flag)) {
+          *abort_flag = 1;
+          break;
+        }
+        mbar_arrive_expect_tx(&full[s], C::STAGE);
+        uint8_t* sa = smem + s * C::STAGE;
+#pragma unroll
+        for (int p = 0; p < kSplitPanels; ++p) {
+          const int k = ((k_first + it) * kSplitPanels + p) * KE;
+          tma_load_2d(sa + p * C::A_PANEL, &map_w, k, n0, &full[s]);
+          tma_load_2d(sa + kSplitPanels * C::A_PANEL + p * C::B_PANEL, &map_x, k, m0, &full[s]);
+        }
+      }
+      // no copy may be in flight when the block ends or reuses the ring
+      for (int i = max(0, it - C::STAGES); i < it; ++i)
+        if (!mbar_wait(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, a.err)) break;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = lin_idesc(E4M3, 128, BN);
+      int seg = 0;
+      bool ok = true;
+      for (int it = 0; it < k_n; ++it) {
+        const int buf = OUT32 ? seg & 1 : 0;
+        const bool begin = OUT32 ? it % kSplitSegment == 0 : it == 0;
+        if (OUT32 && begin) ok = mbar_wait(&acce[buf], ((uint32_t)(seg >> 1) & 1u) ^ 1u, a.err, abort_flag);
+        const int s = it % C::STAGES;
+        ok = ok && mbar_wait(&full[s], (uint32_t)(it / C::STAGES) & 1u, a.err, abort_flag);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t sa = smem_u32(smem + s * C::STAGE);
+        const uint64_t da = umma_desc_sw128(sa), db = umma_desc_sw128(sa + kSplitPanels * C::A_PANEL);
+#pragma unroll
+        for (int p = 0; p < kSplitPanels; ++p)
+#pragma unroll
+          for (int j = 0; j < LIN_KB / 32; ++j)
+            lin_mma<E4M3>(tmem + buf * C::ACC, da + ((p * C::A_PANEL + 32 * j) >> 4), db + ((p * C::B_PANEL + 32 * j) >> 4),
+                          idesc, !(begin && p == 0 && j == 0));
+        umma_commit(&empty[s]);
+        if (it == k_n - 1 || (OUT32 && it % kSplitSegment == kSplitSegment - 1)) {
+          umma_commit(&accf[buf]);
+          ++seg;
+        }
+      }
+      if (!ok) *abort_flag = 1;
+      umma_commit(drain);  // no MMA may be in flight when the tensor memory is released
+      mbar_wait(drain, 0, a.err);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
+    const int nseg = k_n == 0 ? 0 : OUT32 ? (k_n + kSplitSegment - 1) / kSplitSegment : 1;
+    for (int seg = 0; seg < nseg; ++seg) {
+      const int buf = OUT32 ? seg & 1 : 0;
+      const bool ok = mbar_wait(&accf[buf], (uint32_t)(seg >> 1) & 1u, a.err, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) {
+        *abort_flag = 1;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (drains) {
+#pragma unroll
+        for (int h = 0; h < COLS; h += 16) {
+          float v[16];
+          tmem_ld16(tmem + ((uint32_t)(q4 * 32) << 16) + buf * C::ACC + half * COLS + h, v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[h + j] += v[j];
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acce[buf]);
+    }
+  }
+
+  // ---- this CTA's sums [token][channel] into the ring, which nothing uses any more ----
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(smem);
+  if (drains) {
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) sums[(half * COLS + j) * 128 + q4 * 32 + lane] = acc[j];
+  }
+  if (S > 1) cluster_sync_all();
+  else __syncthreads();
+  // ---- tokens rank, rank + S, ..: thread = (channel, every second of them) ----
+  if (warp >= 2) {
+    const int t = threadIdx.x - 64, ch = t & 127, n = n0 + ch;
+    const int live = min(BN, a.M - m0);
+    const float sw = n < a.N ? lin_col_scale(a, n) : 0.f;
+    const float bias = n < a.N && a.bias ? __bfloat162float(a.bias[n]) : 0.f;
+    const int re = a.res_fp32 ? 4 : 2, oe = OUT32 ? 4 : 2;
+    constexpr int U = 4;
+    for (int m1 = rank + (t >> 7) * S; m1 < live; m1 += 2 * U * S) {
+      float v[U], r[U], sx[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int m = m1 + 2 * i * S;
+        const bool on = m < live && n < a.N;
+        r[i] = on && a.res
+                   ? lin_get(reinterpret_cast<const uint8_t*>(a.res) + ((size_t)(m0 + m) * a.ldr + n) * re, a.res_fp32)
+                   : 0.f;
+        sx[i] = on ? lin_row_scale(a, m0 + m) : 0.f;
+        v[i] = 0.f;
+      }
+      for (int s = 0; s < S; ++s) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int m = min(m1 + 2 * i * S, live - 1);
+          v[i] += ld_cluster(smem_u32(sums + m * 128 + ch), (uint32_t)s);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) v[i] = fmaf(v[i] * sx[i], sw, bias);
+      lin_act_switch(a.act, [&](auto act) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) v[i] = lin_act<decltype(act)::value>(v[i]);
+      });
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int m = m1 + 2 * i * S;
+        if (m < live && n < a.N)
+          lin_put<OUT32>(reinterpret_cast<uint8_t*>(a.y) + ((size_t)(m0 + m) * a.ldy + n) * oe, v[i] + r[i]);
+      }
+    }
+  }
+  if (S > 1) cluster_sync_all();  // the others have read this CTA's sums
+  else __syncthreads();
+  if (warp == 0) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * C::ACC));
+  }
+}
+
+template <bool E4M3, bool OUT32, int BN>
+int launch_split_bn(const LinearArgs& a, cudaStream_t stream) {
+  using C = SplitCfg<BN>;
+  CUtensorMap mx, mw;
+  if (!lin_make_map(&mx, a.x, a.K, a.M, a.ldx, BN, E4M3) || !lin_make_map(&mw, a.w, a.K, a.N, a.ldw, 128, E4M3))
+    return OKC_ERR_INVALID;
+  static okc_host::PerDevice configured;
+  if (int st = configured.smem(linear_split_kernel<E4M3, OUT32, BN>, C::SMEM)) return st;
+  const long long tiles = ((long long)a.N + 127) / 128, mt = (a.M + BN - 1) / BN;
+  if (tiles > 65535 || mt > 65535) return OKC_ERR_TOO_LARGE;
+  const int resident = okc_host::num_sms() * (C::SMEM <= 113 * 1024 ? 2 : 1);
+  const int stages = (a.K * (E4M3 ? 1 : 2) + 255) / 256;
+  int S = 1;
+  while (S < 8 && tiles * mt * 2 * S <= resident && stages >= 4 * S) S *= 2;
+  return okc_host::launch_k(linear_split_kernel<E4M3, OUT32, BN>, dim3(S, (unsigned)tiles, (unsigned)mt),
+                            dim3(kSplitThreads), C::SMEM, stream, dim3(S), mx, mw, a);
+}
+
+template <bool E4M3, bool OUT32>
+int launch_split_t(const LinearArgs& a, cudaStream_t stream) {
+  if (a.M <= 16) return launch_split_bn<E4M3, OUT32, 16>(a, stream);
+  if (a.M <= 32) return launch_split_bn<E4M3, OUT32, 32>(a, stream);
+  if (a.M <= 64) return launch_split_bn<E4M3, OUT32, 64>(a, stream);
+  return launch_split_bn<E4M3, OUT32, 128>(a, stream);
+}
+
+}  // namespace
+
+int launch_linear_split(const LinearArgs& a, cudaStream_t stream) {
+  if (a.out_fp32) return a.e4m3 ? launch_split_t<true, true>(a, stream) : launch_split_t<false, true>(a, stream);
+  return a.e4m3 ? launch_split_t<true, false>(a, stream) : launch_split_t<false, false>(a, stream);
+}
+
+}  // namespace okc
