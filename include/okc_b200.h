@@ -425,12 +425,11 @@ int okc_add_rmsnorm_fp8(const void* x, int64_t ldx, const void* residual, int64_
  * NULL.  y bf16 or fp32 (out_fp32) [M][ldy].  act: 0 none, 1 relu, 2 silu, 3 gelu (erf), 4 gelu
  * (tanh form).  fp32 accumulation and epilogue, one rounding.  x and w rows are 16-byte aligned
  * (base, and ld x element size a multiple of 16 bytes); K itself is a multiple of 16 (e4m3) or 8 (bf16).
- * y may be residual.  Beside okc_gemm_bf16. */
-size_t okc_linear_workspace_bytes(int M, int N, int K, int e4m3);
+ * y may be residual.  Takes no workspace.  Beside okc_gemm_bf16. */
 int okc_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int e4m3, const float* x_scale,
                const float* w_scale, int w_scale_one, const void* bias, int act, const void* residual,
                int64_t ldr, int residual_fp32, void* y, int64_t ldy, int out_fp32, int M, int N, int K,
-               void* workspace, size_t workspace_bytes, int32_t* error, okc_stream_t stream);
+               int32_t* error, okc_stream_t stream);
 
 /* Rotary positions with several axes and the FP8 KV-append of a ragged batch.  qkv bf16 [T][ldqkv] =
  * q (Hq*D) | k (Hkv*D) | v (Hkv*D); positions int64 [axes][ld_pos], axes 1..4; pair i < pairs of every q

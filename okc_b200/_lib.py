@@ -87,9 +87,8 @@ SIGNATURES: dict[str, tuple] = {
     "okc_router_logits_workspace_bytes": (_sz, [_i, _i, _i]),
     "okc_router_logits": (_i, [_p, _i, _p, _p, _i, _i, _i, _i, _p, _sz, _p]),
     "okc_add_rmsnorm_fp8": (_i, [_p, _i64, _p, _i64, _i, _p, _p, _i64, _p, _i64, _p, _i, _i, _f, _i, _p]),
-    "okc_linear_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "okc_linear": (_i, [_p, _i64, _p, _i64, _i, _p, _p, _i, _p, _i, _p, _i64, _i, _p, _i64, _i, _i, _i, _i,
-                        _p, _sz, _p, _p]),
+                        _p, _p]),
     "okc_rope_axes_kv_append": (_i, [_p, _i64, _p, _i64, _i, _p, _p, _i, _i, _p, _p, _i, _p, _i64, _i, _p, _p, _p,
                                      _i64, _p, _p, _i, _i, _i, _i, _i, _i64, _p, _p]),
     "okc_attn_chunk_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),

@@ -30,15 +30,10 @@ int okc_add_rmsnorm_fp8(const void* x, int64_t ldx, const void* residual, int64_
                                      eps, unit_offset, stream);
 }
 
-size_t okc_linear_workspace_bytes(int M, int N, int K, int e4m3) {
-  (void)M; (void)N; (void)K; (void)e4m3;
-  return 0;
-}
-
 int okc_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int e4m3, const float* x_scale,
                const float* w_scale, int w_scale_one, const void* bias, int act, const void* residual, int64_t ldr,
-               int residual_fp32, void* y, int64_t ldy, int out_fp32, int M, int N, int K, void* workspace,
-               size_t workspace_bytes, int32_t* error, okc_stream_t stream) {
+               int residual_fp32, void* y, int64_t ldy, int out_fp32, int M, int N, int K, int32_t* error,
+               okc_stream_t stream) {
   if (M == 0) return OKC_OK;
   if (!x || !w || !y || !error || M < 0 || N <= 0 || K <= 0 || act < 0 || act > 4) return OKC_ERR_INVALID;
   const int es = e4m3 ? 1 : 2, ve = 16 / es;
@@ -71,8 +66,6 @@ int okc_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int e4m3,
   a.pairs = ldy % 2 == 0 && aligned_to(y, out_fp32 ? 8 : 4) &&
             (!residual || (ldr % 2 == 0 && aligned_to(residual, residual_fp32 ? 8 : 4)));
   a.err = error;
-  (void)workspace;
-  if (workspace_bytes < okc_linear_workspace_bytes(M, N, K, e4m3)) return OKC_ERR_WORKSPACE;
   return okc::launch_linear(a, stream);
 }
 

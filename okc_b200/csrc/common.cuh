@@ -215,14 +215,20 @@ inline int launch_status() {
 int num_sms();  // cached per device (defined in capi.cu)
 
 // Raises a kernel's dynamic shared-memory limit once per device (the attribute belongs to the
-// device that is current at the call).
+// device that is current at the call).  `regs` > 0: the registers a thread that a kernel which
+// redistributes them (setmaxnreg) must have been compiled to.
 struct PerDevice {
   bool done[64] = {};
   template <typename K>
-  int smem(K kernel, int bytes) {
+  int smem(K kernel, int bytes, int regs = 0) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return OKC_ERR_DEVICE;
     if (done[dev]) return OKC_OK;
+    cudaFuncAttributes fa;
+    if (regs > 0 && (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || fa.numRegs != regs)) {
+      cudaGetLastError();
+      return OKC_ERR_DEVICE;
+    }
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
       cudaGetLastError();
       return OKC_ERR_LAUNCH;

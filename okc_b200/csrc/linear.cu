@@ -10,11 +10,11 @@
 //    pairs in flight share operands in L2; bn (a multiple of 32) is chosen so that the last
 //    wave is full;
 //  * warp 0 streams K blocks of 256 bytes a row with TMA into a ring, warp 1 of the leading CTA issues
-//    the MMAs, warps 2-9 of both CTAs drain the accumulators;
+//    the MMAs, warps 4-11 of both CTAs drain the accumulators;
 //  * the MMA truncates as it accumulates (3e-6 relative over K = 4104 in bf16).  A bf16 output does
 //    not see that; for an fp32 output an accumulator takes kSegment K blocks only, and the draining warps
-//    add the segments in fp32 registers (which bounds bn by 128) while the next one runs in the
-//    other accumulator: 3e-7;
+//    add the segments in fp32 registers while the next one runs in the other accumulator: 3e-7.
+//    A thread holds 128 sums then, with the registers that the first warpgroup gives up;
 //  * the epilogue turns each 32 x 32 block through shared memory, so that a warp reads the residual
 //    and writes y a row at a time whatever their strides and alignment.
 #include "linear.cuh"
@@ -27,18 +27,19 @@ constexpr int kStages = 3;
 constexpr int kPanels = 2;       // 128-byte K panels of a stage: one barrier and one commit for eight MMAs
 constexpr int kSegment = 4;      // stages an accumulator takes, for an fp32 output
 constexpr int kDrainWarps = 8;   // a CTA's
-constexpr int kTallThreads = 64 + 32 * kDrainWarps;
+constexpr int kFirstDrain = 4;   // warps 0 and 1 load and issue; 2 and 3 fill their warpgroup
+constexpr int kTallThreads = 32 * (kFirstDrain + kDrainWarps);
+// Registers a thread: the launch's, and how fp32 outputs split them over the three warpgroups.
+constexpr int kLaunchRegs = 168, kIssueRegs = 40, kDrainRegs = 232;
+static_assert(128 * kIssueRegs + 256 * kDrainRegs <= kTallThreads * kLaunchRegs, "the split must fit the launch");
 constexpr int kGroup = 8;        // token tiles of a group
 
-template <bool OUT32>
 struct TallSmem {
-  static constexpr int BN = OUT32 ? 128 : 256;       // channels of a tile, at most
   static constexpr int A_PANEL = 128 * LIN_KB;       // this CTA's 128 token rows
-  static constexpr int B_PANEL = BN / 2 * LIN_KB;    // its channel rows
+  static constexpr int B_PANEL = 128 * LIN_KB;       // its channel rows, at most
   static constexpr int STAGE = kPanels * (A_PANEL + B_PANEL);
-  static constexpr int BLOCK = 32 * 32;              // a 32 x 32 fp32 block
-  static constexpr int BLOCKS = OUT32 ? 2 : 1;       // per draining warp
-  static constexpr int TURN = kDrainWarps * BLOCKS * BLOCK * 4;
+  static constexpr int BLOCK = 32 * 32;              // a 32 x 32 fp32 block per draining warp
+  static constexpr int TURN = kDrainWarps * BLOCK * 4;
   static constexpr int BAR0 = STAGE * kStages + TURN;
   static constexpr int TOTAL = 1024 + BAR0 + 256;
 };
@@ -137,12 +138,18 @@ __device__ __forceinline__ void tall_block(const float* block, int rows, int col
           }
         }
       } else {
+        auto get = [&](auto type) {
+          using R = decltype(type);
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
-          const int h = 2 * (i0 + i) + odd < rows ? have : 0;
-          r[i].x = h > 0 ? lin_get(res + i * r_step, a.res_fp32) : 0.f;
-          r[i].y = h > 1 ? lin_get(res + i * r_step + re, a.res_fp32) : 0.f;
-        }
+          for (int i = 0; i < B; ++i) {
+            const int h = 2 * (i0 + i) + odd < rows ? have : 0;
+            const R* p = reinterpret_cast<const R*>(res + i * r_step);
+            r[i].x = h > 0 ? (float)p[0] : 0.f;
+            r[i].y = h > 1 ? (float)p[1] : 0.f;
+          }
+        };
+        if (a.res_fp32) get(float());
+        else get(__nv_bfloat16());
       }
       res += B * r_step;
     } else {
@@ -193,7 +200,7 @@ template <bool E4M3, bool OUT32>
 __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __grid_constant__ CUtensorMap map_x,
                                                                       const __grid_constant__ CUtensorMap map_w,
                                                                       const __grid_constant__ LinearArgs a, int bn) {
-  using C = TallSmem<OUT32>;
+  using C = TallSmem;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* turn = reinterpret_cast<float*>(smem + C::STAGE * kStages);
@@ -237,8 +244,9 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < kFirstDrain) {
+    if constexpr (OUT32) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+    if (warp == 0 && lane == 0) {
       const int half = bn / 2;
       const uint32_t bytes = 2 * kPanels * (C::A_PANEL + half * LIN_KB);
       int it = 0;
@@ -268,9 +276,7 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
       // role gave up, it waited for longer than any copy takes)
       for (int i = max(0, it - kStages); i < it; ++i)
         if (!mbar_wait(&empty[i % kStages], (uint32_t)(i / kStages) & 1u, a.err, abort_flag)) break;
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    } else if (warp == 1 && lane == 0 && rank == 0) {
       const uint32_t idesc = lin_idesc(E4M3, 256, bn);
       int it = 0, seg = 0;
       bool ok = true;
@@ -306,11 +312,12 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
       mbar_wait(drain, 0, a.err);
     }
   } else {
-    const int q4 = warp & 3, half = (warp - 2) >> 2;
+    if constexpr (OUT32) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kDrainRegs));
+    const int q4 = warp & 3, half = (warp - kFirstDrain) >> 2;
     const int chunks = bn / 32, c_first = half * ((chunks + 1) / 2), c_n = half ? chunks / 2 : (chunks + 1) / 2;
     const int nseg = OUT32 ? (nkb + kSegment - 1) / kSegment : 1;
     const uint32_t lanes = tmem + ((uint32_t)(q4 * 32) << 16) + c_first * 32;
-    float* st = turn + (warp - 2) * C::BLOCKS * C::BLOCK;
+    float* st = turn + (warp - kFirstDrain) * C::BLOCK;
     int seg = 0;
     bool ok = true;
     auto wait_acc = [&](int buf) {
@@ -329,41 +336,42 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
       lin_tile(u, mt, nt, tm, tn);
       const int m0 = tm * 256 + (int)rank * 128 + q4 * 32, rows = min(32, a.M - m0);
       const float my_sx = lane < rows ? lin_row_scale(a, m0 + lane) : 0.f;
-      auto emit = [&](int c, const float* block) {
+      auto emit = [&](int c) {
         const int n0 = tn * bn + (c_first + c) * 32;
         __syncwarp();
-        tall_block<OUT32>(block, rows, a.N - n0, my_sx, a, m0, n0);
+        tall_block<OUT32>(st, rows, a.N - n0, my_sx, a, m0, n0);
         __syncwarp();
       };
       const int c_live = rows > 0 ? min(c_n, (a.N - tn * bn + 31) / 32 - c_first) : 0;
       if constexpr (OUT32) {
-        float acc[2][32];
+        float acc[4][32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int j = 0; j < 32; ++j) acc[c][j] = 0.f;
         for (int i = 0; i < nseg; ++i, ++seg) {
           if (!wait_acc(seg & 1)) break;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 4; ++c) {
             if (c >= c_n) break;
+            float v[32];
+            tmem_ld32(lanes + (seg & 1) * 256 + c * 32, v);
 #pragma unroll
-            for (int h = 0; h < 32; h += 16) {
-              float v[16];
-              tmem_ld16(lanes + (seg & 1) * 256 + c * 32 + h, v);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) acc[c][h + j] += v[j];
-            }
+            for (int j = 0; j < 32; ++j) acc[c][j] += v[j];
           }
           free_acc(seg & 1);
         }
         if (!ok) break;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) block_put(st + c * C::BLOCK, lane, j, acc[c][2 * j], acc[c][2 * j + 1]);
 #pragma unroll 1
-        for (int c = 0; c < c_live; ++c) emit(c, st + c * C::BLOCK);
+        for (int c = 0; c < c_live; ++c) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (k != c) continue;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) block_put(st, lane, j, acc[k][2 * j], acc[k][2 * j + 1]);
+          }
+          emit(c);
+        }
       } else {
         if (!wait_acc(seg & 1)) break;
 #pragma unroll 1
@@ -373,7 +381,7 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
 #pragma unroll
           for (int j = 0; j < 16; ++j) block_put(st, lane, j, v[2 * j], v[2 * j + 1]);
           if (c == c_live - 1) free_acc(seg & 1);
-          emit(c, st);
+          emit(c);
         }
         if (c_live <= 0) free_acc(seg & 1);
         ++seg;
@@ -391,12 +399,12 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
   }
 }
 
-// Channels a tile: the multiple of 32 from 64 to `most` whose waves cost least (a tile's time goes with its
+// Channels a tile: the multiple of 32 from 64 to 256 whose waves cost least (a tile's time goes with its
 // width, plus a constant of 16 channels' worth for its ends).
-int tall_bn(int M, int N, int pairs, int most) {
-  int best = most;
+int tall_bn(int M, int N, int pairs) {
+  int best = 256;
   long long cost = -1;
-  for (int bn = most; bn >= 64; bn -= 32) {
+  for (int bn = 256; bn >= 64; bn -= 32) {
     const long long tiles = (long long)((M + 255) / 256) * ((N + bn - 1) / bn);
     const long long c = (tiles + pairs - 1) / pairs * (bn + 16);
     if (cost < 0 || c < cost) {
@@ -410,16 +418,16 @@ int tall_bn(int M, int N, int pairs, int most) {
 template <bool E4M3, bool OUT32>
 int launch_tall(const LinearArgs& a, cudaStream_t stream) {
   const int pairs = okc_host::num_sms() / 2;
-  const int bn = tall_bn(a.M, a.N, pairs, OUT32 ? 128 : 256);
+  const int bn = tall_bn(a.M, a.N, pairs);
   CUtensorMap mx, mw;
   if (!lin_make_map(&mx, a.x, a.K, a.M, a.ldx, 128, E4M3) || !lin_make_map(&mw, a.w, a.K, a.N, a.ldw, bn / 2, E4M3))
     return OKC_ERR_INVALID;
   static okc_host::PerDevice configured;
-  if (int st = configured.smem(linear_tall_kernel<E4M3, OUT32>, TallSmem<OUT32>::TOTAL)) return st;
+  if (int st = configured.smem(linear_tall_kernel<E4M3, OUT32>, TallSmem::TOTAL, OUT32 ? kLaunchRegs : 0)) return st;
   const long long tiles = (long long)((a.M + 255) / 256) * ((a.N + bn - 1) / bn);
   if (tiles > 0x7fffffff) return OKC_ERR_TOO_LARGE;
   const int grid = 2 * (int)(tiles < pairs ? tiles : pairs);
-  return okc_host::launch_k(linear_tall_kernel<E4M3, OUT32>, dim3(grid), dim3(kTallThreads), TallSmem<OUT32>::TOTAL, stream, dim3(2),
+  return okc_host::launch_k(linear_tall_kernel<E4M3, OUT32>, dim3(grid), dim3(kTallThreads), TallSmem::TOTAL, stream, dim3(2),
                             mx, mw, a, bn);
 }
 

@@ -58,9 +58,6 @@ __device__ __forceinline__ void lin_act_switch(int act, F&& f) {
   }
 }
 
-__device__ __forceinline__ float lin_get(const uint8_t* p, bool fp32) {
-  return fp32 ? *reinterpret_cast<const float*>(p) : __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p));
-}
 template <bool OUT32>
 __device__ __forceinline__ void lin_put(uint8_t* p, float v) {
   if constexpr (OUT32)

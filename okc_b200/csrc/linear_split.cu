@@ -150,6 +150,15 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
       mbar_wait(drain, 0, a.err);
     }
   } else {
+    if (a.res) {  // the rows of the residual that this CTA will add, into L2 while the weight streams
+      const int re = a.res_fp32 ? 4 : 2, lines = re, t = threadIdx.x - 64;  // 128 channels are `re` lines
+      for (int i = t; i < (min(BN, a.M - m0) - rank + S - 1) / S * lines; i += 32 * kSplitDrain) {
+        const int m = m0 + rank + i / lines * S, n = n0 + i % lines * (128 / re);
+        if (n < a.N)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const uint8_t*>(a.res) +
+                                                         ((size_t)m * a.ldr + n) * re));
+      }
+    }
 #pragma unroll
     for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
     const int nseg = k_n == 0 ? 0 : OUT32 ? (k_n + kSplitSegment - 1) / kSplitSegment : 1;
@@ -192,20 +201,25 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
     const int live = min(BN, a.M - m0);
     const float sw = n < a.N ? lin_col_scale(a, n) : 0.f;
     const float bias = n < a.N && a.bias ? __bfloat162float(a.bias[n]) : 0.f;
-    const int re = a.res_fp32 ? 4 : 2, oe = OUT32 ? 4 : 2;
-    constexpr int U = 4;
+    constexpr int U = 8, oe = OUT32 ? 4 : 2;
     for (int m1 = rank + (t >> 7) * S; m1 < live; m1 += 2 * U * S) {
       float v[U], r[U], sx[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int m = m1 + 2 * i * S;
-        const bool on = m < live && n < a.N;
-        r[i] = on && a.res
-                   ? lin_get(reinterpret_cast<const uint8_t*>(a.res) + ((size_t)(m0 + m) * a.ldr + n) * re, a.res_fp32)
-                   : 0.f;
-        sx[i] = on ? lin_row_scale(a, m0 + m) : 0.f;
-        v[i] = 0.f;
+        sx[i] = m < live ? lin_row_scale(a, m0 + m) : 0.f;
+        v[i] = r[i] = 0.f;
       }
+      auto get = [&](auto type) {
+        using R = decltype(type);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int m = m1 + 2 * i * S;
+          if (m < live && n < a.N) r[i] = (float)reinterpret_cast<const R*>(a.res)[(size_t)(m0 + m) * a.ldr + n];
+        }
+      };
+      if (a.res && a.res_fp32) get(float());
+      else if (a.res) get(__nv_bfloat16());
       for (int s = 0; s < S; ++s) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {

@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from ._lib import check
 
-_lib.load()  # fail loudly at import if the native library is absent
+_LIB = _lib.load()  # fail loudly at import if the native library is absent
 
 _WS: dict[tuple[int, str], torch.Tensor] = {}
 
@@ -382,48 +382,56 @@ def _error_word(dev: int, tag: str) -> int:
     return buf.data_ptr()
 
 
-def _call(dev: int, name: str, *args) -> None:
-    """Calls the C entry point on the current stream of `dev`, with `dev` current."""
-    fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == dev:
-        st = fn(*args, _stream(dev))
+def _call(dev: int, fn, name: str, *args) -> None:
+    """Calls a C entry point on the current stream of `dev`, with `dev` current."""
+    if _current_device() == dev:
+        st = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            st = fn(*args, _stream(dev))
-    if st != _lib.OKC_OK:
+            st = fn(*args, _raw_stream(dev))
+    if st:
         check(st, name)
 
 
-def _tensor(t: torch.Tensor, name: str, dtype, shape: tuple, dev: int, rows: bool = False) -> None:
-    """Checks dtype, device, shape (None = any) and strides: contiguous, or with `rows` only inside
-    each row (the first dimension's stride is free)."""
+# The two queries that torch.cuda.current_device() and current_stream() wrap; a call of a small
+# operator is as long as a few of those.
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _bad(t, name: str, dtype, shape: tuple, dev: int) -> _lib.OkcError:
     if t.dtype != dtype and not (isinstance(dtype, tuple) and t.dtype in dtype):
-        raise _lib.OkcError(f"{name}: expected {dtype}, got {t.dtype}")
-    if not t.is_cuda or t.device.index != dev:
-        raise _lib.OkcError(f"{name}: expected a tensor on cuda:{dev}, got {t.device}")
-    ts = t.shape
-    if len(ts) != len(shape):
-        raise _lib.OkcError(f"{name}: expected shape {shape}, got {tuple(ts)}")
-    for have, want in zip(ts, shape):
-        if want is not None and have != want:
-            raise _lib.OkcError(f"{name}: expected shape {shape}, got {tuple(ts)}")
+        return _lib.OkcError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.get_device() != dev:
+        return _lib.OkcError(f"{name}: expected a tensor on cuda:{dev}, got {t.device}")
+    if t.shape != shape:
+        return _lib.OkcError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+    return _lib.OkcError(f"{name}: unsupported strides {t.stride()} for shape {shape}")
+
+
+def _dense(t: torch.Tensor, name: str, dtype, shape: tuple, dev: int) -> int:
+    """Checks dtype, shape, device and contiguity; returns the address."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise _bad(t, name, dtype, shape, dev)
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, name: str, dtype, shape: tuple, dev: int) -> int:
+    """Checks dtype (one, or a tuple of them), shape, device, and that each row (all but the first
+    dimension) is contiguous and rows do not overlap; returns the row stride in elements."""
+    if (t.dtype is not dtype and not (type(dtype) is tuple and t.dtype in dtype)) or t.shape != shape or t.get_device() != dev:
+        raise _bad(t, name, dtype, shape, dev)
+    row = shape[1] if len(shape) == 2 else shape[1] * shape[2]
     if t.is_contiguous():
-        return
-    if rows:
-        want = 1
-        for d in range(len(ts) - 1, 0, -1):
-            if ts[d] != 1 and t.stride(d) != want:
-                break
-            want *= ts[d]
-        else:
-            if ts[0] <= 1 or t.stride(0) >= want:
-                return
-    raise _lib.OkcError(f"{name}: unsupported strides {t.stride()} for shape {tuple(ts)}")
-
-
-def _ld(t: torch.Tensor) -> int:
-    """Row stride in elements; a single row has the length of one."""
-    return t.stride(0) if t.shape[0] > 1 else math.prod(t.shape[1:])
+        return row
+    st = t.stride()
+    if (st[-1] != 1 and shape[-1] != 1) or (len(shape) == 3 and st[1] != shape[2] and shape[1] != 1):
+        raise _bad(t, name, dtype, shape, dev)
+    if shape[0] <= 1:
+        return row
+    if st[0] < row:
+        raise _bad(t, name, dtype, shape, dev)
+    return st[0]
 
 
 _E4M3 = torch.float8_e4m3fn
@@ -440,25 +448,24 @@ def add_rmsnorm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float, residual: torc
     dev = _dev_index(x)
     if x.dim() != 2:
         raise _lib.OkcError(f"x: expected [T, H], got {tuple(x.shape)}")
-    T, H = x.shape
-    _tensor(x, "x", torch.bfloat16, (T, H), dev, rows=True)
-    _tensor(w, "w", torch.bfloat16, (H,), dev)
-    q = torch.empty((T, H), dtype=_E4M3, device=x.device)
-    scale = torch.empty(T, dtype=torch.float32, device=x.device)
+    T, H = shape = tuple(x.shape)
+    ldx = _rows(x, "x", torch.bfloat16, shape, dev)
+    wp = _dense(w, "w", torch.bfloat16, (H,), dev)
+    q = x.new_empty(shape, dtype=_E4M3)
+    scale = x.new_empty(T, dtype=torch.float32)
     rp, rld, op, old, r32 = None, 0, None, 0, 0
     if residual is not None:
-        _tensor(residual, "residual", _STREAM_TYPES, (T, H), dev, rows=True)
+        rld = _rows(residual, "residual", _STREAM_TYPES, shape, dev)
         if residual_out is None:
-            residual_out = torch.empty((T, H), dtype=residual.dtype, device=x.device)
+            residual_out, old = residual.new_empty(shape), H
         else:
-            _tensor(residual_out, "residual_out", residual.dtype, (T, H), dev, rows=True)
-        rp, rld, op, old = residual.data_ptr(), _ld(residual), residual_out.data_ptr(), _ld(residual_out)
-        r32 = int(residual.dtype == torch.float32)
+            old = _rows(residual_out, "residual_out", residual.dtype, shape, dev)
+        rp, op, r32 = residual.data_ptr(), residual_out.data_ptr(), int(residual.dtype is torch.float32)
     elif residual_out is not None:
         raise _lib.OkcError("residual_out without residual")
     if T:
-        _call(dev, "okc_add_rmsnorm_fp8", x.data_ptr(), _ld(x), rp, rld, r32, w.data_ptr(), op, old, q.data_ptr(), H,
-              scale.data_ptr(), T, H, float(eps), int(unit_offset))
+        _call(dev, _LIB.okc_add_rmsnorm_fp8, "okc_add_rmsnorm_fp8", x.data_ptr(), ldx, rp, rld, r32, wp, op, old,
+              q.data_ptr(), H, scale.data_ptr(), T, H, eps, int(unit_offset))
     return q, scale, residual_out
 
 
@@ -479,35 +486,30 @@ def linear(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor | None = None
     if act not in LINEAR_ACTS:
         raise _lib.OkcError(f"act: expected one of {sorted(k for k in LINEAR_ACTS if k)}, got {act!r}")
     (M, K), N = x.shape, w.shape[0]
-    _tensor(x, "x", (_E4M3, torch.bfloat16), (M, K), dev, rows=True)
-    _tensor(w, "w", x.dtype, (N, K), dev, rows=True)
+    ldx = _rows(x, "x", (_E4M3, torch.bfloat16), (M, K), dev)
+    ldw = _rows(w, "w", x.dtype, (N, K), dev)
     if out is None:
         if out_dtype not in _STREAM_TYPES:
             raise _lib.OkcError(f"out_dtype: expected bfloat16 or float32, got {out_dtype}")
-        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+        out, ldy = x.new_empty((M, N), dtype=out_dtype), N
     else:
-        _tensor(out, "out", _STREAM_TYPES, (M, N), dev, rows=True)
+        ldy = _rows(out, "out", _STREAM_TYPES, (M, N), dev)
     sx = sw = bp = rp = None
     one = rld = r32 = 0
     if x_scale is not None:
-        _tensor(x_scale, "x_scale", torch.float32, (M,), dev)
-        sx = x_scale.data_ptr()
+        sx = _dense(x_scale, "x_scale", torch.float32, (M,), dev)
     if w_scale is not None:
         one = int(w_scale.numel() == 1)
-        _tensor(w_scale, "w_scale", torch.float32, (1,) if one else (N,), dev)
-        sw = w_scale.data_ptr()
+        sw = _dense(w_scale, "w_scale", torch.float32, (1,) if one else (N,), dev)
     if bias is not None:
-        _tensor(bias, "bias", torch.bfloat16, (N,), dev)
-        bp = bias.data_ptr()
+        bp = _dense(bias, "bias", torch.bfloat16, (N,), dev)
     if residual is not None:
-        _tensor(residual, "residual", _STREAM_TYPES, (M, N), dev, rows=True)
-        rp, rld, r32 = residual.data_ptr(), _ld(residual), int(residual.dtype == torch.float32)
-    if not M:
-        return out
-    e4m3 = int(x.dtype == _E4M3)
-    _call(dev, "okc_linear", x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), e4m3, sx, sw, one, bp, LINEAR_ACTS[act], rp,
-          rld, r32, out.data_ptr(), _ld(out), int(out.dtype == torch.float32), M, N, K, None, 0,
-          _error_word(dev, "linear"))
+        rld = _rows(residual, "residual", _STREAM_TYPES, (M, N), dev)
+        rp, r32 = residual.data_ptr(), int(residual.dtype is torch.float32)
+    if M:
+        _call(dev, _LIB.okc_linear, "okc_linear", x.data_ptr(), ldx, w.data_ptr(), ldw, int(x.dtype is _E4M3), sx, sw,
+              one, bp, LINEAR_ACTS[act], rp, rld, r32, out.data_ptr(), ldy, int(out.dtype is torch.float32), M, N, K,
+              _error_word(dev, "linear"))
     return out
 
 
@@ -516,21 +518,26 @@ def rope_sections(sizes) -> tuple[int, ...]:
     return tuple(a for a, n in enumerate(sizes) for _ in range(n))
 
 
-def _ragged(cu_q, seq_lens, page_table, dev: int) -> int:
-    B = seq_lens.shape[0]
-    _tensor(seq_lens, "seq_lens", torch.int32, (B,), dev)
-    _tensor(cu_q, "cu_q", torch.int32, (B + 1,), dev)
-    _tensor(page_table, "page_table", torch.int32, (B, None), dev, rows=True)
-    return B
+def _ragged(cu_q, seq_lens, page_table, dev: int) -> tuple:
+    """(cu_q, seq_lens, B, page_table, its row stride, its columns) as the entry points take them."""
+    B = seq_lens.numel()
+    sl = _dense(seq_lens, "seq_lens", torch.int32, (B,), dev)
+    cq = _dense(cu_q, "cu_q", torch.int32, (B + 1,), dev)
+    cols = page_table.shape[-1]
+    ld = _rows(page_table, "page_table", torch.int32, (B, cols), dev)
+    return cq, sl, B, page_table.data_ptr(), ld, cols
 
 
-def _caches(k_cache, v_cache, k_scale, v_scale, Hkv, D: int, dev: int):
-    _tensor(k_cache, "k_cache", _E4M3, (None, None, Hkv, D), dev)
-    pages, P, Hkv, _ = k_cache.shape
-    _tensor(v_cache, "v_cache", _E4M3, (pages, P, Hkv, D), dev)
-    _tensor(k_scale, "k_scale", torch.float32, (Hkv,), dev)
-    _tensor(v_scale, "v_scale", torch.float32, (Hkv,), dev)
-    return pages, P, Hkv
+def _caches(k_cache, v_cache, k_scale, v_scale, Hkv, D: int, dev: int) -> tuple:
+    """(k_cache, v_cache, k_scale, v_scale, pages, P, Hkv); Hkv None: the cache's."""
+    if k_cache.dim() != 4:
+        raise _lib.OkcError(f"k_cache: expected [pages, P, Hkv, D], got {tuple(k_cache.shape)}")
+    pages, P, h, _ = k_cache.shape
+    Hkv = Hkv or h
+    shape = (pages, P, Hkv, D)
+    return (_dense(k_cache, "k_cache", _E4M3, shape, dev), _dense(v_cache, "v_cache", _E4M3, shape, dev),
+            _dense(k_scale, "k_scale", torch.float32, (Hkv,), dev), _dense(v_scale, "v_scale", torch.float32, (Hkv,), dev),
+            pages, P, Hkv)
 
 
 def rope_axes_kv_append(qkv: torch.Tensor, positions: torch.Tensor, axes, inv_freq: torch.Tensor,
@@ -547,23 +554,25 @@ def rope_axes_kv_append(qkv: torch.Tensor, positions: torch.Tensor, axes, inv_fr
     dev = _dev_index(qkv)
     if qkv.dim() != 2 or positions.dim() != 2:
         raise _lib.OkcError(f"qkv and positions: expected [T, C] and [A, T], got {tuple(qkv.shape)}, {tuple(positions.shape)}")
-    T = qkv.shape[0]
-    _tensor(qkv, "qkv", torch.bfloat16, (T, (Hq + 2 * Hkv) * D), dev, rows=True)
-    _tensor(positions, "positions", torch.int64, (None, T), dev, rows=True)
-    axes = bytes(axes)
-    _tensor(inv_freq, "inv_freq", torch.float32, (len(axes),), dev)
-    B = _ragged(cu_q, seq_lens, page_table, dev)
-    pages, P, _ = _caches(k_cache, v_cache, k_scale, v_scale, Hkv, D, dev)
+    T, A = qkv.shape[0], positions.shape[0]
+    ldqkv = _rows(qkv, "qkv", torch.bfloat16, (T, (Hq + 2 * Hkv) * D), dev)
+    ld_pos = _rows(positions, "positions", torch.int64, (A, T), dev)
+    try:
+        axes = bytes(axes)
+    except (TypeError, ValueError):
+        raise _lib.OkcError(f"axes: expected the axis (0..{A - 1}) of each pair, got {axes!r}") from None
+    R = len(axes)
+    freq = _dense(inv_freq, "inv_freq", torch.float32, (R,), dev)
+    cq, sl, B, table, table_ld, cols = _ragged(cu_q, seq_lens, page_table, dev)
+    kc, vc, ks, vs, pages, P, _ = _caches(k_cache, v_cache, k_scale, v_scale, Hkv, D, dev)
     if q_out is None:
-        q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=qkv.device)
+        q_out, ldq = qkv.new_empty((T, Hq, D)), Hq * D
     else:
-        _tensor(q_out, "q_out", torch.bfloat16, (T, Hq, D), dev, rows=True)
+        ldq = _rows(q_out, "q_out", torch.bfloat16, (T, Hq, D), dev)
     if T:
-        _call(dev, "okc_rope_axes_kv_append", qkv.data_ptr(), _ld(qkv), positions.data_ptr(), _ld(positions),
-              positions.shape[0], axes, inv_freq.data_ptr(), len(axes), int(half), cu_q.data_ptr(),
-              seq_lens.data_ptr(), B, page_table.data_ptr(), _ld(page_table), page_table.shape[1],
-              k_scale.data_ptr(), v_scale.data_ptr(), q_out.data_ptr(), _ld(q_out), k_cache.data_ptr(),
-              v_cache.data_ptr(), T, Hq, Hkv, D, P, pages, _error_word(dev, "rope_axes"))
+        _call(dev, _LIB.okc_rope_axes_kv_append, "okc_rope_axes_kv_append", qkv.data_ptr(), ldqkv, positions.data_ptr(),
+              ld_pos, A, axes, freq, R, int(half), cq, sl, B, table, table_ld, cols, ks, vs, q_out.data_ptr(), ldq,
+              kc, vc, T, Hq, Hkv, D, P, pages, _error_word(dev, "rope_axes"))
     return q_out
 
 
@@ -583,33 +592,28 @@ def attn_chunk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     dev = _dev_index(q)
     if q.dim() != 3:
         raise _lib.OkcError(f"q: expected [T, Hq, D], got {tuple(q.shape)}")
-    T, Hq, D = q.shape
-    _tensor(q, "q", torch.bfloat16, (T, Hq, D), dev, rows=True)
-    B = _ragged(cu_q, seq_lens, page_table, dev)
-    pages, P, Hkv = _caches(k_cache, v_cache, k_scale, v_scale, None, D, dev)
+    T, Hq, D = shape = tuple(q.shape)
+    ldq = _rows(q, "q", torch.bfloat16, shape, dev)
+    cq, sl, B, table, table_ld, cols = _ragged(cu_q, seq_lens, page_table, dev)
+    kc, vc, ks, vs, pages, P, Hkv = _caches(k_cache, v_cache, k_scale, v_scale, None, D, dev)
     sp = pp = dp = None
     if slopes is not None:
-        _tensor(slopes, "slopes", torch.float32, (Hq,), dev)
-        sp = slopes.data_ptr()
+        sp = _dense(slopes, "slopes", torch.float32, (Hq,), dev)
     if prefix_lens is not None:
-        _tensor(prefix_lens, "prefix_lens", torch.int32, (B,), dev)
-        pp = prefix_lens.data_ptr()
+        pp = _dense(prefix_lens, "prefix_lens", torch.int32, (B,), dev)
     if doc_start is not None:
-        _tensor(doc_start, "doc_start", torch.int32, (T,), dev)
-        dp = doc_start.data_ptr()
+        dp = _dense(doc_start, "doc_start", torch.int32, (T,), dev)
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=q.device)
+        out, ldo = q.new_empty(shape), Hq * D
     else:
-        _tensor(out, "out", torch.bfloat16, (T, Hq, D), dev, rows=True)
-    if not T:
-        return out
-    error = _error_word(dev, "attn_chunk")
-    nbytes = _lib.load().okc_attn_chunk_workspace_bytes(T, B, Hq, Hkv, D)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    _call(dev, "okc_attn_chunk_fp8", q.data_ptr(), _ld(q), k_cache.data_ptr(), v_cache.data_ptr(),
-          page_table.data_ptr(), _ld(page_table), page_table.shape[1], cu_q.data_ptr(), seq_lens.data_ptr(),
-          k_scale.data_ptr(), v_scale.data_ptr(), sp, pp, dp, out.data_ptr(), _ld(out), T, B, Hq, Hkv, D, P, pages,
-          float(sm_scale), float(softcap), int(window), int(max_q or 0), ws.data_ptr(), nbytes, error)
+        ldo = _rows(out, "out", torch.bfloat16, shape, dev)
+    if T:
+        error = _error_word(dev, "attn_chunk")
+        nbytes = _LIB.okc_attn_chunk_workspace_bytes(T, B, Hq, Hkv, D)
+        ws = q.new_empty(nbytes, dtype=torch.uint8)
+        _call(dev, _LIB.okc_attn_chunk_fp8, "okc_attn_chunk_fp8", q.data_ptr(), ldq, kc, vc, table, table_ld, cols, cq,
+              sl, ks, vs, sp, pp, dp, out.data_ptr(), ldo, T, B, Hq, Hkv, D, P, pages, sm_scale, softcap, window,
+              max_q or 0, ws.data_ptr(), nbytes, error)
     return out
 
 
