@@ -23,7 +23,8 @@ namespace okc {
 
 namespace {
 
-constexpr int kStages = 3;
+constexpr int kMaxStages = 5;
+constexpr int kRing = 192 * 1024;  // as many stages as fit: 3 of 256 channels, 4 of up to 128
 constexpr int kPanels = 2;       // 128-byte K panels of a stage: one barrier and one commit for eight MMAs
 constexpr int kSegment = 4;      // stages an accumulator takes, for an fp32 output
 constexpr int kDrainWarps = 8;   // a CTA's
@@ -37,10 +38,10 @@ constexpr int kGroup = 8;        // token tiles of a group
 struct TallSmem {
   static constexpr int A_PANEL = 128 * LIN_KB;       // this CTA's 128 token rows
   static constexpr int B_PANEL = 128 * LIN_KB;       // its channel rows, at most
-  static constexpr int STAGE = kPanels * (A_PANEL + B_PANEL);
+  static_assert(kRing >= 3 * kPanels * (A_PANEL + B_PANEL), "three of the widest stages");
   static constexpr int BLOCK = 32 * 32;              // a 32 x 32 fp32 block per draining warp
   static constexpr int TURN = kDrainWarps * BLOCK * 4;
-  static constexpr int BAR0 = STAGE * kStages + TURN;
+  static constexpr int BAR0 = kRing + TURN;
   static constexpr int TOTAL = 1024 + BAR0 + 256;
 };
 
@@ -203,10 +204,10 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
   using C = TallSmem;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* turn = reinterpret_cast<float*>(smem + C::STAGE * kStages);
+  float* turn = reinterpret_cast<float*>(smem + kRing);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR0);  // the leader's count both CTAs' bytes
-  uint64_t* empty = full + kStages;
-  uint64_t* accf = empty + kStages;
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* accf = empty + kMaxStages;
   uint64_t* acce = accf + 2;  // the leader's count both CTAs' draining warps
   uint64_t* drain = acce + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -217,11 +218,12 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
   constexpr int KE = E4M3 ? LIN_KB : LIN_KB / 2;  // K elements of a panel
   const int nkb = (a.K + KE * kPanels - 1) / (KE * kPanels);
   const int mt = (a.M + 255) / 256, nt = (a.N + bn - 1) / bn, tiles = mt * nt;
+  const int b_panel = bn / 2 * LIN_KB, stage = kPanels * (C::A_PANEL + b_panel), stages = min(kMaxStages, kRing / stage);
   const int u_first = blockIdx.x >> 1, u_step = gridDim.x >> 1;
 
   pdl_trigger();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kMaxStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -248,59 +250,66 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
     if constexpr (OUT32) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
     if (warp == 0 && lane == 0) {
       const int half = bn / 2;
-      const uint32_t bytes = 2 * kPanels * (C::A_PANEL + half * LIN_KB);
-      int it = 0;
+      int it = 0, s = 0;
+      uint32_t ph = 0;
       bool ok = true;
       for (int u = u_first; u < tiles && ok; u += u_step) {
         int tm, tn;
         lin_tile(u, mt, nt, tm, tn);
         for (int kb = 0; kb < nkb; ++kb, ++it) {
-          const int s = it % kStages;
-          if (!mbar_wait(&empty[s], ((uint32_t)(it / kStages) & 1u) ^ 1u, a.err, abort_flag)) {
+          if (!mbar_wait(&empty[s], ph ^ 1u, a.err, abort_flag)) {
             ok = false;
             break;
           }
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
-          uint8_t* sa = smem + s * C::STAGE;
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * stage);
+          uint8_t* sa = smem + s * stage;
           const uint32_t bar = in_leader(&full[s]);
 #pragma unroll
           for (int p = 0; p < kPanels; ++p) {
             const int k = (kb * kPanels + p) * KE;
             tma_load_pair(sa + p * C::A_PANEL, &map_x, k, tm * 256 + (int)rank * 128, bar);
-            tma_load_pair(sa + kPanels * C::A_PANEL + p * C::B_PANEL, &map_w, k, tn * bn + (int)rank * half, bar);
+            tma_load_pair(sa + kPanels * C::A_PANEL + p * b_panel, &map_w, k, tn * bn + (int)rank * half, bar);
+          }
+          if (++s == stages) {
+            s = 0;
+            ph ^= 1u;
           }
         }
       }
       if (!ok) *abort_flag = 1;
       // a stage is left once its MMAs are done, so no copy is in flight after these waits (where a
       // role gave up, it waited for longer than any copy takes)
-      for (int i = max(0, it - kStages); i < it; ++i)
-        if (!mbar_wait(&empty[i % kStages], (uint32_t)(i / kStages) & 1u, a.err, abort_flag)) break;
+      for (int i = max(0, it - stages); i < it; ++i)
+        if (!mbar_wait(&empty[i % stages], (uint32_t)(i / stages) & 1u, a.err, abort_flag)) break;
     } else if (warp == 1 && lane == 0 && rank == 0) {
       const uint32_t idesc = lin_idesc(E4M3, 256, bn);
-      int it = 0, seg = 0;
+      int s = 0, seg = 0;
+      uint32_t ph = 0;
       bool ok = true;
       for (int u = u_first; u < tiles && ok; u += u_step) {
-        for (int kb = 0; kb < nkb; ++kb, ++it) {
+        for (int kb = 0; kb < nkb; ++kb) {
           const int buf = seg & 1;
           const bool begin = OUT32 ? kb % kSegment == 0 : kb == 0;
           if (begin) {
             ok = mbar_wait(&acce[buf], ((uint32_t)(seg >> 1) & 1u) ^ 1u, a.err, abort_flag);
             if (!ok) break;
           }
-          const int s = it % kStages;
-          ok = mbar_wait(&full[s], (uint32_t)(it / kStages) & 1u, a.err, abort_flag);
+          ok = mbar_wait(&full[s], ph, a.err, abort_flag);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t sa = smem_u32(smem + s * C::STAGE);
+          const uint32_t sa = smem_u32(smem + s * stage);
           const uint64_t da = umma_desc_sw128(sa), db = umma_desc_sw128(sa + kPanels * C::A_PANEL);
 #pragma unroll
           for (int p = 0; p < kPanels; ++p)
 #pragma unroll
             for (int j = 0; j < LIN_KB / 32; ++j)
               pair_mma<E4M3>(tmem + buf * 256, da + ((p * C::A_PANEL + 32 * j) >> 4),
-                             db + ((p * C::B_PANEL + 32 * j) >> 4), idesc, !(begin && p == 0 && j == 0));
+                             db + ((p * b_panel + 32 * j) >> 4), idesc, !(begin && p == 0 && j == 0));
           pair_commit(&empty[s]);
+          if (++s == stages) {
+            s = 0;
+            ph ^= 1u;
+          }
           if (kb == nkb - 1 || (OUT32 && kb % kSegment == kSegment - 1)) {
             pair_commit(&accf[buf]);
             ++seg;
@@ -336,6 +345,11 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
       lin_tile(u, mt, nt, tm, tn);
       const int m0 = tm * 256 + (int)rank * 128 + q4 * 32, rows = min(32, a.M - m0);
       const float my_sx = lane < rows ? lin_row_scale(a, m0 + lane) : 0.f;
+      if (a.res && lane < rows) {  // this lane's row of the residual, into L2 while the products run
+        const int re = a.res_fp32 ? 4 : 2, n0 = tn * bn + c_first * 32, cols = min(c_n * 32, a.N - n0);
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(a.res) + ((size_t)(m0 + lane) * a.ldr + n0) * re;
+        for (int i = 0; i < cols * re; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
+      }
       auto emit = [&](int c) {
         const int n0 = tn * bn + (c_first + c) * 32;
         __syncwarp();
@@ -433,8 +447,17 @@ int launch_tall(const LinearArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
+// Up to 128 tokens the K-split kernel; beyond, the kernel whose estimate is shorter.  A stage of the
+// K-split kernel's 128 x 128 tiles takes 0.68 us (its ends count as eight), one of a pair's tiles 0.46 us
+// up to 128 channels and 0.58 us at 256, besides 4.5 us at the ends (measured from 192 to 1024 tokens, N 256 to 8192,
+// K 1024 to 8192: the estimate picks the faster one or is within 10%.  256 tokens, N = 256,
+// K = 8192 in bf16: 34.6 us on pairs, 11.5 us split; 512 x 8192 x 8192: 57 and 88 us).
 int launch_linear(const LinearArgs& a, cudaStream_t stream) {
-  if (a.M <= kSplitTokens) return launch_linear_split(a, stream);
+  if (a.M <= 128) return launch_linear_split(a, stream);
+  const int pairs = okc_host::num_sms() / 2, bn = tall_bn(a.M, a.N, pairs);
+  const long long tiles = (long long)((a.M + 255) / 256) * ((a.N + bn - 1) / bn);
+  const double tall = 4.5 + (double)((tiles + pairs - 1) / pairs) * lin_stages(a) * (bn <= 128 ? 0.46 : 0.34 + 0.00094 * bn);
+  if (tiles <= pairs && 0.68 * linear_split_stages(a) < tall) return launch_linear_split(a, stream);
   if (a.out_fp32) return a.e4m3 ? launch_tall<true, true>(a, stream) : launch_tall<false, true>(a, stream);
   return a.e4m3 ? launch_tall<true, false>(a, stream) : launch_tall<false, false>(a, stream);
 }

@@ -13,8 +13,11 @@ namespace okc {
 
 constexpr int LIN_KB = 128;  // bytes of a row per K block
 
-// Up to this many tokens the K-split kernel (linear_split.cu), the CTA-pair kernel (linear.cu) beyond.
-constexpr int kSplitTokens = 128;
+// Both kernels take K in stages of 256 bytes a row.
+inline int lin_stages(const LinearArgs& a) { return (int)(((long long)a.K * (a.e4m3 ? 1 : 2) + 255) / 256); }
+
+// Stages that the K-split kernel (linear_split.cu) runs one after the other for this projection.
+int linear_split_stages(const LinearArgs& a);
 
 // D fp32, both operands K-major, M x N; e4m3 (kind::f8f6f4, type code 0) or bf16 (kind::f16, type code 1).
 __host__ __device__ constexpr uint32_t lin_idesc(bool e4m3, int m, int n) {

@@ -2,8 +2,8 @@
 // side, so one CTA tile covers 128 channels x up to BN tokens and the weight is read once.
 //
 // HBM-bound on the weight stream (N K bytes in e4m3).
-//  * K is split over the S CTAs of a cluster, S the largest of 1, 2, 4, 8 whose CTAs are all resident
-//    at once (every CTA then streams at the same rate whatever N is), so that the whole card reads;
+//  * K is split over the S = 1, 2, 4 or 8 CTAs of a cluster, chosen so that the waves of resident clusters
+//    times a CTA's stages (and ends) are fewest: the whole card reads whatever N is;
 //  * warp 0 streams K blocks of 256 bytes a weight row with TMA into a ring, warp 1 issues the
 //    MMAs, warps 2-9 drain the accumulator; for an fp32 output every kSplitSegment stages, summed in
 //    registers, because the MMA truncates as it accumulates;
@@ -36,11 +36,15 @@ struct SplitCfg {
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t local, uint32_t rank) {
-  uint32_t addr;
+// A float of CTA `rank`'s shared memory at this CTA's address `local`; 0 where !on.
+__device__ __forceinline__ float ld_cluster(uint32_t local, uint32_t rank, bool on) {
   float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(local), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b32 a;\n setp.ne.b32 p, %3, 0;\n mov.f32 %0, 0f00000000;\n"
+      " mapa.shared::cluster.u32 a, %1, %2;\n @p ld.shared::cluster.f32 %0, [a];\n}\n"
+      : "=f"(v)
+      : "r"(local), "r"(rank), "r"((uint32_t)on)
+      : "memory");
   return v;
 }
 
@@ -201,7 +205,9 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
     const int live = min(BN, a.M - m0);
     const float sw = n < a.N ? lin_col_scale(a, n) : 0.f;
     const float bias = n < a.N && a.bias ? __bfloat162float(a.bias[n]) : 0.f;
-    constexpr int U = 8, oe = OUT32 ? 4 : 2;
+    // a thread's tokens in flight; few for small tiles, whose time is the cold fetch of this code
+    // (1 x 10240 x 8192: 16.9 us with short code, 20.4 us with eight tokens unrolled)
+    constexpr int U = BN / 16, oe = OUT32 ? 4 : 2;
     for (int m1 = rank + (t >> 7) * S; m1 < live; m1 += 2 * U * S) {
       float v[U], r[U], sx[U];
 #pragma unroll
@@ -223,8 +229,8 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
       for (int s = 0; s < S; ++s) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-          const int m = min(m1 + 2 * i * S, live - 1);
-          v[i] += ld_cluster(smem_u32(sums + m * 128 + ch), (uint32_t)s);
+          const int m = m1 + 2 * i * S;
+          v[i] += ld_cluster(smem_u32(sums) + (m * 128 + ch) * 4, (uint32_t)s, m < live);
         }
       }
 #pragma unroll
@@ -249,37 +255,89 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
   }
 }
 
+// Clusters of S CTAs that this device holds at once, asked once per kernel, S and device.  The query
+// answers for one CTA an SM (148 for S = 1); the tiles of up to 16 tokens fit twice.
 template <bool E4M3, bool OUT32, int BN>
-int launch_split_bn(const LinearArgs& a, cudaStream_t stream) {
+int resident_clusters(int S) {
+  static int known[64][9];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+  if (known[dev][S] == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(S, 1024);
+    cfg.blockDim = dim3(kSplitThreads);
+    cfg.dynamicSmemBytes = SplitCfg<BN>::SMEM;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = S;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, linear_split_kernel<E4M3, OUT32, BN>, &cfg) != cudaSuccess) cudaGetLastError();
+    constexpr int layers = 2 * (SplitCfg<BN>::SMEM + 1024) <= 228 * 1024 ? 2 : 1;
+    known[dev][S] = n > 0 ? n * layers : 1;
+  }
+  return known[dev][S];
+}
+
+// The K split of `tiles` tiles of `stages` stages: fewest stages in a row, a CTA's ends counted as
+// eight (one token, 28672 x 8192: 40 us as one wave of whole tiles, 52 us as four of a fifth each).
+// Powers of two only: clusters of 3, 5 and 7 left SMs idle (1 x 1280 x 8192: 6.2 us with 8, 11.9 with 7).
+template <bool E4M3, bool OUT32, int BN>
+int split_plan(long long tiles, int stages, int& S) {
+  long long best = -1;
+  for (int s = 1; s <= 8 && s <= stages; s *= 2) {
+    const long long n = resident_clusters<E4M3, OUT32, BN>(s);
+    const long long row = (tiles + n - 1) / n * ((stages + s - 1) / s + 8);
+    if (best < 0 || row < best) {
+      best = row;
+      S = s;
+    }
+  }
+  return best > 0x7fffffff ? 0x7fffffff : (int)best;
+}
+
+template <bool E4M3, bool OUT32, int BN>
+int launch_split_bn(const LinearArgs& a, int* stages_in_a_row, cudaStream_t stream) {
   using C = SplitCfg<BN>;
-  CUtensorMap mx, mw;
-  if (!lin_make_map(&mx, a.x, a.K, a.M, a.ldx, BN, E4M3) || !lin_make_map(&mw, a.w, a.K, a.N, a.ldw, 128, E4M3))
-    return OKC_ERR_INVALID;
   static okc_host::PerDevice configured;
   if (int st = configured.smem(linear_split_kernel<E4M3, OUT32, BN>, C::SMEM)) return st;
   const long long tiles = ((long long)a.N + 127) / 128, mt = (a.M + BN - 1) / BN;
   if (tiles > 65535 || mt > 65535) return OKC_ERR_TOO_LARGE;
-  const int resident = okc_host::num_sms() * (C::SMEM <= 113 * 1024 ? 2 : 1);
-  const int stages = (a.K * (E4M3 ? 1 : 2) + 255) / 256;
   int S = 1;
-  while (S < 8 && tiles * mt * 2 * S <= resident && stages >= 4 * S) S *= 2;
+  const int row = split_plan<E4M3, OUT32, BN>(tiles * mt, lin_stages(a), S);
+  if (stages_in_a_row) {
+    *stages_in_a_row = row;
+    return OKC_OK;
+  }
+  CUtensorMap mx, mw;
+  if (!lin_make_map(&mx, a.x, a.K, a.M, a.ldx, BN, E4M3) || !lin_make_map(&mw, a.w, a.K, a.N, a.ldw, 128, E4M3))
+    return OKC_ERR_INVALID;
   return okc_host::launch_k(linear_split_kernel<E4M3, OUT32, BN>, dim3(S, (unsigned)tiles, (unsigned)mt),
                             dim3(kSplitThreads), C::SMEM, stream, dim3(S), mx, mw, a);
 }
 
 template <bool E4M3, bool OUT32>
-int launch_split_t(const LinearArgs& a, cudaStream_t stream) {
-  if (a.M <= 16) return launch_split_bn<E4M3, OUT32, 16>(a, stream);
-  if (a.M <= 32) return launch_split_bn<E4M3, OUT32, 32>(a, stream);
-  if (a.M <= 64) return launch_split_bn<E4M3, OUT32, 64>(a, stream);
-  return launch_split_bn<E4M3, OUT32, 128>(a, stream);
+int launch_split_t(const LinearArgs& a, int* row, cudaStream_t stream) {
+  if (a.M <= 16) return launch_split_bn<E4M3, OUT32, 16>(a, row, stream);
+  if (a.M <= 32) return launch_split_bn<E4M3, OUT32, 32>(a, row, stream);
+  if (a.M <= 64) return launch_split_bn<E4M3, OUT32, 64>(a, row, stream);
+  return launch_split_bn<E4M3, OUT32, 128>(a, row, stream);
+}
+
+int dispatch(const LinearArgs& a, int* row, cudaStream_t stream) {
+  if (a.out_fp32) return a.e4m3 ? launch_split_t<true, true>(a, row, stream) : launch_split_t<false, true>(a, row, stream);
+  return a.e4m3 ? launch_split_t<true, false>(a, row, stream) : launch_split_t<false, false>(a, row, stream);
 }
 
 }  // namespace
 
-int launch_linear_split(const LinearArgs& a, cudaStream_t stream) {
-  if (a.out_fp32) return a.e4m3 ? launch_split_t<true, true>(a, stream) : launch_split_t<false, true>(a, stream);
-  return a.e4m3 ? launch_split_t<true, false>(a, stream) : launch_split_t<false, false>(a, stream);
+int linear_split_stages(const LinearArgs& a) {
+  int row = 0x7fffffff;
+  return dispatch(a, &row, nullptr) == OKC_OK ? row : 0x7fffffff;
 }
+
+int launch_linear_split(const LinearArgs& a, cudaStream_t stream) { return dispatch(a, nullptr, stream); }
 
 }  // namespace okc
