@@ -26,7 +26,8 @@ struct SplitCfg {
   static constexpr int A_PANEL = 128 * LIN_KB;
   static constexpr int B_PANEL = BN * LIN_KB;
   static constexpr int STAGE = kSplitPanels * (A_PANEL + B_PANEL);
-  static constexpr int STAGES = 3;
+  // up to 16 tokens two CTAs an SM of three stages each, beyond one of as many as fit
+  static constexpr int STAGES = BN <= 16 ? 3 : BN <= 32 ? 5 : BN <= 64 ? 4 : 3;
   static constexpr int BODY = STAGE * STAGES;
   static constexpr int SMEM = 1024 + BODY + 256;
   static constexpr int ACC = BN < 32 ? 32 : BN;  // TMEM columns of an accumulator
