@@ -15,6 +15,8 @@
 //    stays below 2^8 and a rescale is rare after the first blocks.
 // Blocks of a request are taken from its last rows on: the longest causal spans start first.  With few
 // blocks the keys are split over several, which leave fp32 partial sums for a merge.
+#include <type_traits>
+
 #include "chunk_common.cuh"
 #include "tcgen05.cuh"
 
@@ -26,7 +28,11 @@ constexpr int kTile = 128;                 // rows of a tile, keys of a block
 constexpr int kPair = 2 * kTile;           // rows of a CTA
 constexpr int kSoftmaxThreads = 256;
 constexpr int kLoadThreads = 128;
-constexpr int kTcThreads = kSoftmaxThreads + kLoadThreads + 32;
+constexpr int kTcThreads = kSoftmaxThreads + kLoadThreads + 128;  // the last warpgroup's first warp issues
+constexpr int kIssueWarp = (kSoftmaxThreads + kLoadThreads) / 32;
+// Registers a thread: the launch's, and how the warpgroups split them.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kLoadRegs = 120, kIssueRegs = 56;
+static_assert(2 * kSoftmaxRegs + kLoadRegs + kIssueRegs <= 4 * kLaunchRegs, "the split must fit the launch");
 constexpr float kSlack = 8.f;              // log2 growth of the maximum that O tolerates
 
 template <int D>
@@ -81,7 +87,57 @@ __device__ __forceinline__ void tm_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// Waits for this thread's loads; `r` is theirs, so that no use of it moves ahead of the wait.
+__device__ __forceinline__ void tm_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+// Two fp32 operations in one instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair2(float x, float y) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ f32x2 bits2(uint32_t x, uint32_t y) { return pair2(__uint_as_float(x), __uint_as_float(y)); }
+__device__ __forceinline__ float2 split2(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// tanh(x) / x for |x| <= 1 as a polynomial in x^2, fitted for the least |x * error| over that range
+// (2.4e-7; 3.2e-6 relative at 0): eight fused operations where the exponential and the
+// reciprocal of the exact form occupy the special-function unit twice.
+constexpr float kTanhRange = 1.f;
+__device__ __forceinline__ float tanh_coefficient(int k) {
+  return k == 0   ? 0.99999685f
+         : k == 1 ? -0.33324004f
+         : k == 2 ? 0.13253524f
+         : k == 3 ? -0.05097283f
+         : k == 4 ? 0.01611415f
+                  : -0.00283945f;
 }
 __device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -98,7 +154,7 @@ __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_
 
 // Barriers and words shared by the roles.
 struct TcShared {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drain;
+  uint64_t plan, q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drain;
   uint32_t tmem;
   int abort;
   int b, tile;             // the block's request (-1: none) and row tile pair
@@ -119,6 +175,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
 
   pdl_trigger();
   if (threadIdx.x == 0) {
+    mbar_init(&sh.plan, kSoftmaxThreads / 32);
     mbar_init(&sh.q_full, kSoftmaxThreads / 32);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.k_full[i], kLoadThreads / 32);
@@ -138,7 +195,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     sh.full_hi = 0x7fffffff;
     fence_mbar_init();
   }
-  if (warp == kTcThreads / 32 - 1) {
+  if (warp == kIssueWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -179,51 +236,58 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
   tc_before();
   __syncthreads();
   tc_after();
-  const uint32_t tmem = sh.tmem;
   const int b = sh.b;
-  Req rq = {};
-  int rows = 0, row0 = 0, r0 = 0;
-  if (b >= 0) {
-    rq = request(a, b);
-    rows = rq.n * a.G;
-    row0 = a.cu_q[b];
-    r0 = sh.tile * kPair;
-  }
-  // a softmax thread's row
-  RowSpan me = {0, 0, 0};
-  const int r = r0 + threadIdx.x;
-  const bool live = threadIdx.x < kSoftmaxThreads && r < rows;
-  const int tok = live ? row0 + r / a.G : 0, hq = live ? head * a.G + r % a.G : 0;
-  if (live) me = row_span(a, rq, row0, r / a.G);
-  if (threadIdx.x < kSoftmaxThreads) {
-    const int lo = __reduce_min_sync(0xffffffffu, live && me.lo < me.hi ? me.lo : 0x7fffffff);
-    const int hi = __reduce_max_sync(0xffffffffu, live && me.lo < me.hi ? me.hi : 0);
-    const int flo = __reduce_max_sync(0xffffffffu, live ? me.lo : 0);
-    const int fhi = __reduce_min_sync(0xffffffffu, live ? me.hi : 0x7fffffff);
-    if (lane == 0) {
-      atomicMin(&sh.lo, lo);
-      atomicMax(&sh.hi, hi);
-      atomicMax(&sh.full_lo, flo);
-      atomicMin(&sh.full_hi, fhi);
-    }
-  }
-  __syncthreads();
-  // this split's key blocks
-  const int k_lo = sh.lo, k_hi = sh.hi;
-  int nb = k_hi > k_lo ? (k_hi - k_lo + kTile - 1) / kTile : 0, first = 0;
-  if (pl.splits > 1) {
-    const int per = (nb + pl.splits - 1) / pl.splits;
-    first = min(nb, split * per);
-    nb = min(nb, first + per) - first;
-  }
-  const int key0 = k_lo + first * kTile;
-  const bool two = rows - r0 > kTile;
   volatile int* abort_flag = &sh.abort;
+  // The union of the rows' intervals, once the softmax threads have published it, gives the keys:
+  // this split's first one, and its blocks.
+  auto plan = [&](int& key0, int& k_hi) -> int {
+    if (!mbar_wait(&sh.plan, 0, a.err, abort_flag)) *abort_flag = 1;
+    const int k_lo = *reinterpret_cast<volatile int*>(&sh.lo);
+    k_hi = *reinterpret_cast<volatile int*>(&sh.hi);
+    int nb = k_hi > k_lo ? (k_hi - k_lo + kTile - 1) / kTile : 0, first = 0;
+    if (pl.splits > 1) {
+      const int per = (nb + pl.splits - 1) / pl.splits;
+      first = min(nb, split * per);
+      nb = min(nb, first + per) - first;
+    }
+    key0 = k_lo + first * kTile;
+    return nb;
+  };
 
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ------------------------------------------------------------------ softmax
+    const uint32_t tmem = sh.tmem;
+    Req rq = {};
+    int rows = 0, row0 = 0;
+    const int r0 = sh.tile * kPair, r = r0 + threadIdx.x;
+    if (b >= 0) {
+      rq = request(a, b);
+      rows = rq.n * a.G;
+      row0 = a.cu_q[b];
+    }
+    const bool live = r < rows;
+    const int tok = live ? row0 + r / a.G : 0, hq = live ? head * a.G + r % a.G : 0;
+    RowSpan me = {0, 0, 0};
+    if (live) me = row_span(a, rq, row0, r / a.G);
+    {
+      const int lo = __reduce_min_sync(0xffffffffu, live && me.lo < me.hi ? me.lo : 0x7fffffff);
+      const int hi = __reduce_max_sync(0xffffffffu, live && me.lo < me.hi ? me.hi : 0);
+      const int flo = __reduce_max_sync(0xffffffffu, live ? me.lo : 0);
+      const int fhi = __reduce_min_sync(0xffffffffu, live ? me.hi : 0x7fffffff);
+      if (lane == 0) {
+        atomicMin(&sh.lo, lo);
+        atomicMax(&sh.hi, hi);
+        atomicMax(&sh.full_lo, flo);
+        atomicMin(&sh.full_hi, fhi);
+        mbar_arrive(&sh.plan);
+      }
+      __syncwarp();
+    }
+    int key0, k_hi;
+    const int nb = plan(key0, k_hi);
     const int w = warp >> 2;  // tile
-    const bool on = w == 0 || two;
+    const bool on = w == 0 || rows - r0 > kTile;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + w * kTile, to = tmem + lanes + 2 * kTile + w * D;
     float fac = 0.f, slope = 0.f, m_ref = -INFINITY, l = 0.f;
@@ -231,6 +295,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) nan_d[i] = 0;
     const float cap2 = CAP ? a.softcap * 1.4426950408889634f : 0.f;
+    float fac_poly = 0.f, tanh_c[6];  // raw sum -> argument of tanh; cap2 times its polynomial
+#pragma unroll
+    for (int k = 0; k < 6; ++k) tanh_c[k] = cap2 * tanh_coefficient(k);
     if (nb > 0 && on) {
       // the row in f16, scaled by a power of two, into the swizzled panels
       uint4 qv[D / 8];
@@ -248,6 +315,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       // a negative factor goes into the query, so that the largest score is the largest sum
       const float down = fac < 0.f ? -pow2(-shf) : pow2(-shf);
       fac = fabsf(fac);
+      fac_poly = fac * 0.34657359027997264f;  // fac carries 2 log2(e)
       if (BIAS && live) slope = a.slopes[hq] * 1.4426950408889634f;
       uint8_t* qs = smem + C::Q0 + w * C::TILE_B;
       const int lr = threadIdx.x & (kTile - 1);
@@ -275,32 +343,73 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       }
       tc_after();
       const bool edge = !__all_sync(0xffffffffu, !live || (me.lo <= kb && me.hi >= kb + kTile));
-      // the log2 score of raw sum v at key kb + c is u * f, or with a distance bias u * f - slope * distance
+      // visible columns [vis_lo, vis_lo + vis_n)
+      const int vis_lo = live ? me.lo - kb : 0;
+      const unsigned vis_n = live ? max(0, me.hi - me.lo) : 0;
+      // The log2 score of raw sum v at key kb + c is u * f, u = v or its capped form, with a bias less
+      // slope * |ahead - c|.  A block all of whose keys lie behind its rows needs no absolute value.
       const float f = CAP ? cap2 : fac;
-      auto unit = [&](float v) -> float { return CAP ? tanh_from_2l2e(v * fac) : v; };
-      auto biased = [&](float v, int c) -> float {
-        return fmaf(unit(v), f, -__fmul_rn(slope, (float)abs(me.pos - (kb + c))));
+      const float ahead = (float)(me.pos - kb);
+      const bool behind = BIAS && __all_sync(0xffffffffu, !live || me.pos >= kb + kTile - 1);
+      const f32x2 slope2 = pair2(slope, slope), base2 = pair2(-slope * ahead, -slope * ahead);
+      auto exact_unit = [&](float v) -> float { return CAP ? tanh_from_2l2e(v * fac) : v; };
+      auto bias2 = [&](int c) -> f32x2 {  // of columns c and c + 1
+        if (behind) return fma2(pair2((float)c, (float)(c + 1)), slope2, base2);
+        return pair2(-slope * fabsf(ahead - (float)c), -slope * fabsf(ahead - (float)(c + 1)));
       };
-      const int vis_lo = live ? me.lo - kb : 0, vis_n = live ? me.hi - me.lo : 0;  // visible columns [vis_lo, vis_lo + vis_n)
-      // ---- the row's maximum over the block ----
-      float mx = -INFINITY;
-#pragma unroll 1
-      for (int c0 = 0; c0 < kTile; c0 += 32) {
-        uint32_t v[32];
-        tm_ld32(ts + c0, v);
+      auto biased2 = [&](uint32_t v0, uint32_t v1, int c) -> f32x2 {
+        return fma2(pair2(exact_unit(__uint_as_float(v0)), exact_unit(__uint_as_float(v1))), pair2(f, f), bias2(c));
+      };
+      auto seen = [&](int c) { return (unsigned)(c - vis_lo) < vis_n; };
+
+      // ---- the row's maximum over the block; with a cap also the largest magnitude ----
+      float mx = -INFINITY, mag = 0.f;
+      auto maximum = [&](auto masked, const uint32_t (&v)[32], int c0) {
+        constexpr bool MASK = decltype(masked)::value;
+        float m0 = -INFINITY, m1 = -INFINITY, g0 = 0.f, g1 = 0.f;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          float x = __uint_as_float(v[c]);
-          if (BIAS) x = biased(x, c0 + c);
-          if (edge && !((unsigned)(c0 + c - vis_lo) < (unsigned)max(0, vis_n))) x = -INFINITY;
-          mx = fmaxf(mx, x);
+        for (int c = 0; c < 32; c += 2) {
+          float x = __uint_as_float(v[c]), y = __uint_as_float(v[c + 1]);
+          if (BIAS) {
+            const float2 b2 = split2(biased2(v[c], v[c + 1], c0 + c));
+            x = b2.x;
+            y = b2.y;
+          } else if (CAP) {
+            g0 = fmaxf(g0, fabsf(x));
+            g1 = fmaxf(g1, fabsf(y));
+          }
+          if (MASK) {
+            x = seen(c0 + c) ? x : -INFINITY;
+            y = seen(c0 + c + 1) ? y : -INFINITY;
+          }
+          m0 = fmaxf(m0, x);
+          m1 = fmaxf(m1, y);
         }
-      }
+        mx = fmaxf(mx, fmaxf(m0, m1));
+        mag = fmaxf(mag, fmaxf(g0, g1));
+      };
+      // walks the block in chunks of 32 columns, the next one's load in flight
+      auto walk = [&](auto&& chunk) {
+        uint32_t va[32], vb[32];
+        tm_ld32(ts, va);
+        tm_wait_ld(va);
+#pragma unroll
+        for (int c0 = 0; c0 < kTile; c0 += 64) {
+          tm_ld32(ts + c0 + 32, vb);
+          chunk(va, c0);
+          tm_wait_ld(vb);
+          if (c0 + 64 < kTile) tm_ld32(ts + c0 + 64, va);
+          chunk(vb, c0 + 32);
+          if (c0 + 64 < kTile) tm_wait_ld(va);
+        }
+      };
+      if (edge)
+        walk([&](const uint32_t(&v)[32], int c0) { maximum(std::true_type(), v, c0); });
+      else
+        walk([&](const uint32_t(&v)[32], int c0) { maximum(std::false_type(), v, c0); });
       // without a bias the score grows with the raw sum; rounded up, so that no fused u * f - org is positive
-      if (!BIAS && mx != -INFINITY) mx = __fmul_ru(unit(mx), f);
-      if (m_ref == -INFINITY) {
-        m_ref = mx;  // nothing before it: O and l are zero
-      }
+      if (!BIAS && mx != -INFINITY) mx = __fmul_ru(exact_unit(mx), f);
+      if (m_ref == -INFINITY) m_ref = mx;  // nothing before it: O and l are zero
       const bool grow = mx > m_ref + kSlack;
       if (__any_sync(0xffffffffu, grow)) {
         // the block before is complete: its product was issued before this block's scores
@@ -311,6 +420,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
         for (int c0 = 0; c0 < D; c0 += 32) {
           uint32_t v[32];
           tm_ld32(to + c0, v);
+          tm_wait_ld(v);
           uint32_t o[16];
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh) {
@@ -322,26 +432,52 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       }
       const float org = m_ref == -INFINITY ? 0.f : m_ref;
       // ---- P = 2^(score - org), as f16 over the scores ----
-#pragma unroll 1
-      for (int c0 = 0; c0 < kTile; c0 += 32) {
-        uint32_t v[32], o[16];
-        tm_ld32(ts + c0, v);
-        float sum = 0.f;
+      const f32x2 org2 = pair2(-org, -org), f2 = pair2(f, f);
+      f32x2 sum2 = pair2(0.f, 0.f);
+      auto exponentials = [&](auto masked, auto poly, const uint32_t (&v)[32], int c0) {
+        constexpr bool MASK = decltype(masked)::value, POLY = decltype(poly)::value;
+        uint32_t o[16];
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
-          float p[2];
+          f32x2 x2;
+          if constexpr (BIAS) {
+            x2 = add2(biased2(v[c], v[c + 1], c0 + c), org2);
+          } else if constexpr (POLY) {
+            const f32x2 z = mul2(bits2(v[c], v[c + 1]), pair2(fac_poly, fac_poly)), w2 = mul2(z, z);
+            f32x2 h = fma2(w2, pair2(tanh_c[5], tanh_c[5]), pair2(tanh_c[4], tanh_c[4]));
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float raw = __uint_as_float(v[c + i]);
-            p[i] = ex2(BIAS ? biased(raw, c0 + c + i) - org : fmaf(unit(raw), f, -org));
-            if (edge && !((unsigned)(c0 + c + i - vis_lo) < (unsigned)max(0, vis_n))) p[i] = 0.f;
+            for (int k = 3; k >= 0; --k) h = fma2(w2, h, pair2(tanh_c[k], tanh_c[k]));
+            x2 = fma2(z, h, org2);
+          } else {
+            x2 = fma2(pair2(exact_unit(__uint_as_float(v[c])), exact_unit(__uint_as_float(v[c + 1]))), f2, org2);
           }
-          sum += p[0] + p[1];
-          o[c / 2] = h2(p[0], p[1]);
+          float2 p = split2(x2);
+          p.x = ex2(p.x);
+          p.y = ex2(p.y);
+          if (MASK) {
+            p.x = seen(c0 + c) ? p.x : 0.f;
+            p.y = seen(c0 + c + 1) ? p.y : 0.f;
+          }
+          sum2 = add2(sum2, pair2(p.x, p.y));
+          o[c / 2] = h2(p.x, p.y);
         }
-        l += sum;
         tm_st16(ts + c0 / 2, o);
+      };
+      // the polynomial serves a warp whose rows' scores all lie in its range
+      const bool poly = CAP && !BIAS && __all_sync(0xffffffffu, mag * fac_poly <= kTanhRange);
+      if (edge) {
+        if (poly)
+          walk([&](const uint32_t(&v)[32], int c0) { exponentials(std::true_type(), std::integral_constant<bool, CAP && !BIAS>(), v, c0); });
+        else
+          walk([&](const uint32_t(&v)[32], int c0) { exponentials(std::true_type(), std::false_type(), v, c0); });
+      } else {
+        if (poly)
+          walk([&](const uint32_t(&v)[32], int c0) { exponentials(std::false_type(), std::integral_constant<bool, CAP && !BIAS>(), v, c0); });
+        else
+          walk([&](const uint32_t(&v)[32], int c0) { exponentials(std::false_type(), std::false_type(), v, c0); });
       }
+      const float2 sums = split2(sum2);
+      l += sums.x + sums.y;
       tm_wait_st();
       if (kb < sh.full_lo || kb + kTile > sh.full_hi) {  // as the loading warps decide it
         // NaN values of keys that some rows do not see were taken out of V: put them into the rows that do
@@ -379,6 +515,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       uint32_t v[32];
       if (have) {
         tm_ld32(to + c0, v);
+        tm_wait_ld(v);
       } else {
 #pragma unroll
         for (int c = 0; c < 32; ++c) v[c] = 0u;
@@ -410,9 +547,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
         }
       }
     }
-  } else if (warp < (kSoftmaxThreads + kLoadThreads) / 32) {
+  } else if (warp < kIssueWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
     // ------------------------------------------------------------------ keys and values
     const int lt = threadIdx.x - kSoftmaxThreads;  // 0 .. 127
+    int key0, k_hi;
+    const int nb = plan(key0, k_hi);
     const int f_lo = sh.full_lo, f_hi = sh.full_hi;
     auto offset = [&](int j) {  // where key j * 128 + lt lies; -1: reads zeros
       const int key = key0 + j * kTile + lt;
@@ -437,56 +577,58 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
           : "memory");
       return any != 0;
     };
-    // a thread's 16-byte chunks: eight lanes take four chunks of two neighbouring keys, which the
-    // swizzle puts into different banks
-    constexpr int NCH = D / 16, PER = kTile * NCH / kLoadThreads;
-    auto place = [&](int i, int& key, int& ch) {
-      const int u = i * kLoadThreads + lt;  // (key pair, chunk group of four, key of the pair, chunk)
-      ch = (u & 3) + 4 * ((u >> 3) % (NCH / 4));
-      key = 2 * (u / (2 * NCH)) + ((u >> 2) & 1);
-    };
-    auto store = [&](uint8_t* base, int key, int ch, const uint4& raw) {
-      const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
-      uint32_t o[8];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        o[2 * k] = e4m3x2_h2(x[k] & 0xffffu);
-        o[2 * k + 1] = e4m3x2_h2(x[k] >> 16);
-      }
-      uint8_t* row = base + (ch / 4) * C::SUB + key * 128;
-      const int c8 = 2 * (ch % 4);
-      *reinterpret_cast<uint4*>(row + ((c8 ^ (key & 7)) * 16)) = make_uint4(o[0], o[1], o[2], o[3]);
-      *reinterpret_cast<uint4*>(row + (((c8 + 1) ^ (key & 7)) * 16)) = make_uint4(o[4], o[5], o[6], o[7]);
-    };
-    offset(0);
-    sync_any(false);
-    for (int j = 0; j < nb; ++j) {
-      uint4 kr[PER], vr[PER];
+    // A thread's 16-byte chunks: chunk `ch` of every KSTEP-th key from `kf` on.  Eight lanes take four
+    // chunks of two neighbouring keys, which the swizzle puts into different banks.
+    constexpr int NCH = D / 16, PER = kTile * NCH / kLoadThreads, KSTEP = kTile / PER;
+    const int ch = NCH == 8 ? (lt & 3) + 4 * ((lt >> 3) & 1) : lt & 3;
+    const int kf = 2 * (lt / (2 * NCH)) + ((lt >> 2) & 1);
+    static_assert(KSTEP % 8 == 0, "a thread's keys share a swizzle");
+    const int at0 = (ch / 4) * C::SUB + kf * 128 + (((2 * (ch % 4)) ^ (kf & 7)) * 16);
+    const int at1 = (ch / 4) * C::SUB + kf * 128 + (((2 * (ch % 4) + 1) ^ (kf & 7)) * 16);
+    auto store = [&](uint8_t* base, const uint4 (&r)[PER]) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        int key, ch;
-        place(i, key, ch);
-        const long long off = offs[(j & 1) * kTile + key];
-        kr[i] = vr[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (off >= 0) {
-          kr[i] = *reinterpret_cast<const uint4*>(a.k_cache + off + ch * 16);
-          vr[i] = *reinterpret_cast<const uint4*>(a.v_cache + off + ch * 16);
+        const uint32_t x[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+        uint32_t o[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          o[2 * k] = e4m3x2_h2(x[k] & 0xffffu);
+          o[2 * k + 1] = e4m3x2_h2(x[k] >> 16);
         }
+        *reinterpret_cast<uint4*>(base + at0 + i * KSTEP * 128) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(base + at1 + i * KSTEP * 128) = make_uint4(o[4], o[5], o[6], o[7]);
       }
+    };
+    // a block's K or V chunks of this thread, in flight until their conversion
+    auto fetch = [&](const uint8_t* cache, int j, uint4 (&r)[PER]) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const long long off = offs[(j & 1) * kTile + kf + i * KSTEP];
+        r[i] = off >= 0 ? *reinterpret_cast<const uint4*>(cache + off + ch * 16) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    };
+    uint4 kr[PER], vr[PER];
+    bool ok = true;
+    offset(0);
+    sync_any(false);
+    if (nb > 0) fetch(a.k_cache, 0, kr);
+    for (int j = 0; j < nb; ++j) {
+      fetch(a.v_cache, j, vr);
       offset(j + 1);
       const int st = j & 1;
       const uint32_t ph = ((uint32_t)(j >> 1) & 1u) ^ 1u;
-      bool ok = mbar_wait(&sh.k_empty[st], ph, a.err, abort_flag);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        int key, ch;
-        place(i, key, ch);
-        store(smem + C::K0 + st * C::TILE_B, key, ch, kr[i]);
-      }
+      const bool ok_k = mbar_wait(&sh.k_empty[st], ph, a.err, abort_flag);
+      store(smem + C::K0 + st * C::TILE_B, kr);
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.k_full[st]);
-      ok &= mbar_wait(&sh.v_empty[st], ph, a.err, abort_flag);
+      // the offsets of block j + 1 are there; those of block j are read
+      if (sync_any(!ok_k || !ok)) {
+        *abort_flag = 1;
+        break;
+      }
+      if (j + 1 < nb) fetch(a.k_cache, j + 1, kr);
+      ok = mbar_wait(&sh.v_empty[st], ph, a.err, abort_flag);  // the next block's barrier tells the others
       const int kb = key0 + j * kTile;
       const bool edge = kb < f_lo || kb + kTile > f_hi;
       if (edge) {
@@ -494,8 +636,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
         sync_any(false);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          int key, ch;
-          place(i, key, ch);
+          const int key = kf + i * KSTEP;
           uint32_t x[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w}, bad = 0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -507,78 +648,75 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
           vr[i] = make_uint4(x[0], x[1], x[2], x[3]);
         }
       }
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        int key, ch;
-        place(i, key, ch);
-        store(smem + C::V0 + st * C::TILE_B, key, ch, vr[i]);
-      }
+      store(smem + C::V0 + st * C::TILE_B, vr);
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.v_full[st]);
-      // the offsets of block j + 1 are there, those of block j read
-      if (sync_any(!ok)) {
-        *abort_flag = 1;
-        break;
-      }
     }
-  } else if (lane == 0) {
-    // ------------------------------------------------------------------ MMA issue
-    const uint32_t id_s = umma_idesc_f16(kTile, false), id_o = umma_idesc_f16(D, true);
-    auto scores = [&](int w, int st) {
-      const uint64_t qa = umma_desc_sw128(smem_u32(smem + C::Q0 + w * C::TILE_B));
-      const uint64_t ka = umma_desc_sw128(smem_u32(smem + C::K0 + st * C::TILE_B));
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t at = ((k / 4) * C::SUB + (k % 4) * 32) >> 4;
-        umma_ss(tmem + w * kTile, qa + at, ka + at, id_s, k != 0);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+    if (warp == kIssueWarp && lane == 0) {
+      // ------------------------------------------------------------------ MMA issue
+      const uint32_t tmem = sh.tmem;
+      int key0, k_hi;
+      const int nb = plan(key0, k_hi);
+      const bool two = b >= 0 && (a.cu_q[b + 1] - a.cu_q[b]) * a.G - sh.tile * kPair > kTile;
+      const uint32_t id_s = umma_idesc_f16(kTile, false), id_o = umma_idesc_f16(D, true);
+      auto scores = [&](int w, int st) {
+        const uint64_t qa = umma_desc_sw128(smem_u32(smem + C::Q0 + w * C::TILE_B));
+        const uint64_t ka = umma_desc_sw128(smem_u32(smem + C::K0 + st * C::TILE_B));
+  #pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t at = ((k / 4) * C::SUB + (k % 4) * 32) >> 4;
+          umma_ss(tmem + w * kTile, qa + at, ka + at, id_s, k != 0);
+        }
+        umma_commit(&sh.s_full[w]);
+      };
+      auto output = [&](int w, int st, bool acc) {
+        const uint64_t va = umma_desc_mn(smem_u32(smem + C::V0 + st * C::TILE_B), C::SUB);
+  #pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          umma_ts(tmem + 2 * kTile + w * D, tmem + w * kTile + 8 * k, va + k * (2048 >> 4), id_o, acc || k != 0);
+      };
+      bool ok = nb == 0 || mbar_wait(&sh.q_full, 0, a.err, abort_flag);
+      if (ok && nb > 0) {
+        ok = mbar_wait(&sh.k_full[0], 0, a.err, abort_flag);
+        if (ok) {
+          tc_after();
+          scores(0, 0);
+          if (two) scores(1, 0);
+          umma_commit(&sh.k_empty[0]);
+        }
       }
-      umma_commit(&sh.s_full[w]);
-    };
-    auto output = [&](int w, int st, bool acc) {
-      const uint64_t va = umma_desc_mn(smem_u32(smem + C::V0 + st * C::TILE_B), C::SUB);
-#pragma unroll
-      for (int k = 0; k < kTile / 16; ++k)
-        umma_ts(tmem + 2 * kTile + w * D, tmem + w * kTile + 8 * k, va + k * (2048 >> 4), id_o, acc || k != 0);
-    };
-    bool ok = nb == 0 || mbar_wait(&sh.q_full, 0, a.err, abort_flag);
-    if (ok && nb > 0) {
-      ok = mbar_wait(&sh.k_full[0], 0, a.err, abort_flag);
-      if (ok) {
-        tc_after();
-        scores(0, 0);
-        if (two) scores(1, 0);
-        umma_commit(&sh.k_empty[0]);
-      }
-    }
-    for (int j = 0; ok && j < nb; ++j) {
-      const int st = j & 1, nx = st ^ 1;
-      ok = mbar_wait(&sh.v_full[st], (uint32_t)(j >> 1) & 1u, a.err, abort_flag);
-      if (ok && j + 1 < nb) ok = mbar_wait(&sh.k_full[nx], (uint32_t)((j + 1) >> 1) & 1u, a.err, abort_flag);
-      for (int w = 0; ok && w < (two ? 2 : 1); ++w) {
-        ok = mbar_wait(&sh.p_full[w], (uint32_t)j & 1u, a.err, abort_flag);
+      for (int j = 0; ok && j < nb; ++j) {
+        const int st = j & 1, nx = st ^ 1;
+        ok = mbar_wait(&sh.v_full[st], (uint32_t)(j >> 1) & 1u, a.err, abort_flag);
+        if (ok && j + 1 < nb) ok = mbar_wait(&sh.k_full[nx], (uint32_t)((j + 1) >> 1) & 1u, a.err, abort_flag);
+        for (int w = 0; ok && w < (two ? 2 : 1); ++w) {
+          ok = mbar_wait(&sh.p_full[w], (uint32_t)j & 1u, a.err, abort_flag);
+          if (!ok) break;
+          tc_after();
+          output(w, st, j > 0);
+          if (j + 1 < nb)
+            scores(w, nx);  // over P, which the product above has read by then
+          else
+            umma_commit(&sh.o_full[w]);
+        }
         if (!ok) break;
-        tc_after();
-        output(w, st, j > 0);
-        if (j + 1 < nb)
-          scores(w, nx);  // over P, which the product above has read by then
-        else
-          umma_commit(&sh.o_full[w]);
+        umma_commit(&sh.v_empty[st]);
+        if (j + 1 < nb) umma_commit(&sh.k_empty[nx]);
       }
-      if (!ok) break;
-      umma_commit(&sh.v_empty[st]);
-      if (j + 1 < nb) umma_commit(&sh.k_empty[nx]);
+      if (!ok) *abort_flag = 1;
+      umma_commit(&sh.drain);  // no MMA may be in flight when the tensor memory is released
+      mbar_wait(&sh.drain, 0, a.err);
     }
-    if (!ok) *abort_flag = 1;
-    umma_commit(&sh.drain);  // no MMA may be in flight when the tensor memory is released
-    mbar_wait(&sh.drain, 0, a.err);
   }
 
   tc_before();
   __syncthreads();
-  if (warp == kTcThreads / 32 - 1) {
+  if (warp == kIssueWarp) {
     tc_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh.tmem));
   }
 }
 
@@ -636,7 +774,7 @@ template <int D, bool CAP, bool BIAS>
 int launch_tc(const ChunkArgs& a, const TcPlanA& pl, cudaStream_t stream) {
   using C = TcCfgA<D>;
   static okc_host::PerDevice configured;
-  if (int st = configured.smem(attn_chunk_tc_kernel<D, CAP, BIAS>, C::SMEM)) return st;
+  if (int st = configured.smem(attn_chunk_tc_kernel<D, CAP, BIAS>, C::SMEM, kLaunchRegs)) return st;
   const long long tiles = tc_tiles(a.T, a.B, a.G);
   if (tiles > 65535) return OKC_ERR_TOO_LARGE;
   if (int st = okc_host::launch_k(attn_chunk_tc_kernel<D, CAP, BIAS>, dim3(a.Hkv * pl.splits, (unsigned)tiles),
