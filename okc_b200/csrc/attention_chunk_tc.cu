@@ -5,14 +5,13 @@
 // Compute-bound: 4 D operations per (row, visible key) against 2 D cache bytes per key and 256 rows.
 // A block takes 256 rows (token-major, the G query heads of one KV head side by side) as two tiles
 // of 128 and streams the keys that any of them sees in blocks of 128:
-//  * two softmax warpgroups, one thread a row: S is read from tensor memory twice (the maximum, then the
-//    exponentials), P goes back over S as f16 and is the next product's A operand there.  A row's sums
-//    never leave its thread;
+//  * two softmax warpgroups, one thread a row: P goes back over S as f16 and is the next product's A
+//    operand there.  A row's sums never leave its thread;
 //  * four warps fetch key and value rows by page, turn e4m3 into f16 (exact) and store both as the
 //    swizzled rows that the MMAs read (keys K-major, values MN-major: no transpose);
-//  * one thread issues the MMAs: while one tile's softmax runs, the other tile's products do;
-//  * O is rescaled only when a row's maximum has grown by more than 2^8 since the last time, so P
-//    stays below 2^8 and a rescale is rare after the first blocks.
+//  * one thread issues the MMAs, the tiles in turn: while one tile's softmax runs, the other's products do;
+//  * a block's exponentials are taken against the maximum so far, in one pass over S, and done again with
+//    O rescaled only where a P exceeds 2^8: rare after a row's first block;
 // Blocks of a request are taken from its last rows on: the longest causal spans start first.  With few
 // blocks the keys are split over several, which leave fp32 partial sums for a merge.
 #include <type_traits>
@@ -28,12 +27,14 @@ constexpr int kTile = 128;                 // rows of a tile, keys of a block
 constexpr int kPair = 2 * kTile;           // rows of a CTA
 constexpr int kSoftmaxThreads = 256;
 constexpr int kLoadThreads = 128;
-constexpr int kTcThreads = kSoftmaxThreads + kLoadThreads + 128;  // the last warpgroup's first warp issues
-constexpr int kIssueWarp = (kSoftmaxThreads + kLoadThreads) / 32;
-// Registers a thread: the launch's, and how the warpgroups split them.
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kLoadRegs = 120, kIssueRegs = 56;
+constexpr int kIssueWarp = (kSoftmaxThreads + kLoadThreads) / 32;          // its warpgroup's other warps idle
+constexpr int kTcThreads = kSoftmaxThreads + kLoadThreads + 128;
+// Registers a thread: the launch's, and how the four warpgroups split them.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kLoadRegs = 112, kIssueRegs = 64;
 static_assert(2 * kSoftmaxRegs + kLoadRegs + kIssueRegs <= 4 * kLaunchRegs, "the split must fit the launch");
-constexpr float kSlack = 8.f;              // log2 growth of the maximum that O tolerates
+static_assert(kSoftmaxRegs > kLaunchRegs && kLoadRegs < kLaunchRegs && kIssueRegs < kLaunchRegs,
+              "setmaxnreg.inc raises and .dec lowers; the other way round is an illegal instruction");
+constexpr int kSlack = 8;                  // log2 growth of the maximum that O tolerates
 
 template <int D>
 struct TcCfgA {
@@ -43,8 +44,8 @@ struct TcCfgA {
   static constexpr int Q0 = 0;
   static constexpr int K0 = 2 * TILE_B;                // two K blocks
   static constexpr int V0 = K0 + 2 * TILE_B;           // two V blocks
-  static constexpr int OFF0 = V0 + 2 * TILE_B;         // [2][128] row offsets of the keys
-  static constexpr int BAR0 = OFF0 + 2 * kTile * 8;
+  static constexpr int OFF0 = V0 + 2 * TILE_B;         // [2][128] cache rows of the keys
+  static constexpr int BAR0 = OFF0 + 2 * kTile * 4;
   static constexpr int SMEM = 1024 + BAR0 + 512;
 };
 
@@ -98,6 +99,19 @@ __device__ __forceinline__ void tm_wait_ld(uint32_t (&r)[32]) {
                  "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
+__device__ __forceinline__ void tm_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tm_wait_ld(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+
 // Two fp32 operations in one instruction.
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pair2(float x, float y) {
@@ -131,15 +145,16 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
 // (2.4e-7; 3.2e-6 relative at 0): eight fused operations where the exponential and the
 // reciprocal of the exact form occupy the special-function unit twice.
 constexpr float kTanhRange = 1.f;
-__device__ __forceinline__ float tanh_coefficient(int k) {
-  return k == 0   ? 0.99999685f
+__device__ __forceinline__ f32x2 tanh2(int k) {
+  const float c = k == 0   ? 0.99999685f
          : k == 1 ? -0.33324004f
          : k == 2 ? 0.13253524f
          : k == 3 ? -0.05097283f
          : k == 4 ? 0.01611415f
                   : -0.00283945f;
+  return pair2(c, c);
 }
-__device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
           taddr),
@@ -169,7 +184,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   TcShared& sh = *reinterpret_cast<TcShared*>(smem + C::BAR0);
-  long long* offs = reinterpret_cast<long long*>(smem + C::OFF0);
   static_assert(sizeof(TcShared) <= 512, "barrier area");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -183,7 +197,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       mbar_init(&sh.v_full[i], kLoadThreads / 32);
       mbar_init(&sh.v_empty[i], 1);
       mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.p_full[i], kSoftmaxThreads / 64);
       mbar_init(&sh.o_full[i], 1);
       for (int w = 0; w < 4; ++w) sh.nan[i][w] = 0;
     }
@@ -254,13 +268,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     return nb;
   };
 
-  if (warp < 8) {
+  if (warp < kSoftmaxThreads / 32) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ------------------------------------------------------------------ softmax
-    const uint32_t tmem = sh.tmem;
+    const int w = warp >> 2, lr = (warp & 3) * 32 + lane;  // tile, row of it
     Req rq = {};
     int rows = 0, row0 = 0;
-    const int r0 = sh.tile * kPair, r = r0 + threadIdx.x;
+    const int r0 = sh.tile * kPair, r = r0 + w * kTile + lr;
     if (b >= 0) {
       rq = request(a, b);
       rows = rq.n * a.G;
@@ -286,47 +300,45 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     }
     int key0, k_hi;
     const int nb = plan(key0, k_hi);
-    const int w = warp >> 2;  // tile
     const bool on = w == 0 || rows - r0 > kTile;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + w * kTile, to = tmem + lanes + 2 * kTile + w * D;
+    const uint32_t lanes = sh.tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t ts = lanes + w * kTile, to = lanes + 2 * kTile + w * D;  // P lies over the first half of S
     float fac = 0.f, slope = 0.f, m_ref = -INFINITY, l = 0.f;
     uint32_t nan_d[D / 32];  // output columns that a visible NaN value reaches
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) nan_d[i] = 0;
     const float cap2 = CAP ? a.softcap * 1.4426950408889634f : 0.f;
-    float fac_poly = 0.f, tanh_c[6];  // raw sum -> argument of tanh; cap2 times its polynomial
+    f32x2 tanh_c[6];  // cap2 times the polynomial
 #pragma unroll
-    for (int k = 0; k < 6; ++k) tanh_c[k] = cap2 * tanh_coefficient(k);
+    for (int k = 0; k < 6; ++k) tanh_c[k] = mul2(tanh2(k), pair2(cap2, cap2));
     if (nb > 0 && on) {
       // the row in f16, scaled by a power of two, into the swizzled panels
-      uint4 qv[D / 8];
+      const __nv_bfloat16* qp = a.q + (size_t)tok * a.ldq + (size_t)hq * D;
       uint32_t top = 0;
+      if (live) {
+#pragma unroll 4
+        for (int i = 0; i < D / 8; ++i) {
+          const uint4 v = *reinterpret_cast<const uint4*>(qp + 8 * i);
+          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        qv[i] = live ? *reinterpret_cast<const uint4*>(a.q + (size_t)tok * a.ldq + (size_t)hq * D + 8 * i)
-                     : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t u[4] = {qv[i].x, qv[i].y, qv[i].z, qv[i].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
+          for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
+        }
       }
       const int shf = f16_shift(top);
       fac = a.k_scale[head] * a.sm_scale * (CAP ? 2.f / a.softcap : 1.f) * 1.4426950408889634f * pow2(shf);
       // a negative factor goes into the query, so that the largest score is the largest sum
       const float down = fac < 0.f ? -pow2(-shf) : pow2(-shf);
       fac = fabsf(fac);
-      fac_poly = fac * 0.34657359027997264f;  // fac carries 2 log2(e)
       if (BIAS && live) slope = a.slopes[hq] * 1.4426950408889634f;
-      uint8_t* qs = smem + C::Q0 + w * C::TILE_B;
-      const int lr = threadIdx.x & (kTile - 1);
-#pragma unroll
+      uint8_t* qs = smem + C::Q0 + w * C::TILE_B + lr * 128;
+#pragma unroll 4
       for (int i = 0; i < D / 8; ++i) {
-        const uint32_t u[4] = {qv[i].x, qv[i].y, qv[i].z, qv[i].w};
+        const uint4 v = live ? *reinterpret_cast<const uint4*>(qp + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
         uint32_t o[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = h2(bf16_lo(u[k]) * down, bf16_hi(u[k]) * down);
-        *reinterpret_cast<uint4*>(qs + (i / 8) * C::SUB + lr * 128 + (((i % 8) ^ (lr & 7)) * 16)) =
-            make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(qs + (i / 8) * C::SUB + (((i % 8) ^ (lr & 7)) * 16)) = make_uint4(o[0], o[1], o[2], o[3]);
       }
     }
     fence_async_smem();
@@ -334,150 +346,170 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     if (lane == 0) mbar_arrive(&sh.q_full);
 
     bool ok = true;
+    // keys from the last block on: under a distance bias the largest scores come first
     for (int j = 0; j < nb && on; ++j) {
-      const int kb = key0 + j * kTile;
-      ok = mbar_wait(&sh.s_full[w], (uint32_t)j & 1u, a.err, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) {
+      const int kb = key0 + (nb - 1 - j) * kTile;
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[w], (uint32_t)j & 1u, a.err, abort_flag));
+      if (!ok) {
         *abort_flag = 1;
         break;
       }
       tc_after();
       const bool edge = !__all_sync(0xffffffffu, !live || (me.lo <= kb && me.hi >= kb + kTile));
-      // visible columns [vis_lo, vis_lo + vis_n)
-      const int vis_lo = live ? me.lo - kb : 0;
-      const unsigned vis_n = live ? max(0, me.hi - me.lo) : 0;
+      // visible columns [vis_lo, vis_hi)
+      const int vis_lo = live ? me.lo - kb : 0, vis_hi = live ? me.hi - kb : 0;
+      auto seen = [&](int c) { return c >= vis_lo && c < vis_hi; };
       // The log2 score of raw sum v at key kb + c is u * f, u = v or its capped form, with a bias less
-      // slope * |ahead - c|.  A block all of whose keys lie behind its rows needs no absolute value.
+      // slope * |ahead - c|.  Where no visible key lies ahead of its row, no absolute value is needed.
       const float f = CAP ? cap2 : fac;
       const float ahead = (float)(me.pos - kb);
-      const bool behind = BIAS && __all_sync(0xffffffffu, !live || me.pos >= kb + kTile - 1);
-      const f32x2 slope2 = pair2(slope, slope), base2 = pair2(-slope * ahead, -slope * ahead);
+      const bool behind = BIAS && __all_sync(0xffffffffu, !live || min(me.hi, kb + kTile) - 1 <= me.pos);
       auto exact_unit = [&](float v) -> float { return CAP ? tanh_from_2l2e(v * fac) : v; };
-      auto bias2 = [&](int c) -> f32x2 {  // of columns c and c + 1
-        if (behind) return fma2(pair2((float)c, (float)(c + 1)), slope2, base2);
-        return pair2(-slope * fabsf(ahead - (float)c), -slope * fabsf(ahead - (float)(c + 1)));
-      };
-      auto biased2 = [&](uint32_t v0, uint32_t v1, int c) -> f32x2 {
-        return fma2(pair2(exact_unit(__uint_as_float(v0)), exact_unit(__uint_as_float(v1))), pair2(f, f), bias2(c));
-      };
-      auto seen = [&](int c) { return (unsigned)(c - vis_lo) < vis_n; };
+      auto bias = [&](int c) -> float { return -slope * fabsf(ahead - (float)c); };
 
-      // ---- the row's maximum over the block; with a cap also the largest magnitude ----
-      float mx = -INFINITY, mag = 0.f;
-      auto maximum = [&](auto masked, const uint32_t (&v)[32], int c0) {
-        constexpr bool MASK = decltype(masked)::value;
-        float m0 = -INFINITY, m1 = -INFINITY, g0 = 0.f, g1 = 0.f;
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          float x = __uint_as_float(v[c]), y = __uint_as_float(v[c + 1]);
-          if (BIAS) {
-            const float2 b2 = split2(biased2(v[c], v[c + 1], c0 + c));
-            x = b2.x;
-            y = b2.y;
-          } else if (CAP) {
-            g0 = fmaxf(g0, fabsf(x));
-            g1 = fmaxf(g1, fabsf(y));
-          }
-          if (MASK) {
-            x = seen(c0 + c) ? x : -INFINITY;
-            y = seen(c0 + c + 1) ? y : -INFINITY;
-          }
-          m0 = fmaxf(m0, x);
-          m1 = fmaxf(m1, y);
-        }
-        mx = fmaxf(mx, fmaxf(m0, m1));
-        mag = fmaxf(mag, fmaxf(g0, g1));
-      };
-      // walks the block in chunks of 32 columns, the next one's load in flight
-      auto walk = [&](auto&& chunk) {
-        uint32_t va[32], vb[32];
-        tm_ld32(ts, va);
-        tm_wait_ld(va);
-#pragma unroll
-        for (int c0 = 0; c0 < kTile; c0 += 64) {
-          tm_ld32(ts + c0 + 32, vb);
-          chunk(va, c0);
-          tm_wait_ld(vb);
-          if (c0 + 64 < kTile) tm_ld32(ts + c0 + 64, va);
-          chunk(vb, c0 + 32);
-          if (c0 + 64 < kTile) tm_wait_ld(va);
-        }
-      };
-      if (edge)
-        walk([&](const uint32_t(&v)[32], int c0) { maximum(std::true_type(), v, c0); });
-      else
-        walk([&](const uint32_t(&v)[32], int c0) { maximum(std::false_type(), v, c0); });
-      // without a bias the score grows with the raw sum; rounded up, so that no fused u * f - org is positive
-      if (!BIAS && mx != -INFINITY) mx = __fmul_ru(exact_unit(mx), f);
-      if (m_ref == -INFINITY) m_ref = mx;  // nothing before it: O and l are zero
-      const bool grow = mx > m_ref + kSlack;
-      if (__any_sync(0xffffffffu, grow)) {
-        // the block before is complete: its product was issued before this block's scores
-        const float down = grow ? ex2(m_ref - mx) : 1.f;
-        if (grow) m_ref = mx;
-        l *= down;
+      // Raises m_ref to the row's maximum over the columns from c_first on, with O, l and the P before
+      // c_first scaled down to it.
+      auto raise = [&](int c_first) {
+        float mx = -INFINITY;
 #pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += 32) {
-          uint32_t v[32];
-          tm_ld32(to + c0, v);
+        for (int c0 = c_first; c0 < kTile; c0 += 16) {
+          uint32_t v[16];
+          tm_ld16(ts + c0, v);
           tm_wait_ld(v);
-          uint32_t o[16];
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-#pragma unroll
-            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(v[16 * hh + c]) * down);
-            tm_st16(to + c0 + 16 * hh, o);
+          for (int c = 0; c < 16; ++c) {
+            float x = __uint_as_float(v[c]);
+            if (BIAS) x = fmaf(exact_unit(x), f, bias(c0 + c));
+            if (edge && !seen(c0 + c)) x = -INFINITY;
+            mx = fmaxf(mx, x);
           }
         }
-      }
-      const float org = m_ref == -INFINITY ? 0.f : m_ref;
-      // ---- P = 2^(score - org), as f16 over the scores ----
-      const f32x2 org2 = pair2(-org, -org), f2 = pair2(f, f);
-      f32x2 sum2 = pair2(0.f, 0.f);
-      auto exponentials = [&](auto masked, auto poly, const uint32_t (&v)[32], int c0) {
-        constexpr bool MASK = decltype(masked)::value, POLY = decltype(poly)::value;
-        uint32_t o[16];
+        // without a bias the score grows with the raw sum; rounded up, so that no fused u * f - org is positive
+        if (!BIAS && mx != -INFINITY) mx = __fmul_ru(exact_unit(mx), f);
+        const bool grow = mx > m_ref;
+        const bool scale = m_ref != -INFINITY && grow;  // from -infinity: O, l and P are zero
+        const float down = scale ? ex2(m_ref - mx) : 1.f;
+        if (grow) m_ref = mx;
+        if (!__any_sync(0xffffffffu, scale)) return;
+        l *= down;
+        tm_wait_st();  // what this block has stored so far
+        // the block before is complete: its product was issued before this block's scores
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 16) {
+          uint32_t v[16];
+          tm_ld16(to + c0, v);
+          tm_wait_ld(v);
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          f32x2 x2;
-          if constexpr (BIAS) {
-            x2 = add2(biased2(v[c], v[c + 1], c0 + c), org2);
-          } else if constexpr (POLY) {
-            const f32x2 z = mul2(bits2(v[c], v[c + 1]), pair2(fac_poly, fac_poly)), w2 = mul2(z, z);
-            f32x2 h = fma2(w2, pair2(tanh_c[5], tanh_c[5]), pair2(tanh_c[4], tanh_c[4]));
-#pragma unroll
-            for (int k = 3; k >= 0; --k) h = fma2(w2, h, pair2(tanh_c[k], tanh_c[k]));
-            x2 = fma2(z, h, org2);
-          } else {
-            x2 = fma2(pair2(exact_unit(__uint_as_float(v[c])), exact_unit(__uint_as_float(v[c + 1]))), f2, org2);
-          }
-          float2 p = split2(x2);
-          p.x = ex2(p.x);
-          p.y = ex2(p.y);
-          if (MASK) {
-            p.x = seen(c0 + c) ? p.x : 0.f;
-            p.y = seen(c0 + c + 1) ? p.y : 0.f;
-          }
-          sum2 = add2(sum2, pair2(p.x, p.y));
-          o[c / 2] = h2(p.x, p.y);
+          for (int c = 0; c < 16; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * down);
+          tm_st16(to + c0, v);
         }
-        tm_st16(ts + c0 / 2, o);
+        const __half2 down2 = __float2half2_rn(down);
+#pragma unroll 1
+        for (int c0 = 0; c0 < c_first / 2; c0 += 16) {
+          uint32_t v[16];
+          tm_ld16(ts + c0, v);
+          tm_wait_ld(v);
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&v[c]), down2);
+            v[c] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          tm_st16(ts + c0, v);
+        }
       };
-      // the polynomial serves a warp whose rows' scores all lie in its range
-      const bool poly = CAP && !BIAS && __all_sync(0xffffffffu, mag * fac_poly <= kTanhRange);
-      if (edge) {
-        if (poly)
-          walk([&](const uint32_t(&v)[32], int c0) { exponentials(std::true_type(), std::integral_constant<bool, CAP && !BIAS>(), v, c0); });
-        else
-          walk([&](const uint32_t(&v)[32], int c0) { exponentials(std::true_type(), std::false_type(), v, c0); });
-      } else {
-        if (poly)
-          walk([&](const uint32_t(&v)[32], int c0) { exponentials(std::false_type(), std::integral_constant<bool, CAP && !BIAS>(), v, c0); });
-        else
-          walk([&](const uint32_t(&v)[32], int c0) { exponentials(std::false_type(), std::false_type(), v, c0); });
+
+      // P = 2^(score - org) of the 64 columns from c_first on, as f16, and its sum.  Where !EXACT, against an
+      // m_ref that they may exceed and with the polynomial for the cap: `top` (the largest P) and
+      // `reach` (the largest square of tanh's argument) tell whether that was right.
+      uint32_t o[kTile / 4];
+      float sum = 0.f, reach = 0.f;
+      __half2 top = __floats2half2_rn(0.f, 0.f);
+      auto exponentials = [&](auto masked, auto exact, int c_first) {
+        constexpr bool MASK = decltype(masked)::value, EXACT = decltype(exact)::value;
+        const float org = m_ref == -INFINITY ? 0.f : m_ref;
+        const f32x2 org2 = pair2(-org, -org), f2 = pair2(f, f), step2 = pair2(2.f * slope, 2.f * slope);
+        const float z1 = fac * 0.34657359027997264f;  // fac carries 2 log2(e)
+        f32x2 sum2 = pair2(0.f, 0.f);
+        top = __floats2half2_rn(0.f, 0.f);
+        reach = 0.f;
+        uint32_t va[32], vb[32];
+        tm_ld32(ts + c_first, va);
+        tm_ld32(ts + c_first + 32, vb);
+        tm_wait_ld(va);
+        tm_wait_ld(vb);
+        auto chunk = [&](const uint32_t(&v)[32], int h0) {
+          f32x2 b2 = org2;
+          if (BIAS && !EXACT) {
+            const float b1 = fmaf(slope, (float)(c_first + h0) - ahead, -org);
+            b2 = pair2(b1, b1 + slope);
+          }
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            f32x2 x2;
+            if constexpr (EXACT || (CAP && BIAS)) {
+              const f32x2 u2 = pair2(exact_unit(__uint_as_float(v[c])), exact_unit(__uint_as_float(v[c + 1])));
+              if constexpr (BIAS)
+                x2 = add2(fma2(u2, f2, pair2(bias(c_first + h0 + c), bias(c_first + h0 + c + 1))), org2);
+              else
+                x2 = fma2(u2, f2, org2);
+            } else if constexpr (BIAS) {
+              x2 = fma2(bits2(v[c], v[c + 1]), f2, b2);
+              b2 = add2(b2, step2);
+            } else if constexpr (CAP) {
+              const f32x2 z = mul2(bits2(v[c], v[c + 1]), pair2(z1, z1)), w2 = mul2(z, z);
+              f32x2 h = fma2(w2, tanh_c[5], tanh_c[4]);
+#pragma unroll
+              for (int k = 3; k >= 0; --k) h = fma2(w2, h, tanh_c[k]);
+              x2 = fma2(z, h, org2);
+              const float2 ww = split2(w2);
+              reach = fmaxf(reach, fmaxf(ww.x, ww.y));
+            } else {
+              x2 = fma2(bits2(v[c], v[c + 1]), f2, org2);
+            }
+            float2 p = split2(x2);
+            p.x = ex2(p.x);
+            p.y = ex2(p.y);
+            if (MASK) {
+              p.x = seen(c_first + h0 + c) ? p.x : 0.f;
+              p.y = seen(c_first + h0 + c + 1) ? p.y : 0.f;
+            }
+            sum2 = add2(sum2, pair2(p.x, p.y));
+            const __half2 h = __floats2half2_rn(p.x, p.y);
+            o[(h0 + c) / 2] = *reinterpret_cast<const uint32_t*>(&h);
+            if (!EXACT) top = __hmax2(top, h);
+          }
+        };
+        chunk(va, 0);
+        chunk(vb, 32);
+        const float2 s2 = split2(sum2);
+        sum = s2.x + s2.y;
+      };
+      // The first block that a row sees sets its m_ref.  Later ones rarely exceed it by 2^kSlack: they are
+      // tried against the old one, and done again where some row of the warp does.
+      const bool first =
+          __any_sync(0xffffffffu, live && m_ref == -INFINITY && me.lo < min(me.hi, kb + kTile) && me.hi > kb);
+#pragma unroll 1
+      for (int c_first = 0; c_first < kTile; c_first += kTile / 2) {
+        bool again = (BIAS && !behind) || (first && c_first == 0);
+        if (!again) {
+          if (edge)
+            exponentials(std::true_type(), std::false_type(), c_first);
+          else
+            exponentials(std::false_type(), std::false_type(), c_first);
+          const __half2 most = __float2half2_rn((float)(1 << kSlack));
+          again = __any_sync(0xffffffffu, live && (!__hble2(top, most) || reach > kTanhRange));
+        }
+        if (again) {
+          raise(c_first);
+          if (edge)
+            exponentials(std::true_type(), std::true_type(), c_first);
+          else
+            exponentials(std::false_type(), std::true_type(), c_first);
+        }
+        l += sum;
+        tm_st16(ts + c_first / 2, o);
+        tm_st16(ts + c_first / 2 + 16, o + 16);
       }
-      const float2 sums = split2(sum2);
-      l += sums.x + sums.y;
       tm_wait_st();
       if (kb < sh.full_lo || kb + kTile > sh.full_hi) {  // as the loading warps decide it
         // NaN values of keys that some rows do not see were taken out of V: put them into the rows that do
@@ -503,42 +535,37 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     ok = __all_sync(0xffffffffu, ok);
     tc_after();
     const bool have = nb > 0 && on && ok;
-    const size_t orow = (size_t)tok * a.Hq + hq;
+    const size_t orow = (size_t)tok * a.Hq + hq, part = (size_t)split * a.T * a.Hq + orow;
     const float vs = a.v_scale[head];
     const float inv = l == 0.f ? 0.f : __fdividef(vs, l);
-    if (pl.splits > 1 && live) {
-      const size_t at = (size_t)split * a.T * a.Hq + orow;
-      *reinterpret_cast<float2*>(pl.ml + at * 2) = make_float2(m_ref, l);
-    }
-#pragma unroll 1
-    for (int c0 = 0; c0 < D; c0 += 32) {
-      uint32_t v[32];
+    if (pl.splits > 1 && live) *reinterpret_cast<float2*>(pl.ml + part * 2) = make_float2(m_ref, l);
+#pragma unroll
+    for (int c0 = 0; c0 < D; c0 += 16) {
+      uint32_t v[16];
       if (have) {
-        tm_ld32(to + c0, v);
+        tm_ld16(to + c0, v);
         tm_wait_ld(v);
       } else {
 #pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = 0u;
+        for (int c = 0; c < 16; ++c) v[c] = 0u;
       }
-      uint32_t nan = 0;
+      const uint32_t nan = nan_d[c0 / 32] >> (c0 % 32);
+      if (nan & 0xffffu) {
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) nan = 32 * i == c0 ? nan_d[i] : nan;
-      if (nan) {
-#pragma unroll
-        for (int c = 0; c < 32; ++c)
+        for (int c = 0; c < 16; ++c)
           if ((nan >> c) & 1u) v[c] = 0x7fffffffu;
       }
       if (!live) continue;
       if (pl.splits > 1) {
-        float4* dst = reinterpret_cast<float4*>(pl.acc + ((size_t)split * a.T * a.Hq + orow) * D + c0);
+        float4* dst = reinterpret_cast<float4*>(pl.acc + part * D + c0);
 #pragma unroll
-        for (int c = 0; c < 32; c += 4)
+        for (int c = 0; c < 16; c += 4)
           dst[c / 4] = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]),
                                    __uint_as_float(v[c + 3]));
       } else {
         uint4* dst = reinterpret_cast<uint4*>(a.out + (size_t)tok * a.ldo + (size_t)hq * D + c0);
 #pragma unroll
-        for (int c = 0; c < 32; c += 8) {
+        for (int c = 0; c < 16; c += 8) {
           uint32_t o[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
@@ -554,13 +581,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     int key0, k_hi;
     const int nb = plan(key0, k_hi);
     const int f_lo = sh.full_lo, f_hi = sh.full_hi;
-    auto offset = [&](int j) {  // where key j * 128 + lt lies; -1: reads zeros
-      const int key = key0 + j * kTile + lt;
-      long long off = -1;
+    // The cache row (of D bytes) of the block's key lt; kNoRow: reads zeros.
+    constexpr uint32_t kNoRow = 0xffffffffu;
+    uint32_t* offs = reinterpret_cast<uint32_t*>(smem + C::OFF0);
+    auto offset = [&](int j) {
+      const int key = key0 + (nb - 1 - j) * kTile + lt;
+      uint32_t off = kNoRow;
       if (j < nb && key < k_hi) {
         const int page = a.page_table[(size_t)b * a.table_ld + key / a.P];
         if (page >= 0 && page < a.num_pages)
-          off = (((long long)page * a.P + key % a.P) * a.Hkv + head) * D;
+          off = (uint32_t)(((long long)page * a.P + key % a.P) * a.Hkv + head);
         else
           atomicOr(a.err, OKC_DEVERR_PAGE);
       }
@@ -603,8 +633,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     auto fetch = [&](const uint8_t* cache, int j, uint4 (&r)[PER]) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const long long off = offs[(j & 1) * kTile + kf + i * KSTEP];
-        r[i] = off >= 0 ? *reinterpret_cast<const uint4*>(cache + off + ch * 16) : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t row = offs[(j & 1) * kTile + kf + i * KSTEP];
+        r[i] = row != kNoRow ? *reinterpret_cast<const uint4*>(cache + (size_t)row * D + ch * 16) : make_uint4(0u, 0u, 0u, 0u);
       }
     };
     uint4 kr[PER], vr[PER];
@@ -629,7 +659,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       }
       if (j + 1 < nb) fetch(a.k_cache, j + 1, kr);
       ok = mbar_wait(&sh.v_empty[st], ph, a.err, abort_flag);  // the next block's barrier tells the others
-      const int kb = key0 + j * kTile;
+      const int kb = key0 + (nb - 1 - j) * kTile;
       const bool edge = kb < f_lo || kb + kTile > f_hi;
       if (edge) {
         if (lt < 4) sh.nan[st][lt] = 0;
@@ -655,17 +685,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+    // ------------------------------------------------------------------ MMA issue
     if (warp == kIssueWarp && lane == 0) {
-      // ------------------------------------------------------------------ MMA issue
-      const uint32_t tmem = sh.tmem;
       int key0, k_hi;
       const int nb = plan(key0, k_hi);
-      const bool two = b >= 0 && (a.cu_q[b + 1] - a.cu_q[b]) * a.G - sh.tile * kPair > kTile;
+      const int tiles = b >= 0 && (a.cu_q[b + 1] - a.cu_q[b]) * a.G - sh.tile * kPair > kTile ? 2 : 1;
+      const uint32_t tmem = sh.tmem;
       const uint32_t id_s = umma_idesc_f16(kTile, false), id_o = umma_idesc_f16(D, true);
       auto scores = [&](int w, int st) {
         const uint64_t qa = umma_desc_sw128(smem_u32(smem + C::Q0 + w * C::TILE_B));
         const uint64_t ka = umma_desc_sw128(smem_u32(smem + C::K0 + st * C::TILE_B));
-  #pragma unroll
+#pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t at = ((k / 4) * C::SUB + (k % 4) * 32) >> 4;
           umma_ss(tmem + w * kTile, qa + at, ka + at, id_s, k != 0);
@@ -674,33 +704,35 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       };
       auto output = [&](int w, int st, bool acc) {
         const uint64_t va = umma_desc_mn(smem_u32(smem + C::V0 + st * C::TILE_B), C::SUB);
-  #pragma unroll
+#pragma unroll
         for (int k = 0; k < kTile / 16; ++k)
           umma_ts(tmem + 2 * kTile + w * D, tmem + w * kTile + 8 * k, va + k * (2048 >> 4), id_o, acc || k != 0);
       };
-      bool ok = nb == 0 || mbar_wait(&sh.q_full, 0, a.err, abort_flag);
-      if (ok && nb > 0) {
-        ok = mbar_wait(&sh.k_full[0], 0, a.err, abort_flag);
+      bool ok = true;
+      if (nb > 0) {
+        ok = mbar_wait(&sh.q_full, 0, a.err, abort_flag) && mbar_wait(&sh.k_full[0], 0, a.err, abort_flag);
         if (ok) {
           tc_after();
-          scores(0, 0);
-          if (two) scores(1, 0);
+          for (int w = 0; w < tiles; ++w) scores(w, 0);
           umma_commit(&sh.k_empty[0]);
         }
       }
       for (int j = 0; ok && j < nb; ++j) {
         const int st = j & 1, nx = st ^ 1;
         ok = mbar_wait(&sh.v_full[st], (uint32_t)(j >> 1) & 1u, a.err, abort_flag);
-        if (ok && j + 1 < nb) ok = mbar_wait(&sh.k_full[nx], (uint32_t)((j + 1) >> 1) & 1u, a.err, abort_flag);
-        for (int w = 0; ok && w < (two ? 2 : 1); ++w) {
+        for (int w = 0; ok && w < tiles; ++w) {
           ok = mbar_wait(&sh.p_full[w], (uint32_t)j & 1u, a.err, abort_flag);
           if (!ok) break;
           tc_after();
           output(w, st, j > 0);
-          if (j + 1 < nb)
-            scores(w, nx);  // over P, which the product above has read by then
-          else
+          if (j + 1 < nb) {
+            if (w == 0) ok = mbar_wait(&sh.k_full[nx], (uint32_t)((j + 1) >> 1) & 1u, a.err, abort_flag);
+            if (!ok) break;
+            tc_after();
+            scores(w, nx);  // over P: the tensor core takes a thread's MMAs in order, and the ones above read it
+          } else {
             umma_commit(&sh.o_full[w]);
+          }
         }
         if (!ok) break;
         umma_commit(&sh.v_empty[st]);

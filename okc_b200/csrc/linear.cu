@@ -33,6 +33,8 @@ constexpr int kTallThreads = 32 * (kFirstDrain + kDrainWarps);
 // Registers a thread: the launch's, and how fp32 outputs split them over the three warpgroups.
 constexpr int kLaunchRegs = 168, kIssueRegs = 40, kDrainRegs = 232;
 static_assert(128 * kIssueRegs + 256 * kDrainRegs <= kTallThreads * kLaunchRegs, "the split must fit the launch");
+static_assert(kIssueRegs < kLaunchRegs && kDrainRegs > kLaunchRegs,
+              "setmaxnreg.dec lowers and .inc raises; the other way round is an illegal instruction");
 constexpr int kGroup = 8;        // token tiles of a group
 
 struct TallSmem {
