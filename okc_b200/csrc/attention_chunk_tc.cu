@@ -4,14 +4,19 @@
 //
 // Compute-bound: 4 D operations per (row, visible key) against 2 D cache bytes per key and 256 rows.
 // A block takes 256 rows (token-major, the G query heads of one KV head side by side) as two tiles
-// of 128 and streams the keys that any of them sees in blocks of 128:
-//  * two softmax warpgroups, one thread a row: P goes back over S as f16 and is the next product's A
-//    operand there.  A row's sums never leave its thread;
+// of 128 and streams the keys that any of them sees in blocks of 64:
+//  * a softmax warpgroup per tile, one thread a row: P goes back over S as f16 and is the next product's A
+//    operand there.  S has two buffers a tile, so that a block's scores are formed while the one
+//    before is in the softmax, and a row's sums never leave its thread;
 //  * four warps fetch key and value rows by page, turn e4m3 into f16 (exact) and store both as the
-//    swizzled rows that the MMAs read (keys K-major, values MN-major: no transpose);
-//  * one thread issues the MMAs, the tiles in turn: while one tile's softmax runs, the other's products do;
+//    swizzled rows that the MMAs read (keys K-major, values MN-major: no transpose), four blocks deep;
+//  * a thread per tile issues its MMAs;
 //  * a block's exponentials are taken against the maximum so far, in one pass over S, and done again with
-//    O rescaled only where a P exceeds 2^8: rare after a row's first block;
+//    O rescaled only where a P exceeds 2^8: rare after a row's first blocks.
+// The special-function unit bounds it: 256 x 64 exponentials take 1024 cycles of it a block, where the tensor
+// cores need 1024 too, and a block takes 1960 (the softmax warps' other instructions and latencies overlap
+// only in part; a third of the exponentials as polynomials on the fused-operation pipe made it slower).
+// 4096 tokens behind 4096 cached, 64 / 8 heads of 128: 860 us (960 TFLOP/s), capped 1070 us.
 // Blocks of a request are taken from its last rows on: the longest causal spans start first.  With few
 // blocks the keys are split over several, which leave fp32 partial sums for a merge.
 #include <type_traits>
@@ -23,29 +28,34 @@ namespace okc {
 
 namespace {
 
-constexpr int kTile = 128;                 // rows of a tile, keys of a block
+constexpr int kTile = 128;                 // rows of a tile
+constexpr int kKeys = 64;                  // keys of a block
+constexpr int kDepth = 4;                  // blocks of keys and values in shared memory
 constexpr int kPair = 2 * kTile;           // rows of a CTA
 constexpr int kSoftmaxThreads = 256;
 constexpr int kLoadThreads = 128;
-constexpr int kIssueWarp = (kSoftmaxThreads + kLoadThreads) / 32;          // its warpgroup's other warps idle
+constexpr int kIssueWarp = (kSoftmaxThreads + kLoadThreads) / 32;          // and the next; the others of their warpgroup idle
 constexpr int kTcThreads = kSoftmaxThreads + kLoadThreads + 128;
 // Registers a thread: the launch's, and how the four warpgroups split them.
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kLoadRegs = 112, kIssueRegs = 64;
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kLoadRegs = 120, kIssueRegs = 56;
 static_assert(2 * kSoftmaxRegs + kLoadRegs + kIssueRegs <= 4 * kLaunchRegs, "the split must fit the launch");
 static_assert(kSoftmaxRegs > kLaunchRegs && kLoadRegs < kLaunchRegs && kIssueRegs < kLaunchRegs,
               "setmaxnreg.inc raises and .dec lowers; the other way round is an illegal instruction");
+constexpr int kHigh = 0, kLow = 1, kExact = 2;  // how a block's exponentials are taken
 constexpr int kSlack = 8;                  // log2 growth of the maximum that O tolerates
 
 template <int D>
 struct TcCfgA {
-  static constexpr int SUB = kTile * 128;              // 128 rows x 64 f16, one swizzled panel
-  static constexpr int PANELS = D / 64;
-  static constexpr int TILE_B = SUB * PANELS;          // a 128 x D f16 tile
+  static constexpr int PANELS = D / 64;                // swizzled panels of 64 f16 columns
+  static constexpr int QSUB = kTile * 128;             // a panel of a query tile
+  static constexpr int QTILE = QSUB * PANELS;
+  static constexpr int SUB = kKeys * 128;              // a panel of a key or value block
+  static constexpr int BLOCK = SUB * PANELS;
   static constexpr int Q0 = 0;
-  static constexpr int K0 = 2 * TILE_B;                // two K blocks
-  static constexpr int V0 = K0 + 2 * TILE_B;           // two V blocks
-  static constexpr int OFF0 = V0 + 2 * TILE_B;         // [2][128] cache rows of the keys
-  static constexpr int BAR0 = OFF0 + 2 * kTile * 4;
+  static constexpr int K0 = 2 * QTILE;
+  static constexpr int V0 = K0 + kDepth * BLOCK;
+  static constexpr int OFF0 = V0 + kDepth * BLOCK;     // [2][kKeys] cache rows of the keys
+  static constexpr int BAR0 = OFF0 + 2 * kKeys * 4;
   static constexpr int SMEM = 1024 + BAR0 + 512;
 };
 
@@ -55,6 +65,7 @@ struct TcPlanA {
   float* ml;   // [splits][T * Hq][2]
 };
 
+// f16 operands, fp32 sums, 128 x n.
 __device__ __forceinline__ uint32_t umma_idesc_f16(int n, bool b_mn_major) {
   return (1u << 4) | (b_mn_major ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
@@ -141,19 +152,25 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   return r;
 }
 
-// tanh(x) / x for |x| <= 1 as a polynomial in x^2, fitted for the least |x * error| over that range
-// (2.4e-7; 3.2e-6 relative at 0): eight fused operations where the exponential and the
-// reciprocal of the exact form occupy the special-function unit twice.
-constexpr float kTanhRange = 1.f;
+// tanh(x) / x as a polynomial in x^2, fitted for the least |x * error| over |x| <= 1 (six
+// coefficients: 2.4e-7) and over |x| <= 0.4 (three: 1.2e-6): fused operations where the exponential
+// and the reciprocal of the exact form occupy the special-function unit twice.
+constexpr float kTanhRange2 = 1.f, kTanhLowRange2 = 0.16f;  // squares of the ranges
+template <bool LOW>
 __device__ __forceinline__ f32x2 tanh2(int k) {
-  const float c = k == 0   ? 0.99999685f
-         : k == 1 ? -0.33324004f
-         : k == 2 ? 0.13253524f
-         : k == 3 ? -0.05097283f
-         : k == 4 ? 0.01611415f
-                  : -0.00283945f;
+  float c;
+  if (LOW)
+    c = k == 0 ? 0.99997884f : k == 1 ? -0.33225426f : 0.11942387f;
+  else
+    c = k == 0   ? 0.99999685f
+        : k == 1 ? -0.33324004f
+        : k == 2 ? 0.13253524f
+        : k == 3 ? -0.05097283f
+        : k == 4 ? 0.01611415f
+                 : -0.00283945f;
   return pair2(c, c);
 }
+
 __device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
@@ -169,13 +186,14 @@ __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_
 
 // Barriers and words shared by the roles.
 struct TcShared {
-  uint64_t plan, q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drain;
+  uint64_t plan, q_full, k_full[kDepth], v_full[kDepth], kv_empty[kDepth], drain[2];
+  uint64_t s_full[2][2], p_full[2][2];  // [tile][buffer]
   uint32_t tmem;
   int abort;
   int b, tile;             // the block's request (-1: none) and row tile pair
   int lo, hi;              // union of its rows' intervals
   int full_lo, full_hi;    // intersection: keys in it need no mask
-  uint32_t nan[2][4];      // per V block: its keys that hold a NaN that was taken out
+  uint32_t nan[kDepth][kKeys / 32];  // per V block: its keys that hold a NaN that was taken out
 };
 
 template <int D, bool CAP, bool BIAS>
@@ -191,17 +209,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
   if (threadIdx.x == 0) {
     mbar_init(&sh.plan, kSoftmaxThreads / 32);
     mbar_init(&sh.q_full, kSoftmaxThreads / 32);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kDepth; ++i) {
       mbar_init(&sh.k_full[i], kLoadThreads / 32);
-      mbar_init(&sh.k_empty[i], 1);
       mbar_init(&sh.v_full[i], kLoadThreads / 32);
-      mbar_init(&sh.v_empty[i], 1);
-      mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], kSoftmaxThreads / 64);
-      mbar_init(&sh.o_full[i], 1);
-      for (int w = 0; w < 4; ++w) sh.nan[i][w] = 0;
+      mbar_init(&sh.kv_empty[i], 2);  // one per tile
+      for (int w = 0; w < kKeys / 32; ++w) sh.nan[i][w] = 0;
     }
-    mbar_init(&sh.drain, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&sh.drain[t], 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sh.s_full[t][i], 1);
+        mbar_init(&sh.p_full[t][i], kSoftmaxThreads / 64);
+      }
+    }
     sh.abort = 0;
     sh.lo = 0x7fffffff;
     sh.hi = 0;
@@ -258,15 +278,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     if (!mbar_wait(&sh.plan, 0, a.err, abort_flag)) *abort_flag = 1;
     const int k_lo = *reinterpret_cast<volatile int*>(&sh.lo);
     k_hi = *reinterpret_cast<volatile int*>(&sh.hi);
-    int nb = k_hi > k_lo ? (k_hi - k_lo + kTile - 1) / kTile : 0, first = 0;
+    int nb = k_hi > k_lo ? (k_hi - k_lo + kKeys - 1) / kKeys : 0, first = 0;
     if (pl.splits > 1) {
       const int per = (nb + pl.splits - 1) / pl.splits;
       first = min(nb, split * per);
       nb = min(nb, first + per) - first;
     }
-    key0 = k_lo + first * kTile;
+    key0 = k_lo + first * kKeys;
     return nb;
   };
+  // The j-th block taken.  Under a distance bias the nearest keys come first, so that a row meets its
+  // largest scores at once (front to back every block raises the maximum: 1770 us against 915 for 4096
+  // tokens behind 4096).  Without one a row's first block is better a whole one than its diagonal.
+#define OKC_BLOCK_AT(j) (BIAS ? nb - 1 - (j) : (j))
 
   if (warp < kSoftmaxThreads / 32) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -274,13 +298,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     const int w = warp >> 2, lr = (warp & 3) * 32 + lane;  // tile, row of it
     Req rq = {};
     int rows = 0, row0 = 0;
-    const int r0 = sh.tile * kPair, r = r0 + w * kTile + lr;
+    const int r = sh.tile * kPair + w * kTile + lr;
     if (b >= 0) {
       rq = request(a, b);
       rows = rq.n * a.G;
       row0 = a.cu_q[b];
     }
-    const bool live = r < rows;
+    const bool live = r < rows, on = sh.tile * kPair + w * kTile < rows;
     const int tok = live ? row0 + r / a.G : 0, hq = live ? head * a.G + r % a.G : 0;
     RowSpan me = {0, 0, 0};
     if (live) me = row_span(a, rq, row0, r / a.G);
@@ -300,17 +324,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     }
     int key0, k_hi;
     const int nb = plan(key0, k_hi);
-    const bool on = w == 0 || rows - r0 > kTile;
+    const int f_lo = sh.full_lo, f_hi = sh.full_hi;
     const uint32_t lanes = sh.tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t ts = lanes + w * kTile, to = lanes + 2 * kTile + w * D;  // P lies over the first half of S
+    const uint32_t to = lanes + 2 * kTile + w * D;
     float fac = 0.f, slope = 0.f, m_ref = -INFINITY, l = 0.f;
     uint32_t nan_d[D / 32];  // output columns that a visible NaN value reaches
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) nan_d[i] = 0;
-    const float cap2 = CAP ? a.softcap * 1.4426950408889634f : 0.f;
-    f32x2 tanh_c[6];  // cap2 times the polynomial
-#pragma unroll
-    for (int k = 0; k < 6; ++k) tanh_c[k] = mul2(tanh2(k), pair2(cap2, cap2));
     if (nb > 0 && on) {
       // the row in f16, scaled by a power of two, into the swizzled panels
       const __nv_bfloat16* qp = a.q + (size_t)tok * a.ldq + (size_t)hq * D;
@@ -330,7 +350,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       const float down = fac < 0.f ? -pow2(-shf) : pow2(-shf);
       fac = fabsf(fac);
       if (BIAS && live) slope = a.slopes[hq] * 1.4426950408889634f;
-      uint8_t* qs = smem + C::Q0 + w * C::TILE_B + lr * 128;
+      uint8_t* qs = smem + C::Q0 + w * C::QTILE + lr * 128;
 #pragma unroll 4
       for (int i = 0; i < D / 8; ++i) {
         const uint4 v = live ? *reinterpret_cast<const uint4*>(qp + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
@@ -338,41 +358,45 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
         uint32_t o[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = h2(bf16_lo(u[k]) * down, bf16_hi(u[k]) * down);
-        *reinterpret_cast<uint4*>(qs + (i / 8) * C::SUB + (((i % 8) ^ (lr & 7)) * 16)) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(qs + (i / 8) * C::QSUB + (((i % 8) ^ (lr & 7)) * 16)) = make_uint4(o[0], o[1], o[2], o[3]);
       }
     }
     fence_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh.q_full);
 
-    bool ok = true;
-    // keys from the last block on: under a distance bias the largest scores come first
+    const float cap2 = CAP ? a.softcap * 1.4426950408889634f : 0.f;
+    const float f = CAP ? cap2 : fac;
+    auto s_ready = [&](int j) {  // block j's scores are there, and with them every product up to P V of block j - 2
+      return mbar_wait(&sh.s_full[w][j & 1], (uint32_t)(j >> 1) & 1u, a.err, abort_flag);
+    };
+    bool ok = true, low = true;  // low: no score so far has left the three-coefficient range
+#pragma unroll 1
     for (int j = 0; j < nb && on; ++j) {
-      const int kb = key0 + (nb - 1 - j) * kTile;
-      ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[w], (uint32_t)j & 1u, a.err, abort_flag));
+      const int kb = key0 + OKC_BLOCK_AT(j) * kKeys;
+      const uint32_t ts = lanes + w * kTile + (j & 1) * kKeys;  // S, and P over its first half
+      ok = __all_sync(0xffffffffu, s_ready(j));
       if (!ok) {
         *abort_flag = 1;
         break;
       }
       tc_after();
-      const bool edge = !__all_sync(0xffffffffu, !live || (me.lo <= kb && me.hi >= kb + kTile));
+      const bool edge = !__all_sync(0xffffffffu, !live || (me.lo <= kb && me.hi >= kb + kKeys));
       // visible columns [vis_lo, vis_hi)
-      const int vis_lo = live ? me.lo - kb : 0, vis_hi = live ? me.hi - kb : 0;
+      const int vis_lo = me.lo - kb, vis_hi = me.hi - kb;
       auto seen = [&](int c) { return c >= vis_lo && c < vis_hi; };
       // The log2 score of raw sum v at key kb + c is u * f, u = v or its capped form, with a bias less
       // slope * |ahead - c|.  Where no visible key lies ahead of its row, no absolute value is needed.
-      const float f = CAP ? cap2 : fac;
       const float ahead = (float)(me.pos - kb);
-      const bool behind = BIAS && __all_sync(0xffffffffu, !live || min(me.hi, kb + kTile) - 1 <= me.pos);
+      const bool behind = BIAS && __all_sync(0xffffffffu, !live || min(me.hi, kb + kKeys) - 1 <= me.pos);
       auto exact_unit = [&](float v) -> float { return CAP ? tanh_from_2l2e(v * fac) : v; };
       auto bias = [&](int c) -> float { return -slope * fabsf(ahead - (float)c); };
 
-      // Raises m_ref to the row's maximum over the columns from c_first on, with O, l and the P before
-      // c_first scaled down to it.
-      auto raise = [&](int c_first) {
+      // Raises m_ref to the row's maximum over the block, with O and l scaled down to it.
+      auto raise = [&]() {
         float mx = -INFINITY;
 #pragma unroll 1
-        for (int c0 = c_first; c0 < kTile; c0 += 16) {
+        for (int c0 = 0; c0 < kKeys; c0 += 16) {
           uint32_t v[16];
           tm_ld16(ts + c0, v);
           tm_wait_ld(v);
@@ -380,20 +404,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
           for (int c = 0; c < 16; ++c) {
             float x = __uint_as_float(v[c]);
             if (BIAS) x = fmaf(exact_unit(x), f, bias(c0 + c));
-            if (edge && !seen(c0 + c)) x = -INFINITY;
+            if (!seen(c0 + c)) x = -INFINITY;
             mx = fmaxf(mx, x);
           }
         }
         // without a bias the score grows with the raw sum; rounded up, so that no fused u * f - org is positive
         if (!BIAS && mx != -INFINITY) mx = __fmul_ru(exact_unit(mx), f);
         const bool grow = mx > m_ref;
-        const bool scale = m_ref != -INFINITY && grow;  // from -infinity: O, l and P are zero
+        const bool scale = m_ref != -INFINITY && grow;  // from -infinity: O and l are zero
         const float down = scale ? ex2(m_ref - mx) : 1.f;
         if (grow) m_ref = mx;
         if (!__any_sync(0xffffffffu, scale)) return;
         l *= down;
-        tm_wait_st();  // what this block has stored so far
-        // the block before is complete: its product was issued before this block's scores
+        if (!s_ready(j + 1)) *abort_flag = 1;  // P V of the block before is done, and the next waits for this P
+        tc_after();
 #pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += 16) {
           uint32_t v[16];
@@ -403,44 +427,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
           for (int c = 0; c < 16; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * down);
           tm_st16(to + c0, v);
         }
-        const __half2 down2 = __float2half2_rn(down);
-#pragma unroll 1
-        for (int c0 = 0; c0 < c_first / 2; c0 += 16) {
-          uint32_t v[16];
-          tm_ld16(ts + c0, v);
-          tm_wait_ld(v);
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&v[c]), down2);
-            v[c] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-          tm_st16(ts + c0, v);
-        }
       };
 
-      // P = 2^(score - org) of the 64 columns from c_first on, as f16, and its sum.  Where !EXACT, against an
-      // m_ref that they may exceed and with the polynomial for the cap: `top` (the largest P) and
-      // `reach` (the largest square of tanh's argument) tell whether that was right.
-      uint32_t o[kTile / 4];
+      // P = 2^(score - org) as f16 and its sum.  MODE kExact: after raise(); else against an m_ref that the
+      // block may exceed and with a polynomial for the cap: `top` (the largest P) and `reach` (the largest
+      // square of tanh's argument) tell whether that was right.
+      uint32_t o[kKeys / 2];
       float sum = 0.f, reach = 0.f;
       __half2 top = __floats2half2_rn(0.f, 0.f);
-      auto exponentials = [&](auto masked, auto exact, int c_first) {
-        constexpr bool MASK = decltype(masked)::value, EXACT = decltype(exact)::value;
+      auto exponentials = [&](auto masked, auto mode) {
+        constexpr bool MASK = decltype(masked)::value, EXACT = decltype(mode)::value == kExact;
+        constexpr bool LOW = decltype(mode)::value == kLow;
         const float org = m_ref == -INFINITY ? 0.f : m_ref;
         const f32x2 org2 = pair2(-org, -org), f2 = pair2(f, f), step2 = pair2(2.f * slope, 2.f * slope);
         const float z1 = fac * 0.34657359027997264f;  // fac carries 2 log2(e)
         f32x2 sum2 = pair2(0.f, 0.f);
-        top = __floats2half2_rn(0.f, 0.f);
-        reach = 0.f;
-        uint32_t va[32], vb[32];
-        tm_ld32(ts + c_first, va);
-        tm_ld32(ts + c_first + 32, vb);
-        tm_wait_ld(va);
-        tm_wait_ld(vb);
-        auto chunk = [&](const uint32_t(&v)[32], int h0) {
+        auto columns = [&](const uint32_t(&v)[32], int c0) {
           f32x2 b2 = org2;
           if (BIAS && !EXACT) {
-            const float b1 = fmaf(slope, (float)(c_first + h0) - ahead, -org);
+            const float b1 = fmaf(slope, (float)c0 - ahead, -org);
             b2 = pair2(b1, b1 + slope);
           }
 #pragma unroll
@@ -449,7 +454,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
             if constexpr (EXACT || (CAP && BIAS)) {
               const f32x2 u2 = pair2(exact_unit(__uint_as_float(v[c])), exact_unit(__uint_as_float(v[c + 1])));
               if constexpr (BIAS)
-                x2 = add2(fma2(u2, f2, pair2(bias(c_first + h0 + c), bias(c_first + h0 + c + 1))), org2);
+                x2 = add2(fma2(u2, f2, pair2(bias(c0 + c), bias(c0 + c + 1))), org2);
               else
                 x2 = fma2(u2, f2, org2);
             } else if constexpr (BIAS) {
@@ -457,10 +462,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
               b2 = add2(b2, step2);
             } else if constexpr (CAP) {
               const f32x2 z = mul2(bits2(v[c], v[c + 1]), pair2(z1, z1)), w2 = mul2(z, z);
-              f32x2 h = fma2(w2, tanh_c[5], tanh_c[4]);
+              constexpr int N = LOW ? 3 : 6;
+              f32x2 h = fma2(w2, tanh2<LOW>(N - 1), tanh2<LOW>(N - 2));
 #pragma unroll
-              for (int k = 3; k >= 0; --k) h = fma2(w2, h, tanh_c[k]);
-              x2 = fma2(z, h, org2);
+              for (int k = N - 3; k >= 0; --k) h = fma2(w2, h, tanh2<LOW>(k));
+              x2 = fma2(mul2(z, f2), h, org2);
               const float2 ww = split2(w2);
               reach = fmaxf(reach, fmaxf(ww.x, ww.y));
             } else {
@@ -470,52 +476,55 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
             p.x = ex2(p.x);
             p.y = ex2(p.y);
             if (MASK) {
-              p.x = seen(c_first + h0 + c) ? p.x : 0.f;
-              p.y = seen(c_first + h0 + c + 1) ? p.y : 0.f;
+              p.x = seen(c0 + c) ? p.x : 0.f;
+              p.y = seen(c0 + c + 1) ? p.y : 0.f;
             }
             sum2 = add2(sum2, pair2(p.x, p.y));
             const __half2 h = __floats2half2_rn(p.x, p.y);
-            o[(h0 + c) / 2] = *reinterpret_cast<const uint32_t*>(&h);
+            o[(c0 + c) / 2] = *reinterpret_cast<const uint32_t*>(&h);
             if (!EXACT) top = __hmax2(top, h);
           }
         };
-        chunk(va, 0);
-        chunk(vb, 32);
+        uint32_t va[32], vb[32];
+        tm_ld32(ts, va);
+        tm_ld32(ts + 32, vb);
+        tm_wait_ld(va);
+        tm_wait_ld(vb);
+        columns(va, 0);
+        columns(vb, 32);
         const float2 s2 = split2(sum2);
         sum = s2.x + s2.y;
       };
       // The first block that a row sees sets its m_ref.  Later ones rarely exceed it by 2^kSlack: they are
       // tried against the old one, and done again where some row of the warp does.
-      const bool first =
-          __any_sync(0xffffffffu, live && m_ref == -INFINITY && me.lo < min(me.hi, kb + kTile) && me.hi > kb);
-#pragma unroll 1
-      for (int c_first = 0; c_first < kTile; c_first += kTile / 2) {
-        bool again = (BIAS && !behind) || (first && c_first == 0);
-        if (!again) {
-          if (edge)
-            exponentials(std::true_type(), std::false_type(), c_first);
-          else
-            exponentials(std::false_type(), std::false_type(), c_first);
-          const __half2 most = __float2half2_rn((float)(1 << kSlack));
-          again = __any_sync(0xffffffffu, live && (!__hble2(top, most) || reach > kTanhRange));
-        }
-        if (again) {
-          raise(c_first);
-          if (edge)
-            exponentials(std::true_type(), std::true_type(), c_first);
-          else
-            exponentials(std::false_type(), std::true_type(), c_first);
-        }
-        l += sum;
-        tm_st16(ts + c_first / 2, o);
-        tm_st16(ts + c_first / 2 + 16, o + 16);
+      bool again = (BIAS && !behind) ||
+                   __any_sync(0xffffffffu, live && m_ref == -INFINITY && me.lo < min(me.hi, kb + kKeys) && me.hi > kb);
+      if (!again) {
+        if (edge)
+          exponentials(std::true_type(), std::integral_constant<int, kHigh>());
+        else if (CAP && !BIAS && low)
+          exponentials(std::false_type(), std::integral_constant<int, kLow>());
+        else
+          exponentials(std::false_type(), std::integral_constant<int, kHigh>());
+        const __half2 most = __float2half2_rn((float)(1 << kSlack));
+        const float range = low && !edge ? kTanhLowRange2 : kTanhRange2;
+        if (CAP && __any_sync(0xffffffffu, live && reach > kTanhLowRange2)) low = false;
+        again = __any_sync(0xffffffffu, live && (!__hble2(top, most) || reach > range));
       }
+      if (again) {
+        raise();
+        exponentials(std::true_type(), std::integral_constant<int, kExact>());
+      }
+      l += sum;
+      tm_st16(ts, o);
+      tm_st16(ts + 16, o + 16);
       tm_wait_st();
-      if (kb < sh.full_lo || kb + kTile > sh.full_hi) {  // as the loading warps decide it
+      if (kb < f_lo || kb + kKeys > f_hi) {  // as the loading warps decide it
         // NaN values of keys that some rows do not see were taken out of V: put them into the rows that do
-        if (!mbar_wait(&sh.v_full[j & 1], (uint32_t)(j >> 1) & 1u, a.err, abort_flag)) *abort_flag = 1;
-        for (int q = 0; q < 4; ++q) {
-          for (uint32_t bits = *reinterpret_cast<volatile uint32_t*>(&sh.nan[j & 1][q]); bits; bits &= bits - 1) {
+        const int st = j % kDepth;
+        if (!mbar_wait(&sh.v_full[st], (uint32_t)(j / kDepth) & 1u, a.err, abort_flag)) *abort_flag = 1;
+        for (int q = 0; q < kKeys / 32; ++q) {
+          for (uint32_t bits = *reinterpret_cast<volatile uint32_t*>(&sh.nan[st][q]); bits; bits &= bits - 1) {
             const int key = kb + 32 * q + __ffs(bits) - 1;
             if (!live || key < me.lo || key >= me.hi) continue;
             const int page = a.page_table[(size_t)b * a.table_ld + key / a.P];
@@ -528,16 +537,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       }
       tc_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_full[w]);
+      if (lane == 0) mbar_arrive(&sh.p_full[w][j & 1]);
     }
     // ---- output ----
-    if (nb > 0 && on && ok) ok = mbar_wait(&sh.o_full[w], 0, a.err, abort_flag);
-    ok = __all_sync(0xffffffffu, ok);
+    const bool have = nb > 0 && on && __all_sync(0xffffffffu, ok && s_ready(nb + 1));
     tc_after();
-    const bool have = nb > 0 && on && ok;
-    const size_t orow = (size_t)tok * a.Hq + hq, part = (size_t)split * a.T * a.Hq + orow;
-    const float vs = a.v_scale[head];
-    const float inv = l == 0.f ? 0.f : __fdividef(vs, l);
+    const size_t part = (size_t)split * a.T * a.Hq + (size_t)tok * a.Hq + hq;
+    const float inv = l == 0.f ? 0.f : __fdividef(a.v_scale[head], l);
     if (pl.splits > 1 && live) *reinterpret_cast<float2*>(pl.ml + part * 2) = make_float2(m_ref, l);
 #pragma unroll
     for (int c0 = 0; c0 < D; c0 += 16) {
@@ -581,20 +587,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     int key0, k_hi;
     const int nb = plan(key0, k_hi);
     const int f_lo = sh.full_lo, f_hi = sh.full_hi;
-    // The cache row (of D bytes) of the block's key lt; kNoRow: reads zeros.
+    // Threads 0 .. 63: the cache row (of D bytes) of the block's key lt; kNoRow: reads zeros.
     constexpr uint32_t kNoRow = 0xffffffffu;
     uint32_t* offs = reinterpret_cast<uint32_t*>(smem + C::OFF0);
     auto offset = [&](int j) {
-      const int key = key0 + (nb - 1 - j) * kTile + lt;
+      if (lt >= kKeys || j >= nb) return;
+      const int key = key0 + OKC_BLOCK_AT(j) * kKeys + lt;
       uint32_t off = kNoRow;
-      if (j < nb && key < k_hi) {
+      if (key < k_hi) {
         const int page = a.page_table[(size_t)b * a.table_ld + key / a.P];
         if (page >= 0 && page < a.num_pages)
           off = (uint32_t)(((long long)page * a.P + key % a.P) * a.Hkv + head);
         else
           atomicOr(a.err, OKC_DEVERR_PAGE);
       }
-      offs[(j & 1) * kTile + lt] = off;
+      offs[(j & 1) * kKeys + lt] = off;
     };
     // the loading warps' barrier: whether any of them gave up (they leave together)
     auto sync_any = [&](bool bad) {
@@ -609,7 +616,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     };
     // A thread's 16-byte chunks: chunk `ch` of every KSTEP-th key from `kf` on.  Eight lanes take four
     // chunks of two neighbouring keys, which the swizzle puts into different banks.
-    constexpr int NCH = D / 16, PER = kTile * NCH / kLoadThreads, KSTEP = kTile / PER;
+    constexpr int NCH = D / 16, PER = kKeys * NCH / kLoadThreads, KSTEP = kKeys / PER;
     const int ch = NCH == 8 ? (lt & 3) + 4 * ((lt >> 3) & 1) : lt & 3;
     const int kf = 2 * (lt / (2 * NCH)) + ((lt >> 2) & 1);
     static_assert(KSTEP % 8 == 0, "a thread's keys share a swizzle");
@@ -629,45 +636,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
         *reinterpret_cast<uint4*>(base + at1 + i * KSTEP * 128) = make_uint4(o[4], o[5], o[6], o[7]);
       }
     };
-    // a block's K or V chunks of this thread, in flight until their conversion
-    auto fetch = [&](const uint8_t* cache, int j, uint4 (&r)[PER]) {
+    // a block's K and V chunks of this thread, in flight while the block before is converted
+    struct Chunks {
+      uint4 k[PER], v[PER];
+    };
+    auto fetch = [&](int j, Chunks& c) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const uint32_t row = offs[(j & 1) * kTile + kf + i * KSTEP];
-        r[i] = row != kNoRow ? *reinterpret_cast<const uint4*>(cache + (size_t)row * D + ch * 16) : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t row = offs[(j & 1) * kKeys + kf + i * KSTEP];
+        const size_t at = (size_t)row * D + ch * 16;
+        c.k[i] = c.v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row != kNoRow) {
+          c.k[i] = *reinterpret_cast<const uint4*>(a.k_cache + at);
+          c.v[i] = *reinterpret_cast<const uint4*>(a.v_cache + at);
+        }
       }
     };
-    uint4 kr[PER], vr[PER];
     bool ok = true;
-    offset(0);
-    sync_any(false);
-    if (nb > 0) fetch(a.k_cache, 0, kr);
-    for (int j = 0; j < nb; ++j) {
-      fetch(a.v_cache, j, vr);
-      offset(j + 1);
-      const int st = j & 1;
-      const uint32_t ph = ((uint32_t)(j >> 1) & 1u) ^ 1u;
-      const bool ok_k = mbar_wait(&sh.k_empty[st], ph, a.err, abort_flag);
-      store(smem + C::K0 + st * C::TILE_B, kr);
+    auto block = [&](int j, Chunks& now, Chunks& next) {  // false: given up
+      // the offsets of block j + 1 are there, and those of block j are read
+      if (sync_any(!ok)) return false;
+      if (j + 1 < nb) fetch(j + 1, next);
+      offset(j + 2);
+      const int st = j % kDepth, kb = key0 + OKC_BLOCK_AT(j) * kKeys;
+      ok = mbar_wait(&sh.kv_empty[st], ((uint32_t)(j / kDepth) & 1u) ^ 1u, a.err, abort_flag);
+      store(smem + C::K0 + st * C::BLOCK, now.k);
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.k_full[st]);
-      // the offsets of block j + 1 are there; those of block j are read
-      if (sync_any(!ok_k || !ok)) {
-        *abort_flag = 1;
-        break;
-      }
-      if (j + 1 < nb) fetch(a.k_cache, j + 1, kr);
-      ok = mbar_wait(&sh.v_empty[st], ph, a.err, abort_flag);  // the next block's barrier tells the others
-      const int kb = key0 + (nb - 1 - j) * kTile;
-      const bool edge = kb < f_lo || kb + kTile > f_hi;
-      if (edge) {
-        if (lt < 4) sh.nan[st][lt] = 0;
+      if (kb < f_lo || kb + kKeys > f_hi) {
+        if (lt < kKeys / 32) sh.nan[st][lt] = 0;
         sync_any(false);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const int key = kf + i * KSTEP;
-          uint32_t x[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w}, bad = 0;
+          uint32_t x[4] = {now.v[i].x, now.v[i].y, now.v[i].z, now.v[i].w}, bad = 0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t nan = ((x[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
@@ -675,72 +678,78 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
             x[k] &= ~((nan >> 7) * 0xffu);
           }
           if (bad) atomicOr(&sh.nan[st][key >> 5], 1u << (key & 31));
-          vr[i] = make_uint4(x[0], x[1], x[2], x[3]);
+          now.v[i] = make_uint4(x[0], x[1], x[2], x[3]);
         }
       }
-      store(smem + C::V0 + st * C::TILE_B, vr);
+      store(smem + C::V0 + st * C::BLOCK, now.v);
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.v_full[st]);
+      return true;
+    };
+    offset(0);
+    offset(1);
+    sync_any(false);
+    Chunks c0, c1;
+    if (nb > 0) fetch(0, c0);
+    for (int j = 0; j < nb; j += 2) {
+      if (!block(j, c0, c1) || (j + 1 < nb && !block(j + 1, c1, c0))) {
+        *abort_flag = 1;
+        break;
+      }
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-    // ------------------------------------------------------------------ MMA issue
-    if (warp == kIssueWarp && lane == 0) {
+    // ------------------------------------------------------------------ MMA issue, a warp per tile
+    const int w = warp - kIssueWarp;
+    if (w < 2 && lane == 0) {
       int key0, k_hi;
       const int nb = plan(key0, k_hi);
-      const int tiles = b >= 0 && (a.cu_q[b + 1] - a.cu_q[b]) * a.G - sh.tile * kPair > kTile ? 2 : 1;
-      const uint32_t tmem = sh.tmem;
-      const uint32_t id_s = umma_idesc_f16(kTile, false), id_o = umma_idesc_f16(D, true);
-      auto scores = [&](int w, int st) {
-        const uint64_t qa = umma_desc_sw128(smem_u32(smem + C::Q0 + w * C::TILE_B));
-        const uint64_t ka = umma_desc_sw128(smem_u32(smem + C::K0 + st * C::TILE_B));
+      const bool two = b >= 0 && (a.cu_q[b + 1] - a.cu_q[b]) * a.G - sh.tile * kPair > kTile;
+      const uint32_t t_s = sh.tmem + w * kTile, t_o = sh.tmem + 2 * kTile + w * D;
+      const uint32_t id_s = umma_idesc_f16(kKeys, false), id_o = umma_idesc_f16(D, true);
+      const uint64_t qa = umma_desc_sw128(smem_u32(smem + C::Q0 + w * C::QTILE));
+      auto scores = [&](int j) {  // S of block j
+        const uint64_t ka = umma_desc_sw128(smem_u32(smem + C::K0 + j % kDepth * C::BLOCK));
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t at = ((k / 4) * C::SUB + (k % 4) * 32) >> 4;
-          umma_ss(tmem + w * kTile, qa + at, ka + at, id_s, k != 0);
-        }
-        umma_commit(&sh.s_full[w]);
-      };
-      auto output = [&](int w, int st, bool acc) {
-        const uint64_t va = umma_desc_mn(smem_u32(smem + C::V0 + st * C::TILE_B), C::SUB);
-#pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          umma_ts(tmem + 2 * kTile + w * D, tmem + w * kTile + 8 * k, va + k * (2048 >> 4), id_o, acc || k != 0);
+        for (int k = 0; k < D / 16; ++k)
+          umma_ss(t_s + (j & 1) * kKeys, qa + (((k / 4) * C::QSUB + (k % 4) * 32) >> 4),
+                  ka + (((k / 4) * C::SUB + (k % 4) * 32) >> 4), id_s, k != 0);
       };
       bool ok = true;
-      if (nb > 0) {
-        ok = mbar_wait(&sh.q_full, 0, a.err, abort_flag) && mbar_wait(&sh.k_full[0], 0, a.err, abort_flag);
-        if (ok) {
-          tc_after();
-          for (int w = 0; w < tiles; ++w) scores(w, 0);
-          umma_commit(&sh.k_empty[0]);
-        }
-      }
-      for (int j = 0; ok && j < nb; ++j) {
-        const int st = j & 1, nx = st ^ 1;
-        ok = mbar_wait(&sh.v_full[st], (uint32_t)(j >> 1) & 1u, a.err, abort_flag);
-        for (int w = 0; ok && w < tiles; ++w) {
-          ok = mbar_wait(&sh.p_full[w], (uint32_t)j & 1u, a.err, abort_flag);
+      if (nb > 0 && (w == 0 || two)) {
+        ok = mbar_wait(&sh.q_full, 0, a.err, abort_flag);
+        for (int j = 0; ok && j < 2 && j < nb; ++j) {
+          ok = mbar_wait(&sh.k_full[j], 0, a.err, abort_flag);
           if (!ok) break;
           tc_after();
-          output(w, st, j > 0);
-          if (j + 1 < nb) {
-            if (w == 0) ok = mbar_wait(&sh.k_full[nx], (uint32_t)((j + 1) >> 1) & 1u, a.err, abort_flag);
+          scores(j);
+          umma_commit(&sh.s_full[w][j]);
+        }
+        for (int j = 0; ok && j < nb; ++j) {
+          const int st = j % kDepth;
+          ok = mbar_wait(&sh.v_full[st], (uint32_t)(j / kDepth) & 1u, a.err, abort_flag) &&
+               mbar_wait(&sh.p_full[w][j & 1], (uint32_t)(j >> 1) & 1u, a.err, abort_flag);
+          if (!ok) break;
+          tc_after();
+          const uint64_t va = umma_desc_mn(smem_u32(smem + C::V0 + st * C::BLOCK), C::SUB);
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            umma_ts(t_o, t_s + (j & 1) * kKeys + 8 * k, va + k * (2048 >> 4), id_o, (j | k) != 0);
+          umma_commit(&sh.kv_empty[st]);
+          if (!two) umma_commit(&sh.kv_empty[st]);  // (the barrier counts both tiles)
+          if (j + 2 < nb) {
+            ok = mbar_wait(&sh.k_full[(j + 2) % kDepth], (uint32_t)((j + 2) / kDepth) & 1u, a.err, abort_flag);
             if (!ok) break;
             tc_after();
-            scores(w, nx);  // over P: the tensor core takes a thread's MMAs in order, and the ones above read it
-          } else {
-            umma_commit(&sh.o_full[w]);
+            scores(j + 2);  // over P: the tensor core takes a thread's MMAs in order, and the ones above read it
           }
+          umma_commit(&sh.s_full[w][j & 1]);  // behind the last block: that P V of block j is done
         }
-        if (!ok) break;
-        umma_commit(&sh.v_empty[st]);
-        if (j + 1 < nb) umma_commit(&sh.k_empty[nx]);
+        if (!ok) *abort_flag = 1;
+        umma_commit(&sh.drain[w]);  // no MMA may be in flight when the tensor memory is released
+        mbar_wait(&sh.drain[w], 0, a.err);
       }
-      if (!ok) *abort_flag = 1;
-      umma_commit(&sh.drain);  // no MMA may be in flight when the tensor memory is released
-      mbar_wait(&sh.drain, 0, a.err);
     }
   }
 
