@@ -147,52 +147,23 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
     // ---- the lane's two rows ----
     const int rows = rq.n * a.G, r0 = rt * kRows;
     const int row0 = a.cu_q[b];
-    int lo[2], hi[2], pos[2];
+    int lo[2], hi[2], pos[2], tok[2], hq[2];
     bool live[2];
-    float slope[2], fac[2];
-    uint32_t qf[KS][4];
     const bool two = rows - r0 > 8;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = r0 + g + 8 * e;
       live[e] = r < rows;
-      const int i = live[e] ? r / a.G : 0, hq = head * a.G + (live[e] ? r - i * a.G : 0);
-      pos[e] = 0;
-      lo[e] = hi[e] = 0;
-      slope[e] = 0.f;
-      uint2 qv[KS];
-#pragma unroll
-      for (int k = 0; k < KS; ++k) qv[k] = make_uint2(0u, 0u);
+      tok[e] = live[e] ? r / a.G : 0;
+      hq[e] = head * a.G + (live[e] ? r - tok[e] * a.G : 0);
+      pos[e] = lo[e] = hi[e] = 0;
       if (live[e]) {
-        const RowSpan sp = row_span(a, rq, row0, i);
+        const RowSpan sp = row_span(a, rq, row0, tok[e]);
         pos[e] = sp.pos;
         lo[e] = sp.lo;
         hi[e] = sp.hi;
-        if (a.slopes) slope[e] = a.slopes[hq] * 1.4426950408889634f;
-        const __nv_bfloat16* qp = a.q + (size_t)(row0 + i) * a.ldq + (size_t)hq * D;
-#pragma unroll
-        for (int k = 0; k < KS; ++k)  // the four elements of step k's slots
-          qv[k] = *reinterpret_cast<const uint2*>(qp + 64 * (k >> 2) + 16 * c + 4 * (k & 3));
       }
-      uint32_t top = 0;
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-        top = max(max(top, max(qv[k].x & 0x7fffu, (qv[k].x >> 16) & 0x7fffu)),
-                  max(qv[k].y & 0x7fffu, (qv[k].y >> 16) & 0x7fffu));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int sh = f16_shift(top);
-      const float down = pow2(-sh);
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        qf[k][e] = h2(bf16_lo(qv[k].x) * down, bf16_hi(qv[k].x) * down);
-        qf[k][2 + e] = h2(bf16_lo(qv[k].y) * down, bf16_hi(qv[k].y) * down);
-      }
-      // without a cap: log2 units; with one: the argument of tanh times 2 log2(e)
-      fac[e] = a.k_scale[head] * a.sm_scale * (CAP ? 2.f / a.softcap : 1.f) * 1.4426950408889634f *
-               pow2(sh);
     }
-    const float cap2 = CAP ? a.softcap * 1.4426950408889634f : 0.f;
     // keys that every live row sees need no mask; keys outside [t_lo, t_hi) are not read
     int full_lo = max(live[0] ? lo[0] : 0, live[1] ? lo[1] : 0);
     int full_hi = min(live[0] ? hi[0] : 0x7fffffff, live[1] ? hi[1] : 0x7fffffff);
@@ -243,10 +214,6 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
 
-    float o_acc[ND][4];
-#pragma unroll
-    for (int n = 0; n < ND; ++n) o_acc[n][0] = o_acc[n][1] = o_acc[n][2] = o_acc[n][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     int page = fetch_page(s_lo);
 #pragma unroll
     for (int i = 0; i < C::STAGES - 1; ++i) {
@@ -254,6 +221,46 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
       issue(s_lo + i, page);
       page = next;
     }
+    // ---- the query, while the first keys are on their way ----
+    float slope[2], fac[2];
+    uint32_t qf[KS][4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      slope[e] = 0.f;
+      uint2 qv[KS];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) qv[k] = make_uint2(0u, 0u);
+      if (live[e]) {
+        if (a.slopes) slope[e] = a.slopes[hq[e]] * 1.4426950408889634f;
+        const __nv_bfloat16* qp = a.q + (size_t)(row0 + tok[e]) * a.ldq + (size_t)hq[e] * D;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)  // the four elements of step k's slots
+          qv[k] = *reinterpret_cast<const uint2*>(qp + 64 * (k >> 2) + 16 * c + 4 * (k & 3));
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        top = max(max(top, max(qv[k].x & 0x7fffu, (qv[k].x >> 16) & 0x7fffu)),
+                  max(qv[k].y & 0x7fffu, (qv[k].y >> 16) & 0x7fffu));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int sh = f16_shift(top);
+      const float down = pow2(-sh);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        qf[k][e] = h2(bf16_lo(qv[k].x) * down, bf16_hi(qv[k].x) * down);
+        qf[k][2 + e] = h2(bf16_lo(qv[k].y) * down, bf16_hi(qv[k].y) * down);
+      }
+      // without a cap: log2 units; with one: the argument of tanh times 2 log2(e)
+      fac[e] = a.k_scale[head] * a.sm_scale * (CAP ? 2.f / a.softcap : 1.f) * 1.4426950408889634f *
+               pow2(sh);
+    }
+    const float cap2 = CAP ? a.softcap * 1.4426950408889634f : 0.f;
+
+    float o_acc[ND][4];
+#pragma unroll
+    for (int n = 0; n < ND; ++n) o_acc[n][0] = o_acc[n][1] = o_acc[n][2] = o_acc[n][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
     for (int s = s_lo; s < s_hi; ++s) {
       const int next = fetch_page(s + C::STAGES);
@@ -483,8 +490,8 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
   }
 }
 
-// Joins the segments of one output row (token, query head): warps w, w + WPR, .. of the row take
-// its segments, then warp 0 the warps' sums.  o = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s.
+// Joins the segments of one output row (token, query head): WPR warps take its segments in turn, then
+// the first the warps' sums.  o = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s.
 template <int D, int WPR>
 __global__ void __launch_bounds__(256) attn_chunk_merge_kernel(ChunkArgs a, SplitPlan pl) {
   constexpr int E = D / 32;  // elements a lane
@@ -518,20 +525,21 @@ __global__ void __launch_bounds__(256) attn_chunk_merge_kernel(ChunkArgs a, Spli
       const int U = pl.pre_u[a.B], first = pl.pre_u[b] + in_t * nc;
       const int s0 = unit_owner(U, pl.ctas, first), s1 = unit_owner(U, pl.ctas, first + nc - 1) + 1;
       const size_t in_slot = (size_t)(h % pl.nh) * kRows + r % kRows, per = (size_t)pl.nh * kRows;
-      for (int base = s0 + sub * 32; base < s1; base += 32 * WPR) {
+      for (int base = s0 + sub; base < s1; base += 32 * WPR) {  // segments base, base + WPR, ..: a lane each
+        const int mine_at = base + lane * WPR;
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (base + lane < s1) ml = *reinterpret_cast<const float2*>(pl.ml + ((size_t)(base + lane + tile) * per + in_slot) * 2);
+        if (mine_at < s1) ml = *reinterpret_cast<const float2*>(pl.ml + ((size_t)(mine_at + tile) * per + in_slot) * 2);
         const float nm = fmaxf(M, warp_max(ml.x)), org = nm == -INFINITY ? 0.f : nm;
         const float old = ex2(M - org), w = ex2(ml.x - org);
         M = nm;
         L = L * old + warp_sum(w * ml.y);
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] *= old;
-        const int cnt = min(32, s1 - base);
-#pragma unroll 4
+        const int cnt = min(32, (s1 - base + WPR - 1) / WPR);
+#pragma unroll 8
         for (int i = 0; i < cnt; ++i) {
           const float wi = __shfl_sync(0xffffffffu, w, i);
-          const float* src = pl.acc + ((size_t)(base + i + tile) * per + in_slot) * D + lane * E;
+          const float* src = pl.acc + ((size_t)(base + i * WPR + tile) * per + in_slot) * D + lane * E;
           if (E == 4) {
             const float4 v = *reinterpret_cast<const float4*>(src);
             o[0] += wi * v.x;
