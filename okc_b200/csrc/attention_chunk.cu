@@ -9,8 +9,9 @@
 // and a row that sees nothing is zero.
 //
 // Bound by the cache read (2 D bytes a key and KV head).  The rows of one KV head's query group
-// (token-major, G heads a token) fill the 16 rows of mma.sync tiles; e4m3 keys and values are exact in
-// f16, the query too once its row is scaled by a power of two, and P is rounded to f16 (2^-11).
+// (token-major, G heads a token) fill the 16 rows of mma.sync tiles, or, where no request has more than 8,
+// their 8 columns with keys and outputs as the rows: half the MMAs and half the accumulators.  e4m3 keys and
+// values are exact in f16, the query too once its row is scaled by a power of two, and P is rounded to f16 (2^-11).
 //  * units of 32 keys x (8 / nh) subgroups of a (request, row tile, nh heads) are numbered in order
 //    and split evenly over a persistent grid (ragged contexts stay balanced); the nh heads of a
 //    key lie side by side in the cache, so the block's warps read whole token rows together;
@@ -29,7 +30,6 @@ namespace {
 
 constexpr int kStep = 32;      // keys per warp step
 constexpr int kWarps = 8;
-constexpr int kRows = 16;
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
@@ -46,6 +46,7 @@ struct ChunkCfg {
 struct SplitPlan {
   int nh, nsub, hg;   // heads side by side in a block, key subgroups, head groups
   int step_keys;      // keys of a unit
+  int rows;           // rows of a tile: 16, or 8 where no request has more
   int ctas;
   int* pre_u;         // [B + 1] units before a request
   int* pre_t;         // [B + 1] row tiles (times head groups) before a request
@@ -77,7 +78,7 @@ __device__ __forceinline__ void split_prefix(const ChunkArgs& a, const SplitPlan
       const int rows = r.n * a.G;
       if (r.len > a.max_keys && blockIdx.x == 0) atomicOr(a.err, OKC_DEVERR_PAGE);
       if (rows <= pl.most_rows) {
-        t = (rows + kRows - 1) / kRows * pl.hg;
+        t = (rows + pl.rows - 1) / pl.rows * pl.hg;
         u = t * ((max(0, r.hi - r.lo) + pl.step_keys - 1) / pl.step_keys);
       }
     }
@@ -103,11 +104,12 @@ __device__ __forceinline__ void split_prefix(const ChunkArgs& a, const SplitPlan
   }
 }
 
-template <int D, bool CAP>
+template <int D, bool CAP, int R>
 __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs a, SplitPlan pl) {
   using C = ChunkCfg<D>;
   constexpr int KS = D / 16;   // k16 steps of QK
-  constexpr int ND = D / 8;    // n8 blocks of PV
+  constexpr int ND = R == 16 ? D / 8 : D / 16;  // PV blocks: 8 columns, or 16 rows, of the output
+  constexpr int GAP = R == 16 ? 8 : 1;          // a lane's two rows in the softmax: first and first + GAP
   constexpr int NCH = D / 16;  // 16-byte chunks of a key
   extern __shared__ __align__(128) uint8_t smem[];
   int* pre_u = reinterpret_cast<int*>(smem + C::SMEM);
@@ -145,14 +147,15 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
     u0 += c1 - c0;
 
     // ---- the lane's two rows ----
-    const int rows = rq.n * a.G, r0 = rt * kRows;
+    const int rows = rq.n * a.G, r0 = rt * R;
+    const int first = R == 16 ? g : 2 * c;
     const int row0 = a.cu_q[b];
     int lo[2], hi[2], pos[2], tok[2], hq[2];
     bool live[2];
-    const bool two = rows - r0 > 8;
+    const bool two = R == 8 || rows - r0 > 8;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = r0 + g + 8 * e;
+      const int r = r0 + first + GAP * e;
       live[e] = r < rows;
       tok[e] = live[e] ? r / a.G : 0;
       hq[e] = head * a.G + (live[e] ? r - tok[e] * a.G : 0);
@@ -222,17 +225,19 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
       page = next;
     }
     // ---- the query, while the first keys are on their way ----
+    // R = 16: rows g and g + 8 as the A operand.  R = 8: row g as the B operand, whose scale the lanes that
+    // have the row in the softmax fetch from it.
     float slope[2], fac[2];
-    uint32_t qf[KS][4];
+    uint32_t qf[KS][R == 16 ? 4 : 2];
+    float up[2];  // what undoes the row's scale
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      slope[e] = 0.f;
+    for (int e = 0; e < R / 8; ++e) {
+      const int r = r0 + g + 8 * e, t = r / a.G;
       uint2 qv[KS];
 #pragma unroll
       for (int k = 0; k < KS; ++k) qv[k] = make_uint2(0u, 0u);
-      if (live[e]) {
-        if (a.slopes) slope[e] = a.slopes[hq[e]] * 1.4426950408889634f;
-        const __nv_bfloat16* qp = a.q + (size_t)(row0 + tok[e]) * a.ldq + (size_t)hq[e] * D;
+      if (r < rows) {
+        const __nv_bfloat16* qp = a.q + (size_t)(row0 + t) * a.ldq + (size_t)(head * a.G + r - t * a.G) * D;
 #pragma unroll
         for (int k = 0; k < KS; ++k)  // the four elements of step k's slots
           qv[k] = *reinterpret_cast<const uint2*>(qp + 64 * (k >> 2) + 16 * c + 4 * (k & 3));
@@ -246,14 +251,23 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int sh = f16_shift(top);
       const float down = pow2(-sh);
+      up[e] = pow2(sh);
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         qf[k][e] = h2(bf16_lo(qv[k].x) * down, bf16_hi(qv[k].x) * down);
-        qf[k][2 + e] = h2(bf16_lo(qv[k].y) * down, bf16_hi(qv[k].y) * down);
+        qf[k][R / 8 + e] = h2(bf16_lo(qv[k].y) * down, bf16_hi(qv[k].y) * down);
       }
+    }
+    if (R == 8) {
+      const float mine = up[0];
+      up[0] = __shfl_sync(0xffffffffu, mine, 8 * c);
+      up[1] = __shfl_sync(0xffffffffu, mine, 8 * c + 4);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      slope[e] = live[e] && a.slopes ? a.slopes[hq[e]] * 1.4426950408889634f : 0.f;
       // without a cap: log2 units; with one: the argument of tanh times 2 log2(e)
-      fac[e] = a.k_scale[head] * a.sm_scale * (CAP ? 2.f / a.softcap : 1.f) * 1.4426950408889634f *
-               pow2(sh);
+      fac[e] = a.k_scale[head] * a.sm_scale * (CAP ? 2.f / a.softcap : 1.f) * 1.4426950408889634f * up[e];
     }
     const float cap2 = CAP ? a.softcap * 1.4426950408889634f : 0.f;
 
@@ -273,94 +287,128 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
       const uint8_t* vs = ks + kStep * D;
       const int kb0 = k0 + s * pl.step_keys;
 
-      // S: block 2 kb + h, column n <-> key 16 kb + 4 (n / 2) + n % 2 + 2 h
+      // S, keys permuted: within 16 of them, block h's n-th is 4 (n / 2) + n % 2 + 2 h.
+      // R = 16: sc[2 kb + h], rows g and g + 8, column n = key.  R = 8: sc[2 kb] and sc[2 kb + 1] are the halves
+      // h of a 16-key tile, row n = key g, columns 2 c, 2 c + 1 the lane's two rows.
       float sc[4][4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+      for (int n = 0; n < 4; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+      auto key_words = [&](int n, int v) {  // the lane's chunk of its key of block n
         const int k = 16 * (n >> 1) + 4 * (g >> 1) + (g & 1) + 2 * (n & 1);
+        int ch = c + 4 * v;
+        if (D == 128) ch ^= 4 * (k & 1);
+        return *reinterpret_cast<const uint4*>(ks + k * D + ch * 16);
+      };
+      if constexpr (R == 16) {
 #pragma unroll
-        for (int v = 0; v < D / 64; ++v) {
-          int ch = c + 4 * v;
-          if (D == 128) ch ^= 4 * (k & 1);
-          const uint4 kv = *reinterpret_cast<const uint4*>(ks + k * D + ch * 16);
-          const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            mma_f16_16816(sc[n], qf[4 * v + i][0], qf[4 * v + i][1], qf[4 * v + i][2], qf[4 * v + i][3],
-                          e4m3x2_h2(w[i] & 0xffffu), e4m3x2_h2(w[i] >> 16));
+          for (int v = 0; v < D / 64; ++v) {
+            const uint4 kv = key_words(n, v);
+            const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              mma_f16_16816(sc[n], qf[4 * v + i][0], qf[4 * v + i][1], qf[4 * v + i][R / 8], qf[4 * v + i][R / 8 + 1],
+                            e4m3x2_h2(w[i] & 0xffffu), e4m3x2_h2(w[i] >> 16));
+          }
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int v = 0; v < D / 64; ++v) {
+            const uint4 k0v = key_words(2 * kb, v), k1v = key_words(2 * kb + 1, v);
+            const uint32_t w0[4] = {k0v.x, k0v.y, k0v.z, k0v.w}, w1[4] = {k1v.x, k1v.y, k1v.z, k1v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              mma_f16_16816(sc[2 * kb], e4m3x2_h2(w0[i] & 0xffffu), e4m3x2_h2(w1[i] & 0xffffu), e4m3x2_h2(w0[i] >> 16),
+                            e4m3x2_h2(w1[i] >> 16), qf[4 * v + i][0], qf[4 * v + i][1]);
+          }
+        // to the order of the other form: sc[2 kb + h][i], i = the lane's row
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          sc[2 * kb + 1][0] = sc[2 * kb][2];
+          sc[2 * kb + 1][1] = sc[2 * kb][3];
         }
       }
       // scores, running maximum, P
       const bool edge = kb0 < full_lo || kb0 + kStep > full_hi;
-      uint32_t pf[2][4];
+      constexpr int X = R == 16 ? 8 : 4;  // a lane's keys of a row
+      auto key_of = [&](int i) {          // its i-th
+        return R == 16 ? kb0 + 16 * (i >> 2) + 4 * c + (i & 1) + 2 * ((i >> 1) & 1)
+                       : kb0 + 16 * (i >> 1) + 4 * (g >> 1) + (g & 1) + 2 * (i & 1);
+      };
+      float x[2][X];
       float corr[2] = {1.f, 1.f};
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         if (e == 1 && !two) {
-          pf[0][1] = pf[0][3] = pf[1][1] = pf[1][3] = 0u;
+#pragma unroll
+          for (int i = 0; i < X; ++i) x[1][i] = 0.f;
           break;
         }
-        float x[8];  // block n, column 2 c + i: key 16 (n / 2) + 4 c + i + 2 (n % 2)
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            // rounded here: fused into the subtraction below, a large score could exceed the maximum
-            float v = __fmul_rn(sc[n][2 * e + i], fac[e]);
-            if (CAP) v = __fmul_rn(cap2, tanh_from_2l2e(v));
-            x[2 * n + i] = v;
-          }
+        for (int i = 0; i < X; ++i) {
+          // rounded here: fused into the subtraction below, a large score could exceed the maximum
+          float v = __fmul_rn(R == 16 ? sc[i >> 1][2 * e + (i & 1)] : sc[i][e], fac[e]);
+          if (CAP) v = __fmul_rn(cap2, tanh_from_2l2e(v));
+          x[e][i] = v;
+        }
         if (a.slopes) {
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int key = kb0 + 16 * (n >> 1) + 4 * c + i + 2 * (n & 1);
-              x[2 * n + i] -= slope[e] * (float)abs(pos[e] - key);
-            }
+          for (int i = 0; i < X; ++i) x[e][i] -= slope[e] * fabsf((float)(pos[e] - kb0) - (float)(key_of(i) - kb0));
         }
         if (edge) {
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int key = kb0 + 16 * (n >> 1) + 4 * c + i + 2 * (n & 1);
-              if (key < lo[e] || key >= hi[e]) x[2 * n + i] = -INFINITY;
-            }
+          for (int i = 0; i < X; ++i)
+            if (key_of(i) < lo[e] || key_of(i) >= hi[e]) x[e][i] = -INFINITY;
         }
-        float top = x[0];
+        float top = x[e][0];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        for (int i = 1; i < X; ++i) top = fmaxf(top, x[e][i]);
+        // over the lanes that have the row: c, or g
+#pragma unroll
+        for (int s = R == 16 ? 1 : 4; s < (R == 16 ? 4 : 32); s *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
         const float nm = fmaxf(m[e], top);
         const float org = nm == -INFINITY ? 0.f : nm;  // nothing seen yet: any finite origin
         corr[e] = ex2(m[e] - org);
         m[e] = nm;
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = ex2(x[i] - org);
-          sum += x[i];
+        for (int i = 0; i < X; ++i) {
+          x[e][i] = ex2(x[e][i] - org);
+          sum += x[e][i];
         }
         l[e] = l[e] * corr[e] + sum;
+      }
+      // P: the A operand (R = 16), or turned into the B operand, block by block
+      uint32_t pf[2][R == 16 ? 4 : 2];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          pf[kb][e] = h2(x[4 * kb], x[4 * kb + 1]);
-          pf[kb][2 + e] = h2(x[4 * kb + 2], x[4 * kb + 3]);
+      for (int kb = 0; kb < 2; ++kb) {
+        if constexpr (R == 16) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            pf[kb][e] = h2(x[e][4 * kb], x[e][4 * kb + 1]);
+            pf[kb][R / 8 + e] = h2(x[e][4 * kb + 2], x[e][4 * kb + 3]);
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t own = h2(x[0][2 * kb + h], x[1][2 * kb + h]);
+            asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pf[kb][h]) : "r"(own));
+          }
         }
       }
       if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
           o_acc[n][0] *= corr[0];
-          o_acc[n][1] *= corr[0];
-          o_acc[n][2] *= corr[1];
+          o_acc[n][1] *= corr[R == 16 ? 0 : 1];
+          o_acc[n][2] *= corr[R == 16 ? 1 : 0];
           o_acc[n][3] *= corr[1];
         }
       }
-      // O += P V: column n of block nb <-> d = (D / 8) n + nb
+      // O += P V.  R = 16: column n of block nb <-> d = (D / 8) n + nb.  R = 8, transposed: rows n and n + 8 of block nb
+      // <-> d = (D / 8) n + 2 nb and the next.
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         constexpr int W = D / 32;  // words of a lane's share of a key
@@ -398,12 +446,13 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
               for (int n = 0; n < ND; ++n)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                  const int kk = 16 * kb + k, d = (D / 8) * (2 * c + i) + n, key = kb0 + kk;
+                  const int kk = 16 * kb + k, key = kb0 + kk;
+                  const int d = R == 16 ? (D / 8) * (2 * c + i) + n : (D / 8) * g + 2 * n + i;
                   int ch = d / 16;
                   if (D == 128) ch ^= 2 * ((kk >> 2) & 3);
                   if ((vs[kk * D + ch * 16 + d % 16] & 0x7f) == 0x7f) {
-                    if (key >= lo[0] && key < hi[0]) o_acc[n][i] = __uint_as_float(0x7fffffffu);
-                    if (key >= lo[1] && key < hi[1]) o_acc[n][2 + i] = __uint_as_float(0x7fffffffu);
+                    if (key >= lo[0] && key < hi[0]) o_acc[n][R == 16 ? i : 2 * i] = __uint_as_float(0x7fffffffu);
+                    if (key >= lo[1] && key < hi[1]) o_acc[n][R == 16 ? 2 + i : 2 * i + 1] = __uint_as_float(0x7fffffffu);
                   }
                 }
           }
@@ -412,40 +461,53 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
         for (int w = 0; w < W; ++w) {
           const uint32_t a01 = prmt(vw[0][w], vw[1][w], 0x5140), b01 = prmt(vw[0][w], vw[1][w], 0x7362);
           const uint32_t a23 = prmt(vw[2][w], vw[3][w], 0x5140), b23 = prmt(vw[2][w], vw[3][w], 0x7362);
-          mma_f16_16816(o_acc[4 * w + 0], pf[kb][0], pf[kb][1], pf[kb][2], pf[kb][3], e4m3x2_h2(a01 & 0xffffu),
-                        e4m3x2_h2(a23 & 0xffffu));
-          mma_f16_16816(o_acc[4 * w + 1], pf[kb][0], pf[kb][1], pf[kb][2], pf[kb][3], e4m3x2_h2(a01 >> 16),
-                        e4m3x2_h2(a23 >> 16));
-          mma_f16_16816(o_acc[4 * w + 2], pf[kb][0], pf[kb][1], pf[kb][2], pf[kb][3], e4m3x2_h2(b01 & 0xffffu),
-                        e4m3x2_h2(b23 & 0xffffu));
-          mma_f16_16816(o_acc[4 * w + 3], pf[kb][0], pf[kb][1], pf[kb][2], pf[kb][3], e4m3x2_h2(b01 >> 16),
-                        e4m3x2_h2(b23 >> 16));
+          if constexpr (R == 16) {
+            auto col = [&](int n, uint32_t b0, uint32_t b1) {
+              mma_f16_16816(o_acc[4 * w + n], pf[kb][0], pf[kb][1], pf[kb][R / 8], pf[kb][R / 8 + 1], e4m3x2_h2(b0),
+                            e4m3x2_h2(b1));
+            };
+            col(0, a01 & 0xffffu, a23 & 0xffffu);
+            col(1, a01 >> 16, a23 >> 16);
+            col(2, b01 & 0xffffu, b23 & 0xffffu);
+            col(3, b01 >> 16, b23 >> 16);
+          } else {
+            mma_f16_16816(o_acc[2 * w], e4m3x2_h2(a01 & 0xffffu), e4m3x2_h2(a01 >> 16), e4m3x2_h2(a23 & 0xffffu),
+                          e4m3x2_h2(a23 >> 16), pf[kb][0], pf[kb][1]);
+            mma_f16_16816(o_acc[2 * w + 1], e4m3x2_h2(b01 & 0xffffu), e4m3x2_h2(b01 >> 16), e4m3x2_h2(b23 & 0xffffu),
+                          e4m3x2_h2(b23 >> 16), pf[kb][0], pf[kb][1]);
+          }
         }
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+#pragma unroll
+      for (int s = R == 16 ? 1 : 4; s < (R == 16 ? 4 : 32); s *= 2) l[e] += __shfl_xor_sync(0xffffffffu, l[e], s);
     }
+
+    // Row first + GAP e of the tile: this lane's part of its outputs, from d0 on, is part(e, 0 .. NP - 1).
+    constexpr int NP = R == 16 ? D / 4 : D / 8;
+    const int d0 = R == 16 ? (D / 4) * c : (D / 8) * g;
+    auto part = [&](int e, int i) -> float& {
+      if constexpr (R == 16) return o_acc[i % ND][2 * e + i / ND];
+      else return o_acc[i / 2][2 * (i % 2) + e];
+    };
+    const bool leads = R == 16 ? c == 0 : g == 0;  // the lane that tells a row's maximum and sum
 
     // ---- join the key subgroups of a head in shared memory, in order ----
     if (pl.nsub > 1) {
-      float* mine = reinterpret_cast<float*>(ring);  // [16][D] and [16][2]
+      float* mine = reinterpret_cast<float*>(ring);  // [R][D] and [R][2]
       __syncwarp();
       if (sub > 0) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float* dst = mine + (g + 8 * e) * D + (D / 4) * c;
+          const int r = first + GAP * e;
 #pragma unroll
-          for (int n = 0; n < ND; ++n) {
-            dst[n] = o_acc[n][2 * e];
-            dst[D / 8 + n] = o_acc[n][2 * e + 1];
-          }
-          if (c == 0) {
-            mine[kRows * D + 2 * (g + 8 * e)] = m[e];
-            mine[kRows * D + 2 * (g + 8 * e) + 1] = l[e];
+          for (int i = 0; i < NP; ++i) mine[r * D + d0 + i] = part(e, i);
+          if (leads) {
+            mine[R * D + 2 * r] = m[e];
+            mine[R * D + 2 * r + 1] = l[e];
           }
         }
       }
@@ -455,17 +517,14 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
           const float* from = reinterpret_cast<const float*>(smem + (warp + s2 * pl.nh) * C::RING);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float om = from[kRows * D + 2 * (g + 8 * e)], ol = from[kRows * D + 2 * (g + 8 * e) + 1];
+            const int r = first + GAP * e;
+            const float om = from[R * D + 2 * r], ol = from[R * D + 2 * r + 1];
             const float nm = fmaxf(m[e], om), org = nm == -INFINITY ? 0.f : nm;
             const float fa = ex2(m[e] - org), fb = ex2(om - org);
             m[e] = nm;
             l[e] = l[e] * fa + ol * fb;
-            const float* src = from + (g + 8 * e) * D + (D / 4) * c;
 #pragma unroll
-            for (int n = 0; n < ND; ++n) {
-              o_acc[n][2 * e] = o_acc[n][2 * e] * fa + src[n] * fb;
-              o_acc[n][2 * e + 1] = o_acc[n][2 * e + 1] * fa + src[D / 8 + n] * fb;
-            }
+            for (int i = 0; i < NP; ++i) part(e, i) = part(e, i) * fa + from[r * D + d0 + i] * fb;
           }
         }
       }
@@ -475,15 +534,11 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         if (!live[e]) continue;
-        const size_t r = ((size_t)slot * pl.nh + hw) * kRows + g + 8 * e;
-        float4* dst = reinterpret_cast<float4*>(pl.acc + r * D + (D / 4) * c);
+        const size_t r = ((size_t)slot * pl.nh + hw) * R + first + GAP * e;
+        float4* dst = reinterpret_cast<float4*>(pl.acc + r * D + d0);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int n = 0; n < ND; n += 4)
-            dst[(i * ND + n) / 4] = make_float4(o_acc[n][2 * e + i], o_acc[n + 1][2 * e + i], o_acc[n + 2][2 * e + i],
-                                                o_acc[n + 3][2 * e + i]);
-        if (c == 0) *reinterpret_cast<float2*>(pl.ml + r * 2) = make_float2(m[e], l[e]);
+        for (int i = 0; i < NP; i += 4) dst[i / 4] = make_float4(part(e, i), part(e, i + 1), part(e, i + 2), part(e, i + 3));
+        if (leads) *reinterpret_cast<float2*>(pl.ml + r * 2) = make_float2(m[e], l[e]);
       }
     }
     __syncwarp();  // the ring is refilled
@@ -521,10 +576,10 @@ __global__ void __launch_bounds__(256) attn_chunk_merge_kernel(ChunkArgs a, Spli
     const int nc = (max(0, rq.hi - rq.lo) + pl.step_keys - 1) / pl.step_keys;
     if (mine && nc > 0) {
       const int h = hq / a.G, r = (t - a.cu_q[b]) * a.G + hq - h * a.G;
-      const int in_t = (r / kRows) * pl.hg + h / pl.nh, tile = pl.pre_t[b] + in_t;
+      const int in_t = (r / pl.rows) * pl.hg + h / pl.nh, tile = pl.pre_t[b] + in_t;
       const int U = pl.pre_u[a.B], first = pl.pre_u[b] + in_t * nc;
       const int s0 = unit_owner(U, pl.ctas, first), s1 = unit_owner(U, pl.ctas, first + nc - 1) + 1;
-      const size_t in_slot = (size_t)(h % pl.nh) * kRows + r % kRows, per = (size_t)pl.nh * kRows;
+      const size_t in_slot = (size_t)(h % pl.nh) * pl.rows + r % pl.rows, per = (size_t)pl.nh * pl.rows;
       for (int base = s0 + sub; base < s1; base += 32 * WPR) {  // segments base, base + WPR, ..: a lane each
         const int mine_at = base + lane * WPR;
         float2 ml = make_float2(-INFINITY, 0.f);
@@ -586,18 +641,18 @@ int heads_a_block(int Hkv) { return Hkv % 8 == 0 ? 8 : Hkv % 4 == 0 ? 4 : Hkv % 
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
-size_t split_slots(int T, int B, int Hq, int Hkv) {
+size_t split_slots(int T, int B, int Hq, int Hkv, int rows) {
   const size_t hg = Hkv / heads_a_block(Hkv);
-  return okc_host::num_sms() + (((size_t)T * (Hq / Hkv) + kRows - 1) / kRows + B) * hg;
+  return okc_host::num_sms() + (((size_t)T * (Hq / Hkv) + rows - 1) / rows + B) * hg;
 }
 
-template <int D, bool CAP>
-int launch_split(const ChunkArgs& a, SplitPlan& pl, cudaStream_t stream) {
+template <int D, bool CAP, int R>
+int launch_split(const ChunkArgs& a, const SplitPlan& pl, cudaStream_t stream) {
   using C = ChunkCfg<D>;
   const int smem = C::SMEM + 2 * (a.B + 1) * 4;
   static okc_host::PerDevice configured;
-  if (int st = configured.smem(attn_chunk_split_kernel<D, CAP>, C::SMEM + 2 * (kMaxChunkRequests + 1) * 4)) return st;
-  if (int st = okc_host::launch_k(attn_chunk_split_kernel<D, CAP>, dim3(pl.ctas), dim3(32 * kWarps), smem, stream,
+  if (int st = configured.smem(attn_chunk_split_kernel<D, CAP, R>, C::SMEM + 2 * (kMaxChunkRequests + 1) * 4)) return st;
+  if (int st = okc_host::launch_k(attn_chunk_split_kernel<D, CAP, R>, dim3(pl.ctas), dim3(32 * kWarps), smem, stream,
                                   dim3(1), a, pl))
     return st;
   const long long items = (long long)(pl.merge_tokens > 0 ? (long long)a.B * pl.merge_tokens : a.T) * a.Hq;
@@ -611,7 +666,8 @@ int launch_split(const ChunkArgs& a, SplitPlan& pl, cudaStream_t stream) {
 }  // namespace
 
 size_t attn_chunk_ws_bytes(int T, int B, int Hq, int Hkv, int D) {
-  const size_t rows = split_slots(T, B, Hq, Hkv) * heads_a_block(Hkv) * kRows;
+  // 16-row tiles need the more: up to B tiles more of twice the rows
+  const size_t rows = split_slots(T, B, Hq, Hkv, 16) * heads_a_block(Hkv) * 16;
   return 2 * up((size_t)(B + 1) * 4) + up(rows * 8) + up(rows * D * 4) + attn_chunk_tc_ws_bytes(T, B, Hq, Hkv, D);
 }
 
@@ -626,7 +682,8 @@ int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
   const bool split_only = a.max_q > 0 ? (long long)a.max_q * a.G <= kSplitRows : (long long)a.T * a.G <= kSplitRows;
   pl.most_rows = split_only ? 0x7fffffff : kSplitRows;
   pl.merge_tokens = split_only ? 0 : kSplitRows / a.G;
-  const size_t rows = split_slots(a.T, a.B, a.Hq, a.Hkv) * pl.nh * kRows;
+  pl.rows = split_only && a.max_q > 0 && (long long)a.max_q * a.G <= 8 ? 8 : 16;
+  const size_t rows = split_slots(a.T, a.B, a.Hq, a.Hkv, pl.rows) * pl.nh * pl.rows;
   uint8_t* p = reinterpret_cast<uint8_t*>(a.ws);
   pl.pre_u = reinterpret_cast<int*>(p);
   p += up((size_t)(a.B + 1) * 4);
@@ -640,8 +697,13 @@ int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
     if (int st = launch_attn_chunk_tc(a, p, stream)) return st;
     if (pl.merge_tokens == 0) return OKC_OK;  // no request is short enough
   }
-  if (a.D == 64) return a.softcap > 0.f ? launch_split<64, true>(a, pl, stream) : launch_split<64, false>(a, pl, stream);
-  return a.softcap > 0.f ? launch_split<128, true>(a, pl, stream) : launch_split<128, false>(a, pl, stream);
+  const bool cap = a.softcap > 0.f;
+  if (a.D == 64) {
+    if (pl.rows == 8) return cap ? launch_split<64, true, 8>(a, pl, stream) : launch_split<64, false, 8>(a, pl, stream);
+    return cap ? launch_split<64, true, 16>(a, pl, stream) : launch_split<64, false, 16>(a, pl, stream);
+  }
+  if (pl.rows == 8) return cap ? launch_split<128, true, 8>(a, pl, stream) : launch_split<128, false, 8>(a, pl, stream);
+  return cap ? launch_split<128, true, 16>(a, pl, stream) : launch_split<128, false, 16>(a, pl, stream);
 }
 
 }  // namespace okc
