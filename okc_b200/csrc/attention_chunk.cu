@@ -24,6 +24,8 @@
 // in block order, so results repeat bit for bit.
 #include "chunk_common.cuh"
 
+#include <type_traits>
+
 namespace okc {
 
 namespace {
@@ -105,7 +107,7 @@ __device__ __forceinline__ void split_prefix(const ChunkArgs& a, const SplitPlan
 }
 
 template <int D, bool CAP, int R>
-__global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs a, SplitPlan pl) {
+__global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) attn_chunk_split_kernel(ChunkArgs a, SplitPlan pl) {
   using C = ChunkCfg<D>;
   constexpr int KS = D / 16;   // k16 steps of QK
   constexpr int ND = R == 16 ? D / 8 : D / 16;  // PV blocks: 8 columns, or 16 rows, of the output
@@ -183,36 +185,35 @@ __global__ void __launch_bounds__(32 * kWarps) attn_chunk_split_kernel(ChunkArgs
     if (t_lo > k0 + kStep - 1) s_lo = (t_lo - (k0 + kStep - 1) + pl.step_keys - 1) / pl.step_keys;
     if (t_hi < k0 + (s_hi - 1) * pl.step_keys + 1) s_hi = t_hi <= k0 ? 0 : (t_hi - k0 + pl.step_keys - 1) / pl.step_keys;
     const int32_t* trow = a.page_table + (size_t)b * a.table_ld;
-    const size_t hoff = (size_t)head * D;
-    auto fetch_page = [&](int s) -> int {  // this lane's key of step s; -1: not read
+    auto fetch_page = [&](int s) -> int {  // of this lane's key of step s; what it is, issue() checks
       const int key = k0 + s * pl.step_keys + lane;
-      if (s >= s_hi || key < t_lo || key >= t_hi) return -1;
-      const int page = trow[key / a.P];
-      if (page < 0 || page >= a.num_pages) {
-        atomicOr(a.err, OKC_DEVERR_PAGE);
-        return -1;
-      }
-      return page;
+      return s < s_hi && lane < kStep && key >= t_lo && key < t_hi ? trow[page_of(a, key)] : -1;
     };
     auto issue = [&](int s, int page) {
       if (s < s_hi) {
         const int key = k0 + s * pl.step_keys + lane;
-        const long long off = page < 0 ? -1 : ((long long)page * a.P + key % a.P) * a.Hkv * D + (long long)hoff;
-        const uint32_t st = ring_s + (uint32_t)((s - s_lo) % C::STAGES) * C::STAGE;
+        const bool on = page >= 0 && page < a.num_pages;
+        if (!on && lane < kStep && key >= t_lo && key < t_hi) atomicOr(a.err, OKC_DEVERR_PAGE);
+        // rows of D bytes, below 2^32
+        const uint32_t row = on ? ((uint32_t)page * a.P + key - page_of(a, key) * a.P) * a.Hkv + head : 0u;
+        const uint32_t mask = __ballot_sync(0xffffffffu, on);
+        constexpr int KI = 32 / NCH;  // keys of an instruction
+        const int kl = lane / NCH, ch = lane % NCH;
+        const uint32_t st = ring_s + (uint32_t)((s - s_lo) % C::STAGES) * C::STAGE + kl * D;
+        const uint32_t kd = st + (D == 128 ? ch ^ (4 * (kl & 1)) : ch) * 16, vd = st + kStep * D;
+        const uint8_t* kp = a.k_cache + ch * 16;
+        const uint8_t* vp = a.v_cache + ch * 16;
+        auto copy = [&](auto whole) {
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-          const int k = i * (32 / NCH) + lane / NCH, ch = lane % NCH;
-          const long long o = __shfl_sync(0xffffffffu, off, k);
-          const bool on = o >= 0;
-          const size_t src = on ? (size_t)o + ch * 16 : 0;
-          int kc = ch, vc = ch;
-          if (D == 128) {
-            kc ^= 4 * (k & 1);
-            vc ^= 2 * ((k >> 2) & 3);
+          for (int i = 0; i < kStep / KI; ++i) {
+            const size_t src = (size_t)__shfl_sync(0xffffffffu, row, i * KI + kl) * D;
+            const bool in = decltype(whole)::value || (mask >> (i * KI + kl) & 1u);
+            cp16(kd + i * KI * D, kp + src, in);
+            cp16(vd + i * KI * D + (D == 128 ? ch ^ (2 * (i & 3)) : ch) * 16, vp + src, in);
           }
-          cp16(st + k * D + kc * 16, a.k_cache + src, on);
-          cp16(st + kStep * D + k * D + vc * 16, a.v_cache + src, on);
-        }
+        };
+        if (mask == (kStep == 32 ? 0xffffffffu : 0xffffu)) copy(std::true_type{});
+        else copy(std::false_type{});
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };

@@ -527,8 +527,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
           for (uint32_t bits = *reinterpret_cast<volatile uint32_t*>(&sh.nan[st][q]); bits; bits &= bits - 1) {
             const int key = kb + 32 * q + __ffs(bits) - 1;
             if (!live || key < me.lo || key >= me.hi) continue;
-            const int page = a.page_table[(size_t)b * a.table_ld + key / a.P];
-            const uint8_t* vr = a.v_cache + (((size_t)page * a.P + key % a.P) * a.Hkv + head) * D;
+            const int page = a.page_table[(size_t)b * a.table_ld + page_of(a, key)];
+            const uint8_t* vr = a.v_cache + (((size_t)page * a.P + key - page_of(a, key) * a.P) * a.Hkv + head) * D;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i)
               for (int c = 0; c < 32; ++c) nan_d[i] |= (uint32_t)((vr[32 * i + c] & 0x7f) == 0x7f) << c;
@@ -595,9 +595,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       const int key = key0 + OKC_BLOCK_AT(j) * kKeys + lt;
       uint32_t off = kNoRow;
       if (key < k_hi) {
-        const int page = a.page_table[(size_t)b * a.table_ld + key / a.P];
+        const int page = a.page_table[(size_t)b * a.table_ld + page_of(a, key)];
         if (page >= 0 && page < a.num_pages)
-          off = (uint32_t)(((long long)page * a.P + key % a.P) * a.Hkv + head);
+          off = (uint32_t)(((long long)page * a.P + key - page_of(a, key) * a.P) * a.Hkv + head);
         else
           atomicOr(a.err, OKC_DEVERR_PAGE);
       }
