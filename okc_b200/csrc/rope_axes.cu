@@ -20,9 +20,20 @@ namespace {
 constexpr int kRopeThreads = 256;
 constexpr int kMaxPairs = 128;
 
+// Four values to e4m3, to the nearest even one, overflow -> NaN.  The hardware's conversion saturates: it is
+// right up to 464, half a step above the largest number, where the tie goes to the even 448.
 __device__ __forceinline__ uint32_t e4m3x4_nosat(float a, float b, float c, float d) {
-  return (uint32_t)f_to_e4m3_nosat(a) | ((uint32_t)f_to_e4m3_nosat(b) << 8) | ((uint32_t)f_to_e4m3_nosat(c) << 16) |
-         ((uint32_t)f_to_e4m3_nosat(d) << 24);
+  uint32_t w;
+  asm("{\n .reg .b16 l, h;\n cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n"
+      " mov.b32 %0, {l, h};\n}"
+      : "=r"(w) : "f"(a), "f"(b), "f"(c), "f"(d));
+  if (fmaxf(fmaxf(fabsf(a), fabsf(b)), fmaxf(fabsf(c), fabsf(d))) > 464.f) {
+    if (fabsf(a) > 464.f) w |= 0x7fu;
+    if (fabsf(b) > 464.f) w |= 0x7f00u;
+    if (fabsf(c) > 464.f) w |= 0x7f0000u;
+    if (fabsf(d) > 464.f) w |= 0x7f000000u;
+  }
+  return w;
 }
 
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
@@ -49,45 +60,78 @@ __device__ __forceinline__ void store8_e4m3(uint8_t* p, const float (&f)[8], flo
 __global__ void __launch_bounds__(kRopeThreads) rope_axes_append_kernel(RopeAxesArgs a) {
   __shared__ float cs[kMaxPairs], sn[kMaxPairs];
   __shared__ int req;
+  __shared__ long long slot_of;
   pdl_trigger();
   pdl_wait();
   const int t = blockIdx.x;
-  if (threadIdx.x < 32) {
-    const int b = find_request(a.cu_q, a.B, t);
-    if (threadIdx.x == 0) req = b;
-  }
-  for (int i = threadIdx.x; i < a.R; i += kRopeThreads) {
-    const int axis = (int)((a.axis_bits[i >> 5] >> (2 * (i & 31))) & 3u);
-    const double ang = (double)a.positions[(size_t)axis * a.ld_pos + t] * (double)a.inv_freq[i];
-    const double turns = rint(ang * 0.15915494309189535);                 // 1 / (2 pi)
-    const float r = (float)fma(turns, -6.283185307179586, ang);           // 2 pi; in [-pi, pi]
-    sincosf(r, &sn[i], &cs[i]);
-  }
-  __syncthreads();
-  const int b = req;
-  if (b < 0) return;  // a row behind the last request
-  const long long pos = (long long)a.seq_lens[b] - a.cu_q[b + 1] + t;
-  long long slot = -1;
-  if (pos >= 0 && pos / a.P < a.max_pages) {
-    const int page = a.page_table[(size_t)b * a.table_ld + pos / a.P];
-    if (page >= 0 && page < a.num_pages) slot = (long long)page * a.P + pos % a.P;
-  }
-  if (slot < 0 && threadIdx.x == 0) atomicOr(a.err, OKC_DEVERR_PAGE);
-
   const __nv_bfloat16* row = a.qkv + (size_t)t * a.ldqkv;
-  __nv_bfloat16* qo = a.q_out + (size_t)t * a.ldq;
-  const size_t kv_row = slot < 0 ? 0 : (size_t)slot * a.Hkv * a.D;
   const int D = a.D, R = a.R;
   // items: 8 pairs of a q or k head, then 8 passed elements of a q or k head, then 8 of a v head
   const int rp = R / 8, pp = (D - 2 * R) / 8, vp = D / 8, hqk = a.Hq + a.Hkv;
   const int n_rot = hqk * rp, n_pass = hqk * pp, n_all = n_rot + n_pass + a.Hkv * vp;
-  for (int it = threadIdx.x; it < n_all; it += kRopeThreads) {
+  struct Item {
+    int head, u0, u1;  // elements u0 .. + 8 and, of pairs, u1 .. + 8
+    uint4 x, y;
+  };
+  auto fetch = [&](int it) {
+    Item m = {};
     if (it < n_rot) {
-      const int head = it / rp, i0 = (it - head * rp) * 8;
-      const int u0 = a.half ? i0 : 2 * i0, u1 = a.half ? i0 + R : 2 * i0 + 8;
-      float x[8], y[8], p[8], q[8];
-      unpack8(*reinterpret_cast<const uint4*>(row + (size_t)head * D + u0), x);
-      unpack8(*reinterpret_cast<const uint4*>(row + (size_t)head * D + u1), y);
+      m.head = it / rp;
+      const int i0 = (it - m.head * rp) * 8;
+      m.u0 = a.half ? i0 : 2 * i0;
+      m.u1 = a.half ? i0 + R : 2 * i0 + 8;
+      m.y = *reinterpret_cast<const uint4*>(row + (size_t)m.head * D + m.u1);
+    } else if (it < n_all) {
+      const bool is_v = it - n_rot >= n_pass;
+      const int per = is_v ? vp : pp, k = it - n_rot - (is_v ? n_pass : 0), h = k / per;
+      m.u0 = (k - h * per) * 8 + (is_v ? 0 : 2 * R);
+      m.head = is_v ? hqk + h : h;
+    }
+    if (it < n_all) m.x = *reinterpret_cast<const uint4*>(row + (size_t)m.head * D + m.u0);
+    return m;
+  };
+  Item next = fetch(threadIdx.x);  // on its way while the block finds its place in the cache
+
+  if (threadIdx.x < 32) {
+    const int b = find_request(a.cu_q, a.B, t);
+    if (threadIdx.x == 0) {
+      long long slot = -1;
+      if (b >= 0) {
+        const long long pos = (long long)a.seq_lens[b] - a.cu_q[b + 1] + t;
+        if (pos >= 0 && pos <= 0x7fffffff && (uint32_t)pos / (uint32_t)a.P < (uint32_t)a.max_pages) {
+          const uint32_t in_row = (uint32_t)pos / (uint32_t)a.P;
+          const int page = a.page_table[(size_t)b * a.table_ld + in_row];
+          if (page >= 0 && page < a.num_pages) slot = (long long)page * a.P + ((uint32_t)pos - in_row * a.P);
+        }
+        if (slot < 0) atomicOr(a.err, OKC_DEVERR_PAGE);
+      }
+      req = b;
+      slot_of = slot;
+    }
+  } else {
+    for (int i = threadIdx.x - 32; i < R; i += kRopeThreads - 32) {
+      const int axis = (int)((a.axis_bits[i >> 5] >> (2 * (i & 31))) & 3u);
+      const double ang = (double)a.positions[(size_t)axis * a.ld_pos + t] * (double)a.inv_freq[i];
+      const double turns = rint(ang * 0.15915494309189535);        // 1 / (2 pi)
+      const float r = (float)fma(turns, -6.283185307179586, ang);  // 2 pi; in [-pi, pi]
+      sincosf(r, &sn[i], &cs[i]);
+    }
+  }
+  __syncthreads();
+  if (req < 0) return;  // a row behind the last request
+  const long long slot = slot_of;
+  __nv_bfloat16* qo = a.q_out + (size_t)t * a.ldq;
+  const size_t kv_row = slot < 0 ? 0 : (size_t)slot * a.Hkv * D;
+  for (int it = threadIdx.x; it < n_all; it += kRopeThreads) {
+    const Item m = next;
+    next = fetch(it + kRopeThreads);
+    const int head = m.head;
+    float x[8];
+    unpack8(m.x, x);
+    if (it < n_rot) {
+      const int i0 = a.half ? m.u0 : m.u0 / 2;
+      float y[8], p[8], q[8];
+      unpack8(m.y, y);
       if (a.half) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -106,27 +150,20 @@ __global__ void __launch_bounds__(kRopeThreads) rope_axes_append_kernel(RopeAxes
         }
       }
       if (head < a.Hq) {
-        store8_bf16(qo + (size_t)head * D + u0, p);
-        store8_bf16(qo + (size_t)head * D + u1, q);
+        store8_bf16(qo + (size_t)head * D + m.u0, p);
+        store8_bf16(qo + (size_t)head * D + m.u1, q);
       } else if (slot >= 0) {
         uint8_t* dst = a.k_cache + kv_row + (size_t)(head - a.Hq) * D;
-        store8_e4m3(dst + u0, p, a.k_scale[head - a.Hq]);
-        store8_e4m3(dst + u1, q, a.k_scale[head - a.Hq]);
+        store8_e4m3(dst + m.u0, p, a.k_scale[head - a.Hq]);
+        store8_e4m3(dst + m.u1, q, a.k_scale[head - a.Hq]);
       }
-    } else {
-      const int j = it - n_rot;
-      const bool is_v = j >= n_pass;
-      const int per = is_v ? vp : pp, k = is_v ? j - n_pass : j;
-      const int h = k / per, d = (k - h * per) * 8 + (is_v ? 0 : 2 * R);
-      const int head = is_v ? hqk + h : h;
-      float x[8];
-      unpack8(*reinterpret_cast<const uint4*>(row + (size_t)head * D + d), x);
-      if (head < a.Hq) {
-        store8_bf16(qo + (size_t)head * D + d, x);
-      } else if (slot >= 0) {
-        const int kh = is_v ? h : h - a.Hq;
-        store8_e4m3((is_v ? a.v_cache : a.k_cache) + kv_row + (size_t)kh * D + d, x, is_v ? a.v_scale[kh] : a.k_scale[kh]);
-      }
+    } else if (head < a.Hq) {
+      store8_bf16(qo + (size_t)head * D + m.u0, x);
+    } else if (slot >= 0) {
+      const bool is_v = head >= hqk;
+      const int kh = is_v ? head - hqk : head - a.Hq;
+      store8_e4m3((is_v ? a.v_cache : a.k_cache) + kv_row + (size_t)kh * D + m.u0, x,
+                  is_v ? a.v_scale[kh] : a.k_scale[kh]);
     }
   }
 }
