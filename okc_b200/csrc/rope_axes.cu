@@ -17,7 +17,7 @@ namespace okc {
 
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 256;  // at most
 constexpr int kMaxPairs = 128;
 
 // Four values to e4m3, to the nearest even one, overflow -> NaN.  The hardware's conversion saturates: it is
@@ -57,8 +57,11 @@ __device__ __forceinline__ void store8_e4m3(uint8_t* p, const float (&f)[8], flo
   *reinterpret_cast<uint2*>(p) = make_uint2(e4m3x4_nosat(e[0], e[1], e[2], e[3]), e4m3x4_nosat(e[4], e[5], e[6], e[7]));
 }
 
+// n / d from ceil(2^31 / d): exact for n < 2^31 / d.
+__device__ __forceinline__ int over(int n, uint32_t by) { return (int)((uint64_t)(uint32_t)n * by >> 31); }
+
 __global__ void __launch_bounds__(kRopeThreads) rope_axes_append_kernel(RopeAxesArgs a) {
-  __shared__ float cs[kMaxPairs], sn[kMaxPairs];
+  __shared__ __align__(16) float cs[kMaxPairs], sn[kMaxPairs];
   __shared__ int req;
   __shared__ long long slot_of;
   pdl_trigger();
@@ -76,14 +79,14 @@ __global__ void __launch_bounds__(kRopeThreads) rope_axes_append_kernel(RopeAxes
   auto fetch = [&](int it) {
     Item m = {};
     if (it < n_rot) {
-      m.head = it / rp;
+      m.head = over(it, a.by_rp);
       const int i0 = (it - m.head * rp) * 8;
       m.u0 = a.half ? i0 : 2 * i0;
       m.u1 = a.half ? i0 + R : 2 * i0 + 8;
       m.y = *reinterpret_cast<const uint4*>(row + (size_t)m.head * D + m.u1);
     } else if (it < n_all) {
       const bool is_v = it - n_rot >= n_pass;
-      const int per = is_v ? vp : pp, k = it - n_rot - (is_v ? n_pass : 0), h = k / per;
+      const int per = is_v ? vp : pp, k = it - n_rot - (is_v ? n_pass : 0), h = over(k, is_v ? a.by_vp : a.by_pp);
       m.u0 = (k - h * per) * 8 + (is_v ? 0 : 2 * R);
       m.head = is_v ? hqk + h : h;
     }
@@ -109,12 +112,11 @@ __global__ void __launch_bounds__(kRopeThreads) rope_axes_append_kernel(RopeAxes
       slot_of = slot;
     }
   } else {
-    for (int i = threadIdx.x - 32; i < R; i += kRopeThreads - 32) {
+    for (int i = threadIdx.x - 32; i < R; i += blockDim.x - 32) {
       const int axis = (int)((a.axis_bits[i >> 5] >> (2 * (i & 31))) & 3u);
       const double ang = (double)a.positions[(size_t)axis * a.ld_pos + t] * (double)a.inv_freq[i];
-      const double turns = rint(ang * 0.15915494309189535);        // 1 / (2 pi)
-      const float r = (float)fma(turns, -6.283185307179586, ang);  // 2 pi; in [-pi, pi]
-      sincosf(r, &sn[i], &cs[i]);
+      const double turns = ang * 0.15915494309189535;  // 1 / (2 pi)
+      sincospif(2.f * (float)(turns - rint(turns)), &sn[i], &cs[i]);
     }
   }
   __syncthreads();
@@ -122,31 +124,34 @@ __global__ void __launch_bounds__(kRopeThreads) rope_axes_append_kernel(RopeAxes
   const long long slot = slot_of;
   __nv_bfloat16* qo = a.q_out + (size_t)t * a.ldq;
   const size_t kv_row = slot < 0 ? 0 : (size_t)slot * a.Hkv * D;
-  for (int it = threadIdx.x; it < n_all; it += kRopeThreads) {
+  for (int it = threadIdx.x; it < n_all; it += blockDim.x) {
     const Item m = next;
-    next = fetch(it + kRopeThreads);
+    next = fetch(it + blockDim.x);
     const int head = m.head;
     float x[8];
     unpack8(m.x, x);
     if (it < n_rot) {
       const int i0 = a.half ? m.u0 : m.u0 / 2;
-      float y[8], p[8], q[8];
+      float y[8], p[8], q[8], c[8], s[8];
       unpack8(m.y, y);
+#pragma unroll
+      for (int k = 0; k < 8; k += 4) {
+        *reinterpret_cast<float4*>(c + k) = *reinterpret_cast<const float4*>(cs + i0 + k);
+        *reinterpret_cast<float4*>(s + k) = *reinterpret_cast<const float4*>(sn + i0 + k);
+      }
       if (a.half) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float c = cs[i0 + k], s = sn[i0 + k];
-          p[k] = x[k] * c - y[k] * s;
-          q[k] = x[k] * s + y[k] * c;
+          p[k] = x[k] * c[k] - y[k] * s[k];
+          q[k] = x[k] * s[k] + y[k] * c[k];
         }
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float c0 = cs[i0 + k], s0 = sn[i0 + k], c1 = cs[i0 + 4 + k], s1 = sn[i0 + 4 + k];
-          p[2 * k] = x[2 * k] * c0 - x[2 * k + 1] * s0;
-          p[2 * k + 1] = x[2 * k] * s0 + x[2 * k + 1] * c0;
-          q[2 * k] = y[2 * k] * c1 - y[2 * k + 1] * s1;
-          q[2 * k + 1] = y[2 * k] * s1 + y[2 * k + 1] * c1;
+          p[2 * k] = x[2 * k] * c[k] - x[2 * k + 1] * s[k];
+          p[2 * k + 1] = x[2 * k] * s[k] + x[2 * k + 1] * c[k];
+          q[2 * k] = y[2 * k] * c[4 + k] - y[2 * k + 1] * s[4 + k];
+          q[2 * k + 1] = y[2 * k] * s[4 + k] + y[2 * k + 1] * c[4 + k];
         }
       }
       if (head < a.Hq) {
@@ -170,8 +175,16 @@ __global__ void __launch_bounds__(kRopeThreads) rope_axes_append_kernel(RopeAxes
 
 }  // namespace
 
-int launch_rope_axes_append(const RopeAxesArgs& a, cudaStream_t stream) {
-  return okc_host::launch_k(rope_axes_append_kernel, dim3(a.T), dim3(kRopeThreads), 0, stream, dim3(1), a);
+int launch_rope_axes_append(const RopeAxesArgs& args, cudaStream_t stream) {
+  RopeAxesArgs a = args;
+  auto by = [](int d) { return d > 0 ? (uint32_t)(((1ull << 31) + d - 1) / d) : 0u; };
+  a.by_rp = by(a.R / 8);
+  a.by_pp = by((a.D - 2 * a.R) / 8);
+  a.by_vp = by(a.D / 8);
+  // a thread for each item (see the kernel), within two to eight warps
+  const int items = (a.Hq + a.Hkv) * (a.D / 8 - a.R / 8) + a.Hkv * (a.D / 8);
+  const int threads = items <= 64 ? 64 : items >= kRopeThreads ? kRopeThreads : (items + 31) / 32 * 32;
+  return okc_host::launch_k(rope_axes_append_kernel, dim3(a.T), dim3(threads), 0, stream, dim3(1), a);
 }
 
 }  // namespace okc
