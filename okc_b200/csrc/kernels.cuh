@@ -111,7 +111,7 @@ struct RopeAxesArgs {
   int T, B, Hq, Hkv, D, P;
   long long num_pages;
   int* err;
-  uint32_t by_rp, by_pp, by_vp;  // set by the launcher: see over()
+  uint32_t by_rp, by_pp, by_vp, by_r;  // set by the launcher: see over()
 };
 int launch_rope_axes_append(const RopeAxesArgs& a, cudaStream_t stream);
 // Ragged chunk attention over the paged cache (attention_chunk.cu).
