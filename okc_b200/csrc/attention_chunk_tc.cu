@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
   // The j-th block taken.  Under a distance bias the nearest keys come first, so that a row meets its
   // largest scores at once (front to back every block raises the maximum: 1770 us against 915 for 4096
   // tokens behind 4096).  Without one a row's first block is better a whole one than its diagonal.
-#define OKC_BLOCK_AT(j) (BIAS ? nb - 1 - (j) : (j))
+  auto block_at = [](int j, int nb) { return BIAS ? nb - 1 - j : j; };
 
   if (warp < kSoftmaxThreads / 32) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     bool ok = true, low = true;  // low: no score so far has left the three-coefficient range
 #pragma unroll 1
     for (int j = 0; j < nb && on; ++j) {
-      const int kb = key0 + OKC_BLOCK_AT(j) * kKeys;
+      const int kb = key0 + block_at(j, nb) * kKeys;
       const uint32_t ts = lanes + w * kTile + (j & 1) * kKeys;  // S, and P over its first half
       ok = __all_sync(0xffffffffu, s_ready(j));
       if (!ok) {
@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     uint32_t* offs = reinterpret_cast<uint32_t*>(smem + C::OFF0);
     auto offset = [&](int j) {
       if (lt >= kKeys || j >= nb) return;
-      const int key = key0 + OKC_BLOCK_AT(j) * kKeys + lt;
+      const int key = key0 + block_at(j, nb) * kKeys + lt;
       uint32_t off = kNoRow;
       if (key < k_hi) {
         const int page = a.page_table[(size_t)b * a.table_ld + page_of(a, key)];
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       if (sync_any(!ok)) return false;
       if (j + 1 < nb) fetch(j + 1, next);
       offset(j + 2);
-      const int st = j % kDepth, kb = key0 + OKC_BLOCK_AT(j) * kKeys;
+      const int st = j % kDepth, kb = key0 + block_at(j, nb) * kKeys;
       ok = mbar_wait(&sh.kv_empty[st], ((uint32_t)(j / kDepth) & 1u) ^ 1u, a.err, abort_flag);
       store(smem + C::K0 + st * C::BLOCK, now.k);
       fence_async_smem();

@@ -104,55 +104,36 @@ __device__ __forceinline__ void block_put(float* block, int row, int pair, float
   reinterpret_cast<float2*>(block)[row * 16 + (pair ^ (row & 15))] = make_float2(x, y);
 }
 
-// Writes a 32 x 32 block of y (`rows` x `cols` of it exist): a lane has two neighbouring columns of
-// every second row.  Residual rows are fetched eight at a time ahead of the stores, which may
-// overwrite them.  Whole blocks whose rows take aligned accesses of two columns use them.
+// Writes a 32 x 32 block of y whose rows take aligned accesses of two columns: a lane has two neighbouring
+// columns of every second row.  Residual rows are fetched ahead of the stores, which may overwrite them.
 template <bool OUT32>
-__device__ __forceinline__ void tall_block(const float* block, int rows, int cols, float my_sx, const LinearArgs& a,
-                                           int m0, int n0) {
+__device__ __forceinline__ void tall_block(const float* block, float my_sx, const LinearArgs& a, int m0, int n0) {
   constexpr int B = 4;  // a lane's rows in flight
   const int lane = threadIdx.x & 31, odd = lane >> 4, pair = lane & 15;
   const int oe = OUT32 ? 4 : 2, re = a.res_fp32 ? 4 : 2;
-  const int have = min(2, max(0, cols - 2 * pair));  // columns this lane has
   float sw[2], bias[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int n = n0 + 2 * pair + i;
-    sw[i] = i < have ? lin_col_scale(a, n) : 0.f;
-    bias[i] = i < have && a.bias ? __bfloat162float(a.bias[n]) : 0.f;
+    sw[i] = lin_col_scale(a, n);
+    bias[i] = a.bias ? __bfloat162float(a.bias[n]) : 0.f;
   }
   uint8_t* y = reinterpret_cast<uint8_t*>(a.y) + ((size_t)(m0 + odd) * a.ldy + n0 + 2 * pair) * oe;
   const uint8_t* res = reinterpret_cast<const uint8_t*>(a.res) + ((size_t)(m0 + odd) * a.ldr + n0 + 2 * pair) * re;
   const long long y_step = 2 * a.ldy * oe, r_step = 2 * a.ldr * re;
-  const bool whole = a.pairs && rows == 32 && cols >= 32;
 #pragma unroll 1
   for (int i0 = 0; i0 < 16; i0 += B) {
     float2 r[B], v[B];
     if (a.res) {
-      if (whole) {
-        if (a.res_fp32) {
+      if (a.res_fp32) {
 #pragma unroll
-          for (int i = 0; i < B; ++i) r[i] = *reinterpret_cast<const float2*>(res + i * r_step);
-        } else {
-#pragma unroll
-          for (int i = 0; i < B; ++i) {
-            const uint32_t b = *reinterpret_cast<const uint32_t*>(res + i * r_step);
-            r[i] = make_float2(bf16_lo(b), bf16_hi(b));
-          }
-        }
+        for (int i = 0; i < B; ++i) r[i] = *reinterpret_cast<const float2*>(res + i * r_step);
       } else {
-        auto get = [&](auto type) {
-          using R = decltype(type);
 #pragma unroll
-          for (int i = 0; i < B; ++i) {
-            const int h = 2 * (i0 + i) + odd < rows ? have : 0;
-            const R* p = reinterpret_cast<const R*>(res + i * r_step);
-            r[i].x = h > 0 ? (float)p[0] : 0.f;
-            r[i].y = h > 1 ? (float)p[1] : 0.f;
-          }
-        };
-        if (a.res_fp32) get(float());
-        else get(__nv_bfloat16());
+        for (int i = 0; i < B; ++i) {
+          const uint32_t b = *reinterpret_cast<const uint32_t*>(res + i * r_step);
+          r[i] = make_float2(bf16_lo(b), bf16_hi(b));
+        }
       }
       res += B * r_step;
     } else {
@@ -178,23 +159,59 @@ __device__ __forceinline__ void tall_block(const float* block, int rows, int col
     for (int i = 0; i < B; ++i) {
       v[i].x += r[i].x;
       v[i].y += r[i].y;
+      if (OUT32)
+        *reinterpret_cast<float2*>(y + i * y_step) = v[i];
+      else
+        *reinterpret_cast<uint32_t*>(y + i * y_step) = pack_bf16x2(v[i].x, v[i].y);
     }
-    if (whole) {
+    y += B * y_step;
+  }
+}
+
+// The same for any block, of which `rows` x `cols` exist: a lane has one column, so that a row takes one access
+// whatever its alignment (777 x 4095 x 4104 in bf16, fp32 out, bf16
+// residual: 45 us; two columns a lane and a branch at each load 57).
+template <bool OUT32>
+__device__ __forceinline__ void ragged_block(const float* block, int rows, int cols, float my_sx, const LinearArgs& a,
+                                             int m0, int n0) {
+  constexpr int B = 16;  // rows in flight
+  const int lane = threadIdx.x & 31;
+  const bool on = lane < cols;
+  const int oe = OUT32 ? 4 : 2, re = a.res_fp32 ? 4 : 2;
+  const float sw = on ? lin_col_scale(a, n0 + lane) : 0.f;
+  const float bias = on && a.bias ? __bfloat162float(a.bias[n0 + lane]) : 0.f;
+  uint8_t* y = reinterpret_cast<uint8_t*>(a.y) + ((size_t)m0 * a.ldy + n0 + lane) * oe;
+  const uint8_t* res = reinterpret_cast<const uint8_t*>(a.res) + ((size_t)m0 * a.ldr + n0 + lane) * re;
+  const long long y_step = a.ldy * oe, r_step = a.ldr * re;
+#pragma unroll 1
+  for (int i0 = 0; i0 < rows; i0 += B) {
+    float v[B], r[B];
 #pragma unroll
-      for (int i = 0; i < B; ++i) {
-        if (OUT32)
-          *reinterpret_cast<float2*>(y + i * y_step) = v[i];
-        else
-          *reinterpret_cast<uint32_t*>(y + i * y_step) = pack_bf16x2(v[i].x, v[i].y);
-      }
-    } else {
+    for (int i = 0; i < B; ++i) r[i] = 0.f;
+    if (a.res) {
+      if (a.res_fp32) {
 #pragma unroll
-      for (int i = 0; i < B; ++i) {
-        const int h = 2 * (i0 + i) + odd < rows ? have : 0;
-        if (h > 0) lin_put<OUT32>(y + i * y_step, v[i].x);
-        if (h > 1) lin_put<OUT32>(y + i * y_step + oe, v[i].y);
+        for (int i = 0; i < B; ++i)
+          if (on && i0 + i < rows) r[i] = *reinterpret_cast<const float*>(res + i * r_step);
+      } else {
+#pragma unroll
+        for (int i = 0; i < B; ++i) r[i] = ld_bf16_if(res + i * r_step, on && i0 + i < rows);
       }
+      res += B * r_step;
     }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const int row = i0 + i;
+      const float sx = __shfl_sync(0xffffffffu, my_sx, row);
+      v[i] = fmaf(block[row * 32 + 2 * ((lane >> 1) ^ (row & 15)) + (lane & 1)] * sx, sw, bias);
+    }
+    lin_act_switch(a.act, [&](auto act) {
+#pragma unroll
+      for (int i = 0; i < B; ++i) v[i] = lin_act<decltype(act)::value>(v[i]);
+    });
+#pragma unroll
+    for (int i = 0; i < B; ++i)
+      if (on && i0 + i < rows) lin_put<OUT32>(y + i * y_step, v[i] + r[i]);
     y += B * y_step;
   }
 }
@@ -347,15 +364,17 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
       lin_tile(u, mt, nt, tm, tn);
       const int m0 = tm * 256 + (int)rank * 128 + q4 * 32, rows = min(32, a.M - m0);
       const float my_sx = lane < rows ? lin_row_scale(a, m0 + lane) : 0.f;
-      if (a.res && lane < rows) {  // this lane's row of the residual, into L2 while the products run
+      if (a.res && lane < rows) {  // this lane's row of the residual, into L2 while the products run (777 x 4095: 1 to 4 us)
         const int re = a.res_fp32 ? 4 : 2, n0 = tn * bn + c_first * 32, cols = min(c_n * 32, a.N - n0);
         const uint8_t* p = reinterpret_cast<const uint8_t*>(a.res) + ((size_t)(m0 + lane) * a.ldr + n0) * re;
-        for (int i = 0; i < cols * re; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + i));
+        for (int i = 0; i < cols * re + 128; i += 128)  // a row may begin inside a line
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(p + min(i, cols * re - 1)));
       }
       auto emit = [&](int c) {
         const int n0 = tn * bn + (c_first + c) * 32;
         __syncwarp();
-        tall_block<OUT32>(st, rows, a.N - n0, my_sx, a, m0, n0);
+        if (a.pairs && rows == 32 && a.N - n0 >= 32) tall_block<OUT32>(st, my_sx, a, m0, n0);
+        else ragged_block<OUT32>(st, rows, a.N - n0, my_sx, a, m0, n0);
         __syncwarp();
       };
       const int c_live = rows > 0 ? min(c_n, (a.N - tn * bn + 31) / 32 - c_first) : 0;

@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
     }
   } else {
     if (a.res) {  // the rows of the residual that this CTA will add, into L2 while the weight streams
+                  // (128 tokens: 22.1 us, without 23.3)
       const int re = a.res_fp32 ? 4 : 2, lines = re, t = threadIdx.x - 64;  // 128 channels are `re` lines
       for (int i = t; i < (min(BN, a.M - m0) - rank + S - 1) / S * lines; i += 32 * kSplitDrain) {
         const int m = m0 + rank + i / lines * S, n = n0 + i % lines * (128 / re);
@@ -217,16 +218,19 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
         sx[i] = m < live ? lin_row_scale(a, m0 + m) : 0.f;
         v[i] = r[i] = 0.f;
       }
-      auto get = [&](auto type) {
-        using R = decltype(type);
+      if (a.res && a.res_fp32) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
           const int m = m1 + 2 * i * S;
-          if (m < live && n < a.N) r[i] = (float)reinterpret_cast<const R*>(a.res)[(size_t)(m0 + m) * a.ldr + n];
+          if (m < live && n < a.N) r[i] = reinterpret_cast<const float*>(a.res)[(size_t)(m0 + m) * a.ldr + n];
         }
-      };
-      if (a.res && a.res_fp32) get(float());
-      else if (a.res) get(__nv_bfloat16());
+      } else if (a.res) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int m = m1 + 2 * i * S;
+          r[i] = ld_bf16_if(reinterpret_cast<const uint8_t*>(a.res) + ((size_t)(m0 + m) * a.ldr + n) * 2, m < live && n < a.N);
+        }
+      }
       for (int s = 0; s < S; ++s) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
