@@ -61,7 +61,7 @@ __device__ __forceinline__ void store8_e4m3(uint8_t* p, const float (&f)[8], flo
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const float q = f[k] * y;
-      e[k] = fmaf(fmaf(-q, scale, f[k]), y, q);
+      e[k] = copysignf(fmaf(fmaf(-q, scale, f[k]), y, q), q);  // of -0, too
     }
   } else {
 #pragma unroll

@@ -523,7 +523,7 @@ def _ragged(cu_q, seq_lens, page_table, dev: int) -> tuple:
     B = seq_lens.numel()
     sl = _dense(seq_lens, "seq_lens", torch.int32, (B,), dev)
     cq = _dense(cu_q, "cu_q", torch.int32, (B + 1,), dev)
-    cols = page_table.shape[-1]
+    cols = page_table.shape[-1] if page_table.dim() else 0
     ld = _rows(page_table, "page_table", torch.int32, (B, cols), dev)
     return cq, sl, B, page_table.data_ptr(), ld, cols
 
@@ -558,7 +558,7 @@ def rope_axes_kv_append(qkv: torch.Tensor, positions: torch.Tensor, axes, inv_fr
     ldqkv = _rows(qkv, "qkv", torch.bfloat16, (T, (Hq + 2 * Hkv) * D), dev)
     ld_pos = _rows(positions, "positions", torch.int64, (A, T), dev)
     try:
-        axes = bytes(axes)
+        axes = bytes(iter(axes))
     except (TypeError, ValueError):
         raise _lib.OkcError(f"axes: expected the axis (0..{A - 1}) of each pair, got {axes!r}") from None
     R = len(axes)
