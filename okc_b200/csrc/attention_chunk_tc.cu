@@ -306,6 +306,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     }
     const bool live = r < rows, on = sh.tile * kPair + w * kTile < rows;
     const int tok = live ? row0 + r / a.G : 0, hq = live ? head * a.G + r % a.G : 0;
+    // The warp's 32 query rows, on their way while the keys are found: a lane has chunk qc of 16 bytes of every
+    // QR-th row from qr on, so that an access takes whole rows.
+    constexpr int QC = D / 8, QR = 32 / QC, QN = 32 / QR;
+    const int qr = lane / QC, qc = lane % QC;
+    auto at_row = [&](long long mine, int row) {  // a value of the lane that has the row
+      return (long long)__shfl_sync(0xffffffffu, (unsigned long long)mine, row);
+    };
+    const long long q_at = live ? (long long)tok * a.ldq + (long long)hq * D : -1;
+    uint4 qv[QN];
+#pragma unroll
+    for (int i = 0; i < QN; ++i) {
+      const long long at = at_row(q_at, i * QR + qr);
+      qv[i] = at >= 0 ? *reinterpret_cast<const uint4*>(a.q + at + qc * 8) : make_uint4(0u, 0u, 0u, 0u);
+    }
     RowSpan me = {0, 0, 0};
     if (live) me = row_span(a, rq, row0, r / a.G);
     {
@@ -332,34 +346,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) nan_d[i] = 0;
     if (nb > 0 && on) {
-      // the row in f16, scaled by a power of two, into the swizzled panels
-      const __nv_bfloat16* qp = a.q + (size_t)tok * a.ldq + (size_t)hq * D;
-      uint32_t top = 0;
-      if (live) {
-#pragma unroll 4
-        for (int i = 0; i < D / 8; ++i) {
-          const uint4 v = *reinterpret_cast<const uint4*>(qp + 8 * i);
-          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+      // the rows in f16, each scaled by a power of two, into the swizzled panels; a negative factor goes into
+      // the query, so that the largest score is the largest sum
+      const float unit = a.k_scale[head] * a.sm_scale * (CAP ? 2.f / a.softcap : 1.f) * 1.4426950408889634f;
+      uint32_t my_top = 0;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
-        }
-      }
-      const int shf = f16_shift(top);
-      fac = a.k_scale[head] * a.sm_scale * (CAP ? 2.f / a.softcap : 1.f) * 1.4426950408889634f * pow2(shf);
-      // a negative factor goes into the query, so that the largest score is the largest sum
-      const float down = fac < 0.f ? -pow2(-shf) : pow2(-shf);
-      fac = fabsf(fac);
-      if (BIAS && live) slope = a.slopes[hq] * 1.4426950408889634f;
-      uint8_t* qs = smem + C::Q0 + w * C::QTILE + lr * 128;
-#pragma unroll 4
-      for (int i = 0; i < D / 8; ++i) {
-        const uint4 v = live ? *reinterpret_cast<const uint4*>(qp + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-        uint32_t o[4];
+      for (int i = 0; i < QN; ++i) {
+        const uint32_t u[4] = {qv[i].x, qv[i].y, qv[i].z, qv[i].w};
+        uint32_t top = 0, o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
+#pragma unroll
+        for (int k = 1; k < QC; k *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
+        const uint32_t t = __shfl_sync(0xffffffffu, top, lane % QR * QC);
+        if (lane / QR == i) my_top = t;
+        const float down = unit < 0.f ? -pow2(-f16_shift(top)) : pow2(-f16_shift(top));
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = h2(bf16_lo(u[k]) * down, bf16_hi(u[k]) * down);
-        *reinterpret_cast<uint4*>(qs + (i / 8) * C::QSUB + (((i % 8) ^ (lr & 7)) * 16)) = make_uint4(o[0], o[1], o[2], o[3]);
+        const int row = (warp & 3) * 32 + i * QR + qr;
+        *reinterpret_cast<uint4*>(smem + C::Q0 + w * C::QTILE + (qc / 8) * C::QSUB + row * 128 + ((qc % 8) ^ (row & 7)) * 16) =
+            make_uint4(o[0], o[1], o[2], o[3]);
       }
+      fac = fabsf(unit * pow2(f16_shift(my_top)));
+      if (BIAS && live) slope = a.slopes[hq] * 1.4426950408889634f;
     }
     fence_async_smem();
     __syncwarp();
@@ -545,9 +554,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     const size_t part = (size_t)split * a.T * a.Hq + (size_t)tok * a.Hq + hq;
     const float inv = l == 0.f ? 0.f : __fdividef(a.v_scale[head], l);
     if (pl.splits > 1 && live) *reinterpret_cast<float2*>(pl.ml + part * 2) = make_float2(m_ref, l);
-#pragma unroll
-    for (int c0 = 0; c0 < D; c0 += 16) {
-      uint32_t v[16];
+    // The warp's rows are turned in its share of the query tile (2 D bytes a row), which no MMA reads any more,
+    // and leave as whole rows: all of a bf16 row at once, an fp32 one in halves.
+    uint8_t* turn = smem + C::Q0 + w * C::QTILE + (warp & 3) * 32 * 2 * D;
+    auto columns16 = [&](int c0, uint32_t (&v)[16]) {
       if (have) {
         tm_ld16(to + c0, v);
         tm_wait_ld(v);
@@ -561,24 +571,46 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
         for (int c = 0; c < 16; ++c)
           if ((nan >> c) & 1u) v[c] = 0x7fffffffu;
       }
-      if (!live) continue;
-      if (pl.splits > 1) {
-        float4* dst = reinterpret_cast<float4*>(pl.acc + part * D + c0);
+    };
+    auto put = [&](int chunk, uint4 x) { *reinterpret_cast<uint4*>(turn + lane * 2 * D + (chunk ^ (lane % QC)) * 16) = x; };
+    auto leave = [&](uint8_t* base, long long at) {  // `at`: bytes to this lane's row from base, -1: none
+      __syncwarp();
 #pragma unroll
-        for (int c = 0; c < 16; c += 4)
-          dst[c / 4] = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]),
-                                   __uint_as_float(v[c + 3]));
-      } else {
-        uint4* dst = reinterpret_cast<uint4*>(a.out + (size_t)tok * a.ldo + (size_t)hq * D + c0);
+      for (int i = 0; i < QN; ++i) {
+        const int row = i * QR + qr;
+        const long long to_row = at_row(at, row);
+        const uint4 x = *reinterpret_cast<const uint4*>(turn + row * 2 * D + (qc ^ (row % QC)) * 16);
+        if (to_row >= 0) *reinterpret_cast<uint4*>(base + to_row + qc * 16) = x;
+      }
+      __syncwarp();
+    };
+    if (pl.splits > 1) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int c0 = 0; c0 < D / 2; c0 += 16) {
+          uint32_t v[16];
+          columns16(half * (D / 2) + c0, v);
+#pragma unroll
+          for (int c = 0; c < 16; c += 4) put((c0 + c) / 4, make_uint4(v[c], v[c + 1], v[c + 2], v[c + 3]));
+        }
+        leave(reinterpret_cast<uint8_t*>(pl.acc) + half * 2 * D, live ? (long long)(part * D * 4) : -1);
+      }
+    } else {
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 16) {
+        uint32_t v[16];
+        columns16(c0, v);
 #pragma unroll
         for (int c = 0; c < 16; c += 8) {
           uint32_t o[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             o[k] = pack_bf16x2(__uint_as_float(v[c + 2 * k]) * inv, __uint_as_float(v[c + 2 * k + 1]) * inv);
-          dst[c / 8] = make_uint4(o[0], o[1], o[2], o[3]);
+          put((c0 + c) / 8, make_uint4(o[0], o[1], o[2], o[3]));
         }
       }
+      leave(reinterpret_cast<uint8_t*>(a.out), live ? ((long long)tok * a.ldo + (long long)hq * D) * 2 : -1);
     }
   } else if (warp < kIssueWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
