@@ -190,7 +190,8 @@ struct TcShared {
   uint64_t s_full[2][2], p_full[2][2];  // [tile][buffer]
   uint32_t tmem;
   int abort;
-  int b, tile;             // the block's request (-1: none) and row tile pair
+  int b, tile, row0;       // the block's request (-1: none), its row tile pair, the request's first row
+  Req rq;
   int lo, hi;              // union of its rows' intervals
   int full_lo, full_hi;    // intersection: keys in it need no mask
   uint32_t nan[kDepth][kKeys / 32];  // per V block: its keys that hold a NaN that was taken out
@@ -240,8 +241,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     for (int base = 0; base < a.B && found < 0; base += 32) {
       const int b = base + lane;
       int n = 0;
+      Req r = {};
       if (b < a.B) {
-        const Req r = request(a, b);
+        r = request(a, b);
         const int rows = r.n * a.G;
         if (rows > kSplitRows) n = (rows + kPair - 1) / kPair;
         if (r.len > a.max_keys && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(a.err, OKC_DEVERR_PAGE);
@@ -259,6 +261,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
         found = base + l;
         // from the request's last tile pair on
         tile = __shfl_sync(0xffffffffu, before + sum, l) - 1 - (int)blockIdx.y;
+        if (lane == l) {
+          sh.rq = r;
+          sh.row0 = a.cu_q[b];
+        }
       }
       before += __shfl_sync(0xffffffffu, sum, 31);
     }
@@ -296,16 +302,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ------------------------------------------------------------------ softmax
     const int w = warp >> 2, lr = (warp & 3) * 32 + lane;  // tile, row of it
-    Req rq = {};
-    int rows = 0, row0 = 0;
     const int r = sh.tile * kPair + w * kTile + lr;
+    Req rq = {};
+    int row0 = 0;
     if (b >= 0) {
-      rq = request(a, b);
-      rows = rq.n * a.G;
-      row0 = a.cu_q[b];
+      rq = sh.rq;
+      row0 = sh.row0;
     }
+    const int rows = rq.n * a.G, my_tok = (int)((uint64_t)(uint32_t)r * a.group_mul >> a.group_shift);
     const bool live = r < rows, on = sh.tile * kPair + w * kTile < rows;
-    const int tok = live ? row0 + r / a.G : 0, hq = live ? head * a.G + r % a.G : 0;
+    const int tok = live ? row0 + my_tok : 0, hq = live ? head * a.G + r - my_tok * a.G : 0;
     // The warp's 32 query rows, on their way while the keys are found: a lane has chunk qc of 16 bytes of every
     // QR-th row from qr on, so that an access takes whole rows.
     constexpr int QC = D / 8, QR = 32 / QC, QN = 32 / QR;
@@ -314,14 +320,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       return (long long)__shfl_sync(0xffffffffu, (unsigned long long)mine, row);
     };
     const long long q_at = live ? (long long)tok * a.ldq + (long long)hq * D : -1;
-    uint4 qv[QN];
-#pragma unroll
+    uint8_t* q_mine = smem + C::Q0 + w * C::QTILE + (qc / 8) * C::QSUB;
+    auto q_slot = [&](int i) {  // of the lane's i-th chunk, in a swizzled panel
+      const int row = (warp & 3) * 32 + i * QR + qr;
+      return q_mine + row * 128 + ((qc % 8) ^ (row & 7)) * 16;
+    };
+#pragma unroll 4
     for (int i = 0; i < QN; ++i) {
       const long long at = at_row(q_at, i * QR + qr);
-      qv[i] = at >= 0 ? *reinterpret_cast<const uint4*>(a.q + at + qc * 8) : make_uint4(0u, 0u, 0u, 0u);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(q_slot(i))),
+                   "l"(a.q + (at >= 0 ? at + qc * 8 : 0)), "r"(at >= 0 ? 16 : 0)
+                   : "memory");
     }
     RowSpan me = {0, 0, 0};
-    if (live) me = row_span(a, rq, row0, r / a.G);
+    if (live) me = row_span(a, rq, row0, my_tok);
     {
       const int lo = __reduce_min_sync(0xffffffffu, live && me.lo < me.hi ? me.lo : 0x7fffffff);
       const int hi = __reduce_max_sync(0xffffffffu, live && me.lo < me.hi ? me.hi : 0);
@@ -345,14 +357,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     uint32_t nan_d[D / 32];  // output columns that a visible NaN value reaches
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) nan_d[i] = 0;
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (nb > 0 && on) {
       // the rows in f16, each scaled by a power of two, into the swizzled panels; a negative factor goes into
       // the query, so that the largest score is the largest sum
       const float unit = a.k_scale[head] * a.sm_scale * (CAP ? 2.f / a.softcap : 1.f) * 1.4426950408889634f;
       uint32_t my_top = 0;
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < QN; ++i) {
-        const uint32_t u[4] = {qv[i].x, qv[i].y, qv[i].z, qv[i].w};
+        const uint4 qv = *reinterpret_cast<const uint4*>(q_slot(i));
+        const uint32_t u[4] = {qv.x, qv.y, qv.z, qv.w};
         uint32_t top = 0, o[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
@@ -363,9 +377,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
         const float down = unit < 0.f ? -pow2(-f16_shift(top)) : pow2(-f16_shift(top));
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = h2(bf16_lo(u[k]) * down, bf16_hi(u[k]) * down);
-        const int row = (warp & 3) * 32 + i * QR + qr;
-        *reinterpret_cast<uint4*>(smem + C::Q0 + w * C::QTILE + (qc / 8) * C::QSUB + row * 128 + ((qc % 8) ^ (row & 7)) * 16) =
-            make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(q_slot(i)) = make_uint4(o[0], o[1], o[2], o[3]);
       }
       fac = fabsf(unit * pow2(f16_shift(my_top)));
       if (BIAS && live) slope = a.slopes[hq] * 1.4426950408889634f;
@@ -557,25 +569,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     // The warp's rows are turned in its share of the query tile (2 D bytes a row), which no MMA reads any more,
     // and leave as whole rows: all of a bf16 row at once, an fp32 one in halves.
     uint8_t* turn = smem + C::Q0 + w * C::QTILE + (warp & 3) * 32 * 2 * D;
-    auto columns16 = [&](int c0, uint32_t (&v)[16]) {
+    auto columns = [&](int c0, uint32_t (&v)[32]) {
       if (have) {
-        tm_ld16(to + c0, v);
+        tm_ld32(to + c0, v);
         tm_wait_ld(v);
       } else {
 #pragma unroll
-        for (int c = 0; c < 16; ++c) v[c] = 0u;
+        for (int c = 0; c < 32; ++c) v[c] = 0u;
       }
-      const uint32_t nan = nan_d[c0 / 32] >> (c0 % 32);
-      if (nan & 0xffffu) {
+      const uint32_t nan = nan_d[c0 / 32];
+      if (nan) {
 #pragma unroll
-        for (int c = 0; c < 16; ++c)
+        for (int c = 0; c < 32; ++c)
           if ((nan >> c) & 1u) v[c] = 0x7fffffffu;
       }
     };
     auto put = [&](int chunk, uint4 x) { *reinterpret_cast<uint4*>(turn + lane * 2 * D + (chunk ^ (lane % QC)) * 16) = x; };
     auto leave = [&](uint8_t* base, long long at) {  // `at`: bytes to this lane's row from base, -1: none
       __syncwarp();
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < QN; ++i) {
         const int row = i * QR + qr;
         const long long to_row = at_row(at, row);
@@ -588,21 +600,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int c0 = 0; c0 < D / 2; c0 += 16) {
-          uint32_t v[16];
-          columns16(half * (D / 2) + c0, v);
+        for (int c0 = 0; c0 < D / 2; c0 += 32) {
+          uint32_t v[32];
+          columns(half * (D / 2) + c0, v);
 #pragma unroll
-          for (int c = 0; c < 16; c += 4) put((c0 + c) / 4, make_uint4(v[c], v[c + 1], v[c + 2], v[c + 3]));
+          for (int c = 0; c < 32; c += 4) put((c0 + c) / 4, make_uint4(v[c], v[c + 1], v[c + 2], v[c + 3]));
         }
         leave(reinterpret_cast<uint8_t*>(pl.acc) + half * 2 * D, live ? (long long)(part * D * 4) : -1);
       }
     } else {
 #pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 16) {
-        uint32_t v[16];
-        columns16(c0, v);
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t v[32];
+        columns(c0, v);
 #pragma unroll
-        for (int c = 0; c < 16; c += 8) {
+        for (int c = 0; c < 32; c += 8) {
           uint32_t o[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k)

@@ -11,6 +11,15 @@ bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t
 // A finite float (the device math assumes it).
 bool finite(float v) { return v - v == 0.f; }
 
+// n / d = n * mul >> shift for 0 <= n < 2^31: with 2^(l-1) < d <= 2^l and mul = ceil(2^(31+l) / d), n * mul is
+// above 2^(31+l) * n / d by less than 2^(31+l) / d, so the quotient is exact.
+void divide_by(int d, uint32_t& mul, int& shift) {
+  int l = 0;
+  while (1ll << l < d) ++l;
+  shift = 31 + l;
+  mul = (uint32_t)(((1ull << shift) + d - 1) / d);
+}
+
 }  // namespace
 
 extern "C" {
@@ -177,10 +186,8 @@ int okc_attn_chunk_fp8(const void* q, int64_t ldq, const void* k_cache, const vo
   a.P = page_size;
   a.window = window;
   a.num_pages = num_pages;
-  int l = 0;
-  while (1ll << l < page_size) ++l;
-  a.page_shift = 31 + l;
-  a.page_mul = (uint32_t)(((1ull << a.page_shift) + page_size - 1) / page_size);
+  divide_by(page_size, a.page_mul, a.page_shift);
+  divide_by(a.G, a.group_mul, a.group_shift);
   a.sm_scale = sm_scale;
   a.softcap = softcap;
   a.max_q = max_q;

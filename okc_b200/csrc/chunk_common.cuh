@@ -47,8 +47,7 @@ __device__ __forceinline__ uint32_t h2(float x, float y) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The page of a position: with 2^(l-1) < P <= 2^l and mul = ceil(2^(31+l) / P), position * mul is above
-// 2^(31+l) * position / P by less than 2^(31+l) / P for every position below 2^31, so the quotient is exact.
+// The page of a position.
 __device__ __forceinline__ int page_of(const ChunkArgs& a, int position) {
   return (int)((uint64_t)(uint32_t)position * a.page_mul >> a.page_shift);
 }

@@ -123,8 +123,8 @@ struct ChunkArgs {
   const int32_t* page_table;
   long long table_ld;
   int max_keys;  // positions that a table row covers
-  uint32_t page_mul;  // position / P = position * page_mul >> page_shift (page_of)
-  int page_shift;
+  uint32_t page_mul, group_mul;  // n / P = n * page_mul >> page_shift (page_of), n / G likewise
+  int page_shift, group_shift;
   const int32_t* cu_q;
   const int32_t* seq_lens;
   const float* k_scale;
