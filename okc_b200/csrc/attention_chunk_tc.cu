@@ -320,15 +320,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       return (long long)__shfl_sync(0xffffffffu, (unsigned long long)mine, row);
     };
     const long long q_at = live ? (long long)tok * a.ldq + (long long)hq * D : -1;
-    uint8_t* q_mine = smem + C::Q0 + w * C::QTILE + (qc / 8) * C::QSUB;
-    auto q_slot = [&](int i) {  // of the lane's i-th chunk, in a swizzled panel
-      const int row = (warp & 3) * 32 + i * QR + qr;
-      return q_mine + row * 128 + ((qc % 8) ^ (row & 7)) * 16;
+    auto q_slot = [&](int row, int chunk) {  // of the warp's rows, in a swizzled panel
+      const int r128 = (warp & 3) * 32 + row;
+      return smem + C::Q0 + w * C::QTILE + (chunk / 8) * C::QSUB + r128 * 128 + ((chunk % 8) ^ (r128 & 7)) * 16;
     };
 #pragma unroll 4
     for (int i = 0; i < QN; ++i) {
       const long long at = at_row(q_at, i * QR + qr);
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(q_slot(i))),
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(q_slot(i * QR + qr, qc))),
                    "l"(a.q + (at >= 0 ? at + qc * 8 : 0)), "r"(at >= 0 ? 16 : 0)
                    : "memory");
     }
@@ -358,29 +357,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) nan_d[i] = 0;
     asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
     if (nb > 0 && on) {
-      // the rows in f16, each scaled by a power of two, into the swizzled panels; a negative factor goes into
-      // the query, so that the largest score is the largest sum
-      const float unit = a.k_scale[head] * a.sm_scale * (CAP ? 2.f / a.softcap : 1.f) * 1.4426950408889634f;
-      uint32_t my_top = 0;
-#pragma unroll 4
-      for (int i = 0; i < QN; ++i) {
-        const uint4 qv = *reinterpret_cast<const uint4*>(q_slot(i));
-        const uint32_t u[4] = {qv.x, qv.y, qv.z, qv.w};
-        uint32_t top = 0, o[4];
+      // the row in f16, scaled by a power of two, in place; a lane has one row, whose chunks the swizzle puts
+      // into different banks than its neighbours'
+      uint4 v[D / 8];
+      uint32_t two = 0;  // the largest magnitudes of the even and of the odd elements
 #pragma unroll
-        for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
+      for (int i = 0; i < D / 8; ++i) v[i] = *reinterpret_cast<const uint4*>(q_slot(lane, i));
 #pragma unroll
-        for (int k = 1; k < QC; k *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
-        const uint32_t t = __shfl_sync(0xffffffffu, top, lane % QR * QC);
-        if (lane / QR == i) my_top = t;
-        const float down = unit < 0.f ? -pow2(-f16_shift(top)) : pow2(-f16_shift(top));
+      for (int i = 0; i < D / 8; ++i)
+        two = __vmaxu2(__vmaxu2(two, __vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu)),
+                       __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
+      const uint32_t top = max(two & 0xffffu, two >> 16);
+      const int shf = f16_shift(top);
+      fac = a.k_scale[head] * a.sm_scale * (CAP ? 2.f / a.softcap : 1.f) * 1.4426950408889634f * pow2(shf);
+      // a negative factor goes into the query, so that the largest score is the largest sum
+      const float down = fac < 0.f ? -pow2(-shf) : pow2(-shf);
+      fac = fabsf(fac);
+      if (BIAS && live) slope = a.slopes[hq] * 1.4426950408889634f;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        uint32_t o[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = h2(bf16_lo(u[k]) * down, bf16_hi(u[k]) * down);
-        *reinterpret_cast<uint4*>(q_slot(i)) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(q_slot(lane, i)) = make_uint4(o[0], o[1], o[2], o[3]);
       }
-      fac = fabsf(unit * pow2(f16_shift(my_top)));
-      if (BIAS && live) slope = a.slopes[hq] * 1.4426950408889634f;
     }
     fence_async_smem();
     __syncwarp();
