@@ -278,25 +278,36 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
   tc_after();
   const int b = sh.b;
   volatile int* abort_flag = &sh.abort;
-  // The union of the rows' intervals, once the softmax threads have published it, gives the keys:
-  // this split's first one, and its blocks.
-  auto plan = [&](int& key0, int& k_hi) -> int {
+  // The union of the rows' intervals, once the softmax threads have published it, gives the keys: this
+  // split's first one, and its blocks.  The j-th block taken is key0 + block_at(j).  Under a distance bias the
+  // nearest keys come first, so that a row meets its largest scores at once (front to back every block raises
+  // the maximum: 1770 us against 915 for 4096 tokens behind 4096): from the last row's block down, then the
+  // blocks ahead of it, which only a prefix has.  Without a bias a row's first block is better a whole one than
+  // its diagonal.
+  struct Plan {
+    int key0, k_hi, nb, near;
+  };
+  auto plan = [&]() -> Plan {
     if (!mbar_wait(&sh.plan, 0, a.err, abort_flag)) *abort_flag = 1;
     const int k_lo = *reinterpret_cast<volatile int*>(&sh.lo);
-    k_hi = *reinterpret_cast<volatile int*>(&sh.hi);
-    int nb = k_hi > k_lo ? (k_hi - k_lo + kKeys - 1) / kKeys : 0, first = 0;
+    Plan p;
+    p.k_hi = *reinterpret_cast<volatile int*>(&sh.hi);
+    int first = 0;
+    p.nb = p.k_hi > k_lo ? (p.k_hi - k_lo + kKeys - 1) / kKeys : 0;
     if (pl.splits > 1) {
-      const int per = (nb + pl.splits - 1) / pl.splits;
-      first = min(nb, split * per);
-      nb = min(nb, first + per) - first;
+      const int per = (p.nb + pl.splits - 1) / pl.splits;
+      first = min(p.nb, split * per);
+      p.nb = min(p.nb, first + per) - first;
     }
-    key0 = k_lo + first * kKeys;
-    return nb;
+    p.key0 = k_lo + first * kKeys;
+    p.near = 0;
+    if (BIAS && p.nb > 0) {
+      const int last = min(sh.rq.n - 1, (int)((uint64_t)(uint32_t)(sh.tile * kPair + kPair - 1) * a.group_mul >> a.group_shift));
+      p.near = min(p.nb - 1, max(0, sh.rq.len - sh.rq.n + last - p.key0) / kKeys);
+    }
+    return p;
   };
-  // The j-th block taken.  Under a distance bias the nearest keys come first, so that a row meets its
-  // largest scores at once (front to back every block raises the maximum: 1770 us against 915 for 4096
-  // tokens behind 4096).  Without one a row's first block is better a whole one than its diagonal.
-  auto block_at = [](int j, int nb) { return BIAS ? nb - 1 - j : j; };
+  auto block_at = [](const Plan& p, int j) { return (BIAS && j <= p.near ? p.near - j : j) * kKeys; };
 
   if (warp < kSoftmaxThreads / 32) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -347,8 +358,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       }
       __syncwarp();
     }
-    int key0, k_hi;
-    const int nb = plan(key0, k_hi);
+    const Plan keys = plan();
+    const int nb = keys.nb;
     const int f_lo = sh.full_lo, f_hi = sh.full_hi;
     const uint32_t lanes = sh.tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t to = lanes + 2 * kTile + w * D;
@@ -397,7 +408,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     bool ok = true, low = true;  // low: no score so far has left the three-coefficient range
 #pragma unroll 1
     for (int j = 0; j < nb && on; ++j) {
-      const int kb = key0 + block_at(j, nb) * kKeys;
+      const int kb = keys.key0 + block_at(keys, j);
       const uint32_t ts = lanes + w * kTile + (j & 1) * kKeys;  // S, and P over its first half
       ok = __all_sync(0xffffffffu, s_ready(j));
       if (!ok) {
@@ -410,9 +421,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       const int vis_lo = me.lo - kb, vis_hi = me.hi - kb;
       auto seen = [&](int c) { return c >= vis_lo && c < vis_hi; };
       // The log2 score of raw sum v at key kb + c is u * f, u = v or its capped form, with a bias less
-      // slope * |ahead - c|.  Where no visible key lies ahead of its row, no absolute value is needed.
+      // slope * |ahead - c|.  Where the visible keys of all rows lie on one side of them, no absolute value is
+      // needed: the bias is toward * (c - ahead).
       const float ahead = (float)(me.pos - kb);
       const bool behind = BIAS && __all_sync(0xffffffffu, !live || min(me.hi, kb + kKeys) - 1 <= me.pos);
+      const bool beyond = BIAS && !behind && __all_sync(0xffffffffu, !live || max(me.lo, kb) >= me.pos);
+      const float toward = beyond ? -slope : slope;
       auto exact_unit = [&](float v) -> float { return CAP ? tanh_from_2l2e(v * fac) : v; };
       auto bias = [&](int c) -> float { return -slope * fabsf(ahead - (float)c); };
 
@@ -463,14 +477,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
         constexpr bool MASK = decltype(masked)::value, EXACT = decltype(mode)::value == kExact;
         constexpr bool LOW = decltype(mode)::value == kLow;
         const float org = m_ref == -INFINITY ? 0.f : m_ref;
-        const f32x2 org2 = pair2(-org, -org), f2 = pair2(f, f), step2 = pair2(2.f * slope, 2.f * slope);
+        const f32x2 org2 = pair2(-org, -org), f2 = pair2(f, f), step2 = pair2(2.f * toward, 2.f * toward);
         const float z1 = fac * 0.34657359027997264f;  // fac carries 2 log2(e)
         f32x2 sum2 = pair2(0.f, 0.f);
         auto columns = [&](const uint32_t(&v)[32], int c0) {
           f32x2 b2 = org2;
           if (BIAS && !EXACT) {
-            const float b1 = fmaf(slope, (float)c0 - ahead, -org);
-            b2 = pair2(b1, b1 + slope);
+            const float b1 = fmaf(toward, (float)c0 - ahead, -org);
+            b2 = pair2(b1, b1 + toward);
           }
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
@@ -521,7 +535,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       };
       // The first block that a row sees sets its m_ref.  Later ones rarely exceed it by 2^kSlack: they are
       // tried against the old one, and done again where some row of the warp does.
-      bool again = (BIAS && !behind) ||
+      bool again = (BIAS && !CAP && !behind && !beyond) ||
                    __any_sync(0xffffffffu, live && m_ref == -INFINITY && me.lo < min(me.hi, kb + kKeys) && me.hi > kb);
       if (!again) {
         if (edge)
@@ -631,17 +645,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
     // ------------------------------------------------------------------ keys and values
     const int lt = threadIdx.x - kSoftmaxThreads;  // 0 .. 127
-    int key0, k_hi;
-    const int nb = plan(key0, k_hi);
+    const Plan keys = plan();
+    const int nb = keys.nb;
     const int f_lo = sh.full_lo, f_hi = sh.full_hi;
     // Threads 0 .. 63: the cache row (of D bytes) of the block's key lt; kNoRow: reads zeros.
     constexpr uint32_t kNoRow = 0xffffffffu;
     uint32_t* offs = reinterpret_cast<uint32_t*>(smem + C::OFF0);
     auto offset = [&](int j) {
       if (lt >= kKeys || j >= nb) return;
-      const int key = key0 + block_at(j, nb) * kKeys + lt;
+      const int key = keys.key0 + block_at(keys, j) + lt;
       uint32_t off = kNoRow;
-      if (key < k_hi) {
+      if (key < keys.k_hi) {
         const int page = a.page_table[(size_t)b * a.table_ld + page_of(a, key)];
         if (page >= 0 && page < a.num_pages)
           off = (uint32_t)(((long long)page * a.P + key - page_of(a, key) * a.P) * a.Hkv + head);
@@ -705,7 +719,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       if (sync_any(!ok)) return false;
       if (j + 1 < nb) fetch(j + 1, next);
       offset(j + 2);
-      const int st = j % kDepth, kb = key0 + block_at(j, nb) * kKeys;
+      const int st = j % kDepth, kb = keys.key0 + block_at(keys, j);
       ok = mbar_wait(&sh.kv_empty[st], ((uint32_t)(j / kDepth) & 1u) ^ 1u, a.err, abort_flag);
       store(smem + C::K0 + st * C::BLOCK, now.k);
       fence_async_smem();
@@ -750,8 +764,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     // ------------------------------------------------------------------ MMA issue, a warp per tile
     const int w = warp - kIssueWarp;
     if (w < 2 && lane == 0) {
-      int key0, k_hi;
-      const int nb = plan(key0, k_hi);
+      const int nb = plan().nb;
       const bool two = b >= 0 && (a.cu_q[b + 1] - a.cu_q[b]) * a.G - sh.tile * kPair > kTile;
       const uint32_t t_s = sh.tmem + w * kTile, t_o = sh.tmem + 2 * kTile + w * D;
       const uint32_t id_s = umma_idesc_f16(kKeys, false), id_o = umma_idesc_f16(D, true);

@@ -2,8 +2,8 @@
 
 Tolerance, derived: q.k is a sum of D <= 128 exact products in fp32, off by at most (D / 8) * 2^-23 of
 sum |q||k|; with |q| ~ 2, |k| ~ 1, D = 128 that is below 2^-11 of a score unit after the softmax scale, and the
-factors and the cap add 2^-22 of a score of at most 50.  So each p is within 2^-10.5 relative, plus its
-own rounding to f16 (2^-11, or 2^-25 of the row's largest p for the small ones): o is within 2^-9.5 of
+factors add 2^-22 of a score of at most 50, the cap's tanh (within 1.2e-6) 2^-14 at a cap of 50.  So each p is
+within 2^-10.5 relative, plus its own rounding to f16 (2^-11, or 2^-25 of the row's largest p for the small ones): o is within 2^-9.5 of
 a = sum p|v| before, and 2^-8 of itself by, the rounding to bf16."""
 
 import math
@@ -256,3 +256,16 @@ def test_refusals(ops):
     for kw in bad:
         with pytest.raises(OkcError):
             ops.attn_chunk(**{**c, **kw})
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("new,old,prefix", [([150, 40], [300, 10], [430, 50]), ([400], [100], [260]), ([70, 70, 70], [900, 0, 64], [0, 70, 1000]),
+                                            ([2000], [100], [2100])])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (14, 2, 64)])
+def test_a_bias_over_keys_on_both_sides(ops, new, old, prefix, cap, Hq, Hkv, D):
+    """Rows inside a prefix that ends blocks behind them see keys ahead of their position, lowered as those behind are."""
+    c = _case(new, old, Hq, Hkv, D, 16, seed=len(new) + Hq, cap=cap, slopes=True)
+    c["prefix_lens"] = torch.tensor(prefix, dtype=torch.int32)
+    _check(ops, c, max_q=max(new))
+    c["window"] = 90
+    _check(ops, c, max_q=max(new))
