@@ -86,7 +86,8 @@ __device__ __forceinline__ int f16_shift(uint32_t top) { return max(-100, (int)(
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 // A kernel of this file family serves the requests of at most / more than this many rows a KV
-// head (new tokens x query heads of one KV head).
+// head (new tokens x query heads of one KV head).  128 requests of 64 / 8 heads, the short chunks' kernel against the
+// tensor-memory one: 32 rows 416 and 637 us, 64 rows 676 and 767; one request of 64 rows 35 and 35.
 constexpr int kSplitRows = 64;
 
 // The tensor-memory kernel (attention_chunk_tc.cu) for the requests above kSplitRows.

@@ -9,8 +9,10 @@
 // the token, so this costs R 64-bit reductions a token against (Hq + Hkv) D / 2 rotations.
 // Rotations are fp32; q is rounded once to bf16 and k, v once to e4m3 (RNE, overflow -> NaN).
 //
-// HBM-bound: 2 (Hq + 2 Hkv) D bytes in, 2 Hq D + 2 Hkv D bytes out per token.  A block takes one token;
-// each thread moves 16-byte vectors.
+// 2 (Hq + 2 Hkv) D bytes in, 2 Hq D + 2 Hkv D bytes out per token, in 16-byte vectors.  The instructions
+// (about 110 a vector, more for e4m3) weigh more than the bytes, and for few tokens the chain to the page id: row
+// vectors are fetched before it, and a thread fetches its next vector before it turns one.
+// 8000 tokens of 28 + 4 heads of 128, 96 of them turned: 16.7 us, 3.8 TB/s; 128 tokens of 64 + 8 heads: 5 us.
 #include "chunk_common.cuh"
 
 namespace okc {
