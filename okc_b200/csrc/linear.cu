@@ -436,14 +436,15 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
   }
 }
 
-// Channels a tile: the multiple of 32 from 64 to 256 whose waves cost least (a tile's time goes with its
-// width, plus a constant of 16 channels' worth for its ends).
+// Channels a tile: the multiple of 32 from 64 to 256 whose waves cost least.  A stage's time goes with the rows it
+// loads, 256 and bn of them (1024 x 8192 x 8192 in e4m3, a wave of 32 stages: 16.9, 18.9, 21, 26.9, 27 us at 64, 128,
+// 160, 224 and 256 channels), not with its products.
 int tall_bn(int M, int N, int pairs) {
   int best = 256;
   long long cost = -1;
   for (int bn = 256; bn >= 64; bn -= 32) {
     const long long tiles = (long long)((M + 255) / 256) * ((N + bn - 1) / bn);
-    const long long c = (tiles + pairs - 1) / pairs * (bn + 16);
+    const long long c = (tiles + pairs - 1) / pairs * (bn + 256);
     if (cost < 0 || c < cost) {
       cost = c;
       best = bn;
