@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
       if (a.res && lane < rows) {  // this lane's row of the residual, into L2 while the products run (777 x 4095: 1 to 4 us)
         const int re = a.res_fp32 ? 4 : 2, n0 = tn * bn + c_first * 32, cols = min(c_n * 32, a.N - n0);
         const uint8_t* p = reinterpret_cast<const uint8_t*>(a.res) + ((size_t)(m0 + lane) * a.ldr + n0) * re;
-        for (int i = 0; i < cols * re + 128; i += 128)  // a row may begin inside a line
+        for (int i = 0; cols > 0 && i < cols * re + 128; i += 128)  // a row may begin inside a line
           asm volatile("prefetch.global.L2 [%0];" ::"l"(p + min(i, cols * re - 1)));
       }
       auto emit = [&](int c) {

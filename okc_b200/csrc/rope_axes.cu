@@ -12,7 +12,7 @@
 // 2 (Hq + 2 Hkv) D bytes in, 2 Hq D + 2 Hkv D bytes out per token, in 16-byte vectors.  The instructions
 // (about 110 a vector, more for e4m3) weigh more than the bytes, and for few tokens the chain to the page id: row
 // vectors are fetched before it, and a thread fetches its next vector before it turns one.
-// 8000 tokens of 28 + 4 heads of 128, 96 of them turned: 16.7 us, 3.8 TB/s; 128 tokens of 64 + 8 heads: 5 us.
+// 3614 tokens of 28 + 4 heads of 128, 96 elements turned: 16.7 us, 3.8 TB/s; 128 tokens of 64 + 8 heads: 5 us.
 #include "chunk_common.cuh"
 
 namespace okc {
@@ -209,8 +209,8 @@ int launch_rope_axes_append(const RopeAxesArgs& args, cudaStream_t stream) {
   a.by_pp = by((a.D - 2 * a.R) / 8);
   a.by_vp = by(a.D / 8);
   a.by_r = by(a.R);
-  // 8000 tokens of 28 + 4 heads 16.7 us, a token a block 19.4; 2000 tokens 7.1 either way
-  if (a.T >= 2048)
+  // 3614 tokens of 28 + 4 heads 16.7 us, a token a block 19.4; 1806 tokens 10.5 and 11.8; 903 tokens 7.1 either way
+  if (a.T >= 1024)
     return okc_host::launch_k(rope_axes_append_kernel<4>, dim3((a.T + 3) / 4), dim3(kRopeThreads), 0, stream, dim3(1), a);
   // a thread for each item (see the kernel), within two to eight warps
   const int items = (a.Hq + a.Hkv) * (a.D / 8 - a.R / 8) + a.Hkv * (a.D / 8);
