@@ -27,7 +27,7 @@ ERR_NAMES = {
     OKC_ERR_WORKSPACE: "workspace too small",
     OKC_ERR_LAUNCH: "CUDA launch failed",
     OKC_ERR_DEVICE: "no sm_100a device or kernel image",
-    OKC_ERR_TOO_LARGE: "request exceeds the fixed scratch of the no-alloc entry point",
+    OKC_ERR_TOO_LARGE: "request exceeds a fixed limit (scratch of the no-alloc entry point, 32-bit counts)",
 }
 DEVERR_TIMEOUT, DEVERR_PAGE, DEVERR_INDEX = 1, 2, 4
 

@@ -399,6 +399,11 @@ _current_device = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
+def _device(t: torch.Tensor) -> int:
+    dev = t.get_device()
+    return dev if dev >= 0 else _dev_index(t)  # which refuses it
+
+
 def _bad(t, name: str, dtype, shape: tuple, dev: int) -> _lib.OkcError:
     if t.dtype != dtype and not (isinstance(dtype, tuple) and t.dtype in dtype):
         return _lib.OkcError(f"{name}: expected {dtype}, got {t.dtype}")
@@ -445,19 +450,19 @@ def add_rmsnorm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float, residual: torc
     (1 for a row of zeros), q = e4m3(y / scale).  x bf16 [T, H] and w bf16 [H]; residual bf16 or
     fp32 [T, H]; H a multiple of 16 up to 16384.  Returns (q e4m3 [T, H], scale fp32 [T], s or
     None); s goes to `residual_out`, which may be `residual`."""
-    dev = _dev_index(x)
+    dev = _device(x)
     if x.dim() != 2:
         raise _lib.OkcError(f"x: expected [T, H], got {tuple(x.shape)}")
-    T, H = shape = tuple(x.shape)
+    T, H = shape = x.shape
     ldx = _rows(x, "x", torch.bfloat16, shape, dev)
     wp = _dense(w, "w", torch.bfloat16, (H,), dev)
-    q = x.new_empty(shape, dtype=_E4M3)
+    q = torch.empty_like(x, dtype=_E4M3)  # dense, as every output: the rows of x may be strided
     scale = x.new_empty(T, dtype=torch.float32)
     rp, rld, op, old, r32 = None, 0, None, 0, 0
     if residual is not None:
         rld = _rows(residual, "residual", _STREAM_TYPES, shape, dev)
         if residual_out is None:
-            residual_out, old = residual.new_empty(shape), H
+            residual_out, old = torch.empty_like(residual), H
         else:
             old = _rows(residual_out, "residual_out", residual.dtype, shape, dev)
         rp, op, r32 = residual.data_ptr(), residual_out.data_ptr(), int(residual.dtype is torch.float32)
@@ -480,7 +485,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor | None = None
     [N] or [1]; bias bf16 [N]; act None, "relu", "silu", "gelu" or "gelu_tanh"; residual bf16 or
     fp32 [M, N]; y bf16 or fp32 [M, N] (`out`, which may be `residual`, or a new tensor of `out_dtype`).
     K is a multiple of 16 (e4m3) or 8 (bf16), x and w rows 16-byte aligned."""
-    dev = _dev_index(x)
+    dev = _device(x)
     if x.dim() != 2 or w.dim() != 2:
         raise _lib.OkcError(f"x and w: expected [M, K] and [N, K], got {tuple(x.shape)} and {tuple(w.shape)}")
     if act not in LINEAR_ACTS:
@@ -551,7 +556,7 @@ def rope_axes_kv_append(qkv: torch.Tensor, positions: torch.Tensor, axes, inv_fr
     pair (see rope_sections; its length, a multiple of 8, is the number of pairs), inv_freq fp32 [len(axes)].
     A pair is (2i, 2i + 1), or with `half` (i, i + len(axes)); the head's other elements pass.  Returns
     q bf16 [T, Hq, D]; rows behind cu_q[B] are left as they are."""
-    dev = _dev_index(qkv)
+    dev = _device(qkv)
     if qkv.dim() != 2 or positions.dim() != 2:
         raise _lib.OkcError(f"qkv and positions: expected [T, C] and [A, T], got {tuple(qkv.shape)}, {tuple(positions.shape)}")
     T, A = qkv.shape[0], positions.shape[0]
@@ -589,10 +594,10 @@ def attn_chunk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     (0 = uncapped), then lowered by slopes[h] * |p - j| (fp32 [Hq]).  max_q, the longest chunk if the
     caller knows it, only chooses kernels.  Returns bf16 [T, Hq, D]: zero for a row that sees nothing, rows
     behind cu_q[B] as they were."""
-    dev = _dev_index(q)
+    dev = _device(q)
     if q.dim() != 3:
         raise _lib.OkcError(f"q: expected [T, Hq, D], got {tuple(q.shape)}")
-    T, Hq, D = shape = tuple(q.shape)
+    T, Hq, D = shape = q.shape
     ldq = _rows(q, "q", torch.bfloat16, shape, dev)
     cq, sl, B, table, table_ld, cols = _ragged(cu_q, seq_lens, page_table, dev)
     kc, vc, ks, vs, pages, P, Hkv = _caches(k_cache, v_cache, k_scale, v_scale, None, D, dev)
@@ -604,7 +609,7 @@ def attn_chunk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     if doc_start is not None:
         dp = _dense(doc_start, "doc_start", torch.int32, (T,), dev)
     if out is None:
-        out, ldo = q.new_empty(shape), Hq * D
+        out, ldo = torch.empty_like(q), Hq * D
     else:
         ldo = _rows(out, "out", torch.bfloat16, shape, dev)
     if T:
