@@ -52,7 +52,7 @@ struct SplitPlan {
   int nh, nsub, hg;   // heads side by side in a block, key subgroups, head groups
   int step_keys;      // keys of a unit
   int rows;           // rows of a tile: 16, or 8 where no request has more
-  int ctas;
+  int ctas, few;      // CTAs of the grid, and those that share little work (shared_by)
   int* pre_u;         // [B + 1] units before a request
   int* pre_t;         // [B + 1] row tiles (times head groups) before a request
   float* ml;          // [slot][nh][16][2]
@@ -70,6 +70,11 @@ __device__ __forceinline__ int unit_owner(int U, int C, int u) {
   const int q = U / C, r = U % C, big = r * (q + 1);
   return u < big ? u / (q + 1) : r + (u - big) / q;
 }
+
+// How many of the CTAs share U units.  A second one an SM (heads of 64) hides the first's latency where each has some
+// units, and costs the merge twice the segments where not: 128 requests 131 us against 208, 16 requests 31 and 40; one token
+// behind 81919 (4 units an SM) 24.2 and 21.6, behind 2000 11.1 and 10.6.
+__device__ __forceinline__ int shared_by(const SplitPlan& pl, int U) { return U > 6 * pl.few ? pl.ctas : pl.few; }
 
 // Units and row tiles before each request, by one warp.
 __device__ __forceinline__ void split_prefix(const ChunkArgs& a, const SplitPlan& pl, int* pre_u, int* pre_t) {
@@ -131,8 +136,9 @@ __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) attn_chunk_split
       pl.pre_u[i] = pre_u[i];
       pl.pre_t[i] = pre_t[i];
     }
-  int u0, u1;
-  unit_split(pre_u[a.B], gridDim.x, blockIdx.x, u0, u1);
+  const int share = shared_by(pl, pre_u[a.B]);
+  int u0 = 0, u1 = 0;
+  if ((int)blockIdx.x < share) unit_split(pre_u[a.B], share, blockIdx.x, u0, u1);
   const int hw = warp % pl.nh, sub = warp / pl.nh;
   uint8_t* ring = smem + warp * C::RING;
   const uint32_t ring_s = smem_u32(ring);
@@ -582,7 +588,8 @@ __global__ void __launch_bounds__(256) attn_chunk_merge_kernel(ChunkArgs a, Spli
       const int h = hq / a.G, r = (t - a.cu_q[b]) * a.G + hq - h * a.G;
       const int in_t = (r / pl.rows) * pl.hg + h / pl.nh, tile = pl.pre_t[b] + in_t;
       const int U = pl.pre_u[a.B], first = pl.pre_u[b] + in_t * nc;
-      const int s0 = unit_owner(U, pl.ctas, first), s1 = unit_owner(U, pl.ctas, first + nc - 1) + 1;
+      const int share = shared_by(pl, U);
+      const int s0 = unit_owner(U, share, first), s1 = unit_owner(U, share, first + nc - 1) + 1;
       const size_t in_slot = (size_t)(h % pl.nh) * pl.rows + r % pl.rows, per = (size_t)pl.nh * pl.rows;
       for (int base = s0 + sub; base < s1; base += 32 * WPR) {  // segments base, base + WPR, ..: a lane each
         const int mine_at = base + lane * WPR;
@@ -645,9 +652,12 @@ int heads_a_block(int Hkv) { return Hkv % 8 == 0 ? 8 : Hkv % 4 == 0 ? 4 : Hkv % 
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
-size_t split_slots(int T, int B, int Hq, int Hkv, int rows) {
+// CTAs at most: as many as are resident at once.
+int split_ctas(int D) { return okc_host::num_sms() * (D == 64 ? 2 : 1); }
+
+size_t split_slots(int T, int B, int Hq, int Hkv, int D, int rows) {
   const size_t hg = Hkv / heads_a_block(Hkv);
-  return okc_host::num_sms() + (((size_t)T * (Hq / Hkv) + rows - 1) / rows + B) * hg;
+  return split_ctas(D) + (((size_t)T * (Hq / Hkv) + rows - 1) / rows + B) * hg;
 }
 
 template <int D, bool CAP, int R>
@@ -671,7 +681,7 @@ int launch_split(const ChunkArgs& a, const SplitPlan& pl, cudaStream_t stream) {
 
 size_t attn_chunk_ws_bytes(int T, int B, int Hq, int Hkv, int D) {
   // 16-row tiles need the more: up to B tiles more of twice the rows
-  const size_t rows = split_slots(T, B, Hq, Hkv, 16) * heads_a_block(Hkv) * 16;
+  const size_t rows = split_slots(T, B, Hq, Hkv, D, 16) * heads_a_block(Hkv) * 16;
   return 2 * up((size_t)(B + 1) * 4) + up(rows * 8) + up(rows * D * 4) + attn_chunk_tc_ws_bytes(T, B, Hq, Hkv, D);
 }
 
@@ -681,13 +691,17 @@ int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
   pl.nsub = kWarps / pl.nh;
   pl.hg = a.Hkv / pl.nh;
   pl.step_keys = kStep * pl.nsub;
-  pl.ctas = okc_host::num_sms();
+  pl.few = okc_host::num_sms();
+
   // every request short: this kernel alone; else each kernel serves its requests
   const bool split_only = a.max_q > 0 ? (long long)a.max_q * a.G <= kSplitRows : (long long)a.T * a.G <= kSplitRows;
   pl.most_rows = split_only ? 0x7fffffff : kSplitRows;
   pl.merge_tokens = split_only ? 0 : kSplitRows / a.G;
   pl.rows = split_only && a.max_q > 0 && (long long)a.max_q * a.G <= 8 ? 8 : 16;
-  const size_t rows = split_slots(a.T, a.B, a.Hq, a.Hkv, pl.rows) * pl.nh * pl.rows;
+  // the grid by the units that the table's width allows; the kernels know how many there are
+  const long long row_tiles = ((long long)a.T * a.G - a.B) / pl.rows + a.B;
+  pl.ctas = row_tiles * pl.hg * (a.max_keys / pl.step_keys + 1) > 6 * pl.few ? split_ctas(a.D) : pl.few;
+  const size_t rows = split_slots(a.T, a.B, a.Hq, a.Hkv, a.D, pl.rows) * pl.nh * pl.rows;
   uint8_t* p = reinterpret_cast<uint8_t*>(a.ws);
   pl.pre_u = reinterpret_cast<int*>(p);
   p += up((size_t)(a.B + 1) * 4);

@@ -269,3 +269,15 @@ def test_a_bias_over_keys_on_both_sides(ops, new, old, prefix, cap, Hq, Hkv, D):
     _check(ops, c, max_q=max(new))
     c["window"] = 90
     _check(ops, c, max_q=max(new))
+
+
+@pytest.mark.parametrize("new", [1, 3])
+def test_many_steps_of_64_wide_heads(ops, new):
+    """Enough key steps for two blocks an SM, and a table that allows them where few are used."""
+    B = 40
+    c = _case([new] * B, [(331 * i) % 1900 + 300 for i in range(B)], 16, 8, 64, 16, seed=20, cap=30.0)
+    _check(ops, c, max_q=new)
+    c["seq_lens"] = torch.tensor([(5 * i) % 40 + new for i in range(B)], dtype=torch.int32)
+    _check(ops, c, max_q=new)
+    d = _cuda(c)
+    assert torch.equal(ops.attn_chunk(**d, max_q=new), ops.attn_chunk(**d, max_q=new))
