@@ -110,7 +110,7 @@ __device__ __forceinline__ void block_put(float* block, int row, int pair, float
 // columns of every second row.  Residual rows are fetched ahead of the stores, which may overwrite them.
 template <bool OUT32>
 __device__ __forceinline__ void tall_block(const float* block, float my_sx, const LinearArgs& a, int m0, int n0) {
-  constexpr int B = 4;  // a lane's rows in flight
+  constexpr int B = 8;  // a lane's rows in flight
   const int lane = threadIdx.x & 31, odd = lane >> 4, pair = lane & 15;
   const int oe = OUT32 ? 4 : 2, re = a.res_fp32 ? 4 : 2;
   float sw[2], bias[2];
