@@ -693,11 +693,19 @@ int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
   pl.step_keys = kStep * pl.nsub;
   pl.few = okc_host::num_sms();
 
-  // every request short: this kernel alone; else each kernel serves its requests
-  const bool split_only = a.max_q > 0 ? (long long)a.max_q * a.G <= kSplitRows : (long long)a.T * a.G <= kSplitRows;
+  // Every request short: this kernel alone.  Also where all of them make few tiles and steps (as far as T and the
+  // table's width tell), since two kernels and two merges in a row take longer: 8 chunks of up to 44 tokens behind 325
+  // positions, 8 / 1 heads, 19 us against 37, behind 2000 36 and 45; 16 / 8 heads 22 and 36; at 64 / 8 heads (295000 rows
+  // of tiles times keys) 37 either way.  One long request: the tensor-memory kernel alone.  Else each serves its own.
+  const long long longest = a.max_q > 0 && a.max_q < a.T ? a.max_q : a.T;
+  const long long tiles16 = ((long long)a.T * a.G - a.B) / 16 + a.B;
+  const bool split_only =
+      longest * a.G <= kSplitRows || (tiles16 * pl.hg <= okc_host::num_sms() &&
+                                      tiles16 * a.max_keys * a.Hkv * a.D / 128 <= (a.B == 1 ? 20000 : 300000));
+  const bool tc_only = !split_only && a.B == 1;
   pl.most_rows = split_only ? 0x7fffffff : kSplitRows;
   pl.merge_tokens = split_only ? 0 : kSplitRows / a.G;
-  pl.rows = split_only && a.max_q > 0 && (long long)a.max_q * a.G <= 8 ? 8 : 16;
+  pl.rows = split_only && longest * a.G <= 8 ? 8 : 16;
   // the grid by the units that the table's width allows; the kernels know how many there are
   const long long row_tiles = ((long long)a.T * a.G - a.B) / pl.rows + a.B;
   pl.ctas = row_tiles * pl.hg * (a.max_keys / pl.step_keys + 1) > 6 * pl.few ? split_ctas(a.D) : pl.few;
@@ -712,8 +720,8 @@ int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
   pl.acc = reinterpret_cast<float*>(p);
   p += up(rows * a.D * 4);
   if (!split_only) {
-    if (int st = launch_attn_chunk_tc(a, p, stream)) return st;
-    if (pl.merge_tokens == 0) return OKC_OK;  // no request is short enough
+    if (int st = launch_attn_chunk_tc(a, tc_only ? 0 : kSplitRows, p, stream)) return st;
+    if (tc_only || pl.merge_tokens == 0) return OKC_OK;  // no request is short enough
   }
   const bool cap = a.softcap > 0.f;
   if (a.D == 64) {

@@ -63,6 +63,7 @@ struct TcCfgA {
 
 struct TcPlanA {
   int splits;
+  int above;   // requests of more rows than this are served
   float* acc;  // [splits][T * Hq][D]
   float* ml;   // [splits][T * Hq][2]
 };
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
   }
   pdl_wait();
   const int head = blockIdx.x % a.Hkv, split = blockIdx.x / a.Hkv;
-  if (warp == 0) {  // the blockIdx.y-th tile pair of the requests above kSplitRows
+  if (warp == 0) {  // the blockIdx.y-th tile pair of the requests it serves
     int before = 0, found = -1, tile = 0;
     for (int base = 0; base < a.B && found < 0; base += 32) {
       const int b = base + lane;
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       if (b < a.B) {
         r = request(a, b);
         const int rows = r.n * a.G;
-        if (rows > kSplitRows) n = (rows + kPair - 1) / kPair;
+        if (rows > pl.above) n = (rows + kPair - 1) / kPair;
         if (r.len > a.max_keys && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(a.err, OKC_DEVERR_PAGE);
       }
       int sum = n;
@@ -834,7 +835,7 @@ __global__ void __launch_bounds__(256) attn_chunk_tc_merge_kernel(ChunkArgs a, T
   if (item >= all) return;
   const int t = (int)(item / a.Hq), hq = (int)(item - (long long)t * a.Hq);
   const int b = find_request(a.cu_q, a.B, t);
-  if (b < 0 || (a.cu_q[b + 1] - a.cu_q[b]) * a.G <= kSplitRows) return;
+  if (b < 0 || (a.cu_q[b + 1] - a.cu_q[b]) * a.G <= pl.above) return;
   float2 ml = make_float2(-INFINITY, 0.f);
   if (lane < pl.splits) ml = *reinterpret_cast<const float2*>(pl.ml + ((size_t)lane * all + item) * 2);
   const float M = warp_max(ml.x), org = M == -INFINITY ? 0.f : M;
@@ -899,8 +900,9 @@ size_t attn_chunk_tc_ws_bytes(int T, int B, int Hq, int Hkv, int D) {
   return up(rows * D * 4) + up(rows * 8);
 }
 
-int launch_attn_chunk_tc(const ChunkArgs& a, void* ws, cudaStream_t stream) {
+int launch_attn_chunk_tc(const ChunkArgs& a, int above, void* ws, cudaStream_t stream) {
   TcPlanA pl;
+  pl.above = above;
   pl.splits = tc_splits(a.T, a.B, a.Hq, a.Hkv, a.max_keys);
   pl.acc = reinterpret_cast<float*>(ws);
   pl.ml = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + up((size_t)pl.splits * a.T * a.Hq * a.D * 4));

@@ -90,8 +90,9 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 // tensor-memory one: 32 rows 416 and 637 us, 64 rows 676 and 767; one request of 64 rows 35 and 35.
 constexpr int kSplitRows = 64;
 
-// The tensor-memory kernel (attention_chunk_tc.cu) for the requests above kSplitRows.
+// The tensor-memory kernel (attention_chunk_tc.cu) for the requests of more than `above` rows (kSplitRows, or 0
+// where the only request may have more than kSplitRows).
 size_t attn_chunk_tc_ws_bytes(int T, int B, int Hq, int Hkv, int D);
-int launch_attn_chunk_tc(const ChunkArgs& a, void* ws, cudaStream_t stream);
+int launch_attn_chunk_tc(const ChunkArgs& a, int above, void* ws, cudaStream_t stream);
 
 }  // namespace okc

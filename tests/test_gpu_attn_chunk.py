@@ -53,8 +53,24 @@ def _case(new, old, Hq, Hkv, D, P, seed=0, pad=0, cap=0.0, slopes=False, window=
     return c
 
 
+WIDE = False
+
+
+@pytest.fixture(autouse=True, params=[False, True], ids=["narrow", "wide"])
+def table_width(request):
+    """Page tables as wide as the longest request, or with 4096 columns more (which no request reaches): few tiles
+    and a narrow table let the short chunks' kernel take long chunks too, a wide one leaves them to the other."""
+    global WIDE
+    WIDE = request.param
+    yield
+    WIDE = False
+
+
 def _cuda(c):
-    return {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    d = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    if WIDE:
+        d["page_table"] = torch.nn.functional.pad(d["page_table"], (0, 4096), value=-1)
+    return d
 
 
 def _close(o, c, what=""):
@@ -281,3 +297,10 @@ def test_many_steps_of_64_wide_heads(ops, new):
     _check(ops, c, max_q=new)
     d = _cuda(c)
     assert torch.equal(ops.attn_chunk(**d, max_q=new), ops.attn_chunk(**d, max_q=new))
+
+
+def test_one_request_with_rows_behind_it(ops):
+    """A single request of a few rows in a batch padded for many, whatever max_q says."""
+    c = _case([3], [40], 8, 2, 128, 16, seed=21, pad=200, slopes=True)
+    for m in (None, 1, 3, 203, 5000):
+        _check(ops, c, max_q=m)
