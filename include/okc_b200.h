@@ -458,7 +458,8 @@ int okc_rope_axes_kv_append(const void* qkv, int64_t ldqkv, const int64_t* posit
  * [num_pages, P, Hkv, D] with scales fp32 [Hkv], page_table int32 [B][table_ld] (max_pages columns).  A
  * position on a page outside the pool reads zeros, one past the table does not exist (both
  * OKC_DEVERR_PAGE).  max_q: the longest chunk (0 = unknown); it only chooses kernels.  D 64 or
- * 128, B <= 2048, Hq / Hkv whole, 16-byte aligned rows, fewer than 2^32 - 1 cache rows of D.  The
+ * 128, B <= 2048, Hq / Hkv whole, 16-byte aligned rows, fewer than 2^32 - 1 cache rows of D,
+ * T * Hq / Hkv + 256 B below 2^24.  The
  * workspace is scratch of the size that the call's own T and B ask for (fewer requests may need more).
  * Beside okc_attn_decode_fp8 and okc_attn_prefill_fp8. */
 size_t okc_attn_chunk_workspace_bytes(int T, int B, int Hq, int Hkv, int D);

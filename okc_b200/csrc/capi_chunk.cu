@@ -156,6 +156,8 @@ int okc_attn_chunk_fp8(const void* q, int64_t ldq, const void* k_cache, const vo
   const long long keys = (long long)max_pages * page_size < most_keys ? (long long)max_pages * page_size : most_keys;
   const long long tiles = ((long long)T * (Hq / Hkv) + 15) / 16 + B;
   if ((long long)T * Hq > 0x7fffffffll || tiles * Hkv * (keys / 32 + 1) > 0x7fffffffll) return OKC_ERR_TOO_LARGE;
+  // row tile pairs are a grid's second dimension
+  if ((long long)T * (Hq / Hkv) / 256 + B > 65535) return OKC_ERR_TOO_LARGE;
   // ... and so are the cache's rows of D bytes: 256 GB of keys at D = 64
   if (num_pages > 0xfffffffell / page_size / Hkv) return OKC_ERR_TOO_LARGE;
   if (!workspace || workspace_bytes < okc::attn_chunk_ws_bytes(T, B, Hq, Hkv, D)) return OKC_ERR_WORKSPACE;

@@ -83,7 +83,7 @@ def test_attention_refusals(lib, code):
         assert _call(fn, ATTN, **bad) == code.OKC_ERR_ALIGNMENT, bad
     # rows of the cache, of the work list and of the output are counted in 32 bits
     for bad in (dict(num_pages=2 ** 27), dict(num_pages=2 ** 40), dict(page_size=2 ** 30, num_pages=4),
-                dict(T=2 ** 30, Hq=4), dict(T=2 ** 24, max_pages=2 ** 20, table_ld=2 ** 20)):
+                dict(T=2 ** 30, Hq=4), dict(T=2 ** 23, Hq=4), dict(T=2 ** 24, max_pages=2 ** 20, table_ld=2 ** 20)):
         assert _call(fn, ATTN, **bad) == code.OKC_ERR_TOO_LARGE, bad
     assert _call(fn, ATTN) == code.OKC_ERR_WORKSPACE
     assert _call(fn, ATTN, workspace=256, workspace_bytes=100) == code.OKC_ERR_WORKSPACE
