@@ -74,6 +74,7 @@ int okc_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int e4m3,
   a.e4m3 = e4m3;
   a.pairs = ldy % 2 == 0 && aligned_to(y, out_fp32 ? 8 : 4) &&
             (!residual || (ldr % 2 == 0 && aligned_to(residual, residual_fp32 ? 8 : 4)));
+  a.packed = !out_fp32 && !residual && ldy % 8 == 0 && aligned16(y);
   a.err = error;
   return okc::launch_linear(a, stream);
 }

@@ -160,6 +160,7 @@ struct LinearArgs {
   int M, N, K;
   int e4m3;
   int pairs;  // y's and the residual's rows take aligned accesses of two columns
+  int packed; // y is bf16 in rows of whole 16-byte vectors, and there is no residual
   int* err;
 };
 int launch_linear(const LinearArgs& a, cudaStream_t stream);

@@ -159,3 +159,18 @@ def test_refusals(ops):
     for kw in bad:
         with pytest.raises(OkcError):
             ops.linear(**{**d, **kw})
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "bf16"])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+def test_tall_blocks_without_a_residual(ops, act, dtype):
+    """bf16 outputs whose rows take 16-byte accesses, and the same products into rows that do not: equal."""
+    c = _case(300, 352, 272, dtype, seed=31)
+    d = _cuda(c)
+    y = ops.linear(**d, act=act)
+    _check(y, c, act)
+    for cols, first in ((360, 8), (355, 0), (360, 3)):
+        wide = torch.full((300, cols), 7.0, dtype=torch.bfloat16, device="cuda")
+        out = wide[:, first:first + 352]
+        assert torch.equal(ops.linear(**d, act=act, out=out), y)
+        assert (wide[:, :first] == 7).all() and (wide[:, first + 352:] == 7).all()
