@@ -586,17 +586,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     const size_t part = (size_t)split * a.T * a.Hq + (size_t)tok * a.Hq + hq;
     const float inv = l == 0.f ? 0.f : __fdividef(a.v_scale[head], l);
     if (pl.splits > 1 && live) *reinterpret_cast<float2*>(pl.ml + part * 2) = make_float2(m_ref, l);
-    // The warp's rows are turned in its share of the query tile (2 D bytes a row), which no MMA reads any more,
-    // and leave as whole rows: all of a bf16 row at once, an fp32 one in halves.
+    // The warp's rows are turned in its share of the query tile (2 D bytes a row) and leave as whole rows: all of a bf16
+    // row at once, an fp32 one in halves.  That share holds other warps' queries, too: the products that `have` tells of
+    // waited for every warp's, and are done with them.  Without them (no keys: the other warps' copies may still be
+    // landing) zeros leave straight from registers.
     uint8_t* turn = smem + C::Q0 + w * C::QTILE + (warp & 3) * 32 * 2 * D;
     auto columns = [&](int c0, uint32_t (&v)[32]) {
-      if (have) {
-        tm_ld32(to + c0, v);
-        tm_wait_ld(v);
-      } else {
-#pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = 0u;
-      }
+      tm_ld32(to + c0, v);
+      tm_wait_ld(v);
       const uint32_t nan = nan_d[c0 / 32];
       if (nan) {
 #pragma unroll
@@ -611,7 +608,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       for (int i = 0; i < QN; ++i) {
         const int row = i * QR + qr;
         const long long to_row = at_row(at, row);
-        const uint4 x = *reinterpret_cast<const uint4*>(turn + row * 2 * D + (qc ^ (row % QC)) * 16);
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (have) x = *reinterpret_cast<const uint4*>(turn + row * 2 * D + (qc ^ (row % QC)) * 16);
         if (to_row >= 0) *reinterpret_cast<uint4*>(base + to_row + qc * 16) = x;
       }
       __syncwarp();
@@ -621,6 +619,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       for (int half = 0; half < 2; ++half) {
 #pragma unroll
         for (int c0 = 0; c0 < D / 2; c0 += 32) {
+          if (!have) break;
           uint32_t v[32];
           columns(half * (D / 2) + c0, v);
 #pragma unroll
@@ -631,6 +630,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     } else {
 #pragma unroll
       for (int c0 = 0; c0 < D; c0 += 32) {
+        if (!have) break;
         uint32_t v[32];
         columns(c0, v);
 #pragma unroll
@@ -845,6 +845,7 @@ __global__ void __launch_bounds__(256) attn_chunk_tc_merge_kernel(ChunkArgs a, T
   for (int e = 0; e < E; ++e) o[e] = 0.f;
   for (int s = 0; s < pl.splits; ++s) {
     const float ws = __shfl_sync(0xffffffffu, w, s);
+    if (__shfl_sync(0xffffffffu, ml.y, s) == 0.f) continue;  // no key of this segment is the row's
     const float* src = pl.acc + ((size_t)s * all + item) * D + lane * E;
 #pragma unroll
     for (int e = 0; e < E; e += 2) {

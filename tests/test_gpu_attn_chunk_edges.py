@@ -1,0 +1,70 @@
+"""Chunk attention (ops.attn_chunk) where it is told little or extremes: row tiles without a key, limits and
+sentinels of its arguments, caps of every size, weights far below the row's largest.  Tolerances beyond those of
+test_gpu_attn_chunk.py stand beside the tests that need them."""
+
+import math
+
+import pytest
+import torch
+
+import test_gpu_attn_chunk as attn
+from oracle import chunk as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from okc_b200 import ops
+    return ops
+
+
+@pytest.fixture(autouse=True)
+def wide_tables():
+    """Tables much wider than the requests, so that long chunks go to the long chunks' kernel."""
+    attn.WIDE = True
+    yield
+    attn.WIDE = False
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new,Hq,Hkv", [(2600, 8, 8), (700, 2, 1)], ids=["keys-whole", "keys-split"])
+def test_row_tiles_without_keys_are_zero(ops, new, Hq, Hkv, D):
+    """Whole 256-row tile pairs that see nothing, beside pairs that do, their queries NaN, infinite and large: zeros
+    each time, and the other rows as they are without those queries.  2600 rows at 8 heads fill the grid (one
+    segment a row), 1400 rows at one head split the keys, of which most rows have few segments."""
+    c = attn._case([new], [40], Hq, Hkv, D, 16, seed=D + new)
+    rows = 256 * Hkv // Hq  # tokens of a tile pair
+    blind = torch.zeros(new, dtype=torch.bool)
+    for pair in (0, 2, 3, new // rows):  # the last one is not whole
+        blind[pair * rows:(pair + 1) * rows] = True
+    c["doc_start"] = torch.where(blind, 10 ** 6, 0).to(torch.int32)
+    d = attn._cuda(c)
+    blind = blind.cuda()
+    d["q"][blind] = 0
+    want = ops.attn_chunk(**d, max_q=new)
+    assert (want[blind] == 0).all() and torch.isfinite(want.float()).all()
+    for value in (float("nan"), float("inf"), 3e38):
+        d["q"][blind] = value
+        for _ in range(5):
+            out = torch.full_like(want, 9.0)
+            assert torch.equal(ops.attn_chunk(**d, max_q=new, out=out), want)
+    d["seq_lens"][0] = 0  # every row sits before position 0
+    for _ in range(5):
+        out = torch.full_like(want, 9.0)
+        assert (ops.attn_chunk(**d, max_q=new, out=out) == 0).all()
+    assert ops.read_device_error("attn_chunk") == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_nan_query_beside_empty_key_segments(ops, D):
+    """A live row of NaN beside rows whose keys lie in the first segment only."""
+    c = attn._case([300], [0], 2, 1, D, 16, seed=D)
+    d = attn._cuda(c)
+    o = ops.attn_chunk(**d, max_q=300)
+    d["q"][7, 1] = float("nan")
+    for _ in range(5):
+        o2 = ops.attn_chunk(**d, max_q=300)
+        assert torch.isnan(o2[7, 1].float()).all()
+        o2[7, 1] = o[7, 1]
+        attn._close(o2, c)
