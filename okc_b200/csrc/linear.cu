@@ -38,6 +38,7 @@ static_assert(128 * kIssueRegs + 256 * kDrainRegs <= kTallThreads * kLaunchRegs,
 static_assert(kIssueRegs < kLaunchRegs && kDrainRegs > kLaunchRegs,
               "setmaxnreg.dec lowers and .inc raises; the other way round is an illegal instruction");
 constexpr int kGroup = 8;        // token tiles of a group
+constexpr uint16_t kLeader = 1, kBoth = 3;  // of a pair
 
 struct TallSmem {
   static constexpr int A_PANEL = 128 * LIN_KB;       // this CTA's 128 token rows
@@ -83,12 +84,13 @@ __device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uin
         " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
-// Arrives on `bar` of both CTAs when every MMA issued so far is done.
-__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+// Arrives on `bar` of the CTAs in `who` (bit = rank) when every MMA issued so far is done.  A CTA waits for all that is
+// signalled to it before it leaves: its shared memory may be another block's by the time a later signal lands.
+__device__ __forceinline__ void pair_commit(uint64_t* bar, uint16_t who) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
           smem_u32(bar)),
-      "h"((uint16_t)3)
+      "h"(who)
       : "memory");
 }
 
@@ -362,19 +364,19 @@ __global__ void __launch_bounds__(kTallThreads, 1) linear_tall_kernel(const __gr
             for (int j = 0; j < LIN_KB / 32; ++j)
               pair_mma<E4M3>(tmem + buf * 256, da + ((p * C::A_PANEL + 32 * j) >> 4),
                              db + ((p * b_panel + 32 * j) >> 4), idesc, !(begin && p == 0 && j == 0));
-          pair_commit(&empty[s]);
+          pair_commit(&empty[s], kBoth);
           if (++s == stages) {
             s = 0;
             ph ^= 1u;
           }
           if (kb == nkb - 1 || (OUT32 && kb % kSegment == kSegment - 1)) {
-            pair_commit(&accf[buf]);
+            pair_commit(&accf[buf], kBoth);
             ++seg;
           }
         }
       }
       if (!ok) *abort_flag = 1;
-      pair_commit(drain);  // no MMA may be in flight when the tensor memory is released
+      pair_commit(drain, kLeader);  // no MMA may be in flight when the tensor memory is released
       mbar_wait(drain, 0, a.err);
     }
   } else {
