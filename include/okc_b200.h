@@ -459,7 +459,10 @@ int okc_rope_axes_kv_append(const void* qkv, int64_t ldqkv, const int64_t* posit
  * position on a page outside the pool reads zeros, one past the table does not exist (both
  * OKC_DEVERR_PAGE).  max_q: the longest chunk (0 = unknown); it only chooses kernels.  D 64 or
  * 128, B <= 2048, Hq / Hkv whole, 16-byte aligned rows, fewer than 2^32 - 1 cache rows of D,
- * T * Hq / Hkv + 256 B below 2^24.  The
+ * T * Hq < 2^31, T * Hq / Hkv + 256 B below 2^24; positions from 2^31 - 2^17 on count as past the table.  Requests of
+ * at most 64 rows (tokens x Hq / Hkv) have their work numbered in 32 bits: where the call may hold some beside others
+ * (B > 1), or only such (by max_q or T), (T * Hq / Hkv / 8 + B) * Hkv * max_pages * page_size below 2^38 is always
+ * enough, and far more is where they are few (OKC_ERR_TOO_LARGE beyond).  The
  * workspace is scratch of the size that the call's own T and B ask for (fewer requests may need more).
  * Beside okc_attn_decode_fp8 and okc_attn_prefill_fp8. */
 size_t okc_attn_chunk_workspace_bytes(int T, int B, int Hq, int Hkv, int D);

@@ -685,8 +685,18 @@ size_t attn_chunk_ws_bytes(int T, int B, int Hq, int Hkv, int D) {
   return 2 * up((size_t)(B + 1) * 4) + up(rows * 8) + up(rows * D * 4) + attn_chunk_tc_ws_bytes(T, B, Hq, Hkv, D);
 }
 
-int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
-  SplitPlan pl;
+namespace {
+
+// How a call is served, but for the workspace's pieces.
+struct Served {
+  SplitPlan split;
+  bool split_only, tc_only;
+  long long units;  // that the short chunks' kernel may number, as far as T and the table's width tell
+};
+
+Served serve(const ChunkArgs& a) {
+  Served how;
+  SplitPlan& pl = how.split;
   pl.nh = heads_a_block(a.Hkv);
   pl.nsub = kWarps / pl.nh;
   pl.hg = a.Hkv / pl.nh;
@@ -699,16 +709,32 @@ int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
   // of tiles times keys) 37 either way.  One long request: the tensor-memory kernel alone.  Else each serves its own.
   const long long longest = a.max_q > 0 && a.max_q < a.T ? a.max_q : a.T;
   const long long tiles16 = ((long long)a.T * a.G - a.B) / 16 + a.B;
-  const bool split_only =
-      longest * a.G <= kSplitRows || (tiles16 * pl.hg <= okc_host::num_sms() &&
-                                      tiles16 * a.max_keys * a.Hkv * a.D / 128 <= (a.B == 1 ? 20000 : 300000));
-  const bool tc_only = !split_only && a.B == 1;
-  pl.most_rows = split_only ? 0x7fffffff : kSplitRows;
-  pl.merge_tokens = split_only ? 0 : kSplitRows / a.G;
-  pl.rows = split_only && longest * a.G <= 8 ? 8 : 16;
+  how.split_only = longest * a.G <= kSplitRows ||
+                   (tiles16 * pl.hg <= okc_host::num_sms() &&
+                    tiles16 * a.max_keys * a.Hkv * a.D / 128 <= (a.B == 1 ? 20000 : 300000));
+  how.tc_only = !how.split_only && a.B == 1;
+  pl.most_rows = how.split_only ? 0x7fffffff : kSplitRows;
+  pl.merge_tokens = how.split_only ? 0 : kSplitRows / a.G;
+  pl.rows = how.split_only && longest * a.G <= 8 ? 8 : 16;
   // the grid by the units that the table's width allows; the kernels know how many there are
   const long long row_tiles = ((long long)a.T * a.G - a.B) / pl.rows + a.B;
   pl.ctas = row_tiles * pl.hg * (a.max_keys / pl.step_keys + 1) > 6 * pl.few ? split_ctas(a.D) : pl.few;
+
+  // a request that is served beside the tensor-memory kernel has at most kSplitRows rows
+  const long long most_tiles = (long long)a.B * (kSplitRows / 16);
+  const long long tiles = how.split_only || row_tiles < most_tiles ? row_tiles : most_tiles;
+  const bool launched = how.split_only || (!how.tc_only && pl.merge_tokens > 0);
+  how.units = launched ? tiles * pl.hg * (((long long)a.max_keys + pl.step_keys - 1) / pl.step_keys) : 0;
+  return how;
+}
+
+}  // namespace
+
+long long attn_chunk_units(const ChunkArgs& a) { return serve(a).units; }
+
+int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
+  const Served how = serve(a);
+  SplitPlan pl = how.split;
   const size_t rows = split_slots(a.T, a.B, a.Hq, a.Hkv, a.D, pl.rows) * pl.nh * pl.rows;
   uint8_t* p = reinterpret_cast<uint8_t*>(a.ws);
   pl.pre_u = reinterpret_cast<int*>(p);
@@ -719,9 +745,9 @@ int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
   p += up(rows * 8);
   pl.acc = reinterpret_cast<float*>(p);
   p += up(rows * a.D * 4);
-  if (!split_only) {
-    if (int st = launch_attn_chunk_tc(a, tc_only ? 0 : kSplitRows, p, stream)) return st;
-    if (tc_only || pl.merge_tokens == 0) return OKC_OK;  // no request is short enough
+  if (!how.split_only) {
+    if (int st = launch_attn_chunk_tc(a, how.tc_only ? 0 : kSplitRows, p, stream)) return st;
+    if (how.tc_only || pl.merge_tokens == 0) return OKC_OK;  // no request is short enough
   }
   const bool cap = a.softcap > 0.f;
   if (a.D == 64) {

@@ -152,17 +152,13 @@ int okc_attn_chunk_fp8(const void* q, int64_t ldq, const void* k_cache, const vo
   if (table_ld < max_pages || ldq < (int64_t)Hq * D || ldo < (int64_t)Hq * D) return OKC_ERR_INVALID;
   if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || ldq % 8 || ldo % 8)
     return OKC_ERR_ALIGNMENT;
-  // the work list is counted in 32 bits: row tiles x key steps of the longest table row
-  const long long most_keys = (1ll << 31) - (1ll << 17);
-  const long long keys = (long long)max_pages * page_size < most_keys ? (long long)max_pages * page_size : most_keys;
-  const long long tiles = ((long long)T * (Hq / Hkv) + 15) / 16 + B;
-  if ((long long)T * Hq > 0x7fffffffll || tiles * Hkv * (keys / 32 + 1) > 0x7fffffffll) return OKC_ERR_TOO_LARGE;
+  if ((long long)T * Hq > 0x7fffffffll) return OKC_ERR_TOO_LARGE;  // output rows
   // row tile pairs are a grid's second dimension
   if ((long long)T * (Hq / Hkv) / 256 + B > 65535) return OKC_ERR_TOO_LARGE;
-  // ... and so are the cache's rows of D bytes: 256 GB of keys at D = 64
+  // the cache's rows of D bytes are numbered in 32 bits: 256 GB of keys at D = 64
   if (num_pages > 0xfffffffell / page_size / Hkv) return OKC_ERR_TOO_LARGE;
-  if (!workspace || workspace_bytes < okc::attn_chunk_ws_bytes(T, B, Hq, Hkv, D)) return OKC_ERR_WORKSPACE;
-  if (!aligned16(workspace)) return OKC_ERR_ALIGNMENT;
+  const long long most_keys = (1ll << 31) - (1ll << 17);
+  const long long keys = (long long)max_pages * page_size < most_keys ? (long long)max_pages * page_size : most_keys;
   okc::ChunkArgs a;
   a.q = reinterpret_cast<const __nv_bfloat16*>(q);
   a.ldq = ldq;
@@ -196,6 +192,9 @@ int okc_attn_chunk_fp8(const void* q, int64_t ldq, const void* k_cache, const vo
   a.max_q = max_q;
   a.ws = workspace;
   a.err = error;
+  if (okc::attn_chunk_units(a) > 0x7fffffffll) return OKC_ERR_TOO_LARGE;
+  if (!workspace || workspace_bytes < okc::attn_chunk_ws_bytes(T, B, Hq, Hkv, D)) return OKC_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return OKC_ERR_ALIGNMENT;
   return okc::launch_attn_chunk(a, stream);
 }
 

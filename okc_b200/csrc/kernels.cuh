@@ -142,6 +142,8 @@ struct ChunkArgs {
   int* err;
 };
 size_t attn_chunk_ws_bytes(int T, int B, int Hq, int Hkv, int D);
+// Pieces of work that the short chunks' kernel may number for this call (in 32 bits).
+long long attn_chunk_units(const ChunkArgs& a);
 int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream);
 // Projection with an epilogue (linear.cu, linear_split.cu).
 struct LinearArgs {

@@ -95,3 +95,19 @@ def test_workspace_sizes(lib):
     for bad in ((0, 1, 4, 2, 64), (1, 0, 4, 2, 64), (1, 1, 0, 2, 64), (1, 1, 4, 0, 64), (1, 1, 4, 3, 64), (1, 1, 4, 2, 96)):
         assert size(*bad) == 0
     assert 0 < size(1, 1, 4, 2, 64) <= size(100, 1, 4, 2, 64) and size(100, 9, 4, 2, 64) > 0
+
+
+def test_wide_tables_are_taken(lib, code):
+    """Tables far wider than the requests: what limits them is the work that the kernels number, not the width alone.
+    (Past all the other checks these calls stop at the missing workspace.)"""
+    fn = lib.okc_attn_chunk_fp8
+    big = dict(Hq=64, Hkv=8, D=128, ldq=8192, ldo=8192)
+    for good in (dict(T=16384, B=1, max_q=16384, max_pages=2 ** 16),  # one long chunk, a table of 2^20 positions
+                 dict(T=16384, B=1, max_q=0, max_pages=2 ** 26),
+                 dict(T=16384, B=64, max_q=8192, max_pages=2 ** 16),
+                 dict(T=2048 * 8, B=2048, max_q=8, max_pages=2 ** 16),  # verify blocks: one tile each
+                 dict(T=2048 * 8, B=2048, max_q=8, max_pages=2 ** 18),
+                 dict(T=2048, B=2048, max_q=1, max_pages=2 ** 18)):
+        assert _call(fn, ATTN, **big, **good, table_ld=good["max_pages"]) == code.OKC_ERR_WORKSPACE, good
+    for bad in (dict(T=2048 * 8, B=2048, max_q=8, max_pages=2 ** 21), dict(T=2048, B=2048, max_q=0, max_pages=2 ** 26)):
+        assert _call(fn, ATTN, **big, **bad, table_ld=bad["max_pages"]) == code.OKC_ERR_TOO_LARGE, bad

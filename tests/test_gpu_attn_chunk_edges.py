@@ -68,3 +68,19 @@ def test_a_nan_query_beside_empty_key_segments(ops, D):
         assert torch.isnan(o2[7, 1].float()).all()
         o2[7, 1] = o[7, 1]
         attn._close(o2, c)
+
+
+def test_a_long_chunk_behind_a_table_of_a_million_positions(ops):
+    """16384 tokens at 64 / 8 heads, the table's width 2^20 positions: what a table cut to the request gives."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    T, Hq, Hkv, D, P = 16384, 64, 8, 128, 16
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    c = dict(q=rnd(T, Hq, D).to(torch.bfloat16), k_cache=rnd(T // P, P, Hkv, D).to(attn.E4M3),
+             v_cache=rnd(T // P, P, Hkv, D).to(attn.E4M3), cu_q=torch.tensor([0, T], dtype=torch.int32, device="cuda"),
+             seq_lens=torch.tensor([T], dtype=torch.int32, device="cuda"), k_scale=torch.ones(Hkv, device="cuda"),
+             v_scale=torch.ones(Hkv, device="cuda"), sm_scale=1 / math.sqrt(D), max_q=T)
+    table = torch.full((1, 2 ** 20 // P), -1, dtype=torch.int32, device="cuda")
+    table[0, :T // P] = torch.randperm(T // P, generator=g, device="cuda").to(torch.int32)
+    want = ops.attn_chunk(page_table=table[:, :T // P], **c)
+    assert torch.equal(ops.attn_chunk(page_table=table, **c), want)
+    assert ops.read_device_error("attn_chunk") == 0 and want.abs().max() > 0
