@@ -181,8 +181,9 @@ __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) attn_chunk_split
     // keys that every live row sees need no mask; keys outside [t_lo, t_hi) are not read
     int full_lo = max(live[0] ? lo[0] : 0, live[1] ? lo[1] : 0);
     int full_hi = min(live[0] ? hi[0] : 0x7fffffff, live[1] ? hi[1] : 0x7fffffff);
-    int t_lo = min(live[0] ? lo[0] : 0x7fffffff, live[1] ? lo[1] : 0x7fffffff);
-    int t_hi = max(live[0] ? hi[0] : 0, live[1] ? hi[1] : 0);
+    const bool sees[2] = {live[0] && lo[0] < hi[0], live[1] && lo[1] < hi[1]};
+    int t_lo = min(sees[0] ? lo[0] : 0x7fffffff, sees[1] ? lo[1] : 0x7fffffff);
+    int t_hi = max(sees[0] ? hi[0] : 0, sees[1] ? hi[1] : 0);
     full_lo = __reduce_max_sync(0xffffffffu, full_lo);
     full_hi = __reduce_min_sync(0xffffffffu, full_hi);
     t_lo = __reduce_min_sync(0xffffffffu, t_lo);
@@ -191,8 +192,12 @@ __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) attn_chunk_split
     // ---- the warp's steps: keys [k0 + s * step_keys, + 32), those that meet [t_lo, t_hi) ----
     const int k0 = rq.lo + c0 * pl.step_keys + sub * kStep;
     int s_lo = 0, s_hi = c1 - c0;
-    if (t_lo > k0 + kStep - 1) s_lo = (t_lo - (k0 + kStep - 1) + pl.step_keys - 1) / pl.step_keys;
-    if (t_hi < k0 + (s_hi - 1) * pl.step_keys + 1) s_hi = t_hi <= k0 ? 0 : (t_hi - k0 + pl.step_keys - 1) / pl.step_keys;
+    if (t_lo >= t_hi) {
+      s_hi = 0;  // no row of the tile sees a key
+    } else {
+      if (t_lo > k0 + kStep - 1) s_lo = (t_lo - (k0 + kStep - 1) + pl.step_keys - 1) / pl.step_keys;
+      if (t_hi < k0 + (s_hi - 1) * pl.step_keys + 1) s_hi = t_hi <= k0 ? 0 : (t_hi - k0 + pl.step_keys - 1) / pl.step_keys;
+    }
     const int32_t* trow = a.page_table + (size_t)b * a.table_ld;
     auto fetch_page = [&](int s) -> int {  // of this lane's key of step s; what it is, issue() checks
       const int key = k0 + s * pl.step_keys + lane;

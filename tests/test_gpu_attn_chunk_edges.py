@@ -84,3 +84,22 @@ def test_a_long_chunk_behind_a_table_of_a_million_positions(ops):
     want = ops.attn_chunk(page_table=table[:, :T // P], **c)
     assert torch.equal(ops.attn_chunk(page_table=table, **c), want)
     assert ops.read_device_error("attn_chunk") == 0 and want.abs().max() > 0
+
+
+@pytest.mark.parametrize("Hkv", [1, 2, 4, 8])
+@pytest.mark.parametrize("n", [1, 3, 40, 300])
+def test_the_largest_document_start_is_no_work(ops, Hkv, n):
+    """doc_start 2^31 - 1 for rows that see nothing, whole tiles of them and single ones: zeros, in no time."""
+    c = attn._case([n, 5], [70, 40], 4 * Hkv, Hkv, 64, 16, seed=n + Hkv)
+    for first in (0, 4):  # the second time the first tokens see their keys
+        c["doc_start"] = torch.full((n + 5,), 2 ** 31 - 1, dtype=torch.int32)
+        c["doc_start"][:first] = 0
+        attn._check(ops, c, max_q=n)
+        d = attn._cuda(c)
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        ops.attn_chunk(**d, max_q=n)
+        start.record()
+        ops.attn_chunk(**d, max_q=n)
+        end.record()
+        end.synchronize()
+        assert start.elapsed_time(end) < 100  # milliseconds: one empty step for each of 2^31 positions takes seconds
