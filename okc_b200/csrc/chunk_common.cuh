@@ -52,6 +52,12 @@ __device__ __forceinline__ int page_of(const ChunkArgs& a, int position) {
   return (int)((uint64_t)(uint32_t)position * a.page_mul >> a.page_shift);
 }
 
+// The first position that the window leaves a row at position p, which is negative where a request has more new
+// tokens than cached ones (those rows see nothing, whatever the window).
+__device__ __forceinline__ int window_start(const ChunkArgs& a, int p) {
+  return a.window > 0 ? max(0, max(0, p + 1) - a.window) : 0;
+}
+
 // A request: its rows' key intervals all lie in [lo, hi).
 struct Req {
   int n, len, lo, hi, prefix;  // new tokens, cached tokens, union of the rows' key intervals
@@ -62,7 +68,7 @@ __device__ __forceinline__ Req request(const ChunkArgs& a, int b) {
   r.n = max(0, a.cu_q[b + 1] - a.cu_q[b]);
   r.len = max(0, a.seq_lens[b]);
   r.prefix = a.prefix_lens ? a.prefix_lens[b] : 0;
-  r.lo = a.window > 0 ? max(0, r.len - r.n + 1 - a.window) : 0;
+  r.lo = window_start(a, r.len - r.n);
   r.hi = min(r.len, a.max_keys);  // positions past the table's columns do not exist
   return r;
 }
@@ -74,7 +80,7 @@ struct RowSpan {
 __device__ __forceinline__ RowSpan row_span(const ChunkArgs& a, const Req& rq, int row0, int i) {
   RowSpan r;
   r.pos = rq.len - rq.n + i;
-  r.lo = a.window > 0 ? max(0, r.pos + 1 - a.window) : 0;
+  r.lo = window_start(a, r.pos);
   if (a.doc_start) r.lo = max(r.lo, a.doc_start[row0 + i]);
   r.hi = min(rq.hi, max(r.pos + 1, rq.prefix));
   return r;

@@ -103,3 +103,17 @@ def test_the_largest_document_start_is_no_work(ops, Hkv, n):
         end.record()
         end.synchronize()
         assert start.elapsed_time(end) < 100  # milliseconds: one empty step for each of 2^31 positions takes seconds
+
+
+@pytest.mark.parametrize("n", [9, 100])
+def test_the_widest_window_with_rows_before_position_0(ops, n):
+    """More new tokens than cached ones: the rows before position 0 see nothing, a window of 2^31 - 1 leaves the
+    others all their keys."""
+    c = attn._case([n, 2], [0, 30], 8, 2, 64, 16, seed=n)
+    c["seq_lens"][0] = n - 5
+    d = attn._cuda(c)
+    want = ops.attn_chunk(**d, max_q=n)
+    assert (want[:5] == 0).all() and (want[5:].abs().amax((1, 2)) > 0).all()
+    d["window"] = 2 ** 31 - 1
+    assert torch.equal(ops.attn_chunk(**d, max_q=n), want)
+    assert ops.read_device_error("attn_chunk") == 0
