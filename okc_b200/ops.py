@@ -581,6 +581,11 @@ def rope_axes_kv_append(qkv: torch.Tensor, positions: torch.Tensor, axes, inv_fr
     return q_out
 
 
+def _clamped(n: int) -> int:
+    """An integer argument as a C int: -1 for any negative one, 2^31 - 1 from there on (ctypes keeps the low bits)."""
+    return -1 if n < 0 else min(n, 0x7FFFFFFF)
+
+
 def attn_chunk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                cu_q: torch.Tensor, seq_lens: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                sm_scale: float, softcap: float = 0.0, slopes: torch.Tensor | None = None, window: int = 0,
@@ -597,6 +602,8 @@ def attn_chunk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     dev = _device(q)
     if q.dim() != 3:
         raise _lib.OkcError(f"q: expected [T, Hq, D], got {tuple(q.shape)}")
+    # no position reaches 2^31, which is also what the C types hold
+    window, max_q = _clamped(window), _clamped(max_q or 0)
     T, Hq, D = shape = q.shape
     ldq = _rows(q, "q", torch.bfloat16, shape, dev)
     cq, sl, B, table, table_ld, cols = _ragged(cu_q, seq_lens, page_table, dev)
@@ -618,7 +625,7 @@ def attn_chunk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
         ws = q.new_empty(nbytes, dtype=torch.uint8)
         _call(dev, _LIB.okc_attn_chunk_fp8, "okc_attn_chunk_fp8", q.data_ptr(), ldq, kc, vc, table, table_ld, cols, cq,
               sl, ks, vs, sp, pp, dp, out.data_ptr(), ldo, T, B, Hq, Hkv, D, P, pages, sm_scale, softcap, window,
-              max_q or 0, ws.data_ptr(), nbytes, error)
+              max_q, ws.data_ptr(), nbytes, error)
     return out
 
 

@@ -117,3 +117,19 @@ def test_the_widest_window_with_rows_before_position_0(ops, n):
     d["window"] = 2 ** 31 - 1
     assert torch.equal(ops.attn_chunk(**d, max_q=n), want)
     assert ops.read_device_error("attn_chunk") == 0
+
+
+@pytest.mark.parametrize("n", [2, 90])
+def test_windows_past_32_bits(ops, n):
+    """A window wider than a C int is one that leaves every key, not its low bits; a negative one is refused."""
+    from okc_b200._lib import OkcError
+    d = attn._cuda(attn._case([n, 1], [40, 30], 8, 2, 64, 16, seed=n))
+    want = ops.attn_chunk(**d, max_q=n)
+    for window in (2 ** 31, 2 ** 32 + 3, 2 ** 40):
+        d["window"] = window
+        assert torch.equal(ops.attn_chunk(**d, max_q=n), want)
+    d["window"] = 0
+    for more in (dict(window=-(2 ** 32)), dict(window=-1), dict(max_q=-(2 ** 32))):
+        with pytest.raises(OkcError):
+            ops.attn_chunk(**{**d, **more})
+    attn._close(ops.attn_chunk(**d, max_q=2 ** 32 + 1), {k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in d.items()})
