@@ -375,20 +375,24 @@ def attn_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
 def _error_word(dev: int, tag: str) -> int:
     buf = _WS.get((dev, tag))
     if buf is None:
-        if torch.cuda.is_current_stream_capturing():
+        if _on_device(dev, torch.cuda.is_current_stream_capturing):
             raise _lib.OkcError(f"{tag}: the first call on a device allocates its error word; make it before a capture")
         buf = workspace(dev, tag, 256)
         torch.cuda.current_stream(dev).synchronize()  # zeroed before a call on any stream
     return buf.data_ptr()
 
 
+def _on_device(dev: int, fn, *args):
+    """Calls fn with `dev` current."""
+    if _current_device() == dev:
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
+
+
 def _call(dev: int, fn, name: str, *args) -> None:
     """Calls a C entry point on the current stream of `dev`, with `dev` current."""
-    if _current_device() == dev:
-        st = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            st = fn(*args, _raw_stream(dev))
+    st = _on_device(dev, fn, *args, _raw_stream(dev))
     if st:
         check(st, name)
 
@@ -621,7 +625,7 @@ def attn_chunk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
         ldo = _rows(out, "out", torch.bfloat16, shape, dev)
     if T:
         error = _error_word(dev, "attn_chunk")
-        nbytes = _LIB.okc_attn_chunk_workspace_bytes(T, B, Hq, Hkv, D)
+        nbytes = _on_device(dev, _LIB.okc_attn_chunk_workspace_bytes, T, B, Hq, Hkv, D)  # by its SMs
         ws = q.new_empty(nbytes, dtype=torch.uint8)
         _call(dev, _LIB.okc_attn_chunk_fp8, "okc_attn_chunk_fp8", q.data_ptr(), ldq, kc, vc, table, table_ld, cols, cq,
               sl, ks, vs, sp, pp, dp, out.data_ptr(), ldo, T, B, Hq, Hkv, D, P, pages, sm_scale, softcap, window,

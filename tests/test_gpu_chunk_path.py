@@ -316,3 +316,33 @@ def test_appends_of_thousands_of_tokens(ops, half):
         want = d[t].view(torch.uint8)
         want[page] = c[t].view(torch.uint8)[page].cuda()
         assert torch.equal(e[t].view(torch.uint8), want)
+
+
+def test_everything_is_asked_of_the_tensors_device(ops, monkeypatch):
+    """With another device current, the size of the scratch, which goes with the device's SMs, and the launches are
+    those of the tensors' device.  (The other device is made up: its number is all that is asked of it.)"""
+    c = attn._cuda(attn._case([2], [30], HQ, HKV, D, P))
+    want = ops.attn_chunk(**c, max_q=2)
+    current, seen, real, device = [1], {}, ops._LIB, torch.cuda.device
+
+    class Device(device):
+        def __enter__(self):
+            current[0] = 0
+            return super().__enter__()
+
+        def __exit__(self, *a):
+            current[0] = 1
+            return super().__exit__(*a)
+
+    class Lib:
+        def __getattr__(self, name):
+            def f(*args):
+                seen[name] = current[0]
+                return getattr(real, name)(*args)
+            return f
+
+    monkeypatch.setattr(ops, "_LIB", Lib())
+    monkeypatch.setattr(ops, "_current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    assert torch.equal(ops.attn_chunk(**c, max_q=2), want)
+    assert seen == {"okc_attn_chunk_workspace_bytes": 0, "okc_attn_chunk_fp8": 0}
