@@ -451,8 +451,8 @@ int okc_rope_axes_kv_append(const void* qkv, int64_t ldqkv, const int64_t* posit
  * row of a token at position p sees the positions [lo, hi):
  *   lo = max(0, doc_start[t], p + 1 - window),  hi = min(seq_len, max(p + 1, prefix_lens[b])),
  * doc_start int32 [T] (packed documents), prefix_lens int32 [B] (a prefix that every token sees),
- * window 0 = none; NULL leaves either out.  Scores: s_j = q.k_j * sm_scale, with softcap > 0
- * softcap * tanh(s_j / softcap), then minus slopes[h] * |p - j| (fp32 [Hq] or NULL).  out = softmax(s) v,
+ * window 0 = none; NULL leaves either out.  Scores: s_j = q.k_j * sm_scale, with a softcap (0 = none, else
+ * 1e-6 .. 1e12) softcap * tanh(s_j / softcap), then minus slopes[h] * |p - j| (fp32 [Hq] or NULL).  out = softmax(s) v,
  * zero for a row that sees nothing; a position that a row does not see does not reach it whatever
  * the cache holds there.  q bf16 [T][ldq], out bf16 [T][ldo] (Hq heads of D), caches e4m3
  * [num_pages, P, Hkv, D] with scales fp32 [Hkv], page_table int32 [B][table_ld] (max_pages columns).  A

@@ -362,11 +362,17 @@ __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) attn_chunk_split
           break;
         }
 #pragma unroll
-        for (int i = 0; i < X; ++i) {
+        for (int i = 0; i < X; ++i)
           // rounded here: fused into the subtraction below, a large score could exceed the maximum
-          float v = __fmul_rn(R == 16 ? sc[i >> 1][2 * e + (i & 1)] : sc[i][e], fac[e]);
-          if (CAP) v = __fmul_rn(cap2, tanh_from_2l2e(v));
-          x[e][i] = v;
+          x[e][i] = __fmul_rn(R == 16 ? sc[i >> 1][2 * e + (i & 1)] : sc[i][e], fac[e]);
+        if (CAP) {
+          if (a.softcap <= kPlainCap) {
+#pragma unroll
+            for (int i = 0; i < X; ++i) x[e][i] = __fmul_rn(cap2, tanh_from_2l2e(x[e][i]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < X; ++i) x[e][i] = __fmul_rn(cap2, tanh_fine_from_2l2e(x[e][i]));
+          }
         }
         if (a.slopes) {
 #pragma unroll

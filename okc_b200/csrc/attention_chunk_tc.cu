@@ -155,22 +155,14 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   return r;
 }
 
-// tanh(x) / x as a polynomial in x^2, fitted for the least |x * error| over |x| <= 1 (six
-// coefficients: 2.4e-7) and over |x| <= 0.4 (three: 1.2e-6): fused operations where the exponential
-// and the reciprocal of the exact form occupy the special-function unit twice.
+// tanh(x) / x as a polynomial in x^2: the seven terms of tanh_term over |x| <= 1, or three of the least |x * error|
+// (1.2e-6, 1.5e-4 of a score at kLowCap) over |x| <= 0.4: fused operations where the exponential and the reciprocal
+// of the exact form occupy the special-function unit twice.
 constexpr float kTanhRange2 = 1.f, kTanhLowRange2 = 0.16f;  // squares of the ranges
+constexpr float kLowCap = 128.f;
 template <bool LOW>
 __device__ __forceinline__ f32x2 tanh2(int k) {
-  float c;
-  if (LOW)
-    c = k == 0 ? 0.99997884f : k == 1 ? -0.33225426f : 0.11942387f;
-  else
-    c = k == 0   ? 0.99999685f
-        : k == 1 ? -0.33324004f
-        : k == 2 ? 0.13253524f
-        : k == 3 ? -0.05097283f
-        : k == 4 ? 0.01611415f
-                 : -0.00283945f;
+  const float c = !LOW ? tanh_term(k) : k == 0 ? 0.99997884f : k == 1 ? -0.33225426f : 0.11942387f;
   return pair2(c, c);
 }
 
@@ -408,7 +400,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     auto s_ready = [&](int j) {  // block j's scores are there, and with them every product up to P V of block j - 2
       return mbar_wait(&sh.s_full[w][j & 1], (uint32_t)(j >> 1) & 1u, a.err, abort_flag);
     };
-    bool ok = true, low = true;  // low: no score so far has left the three-coefficient range
+    bool ok = true;
+    bool low = a.softcap <= kLowCap;  // ... and no score so far has left the three-term range
+    const bool fine = CAP && a.softcap > kPlainCap;
 #pragma unroll 1
     for (int j = 0; j < nb && on; ++j) {
       const int kb = keys.key0 + block_at(keys, j);
@@ -430,7 +424,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       const bool behind = BIAS && __all_sync(0xffffffffu, !live || min(me.hi, kb + kKeys) - 1 <= me.pos);
       const bool beyond = BIAS && !behind && __all_sync(0xffffffffu, !live || max(me.lo, kb) >= me.pos);
       const float toward = beyond ? -slope : slope;
-      auto exact_unit = [&](float v) -> float { return CAP ? tanh_from_2l2e(v * fac) : v; };
+      auto unit = [&](float v, auto finely) -> float {
+        if constexpr (!CAP) return v;
+        else if constexpr (decltype(finely)::value) return tanh_fine_from_2l2e(v * fac);
+        else return tanh_from_2l2e(v * fac);
+      };
+      auto exact_unit = [&](float v) { return fine ? unit(v, std::true_type()) : unit(v, std::false_type()); };
       auto bias = [&](int c) -> float { return -slope * fabsf(ahead - (float)c); };
 
       // Raises m_ref to the row's maximum over the block, with O and l scaled down to it.
@@ -476,7 +475,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       uint32_t o[kKeys / 2];
       float sum = 0.f, reach = 0.f;
       __half2 top = __floats2half2_rn(0.f, 0.f);
-      auto exponentials = [&](auto masked, auto mode) {
+      auto form = [&](auto masked, auto mode, auto finely) {
         constexpr bool MASK = decltype(masked)::value, EXACT = decltype(mode)::value == kExact;
         constexpr bool LOW = decltype(mode)::value == kLow;
         const float org = m_ref == -INFINITY ? 0.f : m_ref;
@@ -493,7 +492,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
           for (int c = 0; c < 32; c += 2) {
             f32x2 x2;
             if constexpr (EXACT || (CAP && BIAS)) {
-              const f32x2 u2 = pair2(exact_unit(__uint_as_float(v[c])), exact_unit(__uint_as_float(v[c + 1])));
+              const f32x2 u2 = pair2(unit(__uint_as_float(v[c]), finely), unit(__uint_as_float(v[c + 1]), finely));
               if constexpr (BIAS)
                 x2 = add2(fma2(u2, f2, pair2(bias(c0 + c), bias(c0 + c + 1))), org2);
               else
@@ -503,7 +502,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
               b2 = add2(b2, step2);
             } else if constexpr (CAP) {
               const f32x2 z = mul2(bits2(v[c], v[c + 1]), pair2(z1, z1)), w2 = mul2(z, z);
-              constexpr int N = LOW ? 3 : 6;
+              constexpr int N = LOW ? 3 : kTanhTerms;
               f32x2 h = fma2(w2, tanh2<LOW>(N - 1), tanh2<LOW>(N - 2));
 #pragma unroll
               for (int k = N - 3; k >= 0; --k) h = fma2(w2, h, tanh2<LOW>(k));
@@ -535,6 +534,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
         columns(vb, 32);
         const float2 s2 = split2(sum2);
         sum = s2.x + s2.y;
+      };
+      auto exponentials = [&](auto masked, auto mode) {
+        // the polynomials are fine enough for every cap
+        if constexpr (CAP && (decltype(mode)::value == kExact || BIAS)) {
+          if (fine) return form(masked, mode, std::true_type());
+        }
+        form(masked, mode, std::false_type());
       };
       // The first block that a row sees sets its m_ref.  Later ones rarely exceed it by 2^kSlack: they are
       // tried against the old one, and done again where some row of the warp does.

@@ -148,7 +148,7 @@ int okc_attn_chunk_fp8(const void* q, int64_t ldq, const void* k_cache, const vo
   if (T < 0 || B <= 0 || B > okc::kMaxChunkRequests || Hq <= 0 || Hkv <= 0 || Hq % Hkv || (D != 64 && D != 128) ||
       page_size <= 0 || num_pages <= 0 || max_pages <= 0 || window < 0 || max_q < 0)
     return OKC_ERR_INVALID;
-  if (!finite(sm_scale) || !finite(softcap) || softcap < 0.f) return OKC_ERR_INVALID;
+  if (!finite(sm_scale) || !(softcap == 0.f || (softcap >= 1e-6f && softcap <= 1e12f))) return OKC_ERR_INVALID;
   if (table_ld < max_pages || ldq < (int64_t)Hq * D || ldo < (int64_t)Hq * D) return OKC_ERR_INVALID;
   if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || ldq % 8 || ldo % 8)
     return OKC_ERR_ALIGNMENT;

@@ -32,9 +32,31 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// tanh(x) from exp(2x) given x * 2 log2(e): 1 - 2 / (1 + e^2x); off by a few 2^-24 absolute, which a cap of
-// 50 turns into 10^-5 of a score.
+// tanh(x) from exp(2x) given x * 2 log2(e): 1 - 2 / (1 + e^2x); off by 1.2e-7 absolute, which the cap multiplies: by
+// 6e-6 of a score at a cap of 50, by 1.2e-4 at kPlainCap.
 __device__ __forceinline__ float tanh_from_2l2e(float x) { return 1.f - __fdividef(2.f, 1.f + ex2(x)); }
+constexpr float kPlainCap = 1024.f;
+
+// tanh(x) / x over |x| <= 1 as a polynomial in x^2 of the least relative error: 1.5e-7 in fp32.
+constexpr int kTanhTerms = 7;
+__host__ __device__ constexpr float tanh_term(int k) {
+  return k == 0   ? 0.99999994f
+         : k == 1 ? -0.3333284f
+         : k == 2 ? 0.13325204f
+         : k == 3 ? -0.053457007f
+         : k == 4 ? 0.020289943f
+         : k == 5 ? -0.0062033492f
+                  : 0.0010410136f;
+}
+// The same within 2^-21 of itself however small: for caps above kPlainCap, whose scores of a few units are a tanh of
+// next to nothing.
+__device__ __forceinline__ float tanh_fine_from_2l2e(float v) {
+  const float x = v * 0.34657359027997264f, w = x * x;
+  float p = tanh_term(kTanhTerms - 1);
+#pragma unroll
+  for (int k = kTanhTerms - 2; k >= 0; --k) p = fmaf(w, p, tanh_term(k));
+  return w <= 1.f ? x * p : tanh_from_2l2e(v);
+}
 
 __device__ __forceinline__ uint32_t e4m3x2_h2(uint32_t two) {
   uint32_t h;

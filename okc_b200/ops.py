@@ -600,7 +600,7 @@ def attn_chunk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     position p sees the positions [max(0, doc_start, p + 1 - window), max(p + 1, prefix_len)) of its
     request: doc_start int32 [T] the first position of its packed document, prefix_lens int32 [B] a prefix
     that every token sees, window 0 = none.  Scores are capped as softcap * tanh(s / softcap)
-    (0 = uncapped), then lowered by slopes[h] * |p - j| (fp32 [Hq]).  max_q, the longest chunk if the
+    (0 = uncapped, else 1e-6 to 1e12), then lowered by slopes[h] * |p - j| (fp32 [Hq]).  max_q, the longest chunk if the
     caller knows it, only chooses kernels.  Returns bf16 [T, Hq, D]: zero for a row that sees nothing, rows
     behind cu_q[B] as they were."""
     dev = _device(q)

@@ -111,3 +111,11 @@ def test_wide_tables_are_taken(lib, code):
         assert _call(fn, ATTN, **big, **good, table_ld=good["max_pages"]) == code.OKC_ERR_WORKSPACE, good
     for bad in (dict(T=2048 * 8, B=2048, max_q=8, max_pages=2 ** 21), dict(T=2048, B=2048, max_q=0, max_pages=2 ** 26)):
         assert _call(fn, ATTN, **big, **bad, table_ld=bad["max_pages"]) == code.OKC_ERR_TOO_LARGE, bad
+
+
+def test_caps_out_of_range_are_refused(lib, code):
+    fn = lib.okc_attn_chunk_fp8
+    for cap in (1e-7, 1e-30, 1.1e12, 3e38):
+        assert _call(fn, ATTN, softcap=cap) == code.OKC_ERR_INVALID, cap
+    for cap in (0.0, 1.01e-6, 30.0, 9.9e11):
+        assert _call(fn, ATTN, softcap=cap) == code.OKC_ERR_WORKSPACE, cap

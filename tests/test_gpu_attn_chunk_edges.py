@@ -133,3 +133,30 @@ def test_windows_past_32_bits(ops, n):
         with pytest.raises(OkcError):
             ops.attn_chunk(**{**d, **more})
     attn._close(ops.attn_chunk(**d, max_q=2 ** 32 + 1), {k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in d.items()})
+
+
+@pytest.mark.parametrize("cap", [1e-6, 1e-3, 0.5, 127.0, 129.0, 1000.0, 1030.0, 2e4, 1e6, 1e9, 1e12])
+@pytest.mark.parametrize("n,slopes", [(1, False), (5, True), (40, False), (90, True), (300, False)])
+def test_caps_of_every_size(ops, n, slopes, cap):
+    """A cap far above the scores leaves them as they are.  Scores are under 32: the tanh is within 2^-21 of itself or
+    1.2e-7 of the cap where that is at most 1024, so a score is off by 2^-13 at most: inside the tolerance, which
+    allows 2^-14 for it beside 2^-11 for the products."""
+    c = attn._case([n, 2], [200, 77], 8, 2, 128, 16, seed=n, cap=cap, slopes=slopes)
+    attn._check(ops, c, f"cap {cap}", max_q=n)
+    c = attn._case([n, 2], [200, 77], 8, 4, 64, 16, seed=n, cap=cap, slopes=slopes)
+    attn._check(ops, c, f"cap {cap}", max_q=n)
+
+
+@pytest.mark.parametrize("cap", [100.0, 130.0, 600.0, 1500.0, 1e5])
+@pytest.mark.parametrize("n", [2, 70, 300])
+def test_scores_of_hundreds_under_larger_caps(ops, n, cap):
+    """Scores of up to 350 on both sides of the polynomials' range; off by 350 * 2^-20 more than in
+    test_large_scores, whose 2^-7 allows four times that.  A probability below the f16 normals is off by up to 2^-25 of the
+    row's largest: all of the up to 340 keys' together by 340 * 2^-25 of the largest |v|, which shows where the one key
+    that a row is about has a value of zero."""
+    c = attn._case([2, n], [100, 240], 8, 2, 128, 16, seed=4, cap=cap)
+    c["sm_scale"] = 1.0
+    o = ops.attn_chunk(**attn._cuda(c), max_q=n).cpu().double()
+    want, a = ref.attn_chunk(**c)
+    small = 340 * 2.0 ** -25 * float((c["v_cache"].float() * c["v_scale"][:, None]).abs().max())
+    assert ((o - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -7 * a + small).all()
