@@ -14,7 +14,8 @@
 // the two launches and the chains to the first key and through the merge are 9.  The rows of one KV head's query group
 // (token-major, G heads a token) fill the 16 rows of mma.sync tiles, or, where no request has more than 8,
 // their 8 columns with keys and outputs as the rows: half the MMAs and half the accumulators.  e4m3 keys and
-// values are exact in f16, the query too once its row is scaled by a power of two, and P is rounded to f16 (2^-11).
+// values are exact in f16, the query too once its row is scaled by a power of two, and P is rounded to f16 (2^-11; the
+// sum that divides takes it unrounded).
 //  * units of 32 keys x (8 / nh) subgroups of a (request, row tile, nh heads) are numbered in order
 //    and split evenly over a persistent grid (ragged contexts stay balanced); the nh heads of a
 //    key lie side by side in the cache, so the block's warps read whole token rows together;
@@ -35,6 +36,9 @@ namespace {
 
 constexpr int kStep = 32;      // keys per warp step
 constexpr int kWarps = 8;
+// log2 of the largest P: f16 keeps P down to 2^-25, so that keys are lost from the sum only 2^-(25 + kLift) below the
+// row's largest (from an origin at the largest, a million keys at e^-18 of it lost 1.5% of the weight).
+constexpr int kLift = 14;
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
@@ -389,7 +393,8 @@ __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) attn_chunk_split
         // over the lanes that have the row: c, or g
 #pragma unroll
         for (int s = R == 16 ? 1 : 4; s < (R == 16 ? 4 : 32); s *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-        const float nm = fmaxf(m[e], top);
+        // the origin of the exponentials, kLift below the largest score and rounded up: P reaches 2^kLift
+        const float nm = fmaxf(m[e], __fadd_ru(top, -(float)kLift));
         const float org = nm == -INFINITY ? 0.f : nm;  // nothing seen yet: any finite origin
         corr[e] = ex2(m[e] - org);
         m[e] = nm;

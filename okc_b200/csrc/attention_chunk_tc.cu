@@ -11,8 +11,8 @@
 //  * four warps fetch key and value rows by page, turn e4m3 into f16 (exact) and store both as the
 //    swizzled rows that the MMAs read (keys K-major, values MN-major: no transpose), four blocks deep;
 //  * a thread per tile issues its MMAs;
-//  * a block's exponentials are taken against the maximum so far, in one pass over S, and done again with
-//    O rescaled only where a P exceeds 2^8: rare after a row's first blocks.
+//  * a block's exponentials are taken against the origin so far, in one pass over S, and done again with
+//    O rescaled only where a P exceeds 2^8 of the origin's: rare after a row's first blocks.
 // The special-function unit bounds it: 256 x 64 exponentials take 1024 cycles of it a block, where the tensor
 // cores need 1024 too, and a block takes 1960 (the softmax warps' other instructions and latencies overlap
 // only in part; a third of the exponentials as polynomials on the fused-operation pipe made it slower).
@@ -45,6 +45,10 @@ static_assert(kSoftmaxRegs > kLaunchRegs && kLoadRegs < kLaunchRegs && kIssueReg
               "setmaxnreg.inc raises and .dec lowers; the other way round is an illegal instruction");
 constexpr int kHigh = 0, kLow = 1, kExact = 2;  // how a block's exponentials are taken
 constexpr int kSlack = 8;                  // log2 growth of the maximum that O tolerates
+// log2 of the largest P at the origin of the exponentials: f16 keeps P down to 2^-25, so that keys are lost from the sum only
+// 2^-(25 + kLift) below the largest score that the origin was taken from, and reaches 2^16.
+constexpr int kLift = 7;
+static_assert(kLift + kSlack <= 15, "P stays finite in f16");
 
 template <int D>
 struct TcCfgA {
@@ -432,7 +436,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       auto exact_unit = [&](float v) { return fine ? unit(v, std::true_type()) : unit(v, std::false_type()); };
       auto bias = [&](int c) -> float { return -slope * fabsf(ahead - (float)c); };
 
-      // Raises m_ref to the row's maximum over the block, with O and l scaled down to it.
+      // Raises m_ref to kLift below the row's maximum over the block, with O and l scaled down to it.
       auto raise = [&]() {
         float mx = -INFINITY;
 #pragma unroll 1
@@ -450,6 +454,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
         }
         // without a bias the score grows with the raw sum; rounded up, so that no fused u * f - org is positive
         if (!BIAS && mx != -INFINITY) mx = __fmul_ru(exact_unit(mx), f);
+        mx = __fadd_ru(mx, -(float)kLift);  // the origin, rounded up so that P is 2^kLift at most
         const bool grow = mx > m_ref;
         const bool scale = m_ref != -INFINITY && grow;  // from -infinity: O and l are zero
         const float down = scale ? ex2(m_ref - mx) : 1.f;
@@ -553,7 +558,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
           exponentials(std::false_type(), std::integral_constant<int, kLow>());
         else
           exponentials(std::false_type(), std::integral_constant<int, kHigh>());
-        const __half2 most = __float2half2_rn((float)(1 << kSlack));
+        const __half2 most = __float2half2_rn((float)(1 << (kLift + kSlack)));
         const float range = low && !edge ? kTanhLowRange2 : kTanhRange2;
         if (CAP && __any_sync(0xffffffffu, live && reach > kTanhLowRange2)) low = false;
         again = __any_sync(0xffffffffu, live && (!__hble2(top, most) || reach > range));

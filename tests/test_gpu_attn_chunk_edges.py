@@ -160,3 +160,28 @@ def test_scores_of_hundreds_under_larger_caps(ops, n, cap):
     want, a = ref.attn_chunk(**c)
     small = 340 * 2.0 ** -25 * float((c["v_cache"].float() * c["v_scale"][:, None]).abs().max())
     assert ((o - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -7 * a + small).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap", [0.0, 50.0, 2000.0])
+@pytest.mark.parametrize("n,keys", [(1, 4000), (2, 2 ** 20), (5, 333), (300, 4000)])
+def test_many_keys_far_below_one(ops, n, keys, cap, D):
+    """One key 18 units above all others, its value 0 where theirs is 1: the output is the others' share.  A probability
+    is off by 2^-11 of itself or 2^-32 of the row's largest, whichever is more, the output by 2^-9 more."""
+    Hq, P = 2, 16
+    pages = -(-keys // P)
+    for at in (0, keys // 2, keys - n):  # every row sees it
+        k = torch.zeros(pages, P, 1, D)
+        v = torch.ones(pages, P, 1, D)
+        k[at // P, at % P, 0, 1], v[at // P, at % P] = 18.0, 0.0
+        q = torch.zeros(n, Hq, D, dtype=torch.bfloat16)
+        q[..., 1] = 1.0
+        one = torch.ones(1, device="cuda")
+        o = ops.attn_chunk(q.cuda(), k.cuda().to(attn.E4M3), v.cuda().to(attn.E4M3),
+                           torch.nn.functional.pad(torch.arange(pages, dtype=torch.int32), (0, 4096), value=-1).view(1, -1).cuda(),
+                           torch.tensor([0, n], dtype=torch.int32).cuda(), torch.tensor([keys], dtype=torch.int32).cuda(), one, one,
+                           1.0, softcap=cap, max_q=n).cpu().double()
+        others = (torch.arange(n).double() + keys - n).view(n, 1, 1)  # keys that a row sees, but one
+        share = others * math.exp(-(cap * math.tanh(18 / cap) if cap else 18.0))
+        want = share / (1 + share)
+        assert ((o - want).abs() <= (2.0 ** -9 + 2.0 ** -11 + 2.0 ** -16) * want + others * 2.0 ** -32).all()
