@@ -118,7 +118,7 @@ __device__ __forceinline__ void split_prefix(const ChunkArgs& a, const SplitPlan
   }
 }
 
-template <int D, bool CAP, int R>
+template <int D, int CAP, int R>
 __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) attn_chunk_split_kernel(ChunkArgs a, SplitPlan pl) {
   using C = ChunkCfg<D>;
   constexpr int KS = D / 16;   // k16 steps of QK
@@ -366,17 +366,11 @@ __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) attn_chunk_split
           break;
         }
 #pragma unroll
-        for (int i = 0; i < X; ++i)
+        for (int i = 0; i < X; ++i) {
           // rounded here: fused into the subtraction below, a large score could exceed the maximum
-          x[e][i] = __fmul_rn(R == 16 ? sc[i >> 1][2 * e + (i & 1)] : sc[i][e], fac[e]);
-        if (CAP) {
-          if (a.softcap <= kPlainCap) {
-#pragma unroll
-            for (int i = 0; i < X; ++i) x[e][i] = __fmul_rn(cap2, tanh_from_2l2e(x[e][i]));
-          } else {
-#pragma unroll
-            for (int i = 0; i < X; ++i) x[e][i] = __fmul_rn(cap2, tanh_fine_from_2l2e(x[e][i]));
-          }
+          float v = __fmul_rn(R == 16 ? sc[i >> 1][2 * e + (i & 1)] : sc[i][e], fac[e]);
+          if (CAP) v = __fmul_rn(cap2, CAP == kCapFine ? tanh_fine_from_2l2e(v) : tanh_from_2l2e(v));
+          x[e][i] = v;
         }
         if (a.slopes) {
 #pragma unroll
@@ -676,7 +670,7 @@ size_t split_slots(int T, int B, int Hq, int Hkv, int D, int rows) {
   return split_ctas(D) + (((size_t)T * (Hq / Hkv) + rows - 1) / rows + B) * hg;
 }
 
-template <int D, bool CAP, int R>
+template <int D, int CAP, int R>
 int launch_split(const ChunkArgs& a, const SplitPlan& pl, cudaStream_t stream) {
   using C = ChunkCfg<D>;
   const int smem = C::SMEM + 2 * (a.B + 1) * 4;
@@ -691,6 +685,13 @@ int launch_split(const ChunkArgs& a, const SplitPlan& pl, cudaStream_t stream) {
     return okc_host::launch_k(attn_chunk_merge_kernel<D, 8>, dim3((unsigned)items), dim3(256), 0, stream, dim3(1), a, pl);
   return okc_host::launch_k(attn_chunk_merge_kernel<D, 1>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, stream,
                             dim3(1), a, pl);
+}
+
+template <int CAP>
+int launch_split_cap(const ChunkArgs& a, const SplitPlan& pl, cudaStream_t stream) {
+  if (a.D == 64)
+    return pl.rows == 8 ? launch_split<64, CAP, 8>(a, pl, stream) : launch_split<64, CAP, 16>(a, pl, stream);
+  return pl.rows == 8 ? launch_split<128, CAP, 8>(a, pl, stream) : launch_split<128, CAP, 16>(a, pl, stream);
 }
 
 }  // namespace
@@ -765,13 +766,11 @@ int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
     if (int st = launch_attn_chunk_tc(a, how.tc_only ? 0 : kSplitRows, p, stream)) return st;
     if (how.tc_only || pl.merge_tokens == 0) return OKC_OK;  // no request is short enough
   }
-  const bool cap = a.softcap > 0.f;
-  if (a.D == 64) {
-    if (pl.rows == 8) return cap ? launch_split<64, true, 8>(a, pl, stream) : launch_split<64, false, 8>(a, pl, stream);
-    return cap ? launch_split<64, true, 16>(a, pl, stream) : launch_split<64, false, 16>(a, pl, stream);
+  switch (cap_form(a.softcap)) {
+    case kCapFine: return launch_split_cap<kCapFine>(a, pl, stream);
+    case kCapPlain: return launch_split_cap<kCapPlain>(a, pl, stream);
+    default: return launch_split_cap<kCapNone>(a, pl, stream);
   }
-  if (pl.rows == 8) return cap ? launch_split<128, true, 8>(a, pl, stream) : launch_split<128, false, 8>(a, pl, stream);
-  return cap ? launch_split<128, true, 16>(a, pl, stream) : launch_split<128, false, 16>(a, pl, stream);
 }
 
 }  // namespace okc

@@ -196,7 +196,7 @@ struct TcShared {
   uint32_t nan[kDepth][kKeys / 32];  // per V block: its keys that hold a NaN that was taken out
 };
 
-template <int D, bool CAP, bool BIAS>
+template <int D, int CAP, bool BIAS>
 __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs a, TcPlanA pl) {
   using C = TcCfgA<D>;
   extern __shared__ uint8_t smem_raw[];
@@ -406,7 +406,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     };
     bool ok = true;
     bool low = a.softcap <= kLowCap;  // ... and no score so far has left the three-term range
-    const bool fine = CAP && a.softcap > kPlainCap;
 #pragma unroll 1
     for (int j = 0; j < nb && on; ++j) {
       const int kb = keys.key0 + block_at(keys, j);
@@ -428,12 +427,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       const bool behind = BIAS && __all_sync(0xffffffffu, !live || min(me.hi, kb + kKeys) - 1 <= me.pos);
       const bool beyond = BIAS && !behind && __all_sync(0xffffffffu, !live || max(me.lo, kb) >= me.pos);
       const float toward = beyond ? -slope : slope;
-      auto unit = [&](float v, auto finely) -> float {
-        if constexpr (!CAP) return v;
-        else if constexpr (decltype(finely)::value) return tanh_fine_from_2l2e(v * fac);
-        else return tanh_from_2l2e(v * fac);
+      auto exact_unit = [&](float v) -> float {
+        return CAP == kCapFine ? tanh_fine_from_2l2e(v * fac) : CAP ? tanh_from_2l2e(v * fac) : v;
       };
-      auto exact_unit = [&](float v) { return fine ? unit(v, std::true_type()) : unit(v, std::false_type()); };
       auto bias = [&](int c) -> float { return -slope * fabsf(ahead - (float)c); };
 
       // Raises m_ref to kLift below the row's maximum over the block, with O and l scaled down to it.
@@ -480,7 +476,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
       uint32_t o[kKeys / 2];
       float sum = 0.f, reach = 0.f;
       __half2 top = __floats2half2_rn(0.f, 0.f);
-      auto form = [&](auto masked, auto mode, auto finely) {
+      auto exponentials = [&](auto masked, auto mode) {
         constexpr bool MASK = decltype(masked)::value, EXACT = decltype(mode)::value == kExact;
         constexpr bool LOW = decltype(mode)::value == kLow;
         const float org = m_ref == -INFINITY ? 0.f : m_ref;
@@ -497,7 +493,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
           for (int c = 0; c < 32; c += 2) {
             f32x2 x2;
             if constexpr (EXACT || (CAP && BIAS)) {
-              const f32x2 u2 = pair2(unit(__uint_as_float(v[c]), finely), unit(__uint_as_float(v[c + 1]), finely));
+              const f32x2 u2 = pair2(exact_unit(__uint_as_float(v[c])), exact_unit(__uint_as_float(v[c + 1])));
               if constexpr (BIAS)
                 x2 = add2(fma2(u2, f2, pair2(bias(c0 + c), bias(c0 + c + 1))), org2);
               else
@@ -539,13 +535,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
         columns(vb, 32);
         const float2 s2 = split2(sum2);
         sum = s2.x + s2.y;
-      };
-      auto exponentials = [&](auto masked, auto mode) {
-        // the polynomials are fine enough for every cap
-        if constexpr (CAP && (decltype(mode)::value == kExact || BIAS)) {
-          if (fine) return form(masked, mode, std::true_type());
-        }
-        form(masked, mode, std::false_type());
       };
       // The first block that a row sees sets its m_ref.  Later ones rarely exceed it by 2^kSlack: they are
       // tried against the old one, and done again where some row of the warp does.
@@ -886,7 +875,7 @@ int tc_splits(int T, int B, int Hq, int Hkv, long long max_keys) {
   return s < 1 ? 1 : s > 32 ? 32 : (int)s;
 }
 
-template <int D, bool CAP, bool BIAS>
+template <int D, int CAP, bool BIAS>
 int launch_tc(const ChunkArgs& a, const TcPlanA& pl, cudaStream_t stream) {
   using C = TcCfgA<D>;
   static okc_host::PerDevice configured;
@@ -899,6 +888,13 @@ int launch_tc(const ChunkArgs& a, const TcPlanA& pl, cudaStream_t stream) {
   if (pl.splits == 1) return OKC_OK;
   return okc_host::launch_k(attn_chunk_tc_merge_kernel<D>, dim3((unsigned)(((long long)a.T * a.Hq + 7) / 8)), dim3(256),
                             0, stream, dim3(1), a, pl);
+}
+
+template <int CAP>
+int launch_tc_cap(const ChunkArgs& a, const TcPlanA& pl, cudaStream_t stream) {
+  const bool bias = a.slopes != nullptr;
+  if (a.D == 64) return bias ? launch_tc<64, CAP, true>(a, pl, stream) : launch_tc<64, CAP, false>(a, pl, stream);
+  return bias ? launch_tc<128, CAP, true>(a, pl, stream) : launch_tc<128, CAP, false>(a, pl, stream);
 }
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
@@ -918,13 +914,11 @@ int launch_attn_chunk_tc(const ChunkArgs& a, int above, void* ws, cudaStream_t s
   pl.splits = tc_splits(a.T, a.B, a.Hq, a.Hkv, a.max_keys);
   pl.acc = reinterpret_cast<float*>(ws);
   pl.ml = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + up((size_t)pl.splits * a.T * a.Hq * a.D * 4));
-  const bool cap = a.softcap > 0.f, bias = a.slopes != nullptr;
-  if (a.D == 64) {
-    if (cap) return bias ? launch_tc<64, true, true>(a, pl, stream) : launch_tc<64, true, false>(a, pl, stream);
-    return bias ? launch_tc<64, false, true>(a, pl, stream) : launch_tc<64, false, false>(a, pl, stream);
+  switch (cap_form(a.softcap)) {
+    case kCapFine: return launch_tc_cap<kCapFine>(a, pl, stream);
+    case kCapPlain: return launch_tc_cap<kCapPlain>(a, pl, stream);
+    default: return launch_tc_cap<kCapNone>(a, pl, stream);
   }
-  if (cap) return bias ? launch_tc<128, true, true>(a, pl, stream) : launch_tc<128, true, false>(a, pl, stream);
-  return bias ? launch_tc<128, false, true>(a, pl, stream) : launch_tc<128, false, false>(a, pl, stream);
 }
 
 }  // namespace okc
