@@ -153,6 +153,23 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   return r;
 }
 
+// f / scale for many f, as an fp32 division rounds it: with y the reciprocal rounded to nearest, q = f y is off by at
+// most one unit, the remainder f - q scale is exact, and q + remainder * y rounds to the division's result (Markstein,
+// 1990).  In the scales' range all of it is normal wherever the quotient is at least 2^-10, below which e4m3 is zero;
+// others are divided.
+struct Quotient {
+  float scale, y;
+  static __device__ __forceinline__ bool holds(float scale) { return fabsf(scale) >= 0x1p-60f && fabsf(scale) <= 0x1p60f; }
+  __device__ __forceinline__ explicit Quotient(float s) {
+    scale = s;
+    y = __frcp_rn(s);
+  }
+  __device__ __forceinline__ float operator()(float f) const {
+    const float q = f * y;
+    return copysignf(fmaf(fmaf(-q, scale, f), y, q), q);  // of -0, too
+  }
+};
+
 // Two floats -> two e4m3 bytes (x in the low byte), round-to-nearest-even, saturating.
 __device__ __forceinline__ uint16_t f2_to_e4m3x2_sat(float x, float y) {
   return (uint16_t)__nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);

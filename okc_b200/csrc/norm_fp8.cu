@@ -148,10 +148,9 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rmsnorm_fp8_kernel(
   if (scale == 0.f) scale = 1.f;
   if (!live) return;
   if (tid == 0) a.scale[row] = scale;
-  // one reciprocal a row; where 1 / scale leaves the normal range (below 2^-120) it is a power
-  // of two short of it, and the elements are divided instead
-  const bool tiny = scale < 7.5e-37f;
-  const float rs = __fdiv_rn(1.f, scale);
+  // one reciprocal a row, each quotient as a division rounds it
+  const bool held = Quotient::holds(scale);
+  const Quotient by(scale);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int i = (j * TPR + tid) * 8;
@@ -161,7 +160,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rmsnorm_fp8_kernel(
     for (int k = 0; k < 2; ++k) {
       float e[4];
 #pragma unroll
-      for (int m = 0; m < 4; ++m) e[m] = tiny ? __fdiv_rn(h[j][4 * k + m], scale) : h[j][4 * k + m] * rs;
+      for (int m = 0; m < 4; ++m) e[m] = held ? by(h[j][4 * k + m]) : __fdiv_rn(h[j][4 * k + m], scale);
       o[k] = (uint32_t)f2_to_e4m3x2_sat(e[0], e[1]) | ((uint32_t)f2_to_e4m3x2_sat(e[2], e[3]) << 16);
     }
     *reinterpret_cast<uint2*>(a.q + t * a.ldq + i) = make_uint2(o[0], o[1]);

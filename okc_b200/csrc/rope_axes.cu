@@ -52,19 +52,13 @@ __device__ __forceinline__ void store8_bf16(__nv_bfloat16* p, const float (&f)[8
       make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
 }
 
-// The quotients are those of an fp32 division.  With y the reciprocal rounded to nearest, q = f y is off by at most
-// one unit, the remainder f - q scale is exact, and q + remainder * y rounds to the division's result (Markstein, 1990).
-// The scale's range keeps all of it normal wherever the quotient is at least 2^-10, below which e4m3 is zero;
-// a quotient that overflows ends as NaN either way.
+// The quotients are those of an fp32 division; one that overflows ends as NaN either way.
 __device__ __forceinline__ void store8_e4m3(uint8_t* p, const float (&f)[8], float scale) {
   float e[8];
-  if (fabsf(scale) >= 0x1p-60f && fabsf(scale) <= 0x1p60f) {
-    const float y = __frcp_rn(scale);
+  if (Quotient::holds(scale)) {
+    const Quotient by(scale);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float q = f[k] * y;
-      e[k] = copysignf(fmaf(fmaf(-q, scale, f[k]), y, q), q);  // of -0, too
-    }
+    for (int k = 0; k < 8; ++k) e[k] = by(f[k]);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) e[k] = __fdiv_rn(f[k], scale);
