@@ -130,34 +130,7 @@ __device__ __forceinline__ void tm_wait_ld(uint32_t (&r)[16]) {
                  "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 
-// Two fp32 operations in one instruction.
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pair2(float x, float y) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
 __device__ __forceinline__ f32x2 bits2(uint32_t x, uint32_t y) { return pair2(__uint_as_float(x), __uint_as_float(y)); }
-__device__ __forceinline__ float2 split2(f32x2 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 
 // tanh(x) / x as a polynomial in x^2: the seven terms of tanh_term over |x| <= 1, or three of the least |x * error|
 // (1.2e-6, 1.5e-4 of a score at kLowCap) over |x| <= 0.4: fused operations where the exponential and the reciprocal

@@ -153,6 +153,34 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   return r;
 }
 
+// Two fp32 operations in one instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair2(float x, float y) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 split2(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // f / scale for many f, as an fp32 division rounds it: with y the reciprocal rounded to nearest, q = f y is off by at
 // most one unit, the remainder f - q scale is exact, and q + remainder * y rounds to the division's result (Markstein,
 // 1990).  In the scales' range all of it is normal wherever the quotient is at least 2^-10, below which e4m3 is zero;
@@ -167,6 +195,13 @@ struct Quotient {
   __device__ __forceinline__ float operator()(float f) const {
     const float q = f * y;
     return copysignf(fmaf(fmaf(-q, scale, f), y, q), q);  // of -0, too
+  }
+  // Two of them, for a positive scale.  The remainder rounded down is -0 for f = +-0, which keeps a zero's sign.
+  __device__ __forceinline__ float2 operator()(float f0, float f1) const {
+    const f32x2 y2 = pair2(y, y), f2 = pair2(f0, f1), q2 = mul2(f2, y2);
+    f32x2 r2;
+    asm("fma.rm.f32x2 %0, %1, %2, %3;" : "=l"(r2) : "l"(q2), "l"(pair2(-scale, -scale)), "l"(f2));
+    return split2(fma2(r2, y2, q2));
   }
 };
 
