@@ -413,8 +413,9 @@ int okc_tp_oproj_allreduce_residual(const void* x, int ldx, const void* w, int l
  * (unit_offset); scale[t] = max|y[t]| / 448, 1 for a row of zeros; q = e4m3(y / scale), RNE.  Without
  * residual (NULL, residual_out NULL) s = x.  x bf16 [T][ldx], residual bf16 or fp32
  * (residual_fp32) [T][ldr], residual_out [T][ldo] of the same type, w bf16 [H], q e4m3 [T][ldq],
- * scale fp32 [T].  H a multiple of 16, <= 16384; rows 16-byte aligned.  A row that holds an
- * infinity or a NaN gets an infinite or NaN scale.  Beside okc_rmsnorm_bf16. */
+ * scale fp32 [T].  H a multiple of 16, <= 16384; rows 16-byte aligned.  Squares are summed in fp32: a row
+ * that holds an infinity or a NaN, or whose sum of squares overflows (magnitudes near 2^64), gets a NaN scale;
+ * with eps = 0 a row whose squares all vanish (magnitudes below 2^-75) is one of zeros.  Beside okc_rmsnorm_bf16. */
 int okc_add_rmsnorm_fp8(const void* x, int64_t ldx, const void* residual, int64_t ldr, int residual_fp32,
                         const void* w, void* residual_out, int64_t ldo, void* q, int64_t ldq, float* scale,
                         int T, int H, float eps, int unit_offset, okc_stream_t stream);

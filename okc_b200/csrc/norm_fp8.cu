@@ -14,8 +14,8 @@
 //
 // The sum of squares, the norm and the scale are fp32; q is the one rounding to 8 bits.  The
 // largest magnitude is an integer maximum of the absolute bit patterns, which orders finite
-// values as floats and puts infinities and NaN above them: a row that holds either gets an
-// infinite or NaN scale instead of a finite scale that hides it.
+// values as floats and puts infinities and NaN above them: a row that holds either, or whose squares
+// overflow, gets a NaN scale instead of a finite scale that hides it.
 #include "kernels.cuh"
 
 namespace okc {
@@ -119,7 +119,9 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, V == 4 && TPR > 32 ? 10
 #pragma unroll
     for (int i = 0; i < WPR; ++i) ss += red_s[sub][i];
   }
-  const float inv = rsqrtf(ss / (float)a.H + a.eps);
+  float inv = rsqrtf(ss / (float)a.H + a.eps);
+  if (ss == 0.f && a.eps == 0.f) inv = 0.f;                // a row of zeros
+  if (!(ss < INFINITY)) inv = __uint_as_float(0x7fffffffu);  // no number of its own, whatever 1 / inf would make of it
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < V; ++j) {

@@ -38,3 +38,29 @@ def test_quotients_are_those_of_a_division(ops, H):
             ties += int(((y / want).to(E4M3).float() != (y * (1 / want)).to(E4M3).float()).sum())
             assert torch.equal(q.cpu().view(torch.uint8), expect.view(torch.uint8))
     assert ties > 0
+
+
+@pytest.mark.parametrize("H", [16, 272, 512, 1024, 2048, 4096, 8192, 16384])
+@pytest.mark.parametrize("stream", [None, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+def test_rows_of_zeros_and_rows_whose_squares_overflow(ops, H, stream, eps):
+    """Zeros have a scale of 1 without an epsilon, too; squares beyond fp32 a NaN one.  Ordinary rows between them are
+    what they are alone."""
+    import test_gpu_norm_fp8 as norm
+    x, w, r = norm._case(7, H, stream, seed=H)
+    for row, by in ((1, 0.0), (3, 2.0 ** 90), (4, 0.0), (5, -(2.0 ** 90))):
+        x[row] *= by
+        if r is not None:
+            r[row] *= by
+    x[1, ::2] = -0.0
+    run = lambda rows, unit: ops.add_rmsnorm_fp8(x[rows].cuda(), w.cuda(), eps, None if r is None else r[rows].cuda(), unit_offset=unit)
+    for unit in (False, True):
+        q, scale, _ = run(list(range(7)), unit)
+        for row in (1, 4):
+            assert (q[row].float() == 0).all() and scale[row] == 1
+        assert torch.isnan(scale[[3, 5]]).all()
+        for row in (0, 2, 6):
+            alone = run([row], unit)
+            assert torch.equal(alone[0].view(torch.uint8)[0], q.view(torch.uint8)[row]) and alone[1][0] == scale[row]
+        norm._check([v if v is None else v[[0, 2, 6]] for v in run(list(range(7)), unit)], x[[0, 2, 6]], w,
+                    r if r is None else r[[0, 2, 6]], unit, eps)
