@@ -155,8 +155,8 @@ __device__ __forceinline__ void tall_block(const float* block, float my_sx, cons
     lin_act_switch(a.act, [&](auto act) {
 #pragma unroll
       for (int i = 0; i < B; ++i) {
-        v[i].x = lin_act<decltype(act)::value>(v[i].x);
-        v[i].y = lin_act<decltype(act)::value>(v[i].y);
+        v[i].x = lin_act<decltype(act)::value, OUT32>(v[i].x);
+        v[i].y = lin_act<decltype(act)::value, OUT32>(v[i].y);
       }
     });
 #pragma unroll
@@ -190,7 +190,7 @@ __device__ __forceinline__ void packed_block(uint8_t* block, const float (&v)[32
   }
   lin_act_switch(a.act, [&](auto act) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) z[j] = lin_act<decltype(act)::value>(z[j]);
+    for (int j = 0; j < 32; ++j) z[j] = lin_act<decltype(act)::value, false>(z[j]);
   });
   // rows of 64 bytes; the chunks of two neighbouring rows are permuted by them, against bank conflicts
 #pragma unroll
@@ -247,7 +247,7 @@ __device__ __forceinline__ void ragged_block(const float* block, int rows, int c
     }
     lin_act_switch(a.act, [&](auto act) {
 #pragma unroll
-      for (int i = 0; i < B; ++i) v[i] = lin_act<decltype(act)::value>(v[i]);
+      for (int i = 0; i < B; ++i) v[i] = lin_act<decltype(act)::value, OUT32>(v[i]);
     });
 #pragma unroll
     for (int i = 0; i < B; ++i)

@@ -39,13 +39,24 @@ enum { LIN_ACT_NONE = 0, LIN_ACT_RELU = 1, LIN_ACT_SILU = 2, LIN_ACT_GELU = 3, L
 
 // Activations in fp32.  tanh and the logistic function go through one exponential:
 // 0.5 (1 + tanh(u)) = 1 / (1 + exp(-2u)).  A NaN stays a NaN (relu included: fmaxf would drop it).
-template <int ACT>
+// FINE, for an fp32 output: the exponential's argument in two parts, since one rounding of it (what a bf16 output does not
+// see) is |v| units of the result.
+template <bool FINE>
+__device__ __forceinline__ float lin_exp(float u) {
+  if (!FINE) return __expf(u);
+  constexpr float hi = 1.4426950216293335f, lo = 1.9259629911266175e-8f;  // log2(e)
+  const float t = u * hi, rest = fmaf(u, lo, fmaf(u, hi, -t));
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return fabsf(t) < 128.f ? fmaf(e, rest * 0.6931471805599453f, e) : e;  // at either end it is 0 or infinite
+}
+template <int ACT, bool FINE>
 __device__ __forceinline__ float lin_act(float v) {
+  auto over = [](float n, float u) { return __fdividef(n, 1.f + lin_exp<FINE>(u)); };
   if constexpr (ACT == LIN_ACT_RELU) return v < 0.f ? 0.f : v;
-  if constexpr (ACT == LIN_ACT_SILU) return __fdividef(v, 1.f + __expf(-v));
+  if constexpr (ACT == LIN_ACT_SILU) return over(v, -v);
   if constexpr (ACT == LIN_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.7071067811865476f));
-  if constexpr (ACT == LIN_ACT_GELU_TANH)
-    return __fdividef(v, 1.f + __expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
+  if constexpr (ACT == LIN_ACT_GELU_TANH) return over(v, -1.5957691216057308f * (v + 0.044715f * v * v * v));
   return v;
 }
 

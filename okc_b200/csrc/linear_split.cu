@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
       for (int i = 0; i < U; ++i) v[i] = fmaf(v[i] * sx[i], sw, bias);
       lin_act_switch(a.act, [&](auto act) {
 #pragma unroll
-        for (int i = 0; i < U; ++i) v[i] = lin_act<decltype(act)::value>(v[i]);
+        for (int i = 0; i < U; ++i) v[i] = lin_act<decltype(act)::value, OUT32>(v[i]);
       });
 #pragma unroll
       for (int i = 0; i < U; ++i) {
