@@ -763,7 +763,7 @@ int launch_attn_chunk(const ChunkArgs& a, cudaStream_t stream) {
   pl.acc = reinterpret_cast<float*>(p);
   p += up(rows * a.D * 4);
   if (!how.split_only) {
-    if (int st = launch_attn_chunk_tc(a, how.tc_only ? 0 : kSplitRows, p, stream)) return st;
+    if (int st = launch_attn_chunk_tc(a, how.tc_only ? 0 : kSplitRows, p, pl.acc, pl.ml, stream)) return st;
     if (how.tc_only || pl.merge_tokens == 0) return OKC_OK;  // no request is short enough
   }
   switch (cap_form(a.softcap)) {

@@ -65,11 +65,15 @@ struct TcCfgA {
   static constexpr int SMEM = 1024 + BAR0 + 512;
 };
 
+// The tensor core truncates as it adds to O: 1e-7 of it for 16 keys, always towards zero (0.06% over 131072 keys, 0.6% over
+// 2^20).  After so many blocks a row's O goes into its fp32 sums in the workspace, and starts again.
+constexpr int kFold = 2048;
+
 struct TcPlanA {
   int splits;
   int above;   // requests of more rows than this are served
-  float* acc;  // [splits][T * Hq][D]
-  float* ml;   // [splits][T * Hq][2]
+  float* acc;  // [splits][T * Hq][D]: a split's sums, or what has been folded
+  float* ml;   // [splits][T * Hq][2]: their origin, and the sum of P
 };
 
 // f16 operands, fp32 sums, 128 x n.
@@ -169,7 +173,7 @@ struct TcShared {
   uint32_t nan[kDepth][kKeys / 32];  // per V block: its keys that hold a NaN that was taken out
 };
 
-template <int D, int CAP, bool BIAS>
+template <int D, int CAP, bool BIAS, bool FOLD>
 __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs a, TcPlanA pl) {
   using C = TcCfgA<D>;
   extern __shared__ uint8_t smem_raw[];
@@ -379,8 +383,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     };
     bool ok = true;
     bool low = a.softcap <= kLowCap;  // ... and no score so far has left the three-term range
+    auto part_of = [&] { return (size_t)split * a.T * a.Hq + (size_t)tok * a.Hq + hq; };  // the row in the workspace
+    // O of the blocks before j0 into the row's sums in the workspace, which are brought to its origin.
+    auto fold = [&](int j0) {
+      const size_t part = part_of();
+      if (!s_ready(j0 + 1)) *abort_flag = 1;  // P V of the block before is done, and the next waits for its P
+      tc_after();
+      const float was = j0 > kFold && live ? pl.ml[part * 2] : -INFINITY, down = was == -INFINITY ? 0.f : ex2(was - m_ref);
+      float* sums = pl.acc + part * D;
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 16) {
+        uint32_t v[16];
+        tm_ld16(to + c0, v);
+        tm_wait_ld(v);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          if (!live) continue;
+          const float o = __uint_as_float(v[c]);
+          sums[c0 + c] = j0 > kFold ? fmaf(sums[c0 + c], down, o) : o;
+        }
+      }
+      if (live) pl.ml[part * 2] = m_ref;
+      tc_before();
+    };
 #pragma unroll 1
     for (int j = 0; j < nb && on; ++j) {
+      if (FOLD && j > 0 && j % kFold == 0) fold(j);
       const int kb = keys.key0 + block_at(keys, j);
       const uint32_t ts = lanes + w * kTile + (j & 1) * kKeys;  // S, and P over its first half
       ok = __all_sync(0xffffffffu, s_ready(j));
@@ -556,17 +584,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
     // ---- output ----
     const bool have = nb > 0 && on && __all_sync(0xffffffffu, ok && s_ready(nb + 1));
     tc_after();
-    const size_t part = (size_t)split * a.T * a.Hq + (size_t)tok * a.Hq + hq;
     const float inv = l == 0.f ? 0.f : __fdividef(a.v_scale[head], l);
-    if (pl.splits > 1 && live) *reinterpret_cast<float2*>(pl.ml + part * 2) = make_float2(m_ref, l);
     // The warp's rows are turned in its share of the query tile (2 D bytes a row) and leave as whole rows: all of a bf16
     // row at once, an fp32 one in halves.  That share holds other warps' queries, too: the products that `have` tells of
     // waited for every warp's, and are done with them.  Without them (no keys: the other warps' copies may still be
     // landing) zeros leave straight from registers.
     uint8_t* turn = smem + C::Q0 + w * C::QTILE + (warp & 3) * 32 * 2 * D;
+    const size_t part = part_of();
+    const bool folded = FOLD && nb > kFold && live;
+    const float was = folded ? pl.ml[part * 2] : -INFINITY, down = was == -INFINITY ? 0.f : ex2(was - m_ref);
+    if (pl.splits > 1 && live) *reinterpret_cast<float2*>(pl.ml + part * 2) = make_float2(m_ref, l);
     auto columns = [&](int c0, uint32_t (&v)[32]) {
       tm_ld32(to + c0, v);
       tm_wait_ld(v);
+      if (FOLD && folded) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(fmaf(pl.acc[part * D + c0 + c], down, __uint_as_float(v[c])));
+      }
       const uint32_t nan = nan_d[c0 / 32];
       if (nan) {
 #pragma unroll
@@ -771,7 +805,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_chunk_tc_kernel(ChunkArgs 
           const uint64_t va = umma_desc_mn(smem_u32(smem + C::V0 + st * C::BLOCK), C::SUB);
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k)
-            umma_ts(t_o, t_s + (j & 1) * kKeys + 8 * k, va + k * (2048 >> 4), id_o, (j | k) != 0);
+            umma_ts(t_o, t_s + (j & 1) * kKeys + 8 * k, va + k * (2048 >> 4), id_o, ((FOLD ? j % kFold : j) | k) != 0);
           umma_commit(&sh.kv_empty[st]);
           if (!two) umma_commit(&sh.kv_empty[st]);  // (the barrier counts both tiles)
           if (j + 2 < nb) {
@@ -848,19 +882,27 @@ int tc_splits(int T, int B, int Hq, int Hkv, long long max_keys) {
   return s < 1 ? 1 : s > 32 ? 32 : (int)s;
 }
 
-template <int D, int CAP, bool BIAS>
-int launch_tc(const ChunkArgs& a, const TcPlanA& pl, cudaStream_t stream) {
+template <int D, int CAP, bool BIAS, bool FOLD>
+int launch_tc_as(const ChunkArgs& a, const TcPlanA& pl, cudaStream_t stream) {
   using C = TcCfgA<D>;
   static okc_host::PerDevice configured;
-  if (int st = configured.smem(attn_chunk_tc_kernel<D, CAP, BIAS>, C::SMEM, kLaunchRegs)) return st;
+  if (int st = configured.smem(attn_chunk_tc_kernel<D, CAP, BIAS, FOLD>, C::SMEM, kLaunchRegs)) return st;
   const long long tiles = tc_tiles(a.T, a.B, a.G);
   if (tiles > 65535) return OKC_ERR_TOO_LARGE;
-  if (int st = okc_host::launch_k(attn_chunk_tc_kernel<D, CAP, BIAS>, dim3(a.Hkv * pl.splits, (unsigned)tiles),
+  if (int st = okc_host::launch_k(attn_chunk_tc_kernel<D, CAP, BIAS, FOLD>, dim3(a.Hkv * pl.splits, (unsigned)tiles),
                                   dim3(kTcThreads), C::SMEM, stream, dim3(1), a, pl))
     return st;
   if (pl.splits == 1) return OKC_OK;
   return okc_host::launch_k(attn_chunk_tc_merge_kernel<D>, dim3((unsigned)(((long long)a.T * a.Hq + 7) / 8)), dim3(256),
                             0, stream, dim3(1), a, pl);
+}
+
+// The variant with sums set aside where the table is wide enough for it: within one kernel it cost 1 to 4% (4096 tokens
+// behind 4096 at heads of 64, capped, 902 and 937 us).
+template <int D, int CAP, bool BIAS>
+int launch_tc(const ChunkArgs& a, const TcPlanA& pl, cudaStream_t stream) {
+  return a.max_keys / pl.splits > kFold * kKeys ? launch_tc_as<D, CAP, BIAS, true>(a, pl, stream)
+                                                : launch_tc_as<D, CAP, BIAS, false>(a, pl, stream);
 }
 
 template <int CAP>
@@ -881,12 +923,16 @@ size_t attn_chunk_tc_ws_bytes(int T, int B, int Hq, int Hkv, int D) {
   return up(rows * D * 4) + up(rows * 8);
 }
 
-int launch_attn_chunk_tc(const ChunkArgs& a, int above, void* ws, cudaStream_t stream) {
+int launch_attn_chunk_tc(const ChunkArgs& a, int above, void* ws, float* sums, float* origins, cudaStream_t stream) {
   TcPlanA pl;
   pl.above = above;
   pl.splits = tc_splits(a.T, a.B, a.Hq, a.Hkv, a.max_keys);
-  pl.acc = reinterpret_cast<float*>(ws);
-  pl.ml = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + up((size_t)pl.splits * a.T * a.Hq * a.D * 4));
+  pl.acc = sums;
+  pl.ml = origins;
+  if (pl.splits > 1) {
+    pl.acc = reinterpret_cast<float*>(ws);
+    pl.ml = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + up((size_t)pl.splits * a.T * a.Hq * a.D * 4));
+  }
   switch (cap_form(a.softcap)) {
     case kCapFine: return launch_tc_cap<kCapFine>(a, pl, stream);
     case kCapPlain: return launch_tc_cap<kCapPlain>(a, pl, stream);

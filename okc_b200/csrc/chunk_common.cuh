@@ -123,8 +123,9 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 constexpr int kSplitRows = 64;
 
 // The tensor-memory kernel (attention_chunk_tc.cu) for the requests of more than `above` rows (kSplitRows, or 0
-// where the only request may have more than kSplitRows).
+// where the only request may have more than kSplitRows).  `sums` [T * Hq][D] and `origins` [T * Hq][2]: scratch of very
+// long contexts, which may be what the short chunks' kernel takes behind it.
 size_t attn_chunk_tc_ws_bytes(int T, int B, int Hq, int Hkv, int D);
-int launch_attn_chunk_tc(const ChunkArgs& a, int above, void* ws, cudaStream_t stream);
+int launch_attn_chunk_tc(const ChunkArgs& a, int above, void* ws, float* sums, float* origins, cudaStream_t stream);
 
 }  // namespace okc

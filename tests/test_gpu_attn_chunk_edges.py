@@ -185,3 +185,33 @@ def test_many_keys_far_below_one(ops, n, keys, cap, D):
         share = others * math.exp(-(cap * math.tanh(18 / cap) if cap else 18.0))
         want = share / (1 + share)
         assert ((o - want).abs() <= (2.0 ** -9 + 2.0 ** -11 + 2.0 ** -16) * want + others * 2.0 ** -32).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,Hkv,kind", [(1216, 2, "even"), (1216, 2, "rising"), (1216, 2, "slopes"), (256, 8, "rising"),
+                                        (256, 8, "cap")])
+def test_sums_over_a_million_keys(ops, T, Hkv, kind, D):
+    """Values that are the same at every position: so is the output, whatever the weights.  The tensor core's truncation
+    takes at most 2^-22 of a sum for 16 keys (a unit of it and one for the products' alignment), and 131072 keys go into one
+    sum: 2^-9, and 2^-9 for the rounding to bf16.  1216 tokens at 2 / 16 heads fill the grid, 256 at 8 / 64 split the
+    keys in two.  Scores that rise with the position move the origin of the exponentials behind sums that are set
+    aside; some rows see their first key after 600000."""
+    n, P, G = 2 ** 20, 16, 8
+    g = torch.Generator(device="cuda").manual_seed(D + T)
+    k = torch.randn(n // P, P, Hkv, D, generator=g, device="cuda", dtype=torch.float16)
+    q = torch.randn(T, G * Hkv, D, generator=g, device="cuda")
+    if kind == "rising":
+        k[..., 0] = 12 * (torch.arange(n, device="cuda", dtype=torch.float32).view(n // P, P, 1) / n).half()
+        q[..., 0] = 24 * (8 if D == 64 else 11) / 8
+    col = 2.0 ** (torch.arange(D) % 5 - 2).float() * (1 - 2.0 * (torch.arange(D) % 2)) * (1 + torch.arange(D) % 3 / 4)
+    v = col.to(attn.E4M3).cuda().expand(n // P, P, Hkv, D).contiguous()
+    one = torch.ones(Hkv, device="cuda")
+    first = torch.zeros(T, dtype=torch.int32)
+    first[::7] = 600000
+    more = {"slopes": dict(slopes=torch.zeros(G * Hkv, device="cuda")), "cap": dict(softcap=5.0)}.get(kind, {})
+    for _ in range(2):
+        o = ops.attn_chunk(q.to(torch.bfloat16), k.to(attn.E4M3), v, torch.arange(n // P, dtype=torch.int32, device="cuda").view(1, -1),
+                           torch.tensor([0, T], dtype=torch.int32, device="cuda"), torch.tensor([n], dtype=torch.int32, device="cuda"),
+                           one, one, 1 / math.sqrt(D), doc_start=first.cuda(), max_q=T, **more)
+        assert (o.cpu().float() / col - 1).abs().max() <= 2.0 ** -8
+    assert ops.read_device_error("attn_chunk") == 0
