@@ -25,7 +25,9 @@
 //  * a K fragment's k slots and a V fragment's columns are permuted so that each lane's share is
 //    whole 16-byte chunks (a sum over k does not depend on its order).
 // Partial sums go to the workspace as fp32 with their running maximum and sum; segments are joined
-// in block order, so results repeat bit for bit.
+// in block order, so results repeat bit for bit.  mma.sync truncates as it adds to the output, 1.4e-7 of it for 16 keys of a
+// warp: 6e-5 for one request behind 2^20 positions, 0.5% at most, where the keys fill the whole card (594000 of them a
+// warp).  Summed outside of the instruction that goes, and the kernel takes 1 to 4% longer.
 #include "chunk_common.cuh"
 
 #include <type_traits>
@@ -34,7 +36,7 @@ namespace okc {
 
 namespace {
 
-constexpr int kStep = 32;      // keys per warp step
+constexpr int kStep = 32;      // keys of a warp's step: a lane looks one up
 constexpr int kWarps = 8;
 // log2 of the largest P: f16 keeps P down to 2^-25, so that keys are lost from the sum only 2^-(25 + kLift) below the
 // row's largest (from an origin at the largest, a million keys at e^-18 of it lost 1.5% of the weight).
@@ -205,13 +207,13 @@ __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) attn_chunk_split
     const int32_t* trow = a.page_table + (size_t)b * a.table_ld;
     auto fetch_page = [&](int s) -> int {  // of this lane's key of step s; what it is, issue() checks
       const int key = k0 + s * pl.step_keys + lane;
-      return s < s_hi && lane < kStep && key >= t_lo && key < t_hi ? trow[page_of(a, key)] : -1;
+      return s < s_hi && key >= t_lo && key < t_hi ? trow[page_of(a, key)] : -1;
     };
     auto issue = [&](int s, int page) {
       if (s < s_hi) {
         const int key = k0 + s * pl.step_keys + lane;
         const bool on = page >= 0 && page < a.num_pages;
-        if (!on && lane < kStep && key >= t_lo && key < t_hi) atomicOr(a.err, OKC_DEVERR_PAGE);
+        if (!on && key >= t_lo && key < t_hi) atomicOr(a.err, OKC_DEVERR_PAGE);
         // rows of D bytes, below 2^32
         const uint32_t row = on ? ((uint32_t)page * a.P + key - page_of(a, key) * a.P) * a.Hkv + head : 0u;
         const uint32_t mask = __ballot_sync(0xffffffffu, on);
@@ -230,7 +232,7 @@ __global__ void __launch_bounds__(32 * kWarps, D == 64 ? 2 : 1) attn_chunk_split
             cp16(vd + i * KI * D + (D == 128 ? ch ^ (2 * (i & 3)) : ch) * 16, vp + src, in);
           }
         };
-        if (mask == (kStep == 32 ? 0xffffffffu : 0xffffu)) copy(std::true_type{});
+        if (mask == 0xffffffffu) copy(std::true_type{});
         else copy(std::false_type{});
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -659,8 +661,6 @@ __global__ void __launch_bounds__(256) attn_chunk_merge_kernel(ChunkArgs a, Spli
 }
 
 int heads_a_block(int Hkv) { return Hkv % 8 == 0 ? 8 : Hkv % 4 == 0 ? 4 : Hkv % 2 == 0 ? 2 : 1; }
-
-size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
 // CTAs at most: as many as are resident at once.
 int split_ctas(int D) { return okc_host::num_sms() * (D == 64 ? 2 : 1); }

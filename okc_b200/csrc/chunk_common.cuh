@@ -117,6 +117,9 @@ __device__ __forceinline__ RowSpan row_span(const ChunkArgs& a, const Req& rq, i
 __device__ __forceinline__ int f16_shift(uint32_t top) { return max(-100, (int)(top >> 7) - 127 - 13); }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
+// A piece of the workspace.
+inline size_t up(size_t n) { return (n + 255) / 256 * 256; }
+
 // A kernel of this file family serves the requests of at most / more than this many rows a KV
 // head (new tokens x query heads of one KV head).  128 requests of 64 / 8 heads, the short chunks' kernel against the
 // tensor-memory one: 32 rows 416 and 637 us, 64 rows 676 and 767; one request of 64 rows 35 and 35.

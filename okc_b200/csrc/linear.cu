@@ -25,7 +25,7 @@ namespace okc {
 
 namespace {
 
-constexpr int kMaxStages = 5;
+constexpr int kMaxStages = 4;
 constexpr int kRing = 192 * 1024;  // as many stages as fit: 3 of 256 channels, 4 of up to 128
 constexpr int kPanels = 2;       // 128-byte K panels of a stage: one barrier and one commit for eight MMAs
 constexpr int kSegment = 4;      // stages an accumulator takes, for an fp32 output
@@ -54,9 +54,6 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The shared-memory address of `bar` in the pair's leading CTA.
 __device__ __forceinline__ uint32_t in_leader(uint64_t* bar) {

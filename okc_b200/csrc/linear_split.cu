@@ -35,9 +35,6 @@ struct SplitCfg {
   static_assert(BODY >= BN * 128 * 4, "the sums reuse the ring");
 };
 
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // A float of CTA `rank`'s shared memory at this CTA's address `local`; 0 where !on.
 __device__ __forceinline__ float ld_cluster(uint32_t local, uint32_t rank, bool on) {
   float v;
@@ -200,7 +197,7 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
 #pragma unroll
     for (int j = 0; j < COLS; ++j) sums[(half * COLS + j) * 128 + q4 * 32 + lane] = acc[j];
   }
-  if (S > 1) cluster_sync_all();
+  if (S > 1) cluster_sync();
   else __syncthreads();
   // ---- tokens rank, rank + S, ..: thread = (channel, every second of them) ----
   if (warp >= 2) {
@@ -253,7 +250,7 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
       }
     }
   }
-  if (S > 1) cluster_sync_all();  // the others have read this CTA's sums
+  if (S > 1) cluster_sync();  // the others have read this CTA's sums
   else __syncthreads();
   if (warp == 0) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
