@@ -30,6 +30,12 @@ combine), and on rank 0 the single-GPU MoE over the same world * t tokens:
 
     python -m torch.distributed.run --nnodes=1 --nproc-per-node 2 --master-addr 127.0.0.1 \
         --master-port 29514 -m okc_b200.profile_cases moe_ep --t 32
+
+The `ragged` case times an operator case of perf/operators.py (a checkout's, not the package's), `--name`d from its list
+and changed by `--set`: in CUDA graphs of 20 calls, one behind the other and each behind a pass over 256 MB, whose
+own time is taken off.  With --launches it makes that many plain calls instead, for a profiler:
+
+    python -m okc_b200.profile_cases ragged --name attn_b128_decode_cap --set n=4 cap=0.0
 """
 
 from __future__ import annotations
@@ -256,11 +262,45 @@ def case_moe_ep(a):
     return res if rank == 0 else None
 
 
+def case_ragged(a):
+    import ast
+    import importlib.util
+    from pathlib import Path
+
+    spec = importlib.util.spec_from_file_location("operators", Path(__file__).resolve().parent.parent / "perf" / "operators.py")
+    cases = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(cases)
+    cases.own = True
+    case = {c["name"]: c for c in cases.listed()}[a.name]
+    for item in a.set:
+        key, value = item.split("=")
+        case[key] = type(case[key])(ast.literal_eval(value) if not isinstance(case[key], str) else value)
+    state = cases.prepare(case, 1)
+    res = {"case": "ragged", **case, **cases.work(case)}
+    if a.launches:
+        _time(lambda: cases.run(state), a.warmup, a.launches)
+        return res
+    spill = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    n = 20
+
+    def graph_us(fn):
+        fn()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(n):
+                fn()
+        return min(_time(graph.replay, 1, 1) for _ in range(5)) / n
+
+    res["us"] = round(graph_us(lambda: cases.run(state)), 2)
+    res["us_flushed"] = round(graph_us(lambda: (spill.add_(1), cases.run(state))) - graph_us(lambda: spill.add_(1)), 2)
+    return res
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser()
-    ap.add_argument("case", choices=["attn", "gemv", "moe", "tp", "moe_ep", "muse_layer"])
+    ap.add_argument("case", choices=["attn", "gemv", "moe", "tp", "moe_ep", "muse_layer", "ragged"])
     ap.add_argument("--warmup", type=int, default=2)
-    ap.add_argument("--launches", type=int, default=3)
+    ap.add_argument("--launches", type=int, default=None, help="3; ragged: 0, which times graphs")
     ap.add_argument("--b", type=int, default=64)
     ap.add_argument("--ctx-lo", type=int, default=512)
     ap.add_argument("--ctx-hi", type=int, default=4096)
@@ -277,10 +317,14 @@ def main(argv=None):
     ap.add_argument("--d", type=int, default=128, help="attn: head dim")
     ap.add_argument("--window", type=int, default=0, help="muse_layer: sliding window (0: full)")
     ap.add_argument("--kk", default="1024", help="tp: comma-separated O-projection K per rank")
+    ap.add_argument("--name", default="attn_b128_decode_cap", help="ragged: the case")
+    ap.add_argument("--set", nargs="*", default=[], metavar="KEY=VALUE", help="ragged: sizes other than the case's")
     a = ap.parse_args(argv)
+    if a.launches is None:
+        a.launches = 0 if a.case == "ragged" else 3
     torch.cuda.set_device(int(os.environ.get("LOCAL_RANK", "0")))
     res = {"attn": case_attn, "gemv": case_gemv, "moe": case_moe, "tp": case_tp, "moe_ep": case_moe_ep,
-           "muse_layer": case_muse_layer}[a.case](a)
+           "muse_layer": case_muse_layer, "ragged": case_ragged}[a.case](a)
     if res is not None:
         print(json.dumps(res), flush=True)
     return 0
