@@ -405,7 +405,7 @@ int okc_tp_oproj_allreduce_residual(const void* x, int ldx, const void* w, int l
  * Ragged batches: cu_q int32 [B + 1] ascending from 0; request b owns the rows cu_q[b] ..
  * cu_q[b+1]-1, and row t sits at the cache position seq_lens[b] - (cu_q[b+1] - t): seq_lens int32 [B]
  * counts the cached positions with the new ones.  Rows from cu_q[B] to T-1 (a padded batch) are
- * neither read nor written.
+ * not written, and what their inputs hold has no effect (they may be read).
  * ---------------------------------------------------------------------------------- */
 
 /* Residual add + RMSNorm to e4m3: s = x + residual rounded to the residual's type and stored in
@@ -424,7 +424,9 @@ int okc_add_rmsnorm_fp8(const void* x, int64_t ldx, const void* residual, int64_
  * w [N][ldw] both bf16 (e4m3 = 0) or both e4m3 (e4m3 = 1); x_scale fp32 [M], w_scale fp32 [N] or, with
  * w_scale_one, [1]; bias bf16 [N]; residual bf16 or fp32 (residual_fp32) [M][ldr]; each of the four may be
  * NULL.  y bf16 or fp32 (out_fp32) [M][ldy].  act: 0 none, 1 relu, 2 silu, 3 gelu (erf), 4 gelu
- * (tanh form).  fp32 accumulation and epilogue, one rounding.  x and w rows are 16-byte aligned
+ * (tanh form).  Products are summed in fp32 by the tensor core, which truncates: off by 3e-6 of sum |x||w| at K = 4104 and
+ * growing with K for a bf16 output; for an fp32 output in segments that are added with rounding, 3e-7.  fp32
+ * epilogue, one rounding to the output's type.  x and w rows are 16-byte aligned
  * (base, and ld x element size a multiple of 16 bytes); K itself is a multiple of 16 (e4m3) or 8 (bf16).
  * y may be residual.  Takes no workspace.  Beside okc_gemm_bf16. */
 int okc_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int e4m3, const float* x_scale,
@@ -458,7 +460,8 @@ int okc_rope_axes_kv_append(const void* qkv, int64_t ldqkv, const int64_t* posit
  * the cache holds there.  q bf16 [T][ldq], out bf16 [T][ldo] (Hq heads of D), caches e4m3
  * [num_pages, P, Hkv, D] with scales fp32 [Hkv], page_table int32 [B][table_ld] (max_pages columns).  A
  * position on a page outside the pool reads zeros, one past the table does not exist (both
- * OKC_DEVERR_PAGE).  max_q: the longest chunk (0 = unknown); it only chooses kernels.  D 64 or
+ * OKC_DEVERR_PAGE).  max_q: the longest chunk (0 = unknown); it only chooses kernels, as the table's width does where it
+ * rules out long contexts: 128 requests of one token take 218 us with it and 262 without.  D 64 or
  * 128, B <= 2048, Hq / Hkv whole, 16-byte aligned rows, fewer than 2^32 - 1 cache rows of D,
  * T * Hq < 2^31, T * Hq / Hkv + 256 B below 2^24; positions from 2^31 - 2^17 on count as past the table.  Requests of
  * at most 64 rows (tokens x Hq / Hkv) have their work numbered in 32 bits: where the call may hold some beside others

@@ -9,8 +9,8 @@
 // and a row that sees nothing is zero.
 //
 // Bound by the cache read (2 D bytes a key and KV head), nearly: 128 requests of 64 / 8 heads of 128 behind 1050 to
-// 8192 positions take 220 us (5.6 TB/s; capped, the loads alone 198), uncapped 211; 4 tokens each (32 rows: two
-// tiles, the keys converted for each) 416.  One token behind 81919 positions, 16 / 2 heads of 64: 21.5 us, of which
+// 8192 positions take 218 us (5.7 TB/s; capped, the loads alone 198), uncapped 214; 4 tokens each (32 rows: two
+// tiles, the keys converted for each) 417.  One token behind 81919 positions, 16 / 2 heads of 64: 21.7 us, of which
 // the two launches and the chains to the first key and through the merge are 9.  The rows of one KV head's query group
 // (token-major, G heads a token) fill the 16 rows of mma.sync tiles, or, where no request has more than 8,
 // their 8 columns with keys and outputs as the rows: half the MMAs and half the accumulators.  e4m3 keys and

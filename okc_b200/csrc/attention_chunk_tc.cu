@@ -16,7 +16,7 @@
 // The special-function unit bounds it: 256 x 64 exponentials take 1024 cycles of it a block, where the tensor
 // cores need 1024 too, and a block takes 1960 (the softmax warps' other instructions and latencies overlap
 // only in part; a third of the exponentials as polynomials on the fused-operation pipe made it slower).
-// 4096 tokens behind 4096 cached, 64 / 8 heads of 128: 820 us (1010 TFLOP/s), capped 1020 us.  A CTA of one key block
+// 4096 tokens behind 4096 cached, 64 / 8 heads of 128: 825 us (1000 TFLOP/s), capped 1004 us, under a bias 855.  A CTA of one key block
 // takes 11 us (finding its rows, their keys and the query 3, the first keys 2, the first block's two passes 2, the
 // output 2): short spans are bound by that.
 // Blocks of a request are taken from its last rows on: the longest causal spans start first.  With few

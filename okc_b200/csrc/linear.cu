@@ -2,8 +2,8 @@
 // e4m3 or bf16 operands, fp32 accumulation in tensor memory.
 //
 // Compute-bound from a few hundred tokens on (2MNK operations against (M + N) K bytes in).  8192 x 10240 x 8192 in
-// e4m3 with a gelu: 580 us, 2.36 PFLOP/s under the power cap.  777 x 4095 x 4104 in bf16 to fp32 with a residual: 45 us
-// (36 us at 4096 x 4096): 4 token tiles on 148 SMs, and the ends of a tile in the open.
+// e4m3 with a gelu: 478 to 568 us by the card's temperature, 2.4 to 2.9 PFLOP/s under the power cap.  777 x 4099 x 4104 in
+// bf16 to fp32 with a silu and a residual: 47 us (36 us at 4096 x 4096 without the silu): 4 token tiles on 148 SMs, and the ends of a tile in the open.
 //  * a CTA pair owns a tile of 256 tokens x bn channels (tcgen05 cta_group::2): each CTA loads its 128
 //    token rows and half of the channel rows, 32 KB a K block for 256 x 256 x 128 bytes of products,
 //    so shared-memory traffic stays below what the 8-bit MMA rate takes (a single CTA's 128 x 256 tile

@@ -1,8 +1,9 @@
 // Projection with an epilogue, few tokens: the weight is the MMA's 128-row operand and the tokens its N
 // side, so one CTA tile covers 128 channels x up to BN tokens and the weight is read once.
 //
-// HBM-bound on the weight stream (N K bytes in e4m3): one token x 10240 x 8192 16.7 us (5.0 TB/s), of which about 4 are
-// the launch and the pipeline's ends; 128 tokens x 8192 x 8192 with a residual 21 us.
+// HBM-bound on the weight stream (N K bytes in e4m3): one token x 10240 x 8192 17.5 us (4.8 TB/s), of which about 4 are
+// the launch and the pipeline's ends; 8192 x 8192 with a residual (67 MB, half of it in L2 from call to call) 9.8 us at 2
+// tokens, 14 at 32, 18 at 128, in bf16 24, 30 and 35; with L2 flushed between the calls 19, 23 and 27, in bf16 32, 38 and 43.
 //  * K is split over the S = 1, 2, 4 or 8 CTAs of a cluster, chosen so that the waves of resident clusters
 //    times a CTA's stages (and ends) are fewest: the whole card reads whatever N is;
 //  * warp 0 streams K blocks of 256 bytes a weight row with TMA into a ring, warp 1 issues the

@@ -12,7 +12,8 @@
 // 2 (Hq + 2 Hkv) D bytes in, 2 Hq D + 2 Hkv D bytes out per token, in 16-byte vectors.  The instructions
 // (about 110 a vector, more for e4m3) weigh more than the bytes, and for few tokens the chain to the page id: row
 // vectors are fetched before it, and a thread fetches its next vector before it turns one.
-// 3614 tokens of 28 + 4 heads of 128, 96 elements turned: 16.7 us, 3.8 TB/s; 128 tokens of 64 + 8 heads: 5 us.
+// 3614 tokens of 28 + 4 heads of 128, 96 elements turned: 15.4 us, 4.1 TB/s (18.7 with the inputs out of L2); 128 tokens of
+// 64 + 8 heads: 5 us.
 #include "chunk_common.cuh"
 
 namespace okc {
