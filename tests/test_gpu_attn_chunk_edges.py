@@ -215,3 +215,72 @@ def test_sums_over_a_million_keys(ops, T, Hkv, kind, D):
                            one, one, 1 / math.sqrt(D), doc_start=first.cuda(), max_q=T, **more)
         assert (o.cpu().float() / col - 1).abs().max() <= 2.0 ** -8
     assert ops.read_device_error("attn_chunk") == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kind", ["plain", "cap", "slopes"])
+def test_long_contexts_beside_short_chunks(ops, D, kind):
+    """A chunk behind 300000 positions, whose sums are set aside in scratch that the short chunks of the same call take
+    behind it, against 64 bits on rows of each, with random values, a rising origin, pages in any order and a NaN value
+    that some rows see; from a graph twice, and on another stream, the same bits.  The operator's tolerance, and 2^-9
+    of the sums for the tensor core's truncation."""
+    Hq, Hkv, P, n = 32, 4, 16, [1300, 1, 3]
+    full = [300000, 6, 250000]
+    g = torch.Generator(device="cuda").manual_seed(D)
+    width = -(-max(full) // P) + 2
+    pool = 3 * width
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    k = rnd(pool, P, Hkv, D).to(attn.E4M3)
+    v = rnd(pool, P, Hkv, D).to(attn.E4M3)
+    table = torch.randperm(pool, generator=g, device="cuda").to(torch.int32).view(3, width)
+    rise = (torch.arange(width * P, device="cuda") * (20.0 / (width * P))).view(width, P, 1)
+    for b in range(3):
+        k[table[b].long(), :, :, 0] = rise.expand(width, P, Hkv).to(attn.E4M3)
+    T = sum(n)
+    q = rnd(T, Hq, D)
+    q[..., 0] = 1.0 * D ** 0.5
+    q = q.to(torch.bfloat16)
+    cu = torch.tensor([0, 1300, 1301, 1304], dtype=torch.int32, device="cuda")
+    ks, vs = torch.full((Hkv,), 0.75, device="cuda"), torch.full((Hkv,), 1.25, device="cuda")
+    more = {"plain": {}, "cap": dict(softcap=40.0), "slopes": dict(slopes=2.0 ** (-14.0 - torch.arange(Hq, device="cuda") / 8))}[kind]
+    call = lambda **kw: ops.attn_chunk(q, k, v, table, cu, torch.tensor(full, dtype=torch.int32, device="cuda"), ks, vs, 1 / math.sqrt(D),
+                                       max_q=1300, **more, **kw)
+    o = call()
+    lens = torch.tensor(full, dtype=torch.int32, device="cuda")
+    for t, b in ((0, 0), (131, 0), (700, 0), (1299, 0), (1300, 1), (1301, 2), (1303, 2)):
+        p = full[b] - n[b] + t - int(cu[b])
+        j = torch.arange(p + 1, device="cuda")
+        page = table[b].long()[j // P]
+        for h in (0, 13, 31):
+            kk, vv = (x.view(torch.uint8)[page, j % P, h // 8].view(attn.E4M3).float().double() for x in (k, v))
+            s = kk @ q[t, h].double() * (0.75 / math.sqrt(D))
+            if kind == "cap":
+                s = 40 * torch.tanh(s / 40)
+            if kind == "slopes":
+                s = s - more["slopes"][h].double() * (p - j)
+            w = torch.softmax(s, 0)
+            want, a = w @ vv * 1.25, w @ vv.abs() * 1.25
+            assert ((o[t, h].double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -9.5 + 2.0 ** -9) * a).all(), (t, h)
+    graph = torch.cuda.CUDAGraph()
+    out = torch.empty_like(o)
+    args = (q, k, v, table, cu, lens, ks, vs, 1 / math.sqrt(D))
+    with torch.cuda.graph(graph):
+        ops.attn_chunk(*args, max_q=1300, out=out, **more)
+    for _ in range(2):
+        out.fill_(5.0)
+        graph.replay()
+        assert torch.equal(out, o)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        o2 = call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o2, o) and torch.equal(out, o)
+    # position 100000 of the first request: every row of it, and only its head and column
+    v.view(torch.uint8)[int(table[0, 100000 // P]), 100000 % P, 2, 7] = 0x7F
+    nan = torch.isnan(call().float())
+    want = torch.zeros_like(nan)
+    want[:1300, 16:24, 7] = True
+    assert torch.equal(nan, want)
+    assert ops.read_device_error("attn_chunk") == 0
