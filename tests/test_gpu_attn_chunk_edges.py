@@ -284,3 +284,16 @@ def test_long_contexts_beside_short_chunks(ops, D, kind):
     want[:1300, 16:24, 7] = True
     assert torch.equal(nan, want)
     assert ops.read_device_error("attn_chunk") == 0
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("Hq,Hkv,D,P", [(128, 1, 64, 16), (160, 2, 128, 3), (6, 3, 128, 16), (30, 6, 64, 1), (65, 1, 64, 128)])
+@pytest.mark.parametrize("kind", [dict(), dict(cap=1500.0, slopes=True, prefix=True), dict(window=33, docs=True)])
+def test_other_groups_of_heads(ops, Hq, Hkv, D, P, kind, wide):
+    """More query heads a KV head than a short chunk may have rows; head counts that no block of 2, 4 or 8 divides."""
+    attn.WIDE = wide
+    c = attn._case([1, 4, 0, 9], [0, 90, 3, 200], Hq, Hkv, D, P, seed=Hq, pad=2, **kind)
+    for m in (9, None):
+        attn._check(ops, c, max_q=m)
+    c = attn._case([1], [300], Hq, Hkv, D, P, seed=Hq, **kind)
+    attn._check(ops, c, max_q=1)

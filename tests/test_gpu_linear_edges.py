@@ -42,3 +42,13 @@ def test_activations_of_fp32_outputs(ops, M, act):
         tol = 2.0 ** -22 * v.abs()
     off = (y - want).abs()
     assert (off <= tol).all(), f"off by {float((off / tol.clamp(min=1e-300)).max()):.1f} tolerances at {float(v.flatten()[(off / tol.clamp(min=1e-300)).argmax()])}"
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "bf16"])
+@pytest.mark.parametrize("M", [1, 17, 129, 300])
+@pytest.mark.parametrize("N,K", [(1, 16), (2, 32), (7, 1040), (31, 16), (33, 272)])
+def test_the_narrowest_outputs(ops, M, N, K, dtype):
+    import test_gpu_linear as lin
+    c = lin._case(M, N, K, dtype, seed=M + N, residual=torch.float32)
+    for out in (torch.float32, torch.bfloat16):
+        lin._check(ops.linear(**lin._cuda(c), act="silu", out_dtype=out), c, "silu", f"{M} {N} {K} {out}")
