@@ -11,6 +11,7 @@ not on a CUDA device raises.
 from __future__ import annotations
 
 import math
+import threading
 
 import torch
 
@@ -375,11 +376,19 @@ def attn_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
 def _error_word(dev: int, tag: str) -> int:
     buf = _WS.get((dev, tag))
     if buf is None:
-        if _on_device(dev, torch.cuda.is_current_stream_capturing):
-            raise _lib.OkcError(f"{tag}: the first call on a device allocates its error word; make it before a capture")
-        buf = workspace(dev, tag, 256)
-        torch.cuda.current_stream(dev).synchronize()  # zeroed before a call on any stream
+        with _FIRST:  # of the threads that make a first call at once, one makes the word
+            buf = _WS.get((dev, tag))
+            if buf is None:
+                if _on_device(dev, torch.cuda.is_current_stream_capturing):
+                    raise _lib.OkcError(
+                        f"{tag}: the first call on a device allocates its error word; make it before a capture")
+                buf = torch.zeros(4096, dtype=torch.uint8, device=f"cuda:{dev}")
+                torch.cuda.current_stream(dev).synchronize()  # zeroed before a call on any stream
+                _WS[(dev, tag)] = buf
     return buf.data_ptr()
+
+
+_FIRST = threading.Lock()
 
 
 def _on_device(dev: int, fn, *args):
